@@ -53,6 +53,10 @@ EXPORTED_SYMBOLS = (
     "ca_status_string",
     "ca_version",
     "ca_round_bf16_host",
+    "ca_kv8_store",
+    "ca_kv8_load",
+    "ca_attention_kv8_dev",
+    "ca_attention_kv8_workspace",
 )
 
 

@@ -1343,3 +1343,5 @@ const char* ca_version(void) { return "canvas_attn 0.1.0 sm_100a"; }
 
 
 }  // extern "C"
+
+#include "kv8_api.cuh"

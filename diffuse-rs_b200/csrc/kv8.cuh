@@ -1,0 +1,318 @@
+// kv8.cuh -- the 8-bit inter-step cache: quantising K/V rows as they are
+// written and reading them back.
+//
+// K and V are held as e4m3 values with one fp32 scale for each block of T
+// consecutive positions and kv head; the value held is e4m3 * scale. The
+// store writes only powers of two: 2^k with the smallest k in [-64, 120] for
+// which amax <= 448 * 2^k. Dividing by it is exact, so a value is rounded
+// once (to e4m3, nearest even); a held row keeps its bits until its block's
+// scale grows, and then loses nothing but what falls below e4m3's smallest
+// step; and e4m3 * 2^k has at most 4 significant bits, so reading back as
+// bf16 is exact. It replaces StepCache::store and ::gather
+// (src/model/cache.rs:62-81) for a cache of half the bytes.
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+
+#include "sm100.cuh"
+
+namespace ca {
+
+constexpr int kKv8MinExp = -64, kKv8MaxExp = 120;
+constexpr int kErrInvalidRow = -1;
+
+struct Kv8View {
+  uint8_t* k;        // [batch, n_total, Hkv, hd]; position stride row_stride
+  uint8_t* v;
+  float* k_scale;    // [batch, n_blocks, Hkv]
+  float* v_scale;
+  int batch, n_total, Hkv, hd;
+  int T;             // positions per scale: 16, 32, 64 or 128
+  int n_blocks;      // ceil(n_total / T)
+  long long row_stride;
+};
+
+struct Kv8StoreParams {
+  Kv8View c;
+  const __nv_bfloat16* k;  // [rows, Hkv, hd]
+  const __nv_bfloat16* v;
+  const int* pos;          // [rows], ascending within a sequence
+  const int* cu_active;    // [batch + 1] or null (na rows per sequence)
+  const int* kv_len;       // [batch] or null
+  int na;
+  long long rows;
+  int rows_per_job;
+  int* err;
+};
+
+// Two fp32 to two e4m3 (round to nearest even, saturating, NaN kept): lo in
+// the low byte.
+__device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// The four e4m3 values of a word as f16 pairs (exact).
+__device__ __forceinline__ void e4m3x4_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+}
+
+__device__ __forceinline__ float2 f16x2_to_f32(uint32_t h) {
+  float2 r;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+      "cvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "r"(h));
+  return r;
+}
+
+__device__ __forceinline__ void e4m3x4_to_f32(uint32_t w, float (&x)[4]) {
+  uint32_t a, b;
+  e4m3x4_to_f16(w, a, b);
+  const float2 p = f16x2_to_f32(a), q = f16x2_to_f32(b);
+  x[0] = p.x;
+  x[1] = p.y;
+  x[2] = q.x;
+  x[3] = q.y;
+}
+
+// The exponent of the scale that a block of this largest magnitude needs.
+// 448 = 1.75 * 2^8, so amax = m * 2^e (1 <= m < 2) needs e - 8, or e - 7
+// where m > 1.75; read off the fp32 bits, so it is exact.
+__device__ __forceinline__ int kv8_exp(float amax) {
+  if (!(amax > 0.f)) return kKv8MinExp;
+  const uint32_t u = __float_as_uint(amax);
+  const int e = static_cast<int>(u >> 23) - 127;
+  const int k = e - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return min(max(k, kKv8MinExp), kKv8MaxExp);
+}
+
+__device__ __forceinline__ float exp2_int(int k) {  // 2^k, -126 <= k <= 127
+  return __int_as_float((k + 127) << 23);
+}
+
+// One warp writes the rows of one (block, kv head) of K or of V: the largest
+// magnitude of its new rows, the scale, the rounded rows, and, if the scale
+// grew, the rows that stay. A warp's job is rows_per_job consecutive entries
+// of the active list, for one head of K or V; it takes on the blocks whose
+// first active row lies among them and follows each into the next job's
+// entries, so every block has exactly one writer.
+//
+// Bound by HBM (2 bytes read and 1 written for each value) on full passes and
+// by latency on a step's few rows.
+__global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreParams p) {
+  const int lane = threadIdx.x & 31;
+  const long long warp = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int heads2 = 2 * p.c.Hkv;
+  const long long jobs = (p.rows + p.rows_per_job - 1) / p.rows_per_job * heads2;
+  const int T = p.c.T, hd = p.c.hd, upr = hd / 8;  // 8-value units of a row
+  for (long long job = warp; job < jobs; job += static_cast<long long>(gridDim.x) * 8) {
+    const int hh = static_cast<int>(job % heads2);
+    const bool is_v = hh >= p.c.Hkv;
+    const int h = is_v ? hh - p.c.Hkv : hh;
+    const __nv_bfloat16* src = is_v ? p.v : p.k;
+    uint8_t* dst = is_v ? p.c.v : p.c.k;
+    float* scales = is_v ? p.c.v_scale : p.c.k_scale;
+    const long long job0 = job / heads2 * p.rows_per_job;
+    const long long job1 = min(job0 + p.rows_per_job, p.rows);
+    // Each lane looks at one entry (a job has at most 32): its sequence, where
+    // that one's entries end, and whether it is its block's first.
+    const long long mine = job0 + lane;
+    int my_b = 0, my_pos = -1;
+    long long my_end = 0;
+    bool leads = false;
+    if (mine < job1) {
+      long long s0;
+      if (p.cu_active) {
+        int lo = 0, hi = p.c.batch - 1;
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (__ldg(p.cu_active + mid) <= mine) lo = mid;
+          else hi = mid - 1;
+        }
+        my_b = lo;
+        s0 = __ldg(p.cu_active + lo);
+        my_end = min(static_cast<long long>(__ldg(p.cu_active + lo + 1)), p.rows);
+      } else {
+        my_b = static_cast<int>(mine / p.na);
+        s0 = static_cast<long long>(my_b) * p.na;
+        my_end = s0 + p.na;
+      }
+      my_pos = __ldg(p.pos + mine);
+      const int before = mine > s0 ? __ldg(p.pos + mine - 1) : -1;
+      if (my_pos < 0 || my_pos >= p.c.n_total || my_pos <= before || mine >= my_end) {
+        if (p.err) atomicExch(p.err, kErrInvalidRow);
+      } else {
+        leads = before < 0 || before / T != my_pos / T;
+      }
+    }
+    for (uint32_t todo = __ballot_sync(0xffffffffu, leads); todo; todo &= todo - 1u) {
+      const int who = __ffs(todo) - 1;
+      const long long i = job0 + who;
+      const int b = __shfl_sync(0xffffffffu, my_b, who);
+      const int blk = __shfl_sync(0xffffffffu, my_pos, who) / T;
+      const long long s1 = __shfl_sync(0xffffffffu, my_end, who);
+      // The block's entries are i .. i + n - 1 (at most T, ascending), and
+      // its active positions the bits of act.
+      uint32_t act[4] = {0u, 0u, 0u, 0u};
+      int n = 0;
+      int last = -1;
+      bool more = true;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if (more && c * 32 < T) {
+          const long long j = i + c * 32 + lane;
+          const int q = j < s1 ? __ldg(p.pos + j) : -1;
+          int prev = __shfl_up_sync(0xffffffffu, q, 1);
+          if (lane == 0) prev = last;
+          last = __shfl_sync(0xffffffffu, q, 31);
+          const bool in = q >= 0 && q < p.c.n_total && q / T == blk && q > prev;
+          const uint32_t ball = __ballot_sync(0xffffffffu, in);
+          const int got = ball == 0xffffffffu ? 32 : __ffs(~ball) - 1;  // the run from the first
+          n += got;
+          more = got == 32;
+          const int bit = q - blk * T;
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            act[w] |= __reduce_or_sync(
+                0xffffffffu, lane < got && (bit >> 5) == w ? 1u << (bit & 31) : 0u);
+        }
+      }
+      const int in_block = min(T, p.c.n_total - blk * T);
+      const int held = p.kv_len ? min(max(__ldg(p.kv_len + b) - blk * T, 0), in_block) : in_block;
+      bool stays = false;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int bits = min(max(held - 32 * w, 0), 32);
+        const uint32_t want = bits == 32 ? 0xffffffffu : (1u << bits) - 1u;
+        stays |= (want & ~act[w]) != 0u;
+      }
+      // Largest magnitude of the new rows. An infinity counts as the largest
+      // finite value, a NaN not at all.
+      const int units = n * upr;
+      float amax = 0.f;
+      for (int u = lane; u < units; u += 32) {
+        const int r = u / upr, e = (u - r * upr) * 8;
+        const uint4 raw =
+            __ldg(reinterpret_cast<const uint4*>(src + ((i + r) * p.c.Hkv + h) * hd + e));
+        const uint32_t w4[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          amax = fmaxf(amax, fabsf(__uint_as_float(w4[k] << 16)));
+          amax = fmaxf(amax, fabsf(__uint_as_float(w4[k] & 0xffff0000u)));
+        }
+      }
+      amax = fminf(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax))),
+                   __uint_as_float(0x7f7f0000u));
+      const float need = exp2_int(kv8_exp(amax));
+      float* sp = scales + (static_cast<long long>(b) * p.c.n_blocks + blk) * p.c.Hkv + h;
+      const float was = *sp;
+      const bool keep = stays && was > 0.f;
+      const float now = keep ? fmaxf(was, need) : need;
+      __syncwarp();
+      if (lane == 0) *sp = now;
+      const float inv = __fdiv_rn(1.f, now);
+      uint8_t* base = dst + (static_cast<long long>(b) * p.c.n_total) * p.c.row_stride +
+                      static_cast<long long>(h) * hd;
+      for (int u = lane; u < units; u += 32) {
+        const int r = u / upr, e = (u - r * upr) * 8;
+        const uint4 raw =
+            __ldg(reinterpret_cast<const uint4*>(src + ((i + r) * p.c.Hkv + h) * hd + e));
+        const uint32_t w4[4] = {raw.x, raw.y, raw.z, raw.w};
+        uint32_t o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          o[k] = cvt_e4m3x2(__uint_as_float(w4[k] << 16) * inv,
+                            __uint_as_float(w4[k] & 0xffff0000u) * inv);
+        const int q = __ldg(p.pos + i + r);
+        *reinterpret_cast<uint2*>(base + q * p.c.row_stride + e) =
+            make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
+      }
+      if (keep && now > was) {
+        const float ratio = __fdiv_rn(was, now);
+        for (int u = lane; u < in_block * upr; u += 32) {
+          const int r = u / upr, e = (u - r * upr) * 8;
+          if ((act[r >> 5] >> (r & 31)) & 1u) continue;
+          uint2* at = reinterpret_cast<uint2*>(base + (static_cast<long long>(blk) * T + r) *
+                                                          p.c.row_stride + e);
+          const uint2 old = *at;
+          float x[4], y[4];
+          e4m3x4_to_f32(old.x, x);
+          e4m3x4_to_f32(old.y, y);
+          *at = make_uint2(cvt_e4m3x2(x[0] * ratio, x[1] * ratio) |
+                               (cvt_e4m3x2(x[2] * ratio, x[3] * ratio) << 16),
+                           cvt_e4m3x2(y[0] * ratio, y[1] * ratio) |
+                               (cvt_e4m3x2(y[2] * ratio, y[3] * ratio) << 16));
+        }
+      }
+    }
+  }
+}
+
+struct Kv8LoadParams {
+  Kv8View c;
+  void* k_out;     // [rows, Hkv, hd] bf16 or fp32, or null
+  void* v_out;
+  int out_f32;
+  const int* pos;  // [batch, n_pos] or null (positions 0 .. n_pos - 1)
+  int n_pos;
+  long long rows;  // batch * n_pos
+  int* err;
+};
+
+// Rows of the cache as bf16 or fp32. One thread turns 16 values: one 16-byte
+// load, two (four) 16-byte stores. Bound by HBM: 1 byte read and 2 (4)
+// written for each value.
+__global__ void __launch_bounds__(256) kv8_load_kernel(const Kv8LoadParams p) {
+  const int upr = p.c.Hkv * p.c.hd / 16;  // 16-value units of a row
+  const long long units = p.rows * upr;
+  const uint8_t* src = blockIdx.y ? p.c.v : p.c.k;
+  const float* scales = blockIdx.y ? p.c.v_scale : p.c.k_scale;
+  void* dst = blockIdx.y ? p.v_out : p.k_out;
+  if (!dst) return;
+  for (long long u = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; u < units;
+       u += static_cast<long long>(gridDim.x) * blockDim.x) {
+    const long long row = u / upr;
+    const int e = static_cast<int>(u - row * upr) * 16;
+    const int b = static_cast<int>(row / p.n_pos);
+    const int pos = p.pos ? __ldg(p.pos + row) : static_cast<int>(row - static_cast<long long>(b) * p.n_pos);
+    if (pos < 0 || pos >= p.c.n_total) {
+      if (p.err) atomicExch(p.err, kErrInvalidRow);
+      continue;
+    }
+    const float s = __ldg(scales + (static_cast<long long>(b) * p.c.n_blocks + pos / p.c.T) * p.c.Hkv +
+                          e / p.c.hd);
+    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(
+        src + (static_cast<long long>(b) * p.c.n_total + pos) * p.c.row_stride + e));
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    float x[16];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float y[4];
+      e4m3x4_to_f32(w[k], y);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[4 * k + j] = y[j] * s;
+    }
+    const long long o = row * p.c.Hkv * p.c.hd + e;
+    if (p.out_f32) {
+      float4* d = reinterpret_cast<float4*>(static_cast<float*>(dst) + o);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        d[k] = make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+    } else {
+      uint4* d = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(dst) + o);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        d[k] = make_uint4(pack_bf16(x[8 * k], x[8 * k + 1]), pack_bf16(x[8 * k + 2], x[8 * k + 3]),
+                          pack_bf16(x[8 * k + 4], x[8 * k + 5]),
+                          pack_bf16(x[8 * k + 6], x[8 * k + 7]));
+    }
+  }
+}
+
+}  // namespace ca

@@ -1,0 +1,223 @@
+// kv8_api.cuh -- argument checks and launches of the 8-bit cache's entry
+// points (include/canvas_attn.h: ca_kv8_*, ca_attention_kv8_*). Part of the
+// library's single translation unit, after canvas_attn.cu's helpers.
+#pragma once
+
+#include "attn_kv8_rows.cuh"
+#include "kv8.cuh"
+
+namespace ca {
+namespace {
+
+constexpr int kSms = 148;
+
+// The cache as the kernels see it, or why not.
+int kv8_view(const ca_kv8_cache& c, Kv8View* v) {
+  if (!c.k || !c.v || !c.k_scale || !c.v_scale) return CA_ERR_INVALID;
+  if (c.batch < 0 || c.n_total <= 0 || c.n_head_kv <= 0 || c.head_dim <= 0) return CA_ERR_INVALID;
+  if (c.head_dim % 16 || c.head_dim > 512) return CA_ERR_UNSUPPORTED;
+  if (c.block_tokens != 16 && c.block_tokens != 32 && c.block_tokens != 64 &&
+      c.block_tokens != 128)
+    return CA_ERR_UNSUPPORTED;
+  const int64_t dense = static_cast<int64_t>(c.n_head_kv) * c.head_dim;
+  const int64_t rs = c.row_stride ? c.row_stride : dense;
+  if (rs < dense || rs % 16 || !aligned16(c.k) || !aligned16(c.v)) return CA_ERR_INVALID;
+  if (dense > INT_MAX) return CA_ERR_UNSUPPORTED;
+  v->k = static_cast<uint8_t*>(c.k);
+  v->v = static_cast<uint8_t*>(c.v);
+  v->k_scale = c.k_scale;
+  v->v_scale = c.v_scale;
+  v->batch = c.batch;
+  v->n_total = c.n_total;
+  v->Hkv = c.n_head_kv;
+  v->hd = c.head_dim;
+  v->T = c.block_tokens;
+  v->n_blocks = (c.n_total + c.block_tokens - 1) / c.block_tokens;
+  v->row_stride = rs;
+  return CA_OK;
+}
+
+int kv8_store_impl(const ca_kv8_store_args* a, cudaStream_t st) {
+  if (!a || !a->k || !a->v || !a->active_pos) return CA_ERR_INVALID;
+  Kv8StoreParams p{};
+  const int rc = kv8_view(a->cache, &p.c);
+  if (rc != CA_OK) return rc;
+  if (!aligned16(a->k) || !aligned16(a->v)) return CA_ERR_INVALID;
+  if (a->cu_active ? a->total_active < 0 : a->n_active < 0) return CA_ERR_INVALID;
+  p.rows = a->cu_active ? a->total_active : static_cast<int64_t>(p.c.batch) * a->n_active;
+  if (p.c.batch == 0 || p.rows == 0) return CA_OK;
+  if (p.rows > INT_MAX) return CA_ERR_UNSUPPORTED;
+  p.k = static_cast<const __nv_bfloat16*>(a->k);
+  p.v = static_cast<const __nv_bfloat16*>(a->v);
+  p.pos = a->active_pos;
+  p.cu_active = a->cu_active;
+  p.kv_len = a->kv_len;
+  p.na = a->n_active;
+  p.err = a->status;
+  // Entries of the active list a warp looks through: one where that leaves
+  // every warp slot of the GPU at most one job, 32 (a lane each) at most.
+  const int64_t slots = static_cast<int64_t>(kSms) * 64;
+  const int64_t one = p.rows * 2 * p.c.Hkv;
+  p.rows_per_job = static_cast<int>(std::min<int64_t>(32, (one + slots - 1) / slots));
+  const int64_t jobs = (p.rows + p.rows_per_job - 1) / p.rows_per_job * 2 * p.c.Hkv;
+  const int blocks = static_cast<int>(std::min<int64_t>((jobs + 7) / 8, kSms * 64));
+  kv8_store_kernel<<<blocks, 256, 0, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
+}
+
+int kv8_load_impl(const ca_kv8_load_args* a, cudaStream_t st) {
+  if (!a) return CA_ERR_INVALID;
+  Kv8LoadParams p{};
+  const int rc = kv8_view(a->cache, &p.c);
+  if (rc != CA_OK) return rc;
+  if ((!a->k_out && !a->v_out) || a->n_pos < 0 || (!a->pos && a->n_pos > p.c.n_total))
+    return CA_ERR_INVALID;
+  if ((a->k_out && !aligned16(a->k_out)) || (a->v_out && !aligned16(a->v_out)))
+    return CA_ERR_INVALID;
+  p.rows = static_cast<int64_t>(p.c.batch) * a->n_pos;
+  if (p.rows == 0) return CA_OK;
+  p.k_out = a->k_out;
+  p.v_out = a->v_out;
+  p.out_f32 = a->out_f32 ? 1 : 0;
+  p.pos = a->pos;
+  p.n_pos = a->n_pos;
+  p.err = a->status;
+  const int64_t units = p.rows * (static_cast<int64_t>(p.c.Hkv) * p.c.hd / 16);
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((units + 255) / 256, kSms * 32)), 2);
+  kv8_load_kernel<<<grid, 256, 0, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
+}
+
+// How a call is laid out: which kernel, row tiles and splits of the keys.
+struct Kv8Plan {
+  int tiles, splits;
+  int64_t ws_bytes;
+};
+
+// A key axis is split where the row tiles alone would leave SMs idle, into
+// at least 256 keys (two chunks a warp) each.
+int kv8_plan(const ca_attn_kv8_args* a, const Kv8View& c, bool split_ok, Kv8Plan* pl) {
+  const int64_t max_sq = a->cu_q ? a->max_sq : a->sq;
+  const int64_t G = a->n_head / c.Hkv;
+  const int64_t tiles = (max_sq * G + 15) / 16;
+  if (tiles > INT_MAX / 1024) return CA_ERR_UNSUPPORTED;
+  const int64_t cells = tiles * c.Hkv * c.batch;
+  int64_t splits = 1;
+  if (split_ok && cells > 0 && cells < kSms) {
+    splits = kSms / cells;
+    splits = std::max<int64_t>(1, std::min<int64_t>(splits, c.n_total / 256));
+  }
+  pl->tiles = static_cast<int>(tiles);
+  pl->splits = static_cast<int>(splits);
+  pl->ws_bytes =
+      splits == 1 ? 0 : CA_KV8_TICKET_BYTES + cells * splits * (16ll * c.hd + 32) * 4;
+  return CA_OK;
+}
+
+int attn_kv8_check(const ca_attn_kv8_args* a, Kv8View* c) {
+  if (!a) return CA_ERR_INVALID;
+  const int rc = kv8_view(a->cache, c);
+  if (rc != CA_OK) return rc;
+  if (a->n_head <= 0 || a->n_head % c->Hkv) return CA_ERR_INVALID;
+  if (a->cu_q ? (a->max_sq < 0 || a->total_q < 0) : a->sq < 0) return CA_ERR_INVALID;
+  if (c->batch > 65535 || c->Hkv > 65535) return CA_ERR_UNSUPPORTED;
+  const int64_t total_q = a->cu_q ? a->total_q : static_cast<int64_t>(c->batch) * a->sq;
+  if (total_q > INT_MAX) return CA_ERR_UNSUPPORTED;
+  return CA_OK;
+}
+
+template <int HDP>
+int launch_rows(const Kv8AttnParams& p, cudaStream_t st) {
+  static bool attr_done[kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return CA_ERR_CUDA;
+  if (!attr_done[dev]) {
+    if (cudaFuncSetAttribute(attn_kv8_rows_kernel<HDP>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             RowsCfg<HDP>::kSmem) != cudaSuccess)
+      return CA_ERR_CUDA;
+    attr_done[dev] = true;
+  }
+  const dim3 grid(p.tiles * p.splits, p.c.Hkv, p.c.batch);
+  attn_kv8_rows_kernel<HDP><<<grid, 256, RowsCfg<HDP>::kSmem, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
+}
+
+int attn_kv8_impl(const ca_attn_kv8_args* a, cudaStream_t st) {
+  Kv8AttnParams p{};
+  int rc = attn_kv8_check(a, &p.c);
+  if (rc != CA_OK) return rc;
+  if (!a->q || !a->out) return CA_ERR_INVALID;
+  const int H = a->n_head, hd = p.c.hd;
+  const int64_t dense = static_cast<int64_t>(H) * hd;
+  p.q_row_stride = a->q_row_stride ? a->q_row_stride : dense;
+  p.out_row_stride = a->out_row_stride ? a->out_row_stride : dense;
+  if (p.q_row_stride < dense || p.out_row_stride < dense || p.q_row_stride % 8 ||
+      p.out_row_stride % (a->out_f32 ? 4 : 8) || !aligned16(a->q) || !aligned16(a->out))
+    return CA_ERR_INVALID;
+  const int64_t max_sq = a->cu_q ? a->max_sq : a->sq;
+  const int64_t total_q = a->cu_q ? a->total_q : static_cast<int64_t>(p.c.batch) * a->sq;
+  if (p.c.batch == 0 || total_q == 0 || max_sq == 0) return CA_OK;
+  Kv8Plan pl;
+  if ((rc = kv8_plan(a, p.c, a->workspace != nullptr, &pl)) != CA_OK) return rc;
+  if (a->workspace && (!aligned16(a->workspace) || a->workspace_bytes < pl.ws_bytes))
+    return CA_ERR_INVALID;
+  p.q = static_cast<const __nv_bfloat16*>(a->q);
+  p.out = a->out;
+  p.out_f32 = a->out_f32 ? 1 : 0;
+  p.sq = a->sq;
+  p.cu_q = a->cu_q;
+  p.q_pos = a->q_pos;
+  p.kv_len = a->kv_len;
+  p.seq_prefix = a->seq_prefix;
+  p.causal_prefix = clamp_opt(a->causal_prefix);
+  p.window = a->sliding_window < 0 ? kNoWindow
+                                   : static_cast<int>(std::min<int64_t>(a->sliding_window,
+                                                                        INT_MAX - 1));
+  p.H = H;
+  p.G = H / p.c.Hkv;
+  p.scale = a->scale;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.softcap = a->softcap > 0.f ? a->softcap : 0.f;
+  p.splits = pl.splits;
+  p.tiles = pl.tiles;
+  p.err = a->status;
+  if (pl.splits > 1) {
+    const int64_t cells = static_cast<int64_t>(pl.tiles) * p.c.Hkv * p.c.batch;
+    p.tickets = static_cast<int*>(a->workspace);
+    p.part_ml = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + CA_KV8_TICKET_BYTES);
+    p.part_o = p.part_ml + cells * pl.splits * 32;
+  }
+  if (hd <= 64) return launch_rows<64>(p, st);
+  if (hd <= 128) return launch_rows<128>(p, st);
+  if (hd <= 256) return launch_rows<256>(p, st);
+  return launch_rows<512>(p, st);
+}
+
+}  // namespace
+}  // namespace ca
+
+extern "C" {
+
+int ca_kv8_store(const ca_kv8_store_args* a, void* stream) {
+  return ca::kv8_store_impl(a, static_cast<cudaStream_t>(stream));
+}
+
+int ca_kv8_load(const ca_kv8_load_args* a, void* stream) {
+  return ca::kv8_load_impl(a, static_cast<cudaStream_t>(stream));
+}
+
+int ca_attention_kv8_dev(const ca_attn_kv8_args* a, void* stream) {
+  return ca::attn_kv8_impl(a, static_cast<cudaStream_t>(stream));
+}
+
+int64_t ca_attention_kv8_workspace(const ca_attn_kv8_args* a) {
+  ca::Kv8View c;
+  const int rc = ca::attn_kv8_check(a, &c);
+  if (rc != CA_OK) return rc;
+  ca::Kv8Plan pl;
+  const int rp = ca::kv8_plan(a, c, true, &pl);
+  return rp != CA_OK ? rp : pl.ws_bytes;
+}
+
+}  // extern "C"

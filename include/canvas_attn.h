@@ -372,6 +372,123 @@ int ca_linear(const ca_linear_args* a, void* stream);
 int ca_build_rope_table(float* out, int64_t max_seq_len, int64_t rope_dim, float theta,
                         const float* freq_factors);
 
+/*
+ * The 8-bit inter-step cache (StepCache, src/model/cache.rs:25-81, in half
+ * the bytes of the bf16 cache above). K and V are e4m3 values with one fp32
+ * scale for each block of block_tokens consecutive positions and kv head; a
+ * cached value is e4m3 * scale. Blocks start at position 0 of each sequence.
+ * Every sequence has room for n_total positions; how many it holds is kv_len
+ * (device int32 [batch]) of the calls below, or all n_total where that is
+ * NULL.
+ */
+typedef struct {
+    void* k;               /* uint8 (e4m3) [batch, n_total, n_head_kv, head_dim], 16-byte aligned */
+    void* v;               /* the same */
+    float* k_scale;        /* fp32 [batch, ceil(n_total / block_tokens), n_head_kv] */
+    float* v_scale;        /* the same */
+    int32_t batch;
+    int32_t n_total;
+    int32_t n_head_kv;
+    int32_t head_dim;      /* a multiple of 16, at most 512 */
+    int32_t block_tokens;  /* 16, 32, 64 or 128 */
+    int64_t row_stride;    /* bytes between positions of k and v, a multiple of 16;
+                              0 = n_head_kv * head_dim. A sequence is n_total rows */
+} ca_kv8_cache;
+
+typedef struct {
+    ca_kv8_cache cache;
+    const void* k;             /* bf16 [rows, n_head_kv, head_dim], 16-byte aligned */
+    const void* v;             /* the same */
+    int32_t n_active;          /* rows of each sequence (cu_active NULL) */
+    const int32_t* active_pos; /* int32 [rows]: positions, ascending within a sequence */
+    const int32_t* cu_active;  /* int32 [batch + 1] row offsets, or NULL */
+    int64_t total_active;      /* with cu_active: cu_active[batch] */
+    const int32_t* kv_len;     /* int32 [batch]: positions held before this call, or NULL */
+    int32_t* status;           /* device int32 or NULL: set to CA_ERR_INVALID by a position
+                                  out of range or out of order (its row, and later rows
+                                  of the same block, may be skipped) */
+} ca_kv8_store_args;
+
+/*
+ * ca_kv8_store -- StepCache::store (src/model/cache.rs:62-70) into the 8-bit
+ * cache: post-RoPE K and V rows are quantised as they are written. For each
+ * block and kv head that a row falls in, need = 2^k with the smallest k in
+ * [-64, 120] such that no new value of the block exceeds 448 * 2^k. If none
+ * of the block's held positions (those below kv_len) keeps its row, or its
+ * scale is 0 (nothing written yet), the scale becomes need; else the larger
+ * of the old scale and need, and where it grows the rows that stay are
+ * rounded again to the new scale. New values are rounded to nearest even;
+ * infinities saturate, NaN stays NaN and takes no part in the scale.
+ * Deterministic. Asynchronous on `stream`; allocates nothing.
+ */
+int ca_kv8_store(const ca_kv8_store_args* a, void* stream);
+
+typedef struct {
+    ca_kv8_cache cache;
+    const int32_t* pos;  /* int32 [batch, n_pos]: positions to read, any order; NULL: 0 .. n_pos - 1 */
+    int32_t n_pos;
+    void* k_out;         /* [batch, n_pos, n_head_kv, head_dim] bf16, or fp32 when out_f32;
+                            16-byte aligned; NULL: K is not read */
+    void* v_out;
+    int32_t out_f32;
+    int32_t* status;     /* device int32 or NULL: set to CA_ERR_INVALID by a position out of
+                            range (its output row is left as it was) */
+} ca_kv8_load_args;
+
+/*
+ * ca_kv8_load -- StepCache::gather (src/model/cache.rs:73-81) from the 8-bit
+ * cache: rows as bf16 (exact for scales that ca_kv8_store wrote) or fp32.
+ * Asynchronous on `stream`; allocates nothing.
+ */
+int ca_kv8_load(const ca_kv8_load_args* a, void* stream);
+
+typedef struct {
+    ca_kv8_cache cache;
+    const void* q;            /* bf16 [total_q, n_head, head_dim], 16-byte aligned */
+    void* out;                /* [total_q, n_head, head_dim] bf16, or fp32 when out_f32 */
+    int32_t out_f32;
+    int64_t q_row_stride;     /* elements between tokens; 0 = n_head * head_dim */
+    int64_t out_row_stride;   /* 0 = n_head * head_dim */
+    int32_t n_head;
+    int32_t sq;               /* query rows of each sequence (cu_q NULL) */
+    const int32_t* cu_q;      /* int32 [batch + 1] row offsets, or NULL */
+    int32_t max_sq;           /* with cu_q: largest per-sequence query count */
+    int64_t total_q;          /* with cu_q: cu_q[batch] */
+    const int32_t* q_pos;     /* int32 [total_q] positions; NULL: the last held ones,
+                                 kv_len - sq + row */
+    const int32_t* kv_len;    /* int32 [batch]: positions held (clamped to 0 .. n_total);
+                                 NULL: n_total. All of them must have been stored */
+    int64_t sliding_window;   /* as ca_dev_args; -1 = None */
+    int64_t causal_prefix;    /* -1 = None; a prefix past every position is plain causal */
+    const int32_t* seq_prefix; /* int32 [batch], overrides causal_prefix; or NULL */
+    float scale;
+    float softcap;            /* 0 = off */
+    int32_t* status;          /* as ca_dev_args */
+    void* workspace;          /* device, 16-byte aligned, or NULL (long key axes are then not
+                                 split over CTAs: slower, otherwise the same). Its first
+                                 CA_KV8_TICKET_BYTES bytes must be zero before the first call
+                                 that uses it; every call leaves them zero. Calls that may run
+                                 at the same time need one each */
+    int64_t workspace_bytes;  /* at least what ca_attention_kv8_workspace returns */
+} ca_attn_kv8_args;
+#define CA_KV8_TICKET_BYTES 4096
+
+/*
+ * ca_attention_kv8_dev -- attention() (src/model/attention.rs:106-133) over
+ * the 8-bit cache: bf16 queries, K and V taken as they are held, keys at
+ * positions 0 .. kv_len - 1 of each sequence, masks as in ca_attention_dev
+ * (no sequence ids: every sequence has its own cache). Products and sums in
+ * fp32, softmax weights in f16 (11 bits). Scales may be any positive finite
+ * values. A query row with no visible key gets NaN. A NaN held in V may reach
+ * the rows of its sequence and kv head that do not see it. Asynchronous on
+ * `stream`; allocates nothing.
+ */
+int ca_attention_kv8_dev(const ca_attn_kv8_args* a, void* stream);
+
+/* Bytes of workspace a call with these arguments uses (pointers are not
+ * read), or a negative ca_status. */
+int64_t ca_attention_kv8_workspace(const ca_attn_kv8_args* a);
+
 /* Reads and clears the device-wide error word of the current device after
  * synchronising `stream`: CA_OK, or CA_ERR_TIMEOUT if the bounded wait of a
  * kernel launched without a status word of its own (status == NULL) expired
