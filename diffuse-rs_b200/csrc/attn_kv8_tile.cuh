@@ -1,0 +1,703 @@
+// attn_kv8_tile.cuh -- attention of many query rows over the 8-bit cache on
+// the fifth-generation tensor cores.
+//
+// One CTA takes 128 query rows (token, head-of-the-group pairs, token-major)
+// of one (sequence, kv head) and one stretch of its key tiles. Mathematics
+// and the treatment of the scales are those of attn_kv8_rows.cuh:
+//   t = a (q . k8) + L,   p = 2^(t - m),   out = sum p v8 / sum p 2^-L.
+//
+// S = Q K^T runs on K as it is held (kind::f8f6f4, e4m3 x e4m3, fp32
+// accumulators): each row of Q is scaled by a power of two into e4m3's range
+// and split into two e4m3 terms, q = hi + lo, whose products land in the same
+// accumulator. Two terms of 4 significant bits hold bf16's 8 exactly, down to
+// 2^-18 of the row's largest value. The two e4m3 products cost the tensor
+// core what one bf16 product would, and K needs no conversion. P V cannot do
+// the same: a weight's range (2^-31 .. 1 counts in a long row) does not fit
+// two e4m3 terms, so P is f16 (11 bits, in TMEM over S) and V is turned into
+// f16 in shared memory by four warps of its own, which keep out of the
+// softmax warps' issue slots.
+//
+// Warp roles (512 threads at head_dim <= 128, one CTA per SM):
+//   warp 0       K tiles, TMA into a ring (lane 0)
+//   warp 1       TMEM, tcgen05.mma issue (lane 0)
+//   warp 2       V tiles, TMA into a ring (lane 0)
+//   warps 4-11   softmax in two groups of four that take alternate key tiles,
+//                each with its own S and O in TMEM, merged at the end; they
+//                split Q first and write the output last
+//   warps 12-15  V tile -> f16
+// head_dim 256: one softmax group (384 threads), 64-key tiles, three S
+// buffers and one O.
+#pragma once
+
+#include "attn_kv8_rows.cuh"
+
+namespace ca {
+
+template <int HDP_>
+struct TileCfg {
+  static constexpr int HDP = HDP_;                       // 64, 128 or 256
+  static constexpr bool ALT = HDP <= 128;
+  static constexpr int BN = ALT ? 128 : 64;              // keys of a tile
+  static constexpr int kGroups = ALT ? 2 : 1;
+  static constexpr int kSoftThreads = 128 * kGroups;
+  static constexpr int kThreads = 256 + kSoftThreads;
+  static constexpr int kConvWarp0 = 4 + 4 * kGroups;
+  static constexpr int STK = 3, STV = 2;                 // stages: K, V as held; V as f16 has 2
+  static constexpr int SB = ALT ? 2 : 3;                 // S buffers
+  static constexpr int kChunks = (HDP + 127) / 128;      // 128-byte columns of an e4m3 tile
+  static constexpr int kSteps = HDP / 32;                // k-steps of S
+  static constexpr int kQTerm = kChunks * 128 * 128;     // one term of Q
+  static constexpr int kTile8 = kChunks * BN * 128;      // K or V as held
+  static constexpr int kVAtoms = HDP / 64;               // 64-column atoms of V in f16
+  static constexpr int kTile16 = kVAtoms * BN * 128;
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffK = kOffQ + 2 * kQTerm;
+  static constexpr int kOffV8 = kOffK + STK * kTile8;
+  static constexpr int kOffV = kOffV8 + STV * kTile8;
+  static constexpr int kOffBar = kOffV + 2 * kTile16;
+  static constexpr int kBarQ = 0;               // Q's terms are in place
+  static constexpr int kBarK = 1;               // [STK] K landed
+  static constexpr int kBarKE = kBarK + STK;    // [STK] K free
+  static constexpr int kBarV8 = kBarKE + STK;   // [STV] V landed
+  static constexpr int kBarV8E = kBarV8 + STV;  // [STV] V free
+  static constexpr int kBarV = kBarV8E + STV;   // [2] V in f16
+  static constexpr int kBarVE = kBarV + 2;      // [2] free
+  static constexpr int kBarS = kBarVE + 2;      // [SB]
+  static constexpr int kBarP = kBarS + SB;      // [2] P written (per group)
+  static constexpr int kBarO = kBarP + 2;       // [2] P V done (per O)
+  static constexpr int kBarF = kBarO + 2;       // every MMA done
+  static constexpr int kNumBars = kBarF + 1;
+  static constexpr int kOffQs = kOffBar + (kNumBars * 8 + 15) / 16 * 16;  // float [128]
+  static constexpr int kOffXch = kOffQs + 128 * 4;                        // float [2][2][128]
+  static constexpr int kOffMisc = kOffXch + 2 * 2 * 128 * 4;
+  static constexpr int kSmem = kOffMisc + 64;
+  static constexpr int kOCol = SB * BN;
+  static constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(BN >> 3) << 17) |
+                                      (128u >> 4 << 24);  // e4m3 x e4m3, fp32
+  static constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) |
+                                      (static_cast<uint32_t>(HDP >> 3) << 17) |
+                                      (128u >> 4 << 24);  // f16 x f16 (MN-major), fp32
+  static_assert(kOCol + kGroups * HDP <= 512, "TMEM");
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+// D[tmem] (+)= A[smem] x B[smem]^T, kind::f8f6f4 (e4m3 in, fp32 accumulate).
+__device__ __forceinline__ void umma_ss_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                           uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void reg_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// The launch's 512 threads hold 128 registers each: 2 x 128 x 192 for the
+// softmax and 2 x 128 x 64 for the rest are exactly those 65,536.
+constexpr int kTileSoftRegs = 192, kTileOtherRegs = 64;
+
+template <class C>
+__global__ void __launch_bounds__(C::kThreads, 1)
+    attn_kv8_tile_kernel(const __grid_constant__ CUtensorMap tm_k,
+                         const __grid_constant__ CUtensorMap tm_v, const Kv8AttnParams p) {
+  constexpr int BN = C::BN, HDP = C::HDP;
+  constexpr bool ALT = C::ALT;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((smem_u32(smem) & 1023u) != 0) {
+    if (threadIdx.x == 0) atomicExch(p.err ? p.err : &g_device_error, kErrLayout);
+    return;
+  }
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int split = blockIdx.x % p.splits, tile = blockIdx.x / p.splits;
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int hd = p.c.hd;
+
+  const int q_beg = p.cu_q ? p.cu_q[b] : b * p.sq;
+  const int q_len = p.cu_q ? p.cu_q[b + 1] - q_beg : p.sq;
+  const long long n_rows = static_cast<long long>(q_len) * p.G;
+  const long long row0 = static_cast<long long>(tile) * 128;
+  if (row0 >= n_rows) return;
+  const int rows = static_cast<int>(min(128ll, n_rows - row0));
+  const int len = p.kv_len ? min(max(p.kv_len[b], 0), p.c.n_total) : p.c.n_total;
+  const int prefix = p.seq_prefix ? p.seq_prefix[b] : p.causal_prefix;
+
+  const uint32_t sQ = smem_u32(smem + C::kOffQ);
+  const uint32_t sK = smem_u32(smem + C::kOffK);
+  const uint32_t sV8 = smem_u32(smem + C::kOffV8);
+  const uint32_t sV = smem_u32(smem + C::kOffV);
+  const uint32_t bar0 = smem_u32(smem + C::kOffBar);
+  auto bar = [&](int i) -> uint32_t { return bar0 + 8u * i; };
+  float* sQs = reinterpret_cast<float*>(smem + C::kOffQs);
+  int* misc = reinterpret_cast<int*>(smem + C::kOffMisc);  // [0] TMEM, [1..4] key ranges, [5] join
+
+  auto interval = [&](int r, int& lo, int& hi) {
+    const int tok = static_cast<int>((row0 + r) / p.G);
+    const int pos = p.q_pos ? __ldg(p.q_pos + q_beg + tok) : len - q_len + tok;
+    kv8_interval(pos, len, p.window, prefix, lo, hi);
+  };
+
+  if (tid == 0) {
+    mbar_init(bar(C::kBarQ), 1);
+    for (int s = 0; s < C::STK; ++s) {
+      mbar_init(bar(C::kBarK + s), 1);
+      mbar_init(bar(C::kBarKE + s), 1);
+    }
+    for (int s = 0; s < C::STV; ++s) {
+      mbar_init(bar(C::kBarV8 + s), 1);
+      mbar_init(bar(C::kBarV8E + s), 4);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bar(C::kBarV + s), 4);
+      mbar_init(bar(C::kBarVE + s), 1);
+      mbar_init(bar(C::kBarP + s), 4);
+      mbar_init(bar(C::kBarO + s), 1);
+    }
+    for (int s = 0; s < C::SB; ++s) mbar_init(bar(C::kBarS + s), 1);
+    mbar_init(bar(C::kBarF), 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(misc), 512);
+    tmem_relinquish();
+  }
+  if (warp == 3) {
+    // The hull of what the rows see, and what every row sees.
+    int k_lo = INT_MAX, k_hi = 0, f_lo = 0, f_hi = INT_MAX;
+    for (int r = lane; r < rows; r += 32) {
+      int lo, hi;
+      interval(r, lo, hi);
+      if (lo < hi) {
+        k_lo = min(k_lo, lo);
+        k_hi = max(k_hi, hi);
+      }
+      f_lo = max(f_lo, lo);
+      f_hi = min(f_hi, hi);
+    }
+    k_lo = __reduce_min_sync(0xffffffffu, k_lo);
+    k_hi = __reduce_max_sync(0xffffffffu, k_hi);
+    f_lo = __reduce_max_sync(0xffffffffu, f_lo);
+    f_hi = __reduce_min_sync(0xffffffffu, f_hi);
+    if (lane == 0) {
+      misc[1] = k_lo;
+      misc[2] = k_hi;
+      misc[3] = f_lo;
+      misc[4] = f_hi;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = static_cast<uint32_t>(misc[0]);
+  const int k_lo = misc[1], k_hi = misc[2], f_lo = misc[3], f_hi = misc[4];
+  // This CTA's key tiles kt0 .. kt0 + n - 1.
+  int kt0 = 0, n = 0;
+  if (k_lo < k_hi) {
+    const int first = k_lo / BN, all = (k_hi + BN - 1) / BN - first;
+    const int per = (all + p.splits - 1) / p.splits;
+    kt0 = first + min(all, split * per);
+    n = first + min(all, (split + 1) * per) - kt0;
+  }
+  const int tok0 = b * p.c.n_total;  // the sequence's first row of the tensor maps
+  bool dead = false;
+
+  if (warp < 4) {
+    if constexpr (ALT) reg_dec<kTileOtherRegs>();
+    if (warp == 0 || warp == 2) {
+      // ---------------------------------------------------------- producers
+      if (lane == 0) {
+        const bool is_k = warp == 0;
+        const int full = is_k ? C::kBarK : C::kBarV8;
+        const int empty = is_k ? C::kBarKE : C::kBarV8E;
+        const int NS = is_k ? C::STK : C::STV;
+        const uint32_t base = is_k ? sK : sV8;
+        const CUtensorMap* tm = is_k ? &tm_k : &tm_v;
+        for (int u = 0; u < n; ++u) {
+          const int s = u % NS;
+          if (u >= NS && !mbar_wait(bar(empty + s), ((u / NS) - 1) & 1, dead, p.err)) break;
+          mbar_arrive_expect_tx(bar(full + s), C::kTile8);
+#pragma unroll
+          for (int c = 0; c < C::kChunks; ++c)
+            tma_load_3d(base + s * C::kTile8 + c * BN * 128, tm, bar(full + s), c * 128, kvh,
+                        tok0 + (kt0 + u) * BN);
+        }
+        bool d2 = false;  // leave no copy in flight
+        for (int u = max(0, n - NS); u < n; ++u)
+          mbar_wait(bar(full + u % NS), (u / NS) & 1, d2, p.err);
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------- MMA issue
+      if (lane == 0) {
+        auto og = [&](int i) -> int { return ALT ? (i & 1) : 0; };
+        auto ouse = [&](int i) -> int { return ALT ? (i >> 1) : i; };
+        auto issue_s = [&](int j) -> bool {
+          const int s = j % C::STK, sb = j % C::SB;
+          if (!mbar_wait(bar(C::kBarK + s), (j / C::STK) & 1, dead, p.err)) return false;
+          // The buffer last held P[j - SB]: P V[j - SB] has read it. (With one
+          // group S[j] is issued after P V[j - 2], whose issue waited for
+          // P V[j - 3].)
+          if (ALT && j >= C::SB &&
+              !mbar_wait(bar(C::kBarO + og(j - C::SB)), ouse(j - C::SB) & 1, dead, p.err))
+            return false;
+          tc_fence_after();
+          const uint32_t kbase = sK + s * C::kTile8;
+#pragma unroll
+          for (int term = 0; term < 2; ++term)
+#pragma unroll
+            for (int kk = 0; kk < C::kSteps; ++kk) {
+              const uint64_t a = umma_desc_sw128(
+                  sQ + term * C::kQTerm + (kk >> 2) * 128 * 128 + (kk & 3) * 32, 16, 1024);
+              const uint64_t bd =
+                  umma_desc_sw128(kbase + (kk >> 2) * BN * 128 + (kk & 3) * 32, 16, 1024);
+              umma_ss_f8(tmem + sb * BN, a, bd, C::kIdescS, term + kk > 0 ? 1u : 0u);
+            }
+          umma_commit(bar(C::kBarS + sb));
+          umma_commit(bar(C::kBarKE + s));
+          return true;
+        };
+        auto issue_pv = [&](int i) -> bool {
+          const int g = og(i), use = ouse(i), s = i & 1;
+          if (!mbar_wait(bar(C::kBarV + s), (i >> 1) & 1, dead, p.err)) return false;
+          if (!mbar_wait(bar(C::kBarP + g), use & 1, dead, p.err)) return false;
+          if (!ALT && i > 0 && !mbar_wait(bar(C::kBarO), (i - 1) & 1, dead, p.err)) return false;
+          tc_fence_after();
+          const uint32_t vbase = sV + s * C::kTile16;
+          const uint32_t pcol = tmem + (i % C::SB) * BN;
+          const uint32_t dst = tmem + C::kOCol + g * HDP;
+#pragma unroll
+          for (int kk = 0; kk < BN / 16; ++kk) {
+            const uint64_t bd = umma_desc_sw128(vbase + kk * 2048, BN * 128, 1024);
+            umma_ts(dst, pcol + kk * 16, bd, C::kIdescO, use > 0 || kk > 0 ? 1u : 0u);
+          }
+          umma_commit(bar(C::kBarO + g));
+          umma_commit(bar(C::kBarVE + s));
+          return true;
+        };
+        if (n > 0 && mbar_wait(bar(C::kBarQ), 0, dead, p.err)) {
+          bool ok = issue_s(0) && (n < 2 || issue_s(1));
+          for (int j = 0; ok && j < n; ++j) ok = issue_pv(j) && (j + 2 >= n || issue_s(j + 2));
+        }
+        umma_commit(bar(C::kBarF));
+        bool d2 = false;
+        mbar_wait(bar(C::kBarF), 0, d2, p.err);
+      }
+    }
+  } else if (warp >= C::kConvWarp0) {
+    // ------------------------------------------------------------ V to f16
+    if constexpr (ALT) reg_dec<kTileOtherRegs>();
+    const int cw = warp - C::kConvWarp0;
+    for (int j = 0; j < n; ++j) {
+      const int s8 = j % C::STV, s = j & 1;
+      mbar_wait(bar(C::kBarV8 + s8), (j / C::STV) & 1, dead, p.err);
+      if (j >= 2) mbar_wait(bar(C::kBarVE + s), ((j >> 1) - 1) & 1, dead, p.err);
+      dead = __any_sync(0xffffffffu, dead);
+      if (dead) break;
+      const uint32_t src = sV8 + s8 * C::kTile8, dst = sV + s * C::kTile16;
+      const int key0 = (kt0 + j) * BN;
+      // A row's 16-byte unit u (16 values) becomes two units of its atom.
+      // Eight lanes take a row's units; those of the upper half write their
+      // second unit first, so that each store of eight lanes covers all banks.
+      constexpr int UPR = HDP == 64 ? 4 : 8;  // units of a row within a 128-byte column
+      constexpr int RPW = 32 / UPR;           // rows a warp covers at once
+      const int u = lane % UPR;
+#pragma unroll
+      for (int c = 0; c < C::kChunks; ++c) {
+#pragma unroll 4
+        for (int r0 = cw * RPW; r0 < BN; r0 += 4 * RPW) {
+          const int r = r0 + lane / UPR;
+          uint32_t w[4], o[8];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                       : "r"(src + c * BN * 128 + r * 128 + ((u ^ (r & 7)) << 4)));
+          // Keys that no row sees are zeros: what lies there is not data.
+          if (key0 + r < k_lo || key0 + r >= k_hi) w[0] = w[1] = w[2] = w[3] = 0u;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) e4m3x4_to_f16(w[i], o[2 * i], o[2 * i + 1]);
+          const uint32_t row = dst + (c * 2 + (u >> 2)) * BN * 128 + r * 128;
+          const int d = 2 * (u & 3), first = UPR == 8 ? u >> 2 : 0;
+          if (first == 0) {
+            st_shared_v4(row + ((d ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
+            st_shared_v4(row + (((d + 1) ^ (r & 7)) << 4), o[4], o[5], o[6], o[7]);
+          } else {
+            st_shared_v4(row + (((d + 1) ^ (r & 7)) << 4), o[4], o[5], o[6], o[7]);
+            st_shared_v4(row + ((d ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(bar(C::kBarV + s));
+        mbar_arrive(bar(C::kBarV8E + s8));
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    if constexpr (ALT) reg_inc<kTileSoftRegs>();
+    const int grp = (warp - 4) >> 2;
+    const int wq = warp & 3;
+    const int r = wq * 32 + lane;
+    const int st = tid - 128;  // softmax thread
+    const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
+
+    // Q into its two terms. Threads share a row (two at head_dim <= 128, one
+    // at 256 with its single group), each with one half of its units.
+    {
+      constexpr int TPR = C::kGroups;
+      const int qr = st / TPR, part = st % TPR;
+      constexpr int NU = HDP / 16 / TPR;  // 16-value units of this thread
+      const __nv_bfloat16* src = nullptr;
+      if (qr < rows) {
+        const long long rr = row0 + qr;
+        src = p.q + (q_beg + rr / p.G) * p.q_row_stride + (kvh * p.G + rr % p.G) * hd;
+      }
+      float amax = 0.f;
+      for (int i = 0; i < NU; ++i) {
+        const int e = (part * NU + i) * 16;
+        if (src && e < hd) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src + e) + h);
+            const uint32_t w4[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              amax = fmax3(amax, fabsf(__uint_as_float(w4[k] << 16)),
+                           fabsf(__uint_as_float(w4[k] & 0xffff0000u)));
+          }
+        }
+      }
+      if constexpr (TPR == 2) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      const int ex = e4m3_exp(fminf(amax, __uint_as_float(0x7f7f0000u)), -120, 120);
+      // A negative scale turns Q's sign, so that the scores' factor is not.
+      const float inv = p.scale < 0.f ? -exp2_int(-ex) : exp2_int(-ex);
+      if (part == 0) sQs[qr] = exp2_int(ex);
+      for (int i = 0; i < NU; ++i) {
+        const int un = part * NU + i;
+        const int e = un * 16;
+        uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
+        if (src && e < hd) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src + e) + h);
+            const uint32_t w4[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              float x[4] = {__uint_as_float(w4[2 * k] << 16) * inv,
+                            __uint_as_float(w4[2 * k] & 0xffff0000u) * inv,
+                            __uint_as_float(w4[2 * k + 1] << 16) * inv,
+                            __uint_as_float(w4[2 * k + 1] & 0xffff0000u) * inv};
+              const uint32_t top = cvt_e4m3x2(x[0], x[1]) | (cvt_e4m3x2(x[2], x[3]) << 16);
+              float back[4];
+              e4m3x4_to_f32(top, back);
+              hi[2 * h + k] = top;
+              lo[2 * h + k] = cvt_e4m3x2(x[0] - back[0], x[1] - back[1]) |
+                              (cvt_e4m3x2(x[2] - back[2], x[3] - back[3]) << 16);
+            }
+          }
+        }
+        const uint32_t at = sQ + (un >> 3) * 128 * 128 + qr * 128 + (((un & 7) ^ (qr & 7)) << 4);
+        st_shared_v4(at, hi[0], hi[1], hi[2], hi[3]);
+        st_shared_v4(at + C::kQTerm, lo[0], lo[1], lo[2], lo[3]);
+      }
+      fence_proxy_async_smem();
+      named_bar_sync(1, C::kSoftThreads);
+      if (st == 0) mbar_arrive(bar(C::kBarQ));
+    }
+
+    int lo = 0, hi = INT_MAX;  // rows past the end see everything: they slow nothing down
+    if (r < rows) interval(r, lo, hi);
+    const float qs = sQs[r];
+    const bool capped = p.softcap != 0.f;
+    // Score factor without the block's K scale: log2 units, or for the
+    // soft-cap the argument of tanh.
+    const float row_c =
+        qs * fabsf(capped ? p.scale / p.softcap : p.scale_log2);
+    const float cap_l2 = p.softcap * 1.4426950408889634f;
+    const int shift = 31 - __clz(p.c.T);
+    const float* ksc = p.c.k_scale + static_cast<long long>(b) * p.c.n_blocks * p.c.Hkv + kvh;
+    const float* vsc = p.c.v_scale + static_cast<long long>(b) * p.c.n_blocks * p.c.Hkv + kvh;
+    // Lane c < BN / 16 holds the scales of the tile's keys 16 c .. 16 c + 15,
+    // loaded a tile ahead.
+    float nk = 0.f, nv = 1.f;
+    auto scales = [&](int j) {
+      if (j < n) {
+        const long long at = static_cast<long long>(min(
+            ((kt0 + j) * BN + (lane % (BN / 16)) * 16) >> shift, p.c.n_blocks - 1)) * p.c.Hkv;
+        nk = __ldg(ksc + at);
+        nv = __ldg(vsc + at);
+      }
+    };
+    float m = -INFINITY, l = 0.f;
+    int used = 0;
+    constexpr int STEP = C::kGroups;
+    scales(grp);
+    for (int j = grp; j < n; j += STEP) {
+      const int sb = j % C::SB;
+      const float cur_k = nk, cur_L = kv8_log2(nv);
+      const float cur_inv = ex2_approx(-cur_L);
+      scales(j + STEP);
+      mbar_wait(bar(C::kBarS + sb), (j / C::SB) & 1, dead, p.err);
+      dead = __any_sync(0xffffffffu, dead);
+      if (dead) break;
+      tc_fence_after();
+      const uint32_t s_addr = tmem + lane_off + sb * BN;
+      const int key0 = (kt0 + j) * BN;
+      const bool full = key0 >= f_lo && key0 + BN <= f_hi;
+      // Column i of the tile is visible iff (unsigned)(i - v0) < v1.
+      const int v0 = lo - key0;
+      const uint32_t v1 = static_cast<uint32_t>(hi) - static_cast<uint32_t>(lo);
+      float sr[BN];
+      float cmax = -INFINITY, umax = 0.f;
+      float a16[BN / 16], L16[BN / 16];
+#pragma unroll
+      for (int c = 0; c < BN / 16; ++c) {
+        a16[c] = row_c * __shfl_sync(0xffffffffu, cur_k, c);
+        L16[c] = __shfl_sync(0xffffffffu, cur_L, c);
+      }
+#pragma unroll
+      for (int cb = 0; cb < BN / 32; ++cb)
+        tmem_ld32(s_addr + cb * 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[cb * 32]));
+      tmem_wait_ld();
+      if (!full) {
+#pragma unroll
+        for (int i = 0; i < BN; ++i)
+          sr[i] = static_cast<uint32_t>(i - v0) < v1 ? sr[i] : -INFINITY;
+      }
+#pragma unroll
+      for (int c = 0; c < BN / 16; ++c) {
+        const float* x = &sr[c * 16];
+        float m0 = fmax3(x[0], x[1], x[2]), m1 = fmax3(x[3], x[4], x[5]);
+        m0 = fmax3(m0, x[6], x[7]);
+        m1 = fmax3(m1, x[8], x[9]);
+        m0 = fmax3(m0, x[10], x[11]);
+        m1 = fmax3(m1, x[12], x[13]);
+        m0 = fmax3(m0, x[14], x[15]);
+        m0 = fmaxf(m0, m1);
+        if (capped) {
+          float y = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) y = fmaxf(y, x[i] == -INFINITY ? 0.f : fabsf(x[i]));
+          umax = fmaxf(umax, y * a16[c]);
+          m0 = m0 == -INFINITY ? m0 : fmaf(cap_l2, tanh_via_exp2(m0 * a16[c]), L16[c]);
+        } else {
+          m0 = fmaf(m0, a16[c], L16[c]);
+        }
+        cmax = fmaxf(cmax, m0);
+      }
+      const bool resc = cmax > m + kKv8Lazy;
+      float corr = 1.f;
+      if (resc) {
+        corr = ex2_approx(m - cmax);
+        m = cmax;
+      }
+      const float mu = m == -INFINITY ? 0.f : m - kKv8Shift;
+      const bool poly = capped && __all_sync(0xffffffffu, umax <= kTanhPolyMax);
+      float sum = 0.f;
+      auto pass2 = [&](auto cap_c) {
+        constexpr int CAP = decltype(cap_c)::value;  // 0 none, 1 tanh, 2 its polynomial
+#pragma unroll
+        for (int c = 0; c < BN / 16; ++c) {
+          const float off = L16[c] - mu;
+          uint32_t w[8];
+          float2 s2 = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const float x0 = sr[c * 16 + 2 * q], x1 = sr[c * 16 + 2 * q + 1];
+            float2 y;
+            if constexpr (CAP == 0) {
+              y = __ffma2_rn(make_float2(x0, x1), make_float2(a16[c], a16[c]),
+                             make_float2(off, off));
+            } else if constexpr (CAP == 1) {
+              y.x = x0 == -INFINITY ? x0 : fmaf(cap_l2, tanh_via_exp2(x0 * a16[c]), off);
+              y.y = x1 == -INFINITY ? x1 : fmaf(cap_l2, tanh_via_exp2(x1 * a16[c]), off);
+            } else {
+              const float2 t = tanh_poly2(make_float2(x0 * a16[c], x1 * a16[c]));
+              y = __ffma2_rn(make_float2(cap_l2, cap_l2), t, make_float2(off, off));
+              y.x = x0 == -INFINITY ? x0 : y.x;
+              y.y = x1 == -INFINITY ? x1 : y.y;
+            }
+            const float p0 = ex2_approx(y.x), p1 = ex2_approx(y.y);
+            s2 = __fadd2_rn(s2, make_float2(p0, p1));
+            w[q] = pack_f16(p0, p1);
+          }
+          tmem_st8(s_addr + c * 16, w);
+          sum = fmaf(s2.x + s2.y, __shfl_sync(0xffffffffu, cur_inv, c), sum);
+        }
+      };
+      if (!capped) pass2(std::integral_constant<int, 0>{});
+      else if (!poly) pass2(std::integral_constant<int, 1>{});
+      else pass2(std::integral_constant<int, 2>{});
+      l = fmaf(l, corr, sum);
+      // One group: the previous P V may still add to O, and its end shows
+      // that the MMA warp has taken P[j - 1].
+      if (!ALT && used > 0) {
+        mbar_wait(bar(C::kBarO), (j - 1) & 1, dead, p.err);
+        dead = __any_sync(0xffffffffu, dead);
+        if (dead) break;
+        tc_fence_after();
+      }
+      if (used > 0 && __any_sync(0xffffffffu, resc)) {
+#pragma unroll 1
+        for (int c = 0; c < HDP / 32; ++c) {
+          uint32_t o[32];
+          const uint32_t ta = tmem + lane_off + C::kOCol + grp * HDP + c * 32;
+          tmem_ld32(ta, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = f2u(u2f(o[i]) * corr);
+          tmem_st32(ta, o);
+        }
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(C::kBarP + grp));
+      ++used;
+    }
+
+    // ------------------------------------------------------------ epilogue
+    if (n > 0 && !dead) {
+      mbar_wait(bar(C::kBarF), 0, dead, p.err);
+      dead = __any_sync(0xffffffffu, dead);
+      tc_fence_after();
+    }
+    float s_me = 1.f, s_ot = 0.f, lt = l, mt = m;
+    if constexpr (ALT) {
+      // The groups' maxima and sums: [group][l, m][128].
+      float* xch = reinterpret_cast<float*>(smem + C::kOffXch);
+      xch[grp * 256 + r] = l;
+      xch[grp * 256 + 128 + r] = m;
+      named_bar_sync(1, C::kSoftThreads);
+      const float l_ot = xch[(grp ^ 1) * 256 + r], m_ot = xch[(grp ^ 1) * 256 + 128 + r];
+      mt = fmaxf(m, m_ot);
+      const float ref = mt == -INFINITY ? 0.f : mt;
+      s_me = ex2_approx(m - ref);
+      s_ot = ex2_approx(m_ot - ref);
+      lt = grp == 0 ? fmaf(l, s_me, l_ot * s_ot) : fmaf(l_ot, s_ot, l * s_me);
+    }
+    const int n_me = ALT ? (grp == 0 ? (n + 1) / 2 : n / 2) : n;
+    const int n_ot = n - n_me;
+    const bool final_out = p.splits == 1;
+    const float inv = final_out ? __fdiv_rn(1.f, lt) : 1.f;
+    const long long cell = (static_cast<long long>(b) * p.c.Hkv + kvh) * p.tiles + tile;
+    const long long rr = row0 + r;
+    const long long at =
+        (q_beg + rr / p.G) * p.out_row_stride + (kvh * p.G + rr % p.G) * static_cast<long long>(hd);
+    float* po = p.part_o + ((cell * p.splits + split) * 128 + r) * hd;
+    constexpr int WC = HDP / C::kGroups;  // columns this group writes
+#pragma unroll 1
+    for (int c = 0; c < WC / 32; ++c) {
+      const int col0 = grp * WC + c * 32;
+      uint32_t o[32];
+      float v[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = 0.f;
+      if (n_me > 0 && !dead) {
+        tmem_ld32(tmem + lane_off + C::kOCol + grp * HDP + col0, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = u2f(o[i]) * s_me;
+      }
+      if (ALT && n_ot > 0 && !dead) {
+        tmem_ld32(tmem + lane_off + C::kOCol + (grp ^ 1) * HDP + col0, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = fmaf(u2f(o[i]), s_ot, v[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = dead ? __int_as_float(0x7fc00000) : v[i] * inv;
+      if (r < rows) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int col = col0 + 16 * h;
+          if (col < hd) {
+            const float* x = &v[16 * h];
+            if (!final_out || p.out_f32) {
+              float4* d = reinterpret_cast<float4*>(
+                  final_out ? static_cast<float*>(p.out) + at + col : po + col);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                d[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            } else {
+              uint4* d = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + at + col);
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                d[i] = make_uint4(pack_bf16(x[8 * i], x[8 * i + 1]),
+                                  pack_bf16(x[8 * i + 2], x[8 * i + 3]),
+                                  pack_bf16(x[8 * i + 4], x[8 * i + 5]),
+                                  pack_bf16(x[8 * i + 6], x[8 * i + 7]));
+            }
+          }
+        }
+      }
+    }
+    if (!final_out) {
+      float* pml = p.part_ml + (cell * p.splits + split) * 256;
+      if (grp == 0 && r < rows) {
+        pml[r] = mt;
+        pml[128 + r] = lt;
+      }
+      __threadfence();
+      named_bar_sync(1, C::kSoftThreads);
+      if (st == 0) {
+        const int done = atomicAdd(p.tickets + cell, 1);
+        misc[5] = done == p.splits - 1;
+        if (misc[5]) p.tickets[cell] = 0;  // as the next call finds it
+      }
+      named_bar_sync(1, C::kSoftThreads);
+      if (misc[5]) {
+        __threadfence();
+        pml = p.part_ml + cell * p.splits * 256;
+        po = p.part_o + cell * p.splits * 128 * static_cast<long long>(hd);
+        const int upr = hd / 4;
+        for (int i = st; i < rows * upr; i += C::kSoftThreads) {
+          const int jr = i / upr, e = (i - jr * upr) * 4;
+          float mj = -INFINITY;
+          for (int k = 0; k < p.splits; ++k) mj = fmaxf(mj, __ldcg(pml + k * 256 + jr));
+          float lj = 0.f;
+          float4 oj = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (mj != -INFINITY) {
+            for (int k = 0; k < p.splits; ++k) {
+              const float w = ex2_approx(__ldcg(pml + k * 256 + jr) - mj);
+              lj = fmaf(__ldcg(pml + k * 256 + 128 + jr), w, lj);
+              const float4 x = __ldcg(reinterpret_cast<const float4*>(
+                  po + (static_cast<long long>(k) * 128 + jr) * hd + e));
+              oj.x = fmaf(x.x, w, oj.x);
+              oj.y = fmaf(x.y, w, oj.y);
+              oj.z = fmaf(x.z, w, oj.z);
+              oj.w = fmaf(x.w, w, oj.w);
+            }
+          }
+          const float ij = __fdiv_rn(1.f, lj);
+          const long long gr = row0 + jr;
+          const long long d = (q_beg + gr / p.G) * p.out_row_stride +
+                              (kvh * p.G + gr % p.G) * static_cast<long long>(hd) + e;
+          if (p.out_f32)
+            *reinterpret_cast<float4*>(static_cast<float*>(p.out) + d) =
+                make_float4(oj.x * ij, oj.y * ij, oj.z * ij, oj.w * ij);
+          else
+            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + d) =
+                make_uint2(pack_bf16(oj.x * ij, oj.y * ij), pack_bf16(oj.z * ij, oj.w * ij));
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace ca

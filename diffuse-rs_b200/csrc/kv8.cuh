@@ -81,15 +81,15 @@ __device__ __forceinline__ void e4m3x4_to_f32(uint32_t w, float (&x)[4]) {
   x[3] = q.y;
 }
 
-// The exponent of the scale that a block of this largest magnitude needs.
-// 448 = 1.75 * 2^8, so amax = m * 2^e (1 <= m < 2) needs e - 8, or e - 7
-// where m > 1.75; read off the fp32 bits, so it is exact.
-__device__ __forceinline__ int kv8_exp(float amax) {
-  if (!(amax > 0.f)) return kKv8MinExp;
+// The smallest k in [lo, hi] with amax <= 448 * 2^k. 448 = 1.75 * 2^8, so
+// amax = m * 2^e (1 <= m < 2) needs e - 8, or e - 7 where m > 1.75; read off
+// the fp32 bits, so it is exact.
+__device__ __forceinline__ int e4m3_exp(float amax, int lo, int hi) {
+  if (!(amax > 0.f)) return lo;
   const uint32_t u = __float_as_uint(amax);
   const int e = static_cast<int>(u >> 23) - 127;
   const int k = e - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return min(max(k, kKv8MinExp), kKv8MaxExp);
+  return min(max(k, lo), hi);
 }
 
 __device__ __forceinline__ float exp2_int(int k) {  // 2^k, -126 <= k <= 127
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreParams p) 
       }
       amax = fminf(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax))),
                    __uint_as_float(0x7f7f0000u));
-      const float need = exp2_int(kv8_exp(amax));
+      const float need = exp2_int(e4m3_exp(amax, kKv8MinExp, kKv8MaxExp));
       float* sp = scales + (static_cast<long long>(b) * p.c.n_blocks + blk) * p.c.Hkv + h;
       const float was = *sp;
       const bool keep = stays && was > 0.f;

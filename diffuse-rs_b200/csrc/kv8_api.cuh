@@ -4,6 +4,7 @@
 #pragma once
 
 #include "attn_kv8_rows.cuh"
+#include "attn_kv8_tile.cuh"
 #include "kv8.cuh"
 
 namespace ca {
@@ -90,27 +91,37 @@ int kv8_load_impl(const ca_kv8_load_args* a, cudaStream_t st) {
 
 // How a call is laid out: which kernel, row tiles and splits of the keys.
 struct Kv8Plan {
+  bool tile;  // the 128-row tensor-core kernel, else 16 rows a CTA
   int tiles, splits;
   int64_t ws_bytes;
 };
 
-// A key axis is split where the row tiles alone would leave SMs idle, into
-// at least 256 keys (two chunks a warp) each.
+#ifndef CA_KV8_TILE_ROWS
+#define CA_KV8_TILE_ROWS 16
+#endif
+
 int kv8_plan(const ca_attn_kv8_args* a, const Kv8View& c, bool split_ok, Kv8Plan* pl) {
   const int64_t max_sq = a->cu_q ? a->max_sq : a->sq;
   const int64_t G = a->n_head / c.Hkv;
-  const int64_t tiles = (max_sq * G + 15) / 16;
+  const int64_t rows = max_sq * G;
+  pl->tile = rows > CA_KV8_TILE_ROWS && c.hd <= 256 &&
+             static_cast<int64_t>(c.batch) * c.n_total <= INT_MAX;
+  const int tr = pl->tile ? 128 : 16;
+  const int64_t tiles = (rows + tr - 1) / tr;
   if (tiles > INT_MAX / 1024) return CA_ERR_UNSUPPORTED;
   const int64_t cells = tiles * c.Hkv * c.batch;
+  // A key axis is split where the row tiles alone would leave SMs idle, into
+  // stretches of at least 256 keys (16-row kernel: two chunks a warp) or 512.
   int64_t splits = 1;
   if (split_ok && cells > 0 && cells < kSms) {
     splits = kSms / cells;
-    splits = std::max<int64_t>(1, std::min<int64_t>(splits, c.n_total / 256));
+    splits = std::max<int64_t>(1, std::min<int64_t>(splits, c.n_total / (pl->tile ? 512 : 256)));
   }
   pl->tiles = static_cast<int>(tiles);
   pl->splits = static_cast<int>(splits);
-  pl->ws_bytes =
-      splits == 1 ? 0 : CA_KV8_TICKET_BYTES + cells * splits * (16ll * c.hd + 32) * 4;
+  pl->ws_bytes = splits == 1 ? 0
+                             : CA_KV8_TICKET_BYTES +
+                                   cells * splits * (static_cast<int64_t>(tr) * c.hd + 2 * tr) * 4;
   return CA_OK;
 }
 
@@ -140,6 +151,44 @@ int launch_rows(const Kv8AttnParams& p, cudaStream_t st) {
   }
   const dim3 grid(p.tiles * p.splits, p.c.Hkv, p.c.batch);
   attn_kv8_rows_kernel<HDP><<<grid, 256, RowsCfg<HDP>::kSmem, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
+}
+
+// e4m3 rows [tokens][kv heads][head_dim] in boxes of 128 bytes x 1 head x
+// `keys` tokens, 128-byte swizzle; what lies outside reads as zero.
+int make_tmap_kv8(CUtensorMap* m, const uint8_t* base, const Kv8View& c, uint32_t keys) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return CA_ERR_CUDA;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(c.hd), static_cast<cuuint64_t>(c.Hkv),
+                        static_cast<cuuint64_t>(c.batch) * c.n_total};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(c.hd), static_cast<cuuint64_t>(c.row_stride)};
+  cuuint32_t box[3] = {128, 1, keys};
+  cuuint32_t es[3] = {1, 1, 1};
+  const CUresult r =
+      fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(base), dims, strides, box, es,
+         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? CA_OK : CA_ERR_INVALID;
+}
+
+template <int HDP>
+int launch_tile(const Kv8AttnParams& p, cudaStream_t st) {
+  using C = TileCfg<HDP>;
+  static bool attr_done[kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return CA_ERR_CUDA;
+  CUtensorMap tk, tv;
+  int rc;
+  if ((rc = make_tmap_kv8(&tk, p.c.k, p.c, C::BN)) != CA_OK) return rc;
+  if ((rc = make_tmap_kv8(&tv, p.c.v, p.c, C::BN)) != CA_OK) return rc;
+  if (!attr_done[dev]) {
+    if (cudaFuncSetAttribute(attn_kv8_tile_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             C::kSmem) != cudaSuccess)
+      return CA_ERR_CUDA;
+    attr_done[dev] = true;
+  }
+  const dim3 grid(p.tiles * p.splits, p.c.Hkv, p.c.batch);
+  attn_kv8_tile_kernel<C><<<grid, C::kThreads, C::kSmem, st>>>(tk, tv, p);
   return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
 }
 
@@ -186,7 +235,12 @@ int attn_kv8_impl(const ca_attn_kv8_args* a, cudaStream_t st) {
     const int64_t cells = static_cast<int64_t>(pl.tiles) * p.c.Hkv * p.c.batch;
     p.tickets = static_cast<int*>(a->workspace);
     p.part_ml = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + CA_KV8_TICKET_BYTES);
-    p.part_o = p.part_ml + cells * pl.splits * 32;
+    p.part_o = p.part_ml + cells * pl.splits * 2 * (pl.tile ? 128 : 16);
+  }
+  if (pl.tile) {
+    if (hd <= 64) return launch_tile<64>(p, st);
+    if (hd <= 128) return launch_tile<128>(p, st);
+    return launch_tile<256>(p, st);
   }
   if (hd <= 64) return launch_rows<64>(p, st);
   if (hd <= 128) return launch_rows<128>(p, st);
