@@ -17,16 +17,20 @@
 // f16 in shared memory by four warps of its own, which keep out of the
 // softmax warps' issue slots.
 //
-// Warp roles (512 threads at head_dim <= 128, one CTA per SM):
+// Warp roles (one CTA per SM; head_dim <= 128: 768 threads, 256: 512):
 //   warp 0       K tiles, TMA into a ring (lane 0)
 //   warp 1       TMEM, tcgen05.mma issue (lane 0)
 //   warp 2       V tiles, TMA into a ring (lane 0)
-//   warps 4-11   softmax in two groups of four that take alternate key tiles,
-//                each with its own S and O in TMEM, merged at the end; they
-//                split Q first and write the output last
-//   warps 12-15  V tile -> f16
-// head_dim 256: one softmax group (384 threads), 64-key tiles, three S
-// buffers and one O.
+//   warps 4 on   softmax. head_dim <= 128: two tile groups take alternate key
+//                tiles, each with its own S and O in TMEM, merged at the end;
+//                256: one group, 64-key tiles, three S buffers, one O. In a
+//                group two warps share 32 rows, each with half of a tile's
+//                keys and of O's columns; they exchange row maxima through
+//                shared memory and a barrier of their own.
+//   last 4       V tile -> f16
+// The softmax is a chain of latencies (TMEM load, maximum, exponentials, TMEM
+// store), so it wants warps: with one warp for whole 128-key rows a tile took
+// a group about 3100 clocks besides its MMAs.
 #pragma once
 
 #include "attn_kv8_rows.cuh"
@@ -38,10 +42,12 @@ struct TileCfg {
   static constexpr int HDP = HDP_;                       // 64, 128 or 256
   static constexpr bool ALT = HDP <= 128;
   static constexpr int BN = ALT ? 128 : 64;              // keys of a tile
-  static constexpr int kGroups = ALT ? 2 : 1;
-  static constexpr int kSoftThreads = 128 * kGroups;
+  static constexpr int TG = ALT ? 2 : 1;                 // tile groups
+  static constexpr int SC = BN / 2;                      // keys of a softmax thread's half row
+  static constexpr int kSoftWarps = 8 * TG;
+  static constexpr int kSoftThreads = 32 * kSoftWarps;
   static constexpr int kThreads = 256 + kSoftThreads;
-  static constexpr int kConvWarp0 = 4 + 4 * kGroups;
+  static constexpr int kConvWarp0 = 4 + kSoftWarps;
   static constexpr int STK = 3, STV = 2;                 // stages: K, V as held; V as f16 has 2
   static constexpr int SB = ALT ? 2 : 3;                 // S buffers
   static constexpr int kChunks = (HDP + 127) / 128;      // 128-byte columns of an e4m3 tile
@@ -55,8 +61,7 @@ struct TileCfg {
   static constexpr int kOffV8 = kOffK + STK * kTile8;
   static constexpr int kOffV = kOffV8 + STV * kTile8;
   static constexpr int kOffBar = kOffV + 2 * kTile16;
-  static constexpr int kBarQ = 0;               // Q's terms are in place
-  static constexpr int kBarK = 1;               // [STK] K landed
+  static constexpr int kBarK = 0;               // [STK] K landed
   static constexpr int kBarKE = kBarK + STK;    // [STK] K free
   static constexpr int kBarV8 = kBarKE + STK;   // [STV] V landed
   static constexpr int kBarV8E = kBarV8 + STV;  // [STV] V free
@@ -68,8 +73,9 @@ struct TileCfg {
   static constexpr int kBarF = kBarO + 2;       // every MMA done
   static constexpr int kNumBars = kBarF + 1;
   static constexpr int kOffQs = kOffBar + (kNumBars * 8 + 15) / 16 * 16;  // float [128]
-  static constexpr int kOffXch = kOffQs + 128 * 4;                        // float [2][2][128]
-  static constexpr int kOffMisc = kOffXch + 2 * 2 * 128 * 4;
+  static constexpr int kOffXch = kOffQs + 128 * 4;       // float [2 TG][2][128]
+  static constexpr int kOffSc = kOffXch + 2 * TG * 2 * 128 * 4;  // float [warp][2][3][4]
+  static constexpr int kOffMisc = kOffSc + kSoftWarps * 2 * 3 * 4 * 4;
   static constexpr int kSmem = kOffMisc + 64;
   static constexpr int kOCol = SB * BN;
   static constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(BN >> 3) << 17) |
@@ -77,7 +83,7 @@ struct TileCfg {
   static constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) |
                                       (static_cast<uint32_t>(HDP >> 3) << 17) |
                                       (128u >> 4 << 24);  // f16 x f16 (MN-major), fp32
-  static_assert(kOCol + kGroups * HDP <= 512, "TMEM");
+  static_assert(kOCol + TG * HDP <= 512, "TMEM");
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -101,15 +107,15 @@ __device__ __forceinline__ void reg_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// The launch's 512 threads hold 128 registers each: 2 x 128 x 192 for the
-// softmax and 2 x 128 x 64 for the rest are exactly those 65,536.
-constexpr int kTileSoftRegs = 192, kTileOtherRegs = 64;
+// Registers at head_dim <= 128: 768 threads are launched with 80 each; four
+// softmax warpgroups at 96 and the other two at 48 are those 6 x 80.
+constexpr int kTileSoftRegs = 96, kTileOtherRegs = 48;
 
 template <class C>
 __global__ void __launch_bounds__(C::kThreads, 1)
     attn_kv8_tile_kernel(const __grid_constant__ CUtensorMap tm_k,
                          const __grid_constant__ CUtensorMap tm_v, const Kv8AttnParams p) {
-  constexpr int BN = C::BN, HDP = C::HDP;
+  constexpr int BN = C::BN, HDP = C::HDP, SC = C::SC;
   constexpr bool ALT = C::ALT;
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023u) != 0) {
@@ -139,75 +145,175 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   float* sQs = reinterpret_cast<float*>(smem + C::kOffQs);
   int* misc = reinterpret_cast<int*>(smem + C::kOffMisc);  // [0] TMEM, [1..4] key ranges, [5] join
 
+  const bool masked = p.window != kNoWindow || prefix >= 0;
   auto interval = [&](int r, int& lo, int& hi) {
+    lo = 0;
+    hi = len;
+    if (!masked) return;
     const int tok = static_cast<int>((row0 + r) / p.G);
     const int pos = p.q_pos ? __ldg(p.q_pos + q_beg + tok) : len - q_len + tok;
     kv8_interval(pos, len, p.window, prefix, lo, hi);
   };
+  const int tok0 = b * p.c.n_total;  // the sequence's first row of the tensor maps
 
-  if (tid == 0) {
-    mbar_init(bar(C::kBarQ), 1);
-    for (int s = 0; s < C::STK; ++s) {
-      mbar_init(bar(C::kBarK + s), 1);
-      mbar_init(bar(C::kBarKE + s), 1);
-    }
-    for (int s = 0; s < C::STV; ++s) {
-      mbar_init(bar(C::kBarV8 + s), 1);
-      mbar_init(bar(C::kBarV8E + s), 4);
-    }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(bar(C::kBarV + s), 4);
-      mbar_init(bar(C::kBarVE + s), 1);
-      mbar_init(bar(C::kBarP + s), 4);
-      mbar_init(bar(C::kBarO + s), 1);
-    }
-    for (int s = 0; s < C::SB; ++s) mbar_init(bar(C::kBarS + s), 1);
-    mbar_init(bar(C::kBarF), 1);
-    fence_barrier_init();
-    fence_proxy_async_smem();
-  }
-  if (warp == 1) {
-    tmem_alloc(smem_u32(misc), 512);
-    tmem_relinquish();
-  }
-  if (warp == 3) {
-    // The hull of what the rows see, and what every row sees.
-    int k_lo = INT_MAX, k_hi = 0, f_lo = 0, f_hi = INT_MAX;
-    for (int r = lane; r < rows; r += 32) {
-      int lo, hi;
-      interval(r, lo, hi);
-      if (lo < hi) {
-        k_lo = min(k_lo, lo);
-        k_hi = max(k_hi, hi);
+  // Warps 0, 2 and 3 find the keys: the hull of what the rows see, what
+  // every row sees, and this CTA's tiles kt0 .. kt0 + n - 1. The producers
+  // set up their own barriers and start at once, while warps 4-11 split Q.
+  int k_lo = 0, k_hi = 0, f_lo = 0, f_hi = 0, kt0 = 0, n = 0;
+  auto find_keys = [&]() {
+    k_lo = 0;
+    k_hi = f_hi = len;
+    f_lo = 0;
+    if (masked) {
+      k_lo = f_hi = INT_MAX;
+      k_hi = 0;
+      for (int r = lane; r < rows; r += 32) {
+        int lo, hi;
+        interval(r, lo, hi);
+        if (lo < hi) {
+          k_lo = min(k_lo, lo);
+          k_hi = max(k_hi, hi);
+        }
+        f_lo = max(f_lo, lo);
+        f_hi = min(f_hi, hi);
       }
-      f_lo = max(f_lo, lo);
-      f_hi = min(f_hi, hi);
+      k_lo = __reduce_min_sync(0xffffffffu, k_lo);
+      k_hi = __reduce_max_sync(0xffffffffu, k_hi);
+      f_lo = __reduce_max_sync(0xffffffffu, f_lo);
+      f_hi = __reduce_min_sync(0xffffffffu, f_hi);
     }
-    k_lo = __reduce_min_sync(0xffffffffu, k_lo);
-    k_hi = __reduce_max_sync(0xffffffffu, k_hi);
-    f_lo = __reduce_max_sync(0xffffffffu, f_lo);
-    f_hi = __reduce_min_sync(0xffffffffu, f_hi);
+    if (k_lo < k_hi) {
+      const int first = k_lo / BN, all = (k_hi + BN - 1) / BN - first;
+      const int per = (all + p.splits - 1) / p.splits;
+      kt0 = first + min(all, split * per);
+      n = first + min(all, (split + 1) * per) - kt0;
+    }
+  };
+  auto load_tile = [&](const CUtensorMap* tm, uint32_t base, int full, int u, int s) {
+    mbar_arrive_expect_tx(bar(full + s), C::kTile8);
+#pragma unroll
+    for (int c = 0; c < C::kChunks; ++c)
+      tma_load_3d(base + s * C::kTile8 + c * BN * 128, tm, bar(full + s), c * 128, kvh,
+                  tok0 + (kt0 + u) * BN);
+  };
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int s = 0; s < C::STK; ++s) {
+        mbar_init(bar(C::kBarK + s), 1);
+        mbar_init(bar(C::kBarKE + s), 1);
+      }
+      fence_barrier_init();
+      fence_proxy_async_smem();
+    }
+    find_keys();
+    if (lane == 0)
+      for (int u = 0; u < min(n, C::STK); ++u) load_tile(&tm_k, sK, C::kBarK, u, u);
+  } else if (warp == 2) {
+    if (lane == 0) {
+      for (int s = 0; s < C::STV; ++s) {
+        mbar_init(bar(C::kBarV8 + s), 1);
+        mbar_init(bar(C::kBarV8E + s), 4);
+      }
+      fence_barrier_init();
+      fence_proxy_async_smem();
+    }
+    find_keys();
+    if (lane == 0)
+      for (int u = 0; u < min(n, C::STV); ++u) load_tile(&tm_v, sV8, C::kBarV8, u, u);
+  } else if (warp == 3) {
+    if (lane == 0) {
+      for (int s = 0; s < 2; ++s) {
+        mbar_init(bar(C::kBarV + s), 4);
+        mbar_init(bar(C::kBarVE + s), 1);
+        mbar_init(bar(C::kBarP + s), 8);
+        mbar_init(bar(C::kBarO + s), 1);
+      }
+      for (int s = 0; s < C::SB; ++s) mbar_init(bar(C::kBarS + s), 1);
+      mbar_init(bar(C::kBarF), 1);
+      fence_barrier_init();
+      fence_proxy_async_smem();
+    }
+    find_keys();
     if (lane == 0) {
       misc[1] = k_lo;
       misc[2] = k_hi;
       misc[3] = f_lo;
       misc[4] = f_hi;
+      misc[6] = kt0;
+      misc[7] = n;
     }
+  } else if (warp == 1) {
+    tmem_alloc(smem_u32(misc), 512);
+    tmem_relinquish();
+  } else if (warp < 12) {
+    // Q into its two terms: a lane takes 16 values, HDP / 16 lanes a row.
+    constexpr int LPR = HDP / 16, RPW = 32 / LPR, NP = 128 / (8 * RPW);
+    constexpr int NB = NP < 4 ? NP : 4;  // rows a lane has in flight
+    const int un = lane % LPR, e = un * 16;
+#pragma unroll 1
+    for (int p0 = 0; p0 < NP; p0 += NB) {
+      uint4 raw[NB][2];
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int qr = ((p0 + i) * 8 + warp - 4) * RPW + lane / LPR;
+        raw[i][0] = raw[i][1] = make_uint4(0u, 0u, 0u, 0u);
+        if (qr < rows && e < hd) {
+          const unsigned rr = static_cast<unsigned>(row0 + qr);  // < 2^31 (checked on the host)
+          const unsigned tok = rr / static_cast<unsigned>(p.G);
+          const uint4* src = reinterpret_cast<const uint4*>(
+              p.q + (q_beg + static_cast<long long>(tok)) * p.q_row_stride +
+              (kvh * p.G + static_cast<int>(rr - tok * p.G)) * static_cast<long long>(hd) + e);
+          raw[i][0] = __ldg(src);
+          raw[i][1] = __ldg(src + 1);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int qr = ((p0 + i) * 8 + warp - 4) * RPW + lane / LPR;
+        const uint32_t w8[8] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w,
+                                raw[i][1].x, raw[i][1].y, raw[i][1].z, raw[i][1].w};
+        float amax = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          amax = fmax3(amax, fabsf(__uint_as_float(w8[k] << 16)),
+                       fabsf(__uint_as_float(w8[k] & 0xffff0000u)));
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1)
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        const int ex = e4m3_exp(fminf(amax, __uint_as_float(0x7f7f0000u)), -120, 120);
+        // A negative scale turns Q's sign, so that the scores' factor is not.
+        const float inv = p.scale < 0.f ? -exp2_int(-ex) : exp2_int(-ex);
+        if (un == 0) sQs[qr] = exp2_int(ex);
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float x[4] = {__uint_as_float(w8[2 * k] << 16) * inv,
+                              __uint_as_float(w8[2 * k] & 0xffff0000u) * inv,
+                              __uint_as_float(w8[2 * k + 1] << 16) * inv,
+                              __uint_as_float(w8[2 * k + 1] & 0xffff0000u) * inv};
+          hi[k] = cvt_e4m3x2(x[0], x[1]) | (cvt_e4m3x2(x[2], x[3]) << 16);
+          float back[4];
+          e4m3x4_to_f32(hi[k], back);
+          lo[k] = cvt_e4m3x2(x[0] - back[0], x[1] - back[1]) |
+                  (cvt_e4m3x2(x[2] - back[2], x[3] - back[3]) << 16);
+        }
+        const uint32_t at = sQ + (un >> 3) * 128 * 128 + qr * 128 + (((un & 7) ^ (qr & 7)) << 4);
+        st_shared_v4(at, hi[0], hi[1], hi[2], hi[3]);
+        st_shared_v4(at + C::kQTerm, lo[0], lo[1], lo[2], lo[3]);
+      }
+    }
+    fence_proxy_async_smem();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = static_cast<uint32_t>(misc[0]);
-  const int k_lo = misc[1], k_hi = misc[2], f_lo = misc[3], f_hi = misc[4];
-  // This CTA's key tiles kt0 .. kt0 + n - 1.
-  int kt0 = 0, n = 0;
-  if (k_lo < k_hi) {
-    const int first = k_lo / BN, all = (k_hi + BN - 1) / BN - first;
-    const int per = (all + p.splits - 1) / p.splits;
-    kt0 = first + min(all, split * per);
-    n = first + min(all, (split + 1) * per) - kt0;
-  }
-  const int tok0 = b * p.c.n_total;  // the sequence's first row of the tensor maps
+  k_lo = misc[1];
+  k_hi = misc[2];
+  f_lo = misc[3];
+  f_hi = misc[4];
+  kt0 = misc[6];
+  n = misc[7];
   bool dead = false;
 
   if (warp < 4) {
@@ -219,16 +325,10 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         const int full = is_k ? C::kBarK : C::kBarV8;
         const int empty = is_k ? C::kBarKE : C::kBarV8E;
         const int NS = is_k ? C::STK : C::STV;
-        const uint32_t base = is_k ? sK : sV8;
-        const CUtensorMap* tm = is_k ? &tm_k : &tm_v;
-        for (int u = 0; u < n; ++u) {
+        for (int u = NS; u < n; ++u) {
           const int s = u % NS;
-          if (u >= NS && !mbar_wait(bar(empty + s), ((u / NS) - 1) & 1, dead, p.err)) break;
-          mbar_arrive_expect_tx(bar(full + s), C::kTile8);
-#pragma unroll
-          for (int c = 0; c < C::kChunks; ++c)
-            tma_load_3d(base + s * C::kTile8 + c * BN * 128, tm, bar(full + s), c * 128, kvh,
-                        tok0 + (kt0 + u) * BN);
+          if (!mbar_wait(bar(empty + s), ((u / NS) - 1) & 1, dead, p.err)) break;
+          load_tile(is_k ? &tm_k : &tm_v, is_k ? sK : sV8, full, u, s);
         }
         bool d2 = false;  // leave no copy in flight
         for (int u = max(0, n - NS); u < n; ++u)
@@ -282,7 +382,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
           umma_commit(bar(C::kBarVE + s));
           return true;
         };
-        if (n > 0 && mbar_wait(bar(C::kBarQ), 0, dead, p.err)) {
+        if (n > 0) {
           bool ok = issue_s(0) && (n < 2 || issue_s(1));
           for (int j = 0; ok && j < n; ++j) ok = issue_pv(j) && (j + 2 >= n || issue_s(j + 2));
         }
@@ -343,75 +443,14 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   } else {
     // ------------------------------------------------------------ softmax
     if constexpr (ALT) reg_inc<kTileSoftRegs>();
-    const int grp = (warp - 4) >> 2;
+    const int wg = (warp - 4) >> 2;       // warpgroup: tile group, half of the row
+    const int grp = wg >> 1, half = wg & 1;
     const int wq = warp & 3;
     const int r = wq * 32 + lane;
     const int st = tid - 128;  // softmax thread
     const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
-
-    // Q into its two terms. Threads share a row (two at head_dim <= 128, one
-    // at 256 with its single group), each with one half of its units.
-    {
-      constexpr int TPR = C::kGroups;
-      const int qr = st / TPR, part = st % TPR;
-      constexpr int NU = HDP / 16 / TPR;  // 16-value units of this thread
-      const __nv_bfloat16* src = nullptr;
-      if (qr < rows) {
-        const long long rr = row0 + qr;
-        src = p.q + (q_beg + rr / p.G) * p.q_row_stride + (kvh * p.G + rr % p.G) * hd;
-      }
-      float amax = 0.f;
-      for (int i = 0; i < NU; ++i) {
-        const int e = (part * NU + i) * 16;
-        if (src && e < hd) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src + e) + h);
-            const uint32_t w4[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              amax = fmax3(amax, fabsf(__uint_as_float(w4[k] << 16)),
-                           fabsf(__uint_as_float(w4[k] & 0xffff0000u)));
-          }
-        }
-      }
-      if constexpr (TPR == 2) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      const int ex = e4m3_exp(fminf(amax, __uint_as_float(0x7f7f0000u)), -120, 120);
-      // A negative scale turns Q's sign, so that the scores' factor is not.
-      const float inv = p.scale < 0.f ? -exp2_int(-ex) : exp2_int(-ex);
-      if (part == 0) sQs[qr] = exp2_int(ex);
-      for (int i = 0; i < NU; ++i) {
-        const int un = part * NU + i;
-        const int e = un * 16;
-        uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
-        if (src && e < hd) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src + e) + h);
-            const uint32_t w4[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              float x[4] = {__uint_as_float(w4[2 * k] << 16) * inv,
-                            __uint_as_float(w4[2 * k] & 0xffff0000u) * inv,
-                            __uint_as_float(w4[2 * k + 1] << 16) * inv,
-                            __uint_as_float(w4[2 * k + 1] & 0xffff0000u) * inv};
-              const uint32_t top = cvt_e4m3x2(x[0], x[1]) | (cvt_e4m3x2(x[2], x[3]) << 16);
-              float back[4];
-              e4m3x4_to_f32(top, back);
-              hi[2 * h + k] = top;
-              lo[2 * h + k] = cvt_e4m3x2(x[0] - back[0], x[1] - back[1]) |
-                              (cvt_e4m3x2(x[2] - back[2], x[3] - back[3]) << 16);
-            }
-          }
-        }
-        const uint32_t at = sQ + (un >> 3) * 128 * 128 + qr * 128 + (((un & 7) ^ (qr & 7)) << 4);
-        st_shared_v4(at, hi[0], hi[1], hi[2], hi[3]);
-        st_shared_v4(at + C::kQTerm, lo[0], lo[1], lo[2], lo[3]);
-      }
-      fence_proxy_async_smem();
-      named_bar_sync(1, C::kSoftThreads);
-      if (st == 0) mbar_arrive(bar(C::kBarQ));
-    }
+    const int pair_bar = 2 + grp * 4 + wq;  // the two warps of these rows
+    float* xch = reinterpret_cast<float*>(smem + C::kOffXch);
 
     int lo = 0, hi = INT_MAX;  // rows past the end see everything: they slow nothing down
     if (r < rows) interval(r, lo, hi);
@@ -425,55 +464,62 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     const int shift = 31 - __clz(p.c.T);
     const float* ksc = p.c.k_scale + static_cast<long long>(b) * p.c.n_blocks * p.c.Hkv + kvh;
     const float* vsc = p.c.v_scale + static_cast<long long>(b) * p.c.n_blocks * p.c.Hkv + kvh;
-    // Lane c < BN / 16 holds the scales of the tile's keys 16 c .. 16 c + 15,
-    // loaded a tile ahead.
+    // Lane c < SC / 16 takes the scales of this half's keys 16 c .. 16 c + 15,
+    // loaded a tile ahead; they reach the other lanes through shared memory.
+    constexpr int NC = SC / 16;
     float nk = 0.f, nv = 1.f;
     auto scales = [&](int j) {
       if (j < n) {
-        const long long at = static_cast<long long>(min(
-            ((kt0 + j) * BN + (lane % (BN / 16)) * 16) >> shift, p.c.n_blocks - 1)) * p.c.Hkv;
+        const int key = (kt0 + j) * BN + half * SC + (lane % NC) * 16;
+        const long long at = static_cast<long long>(min(key >> shift, p.c.n_blocks - 1)) * p.c.Hkv;
         nk = __ldg(ksc + at);
         nv = __ldg(vsc + at);
       }
     };
+    float* my_sc = reinterpret_cast<float*>(smem + C::kOffSc) + (warp - 4) * 24;
     float m = -INFINITY, l = 0.f;
     int used = 0;
-    constexpr int STEP = C::kGroups;
     scales(grp);
-    for (int j = grp; j < n; j += STEP) {
+    for (int j = grp; j < n; j += C::TG) {
       const int sb = j % C::SB;
-      const float cur_k = nk, cur_L = kv8_log2(nv);
-      const float cur_inv = ex2_approx(-cur_L);
-      scales(j + STEP);
+      float* tab = my_sc + (used & 1) * 12;  // [k scale, L, 2^-L][4]
+      if (lane < NC) {
+        const float L = kv8_log2(nv);
+        tab[lane] = nk;
+        tab[4 + lane] = L;
+        tab[8 + lane] = ex2_approx(-L);
+      }
+      scales(j + C::TG);
+      __syncwarp();
       mbar_wait(bar(C::kBarS + sb), (j / C::SB) & 1, dead, p.err);
       dead = __any_sync(0xffffffffu, dead);
-      if (dead) break;
+      // A pair ends together: neither warp waits for the other below.
       tc_fence_after();
-      const uint32_t s_addr = tmem + lane_off + sb * BN;
-      const int key0 = (kt0 + j) * BN;
-      const bool full = key0 >= f_lo && key0 + BN <= f_hi;
-      // Column i of the tile is visible iff (unsigned)(i - v0) < v1.
+      const uint32_t s_addr = tmem + lane_off + sb * BN + half * SC;
+      const int key0 = (kt0 + j) * BN + half * SC;
+      const bool full = key0 >= f_lo && key0 + SC <= f_hi;
+      // Column i of the half is visible iff (unsigned)(i - v0) < v1.
       const int v0 = lo - key0;
       const uint32_t v1 = static_cast<uint32_t>(hi) - static_cast<uint32_t>(lo);
-      float sr[BN];
-      float cmax = -INFINITY, umax = 0.f;
-      float a16[BN / 16], L16[BN / 16];
+      float sr[SC];
 #pragma unroll
-      for (int c = 0; c < BN / 16; ++c) {
-        a16[c] = row_c * __shfl_sync(0xffffffffu, cur_k, c);
-        L16[c] = __shfl_sync(0xffffffffu, cur_L, c);
-      }
-#pragma unroll
-      for (int cb = 0; cb < BN / 32; ++cb)
+      for (int cb = 0; cb < SC / 32; ++cb)
         tmem_ld32(s_addr + cb * 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[cb * 32]));
+      float a16[NC], L16[NC];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        a16[c] = row_c * tab[c];
+        L16[c] = tab[4 + c];
+      }
       tmem_wait_ld();
       if (!full) {
 #pragma unroll
-        for (int i = 0; i < BN; ++i)
+        for (int i = 0; i < SC; ++i)
           sr[i] = static_cast<uint32_t>(i - v0) < v1 ? sr[i] : -INFINITY;
       }
+      float cmax = -INFINITY, umax = 0.f;
 #pragma unroll
-      for (int c = 0; c < BN / 16; ++c) {
+      for (int c = 0; c < NC; ++c) {
         const float* x = &sr[c * 16];
         float m0 = fmax3(x[0], x[1], x[2]), m1 = fmax3(x[3], x[4], x[5]);
         m0 = fmax3(m0, x[6], x[7]);
@@ -483,15 +529,30 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         m0 = fmax3(m0, x[14], x[15]);
         m0 = fmaxf(m0, m1);
         if (capped) {
-          float y = 0.f;
+          // The largest magnitude: of the visible scores' two ends.
+          float n0 = INFINITY, n1 = INFINITY;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) y = fmaxf(y, x[i] == -INFINITY ? 0.f : fabsf(x[i]));
-          umax = fmaxf(umax, y * a16[c]);
+          for (int i = 0; i < 16; i += 2) {
+            n0 = fminf(n0, x[i] == -INFINITY ? INFINITY : x[i]);
+            n1 = fminf(n1, x[i + 1] == -INFINITY ? INFINITY : x[i + 1]);
+          }
+          n0 = fminf(n0, n1);
+          if (m0 != -INFINITY) umax = fmax3(umax, fabsf(m0) * a16[c], fabsf(n0) * a16[c]);
           m0 = m0 == -INFINITY ? m0 : fmaf(cap_l2, tanh_via_exp2(m0 * a16[c]), L16[c]);
         } else {
           m0 = fmaf(m0, a16[c], L16[c]);
         }
         cmax = fmaxf(cmax, m0);
+      }
+      // The other half's maximum (and whether its warp gave up).
+      {
+        float* mine = xch + ((wg * 2 + (used & 1)) * 128) + r;
+        *mine = dead ? __int_as_float(0x7fc00000) : cmax;  // a maximum is never NaN
+        named_bar_sync(pair_bar, 64);
+        const float other = xch[((wg ^ 1) * 2 + (used & 1)) * 128 + r];
+        dead = __any_sync(0xffffffffu, dead || other != other);
+        if (dead) break;
+        cmax = fmaxf(cmax, other);
       }
       const bool resc = cmax > m + kKv8Lazy;
       float corr = 1.f;
@@ -505,7 +566,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       auto pass2 = [&](auto cap_c) {
         constexpr int CAP = decltype(cap_c)::value;  // 0 none, 1 tanh, 2 its polynomial
 #pragma unroll
-        for (int c = 0; c < BN / 16; ++c) {
+        for (int c = 0; c < NC; ++c) {
           const float off = L16[c] - mu;
           uint32_t w[8];
           float2 s2 = make_float2(0.f, 0.f);
@@ -520,17 +581,20 @@ __global__ void __launch_bounds__(C::kThreads, 1)
               y.x = x0 == -INFINITY ? x0 : fmaf(cap_l2, tanh_via_exp2(x0 * a16[c]), off);
               y.y = x1 == -INFINITY ? x1 : fmaf(cap_l2, tanh_via_exp2(x1 * a16[c]), off);
             } else {
-              const float2 t = tanh_poly2(make_float2(x0 * a16[c], x1 * a16[c]));
+              const float2 t = tanh_poly2(__fmul2_rn(make_float2(x0, x1),
+                                                     make_float2(a16[c], a16[c])));
               y = __ffma2_rn(make_float2(cap_l2, cap_l2), t, make_float2(off, off));
-              y.x = x0 == -INFINITY ? x0 : y.x;
-              y.y = x1 == -INFINITY ? x1 : y.y;
+              if (!full) {
+                y.x = x0 == -INFINITY ? x0 : y.x;
+                y.y = x1 == -INFINITY ? x1 : y.y;
+              }
             }
             const float p0 = ex2_approx(y.x), p1 = ex2_approx(y.y);
             s2 = __fadd2_rn(s2, make_float2(p0, p1));
             w[q] = pack_f16(p0, p1);
           }
           tmem_st8(s_addr + c * 16, w);
-          sum = fmaf(s2.x + s2.y, __shfl_sync(0xffffffffu, cur_inv, c), sum);
+          sum = fmaf(s2.x + s2.y, tab[8 + c], sum);
         }
       };
       if (!capped) pass2(std::integral_constant<int, 0>{});
@@ -542,14 +606,13 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       if (!ALT && used > 0) {
         mbar_wait(bar(C::kBarO), (j - 1) & 1, dead, p.err);
         dead = __any_sync(0xffffffffu, dead);
-        if (dead) break;
         tc_fence_after();
       }
       if (used > 0 && __any_sync(0xffffffffu, resc)) {
 #pragma unroll 1
-        for (int c = 0; c < HDP / 32; ++c) {
+        for (int c = 0; c < HDP / 64; ++c) {
           uint32_t o[32];
-          const uint32_t ta = tmem + lane_off + C::kOCol + grp * HDP + c * 32;
+          const uint32_t ta = tmem + lane_off + C::kOCol + grp * HDP + half * (HDP / 2) + c * 32;
           tmem_ld32(ta, o);
           tmem_wait_ld();
 #pragma unroll
@@ -570,33 +633,38 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       dead = __any_sync(0xffffffffu, dead);
       tc_fence_after();
     }
-    float s_me = 1.f, s_ot = 0.f, lt = l, mt = m;
+    // Maxima and sums of all halves: [warpgroup][l, m][128]. A pair has one
+    // maximum.
+    named_bar_sync(1, C::kSoftThreads);
+    xch[wg * 256 + r] = l;
+    xch[wg * 256 + 128 + r] = m;
+    named_bar_sync(1, C::kSoftThreads);
+    float s_me = 1.f, s_ot = 0.f, mt = m;
+    float lt = xch[(grp * 2) * 256 + r] + xch[(grp * 2 + 1) * 256 + r];
     if constexpr (ALT) {
-      // The groups' maxima and sums: [group][l, m][128].
-      float* xch = reinterpret_cast<float*>(smem + C::kOffXch);
-      xch[grp * 256 + r] = l;
-      xch[grp * 256 + 128 + r] = m;
-      named_bar_sync(1, C::kSoftThreads);
-      const float l_ot = xch[(grp ^ 1) * 256 + r], m_ot = xch[(grp ^ 1) * 256 + 128 + r];
+      const float l_ot = xch[((grp ^ 1) * 2) * 256 + r] + xch[((grp ^ 1) * 2 + 1) * 256 + r];
+      const float m_ot = xch[((grp ^ 1) * 2) * 256 + 128 + r];
       mt = fmaxf(m, m_ot);
       const float ref = mt == -INFINITY ? 0.f : mt;
       s_me = ex2_approx(m - ref);
       s_ot = ex2_approx(m_ot - ref);
-      lt = grp == 0 ? fmaf(l, s_me, l_ot * s_ot) : fmaf(l_ot, s_ot, l * s_me);
+      lt = grp == 0 ? fmaf(lt, s_me, l_ot * s_ot) : fmaf(l_ot, s_ot, lt * s_me);
     }
     const int n_me = ALT ? (grp == 0 ? (n + 1) / 2 : n / 2) : n;
     const int n_ot = n - n_me;
     const bool final_out = p.splits == 1;
     const float inv = final_out ? __fdiv_rn(1.f, lt) : 1.f;
     const long long cell = (static_cast<long long>(b) * p.c.Hkv + kvh) * p.tiles + tile;
-    const long long rr = row0 + r;
-    const long long at =
-        (q_beg + rr / p.G) * p.out_row_stride + (kvh * p.G + rr % p.G) * static_cast<long long>(hd);
-    float* po = p.part_o + ((cell * p.splits + split) * 128 + r) * hd;
-    constexpr int WC = HDP / C::kGroups;  // columns this group writes
+    // Each warp puts 32 columns of its 32 rows into shared memory (the K ring
+    // is idle), 16-byte units turned by the row, and writes them out row by
+    // row, so that global stores are whole 64- or 128-byte pieces.
+    const bool f32 = !final_out || p.out_f32;
+    const uint32_t stage = sK + (warp - 4) * 4096;
+    constexpr int WC = HDP / (2 * C::TG);  // columns a warp writes
+    constexpr int PC = WC < 32 ? WC : 32;  // ... at a time
 #pragma unroll 1
-    for (int c = 0; c < WC / 32; ++c) {
-      const int col0 = grp * WC + c * 32;
+    for (int c = 0; c < WC / PC; ++c) {
+      const int col0 = wg * WC + c * PC;
       uint32_t o[32];
       float v[32];
 #pragma unroll
@@ -615,34 +683,47 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       }
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = dead ? __int_as_float(0x7fc00000) : v[i] * inv;
-      if (r < rows) {
+      // Units of 16 bytes: 4 fp32 or 8 bf16.
+      const int units = f32 ? PC / 4 : PC / 8;
+      const uint32_t my_row = stage + lane * (units * 16);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int col = col0 + 16 * h;
-          if (col < hd) {
-            const float* x = &v[16 * h];
-            if (!final_out || p.out_f32) {
-              float4* d = reinterpret_cast<float4*>(
-                  final_out ? static_cast<float*>(p.out) + at + col : po + col);
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                d[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-            } else {
-              uint4* d = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + at + col);
-#pragma unroll
-              for (int i = 0; i < 2; ++i)
-                d[i] = make_uint4(pack_bf16(x[8 * i], x[8 * i + 1]),
-                                  pack_bf16(x[8 * i + 2], x[8 * i + 3]),
-                                  pack_bf16(x[8 * i + 4], x[8 * i + 5]),
-                                  pack_bf16(x[8 * i + 6], x[8 * i + 7]));
-            }
-          }
+      for (int u = 0; u < PC / 4; ++u) {
+        if (f32) {
+          st_shared_v4(my_row + ((u ^ (lane & (PC / 4 - 1))) << 4), f2u(v[4 * u]),
+                       f2u(v[4 * u + 1]), f2u(v[4 * u + 2]), f2u(v[4 * u + 3]));
+        } else if (u < PC / 8) {
+          st_shared_v4(my_row + ((u ^ (lane & (PC / 8 - 1))) << 4), pack_bf16(v[8 * u], v[8 * u + 1]),
+                       pack_bf16(v[8 * u + 2], v[8 * u + 3]), pack_bf16(v[8 * u + 4], v[8 * u + 5]),
+                       pack_bf16(v[8 * u + 6], v[8 * u + 7]));
         }
       }
+      __syncwarp();
+#pragma unroll 1
+      for (int i = lane; i < 32 * units; i += 32) {
+        const int wr = i / units, u = i - wr * units;
+        const int gr = wq * 32 + wr, col = col0 + u * (f32 ? 4 : 8);
+        if (gr < rows && col < hd) {
+          uint32_t w[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                       : "r"(stage + wr * (units * 16) + ((u ^ (wr & (units - 1))) << 4)));
+          const unsigned rr = static_cast<unsigned>(row0 + gr);
+          const unsigned tok = rr / static_cast<unsigned>(p.G);
+          const long long at = (q_beg + static_cast<long long>(tok)) * p.out_row_stride +
+                               (kvh * p.G + static_cast<int>(rr - tok * p.G)) *
+                                   static_cast<long long>(hd) + col;
+          char* d = !final_out
+                        ? reinterpret_cast<char*>(
+                              p.part_o + ((cell * p.splits + split) * 128 + gr) * hd + col)
+                        : static_cast<char*>(p.out) + at * (f32 ? 4 : 2);
+          *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      __syncwarp();
     }
     if (!final_out) {
       float* pml = p.part_ml + (cell * p.splits + split) * 256;
-      if (grp == 0 && r < rows) {
+      if (wg == 0 && r < rows) {
         pml[r] = mt;
         pml[128 + r] = lt;
       }
@@ -657,7 +738,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       if (misc[5]) {
         __threadfence();
         pml = p.part_ml + cell * p.splits * 256;
-        po = p.part_o + cell * p.splits * 128 * static_cast<long long>(hd);
+        const float* po = p.part_o + cell * p.splits * 128 * static_cast<long long>(hd);
         const int upr = hd / 4;
         for (int i = st; i < rows * upr; i += C::kSoftThreads) {
           const int jr = i / upr, e = (i - jr * upr) * 4;
