@@ -1,23 +1,29 @@
 // attn_kv8_rows.cuh -- attention of a few query rows over the 8-bit cache.
 //
-// One CTA takes 16 query rows (token, head-of-the-group pairs, token-major)
-// of one (sequence, kv head) and one stretch of its keys. Each warp walks
-// chunks of 16 keys of that stretch on its own, K and V going from HBM
-// straight to registers in the layout the tensor core wants: the order of
-// the head dims inside Q K^T, and of the output columns inside P V, is free,
-// so every lane loads whole 16-byte pieces of a row and turns them into f16
-// (exact for e4m3) without a shuffle or shared memory.
+// One CTA takes 8 or 16 query rows (token, head-of-the-group pairs, token-
+// major) of one (sequence, kv head) and one stretch of its keys. Its warps
+// walk that stretch in chunks of 16 keys, each on its own: a ring of K and V
+// chunks filled by TMA, a softmax state, no barrier with the others until
+// their sums meet at the end.
 //
 // Mathematics. A cached value is e4m3 * scale, one scale for each block of
 // keys. With a = scale_k(block) * scale * log2 e and L = log2 scale_v(block),
 //   t = a (q . k8) + L,   p = 2^(t - m),
 //   O = sum p v8,         l = sum p 2^-L,     out = O / l
 // with m a running bound of t: the V scale rides in the exponent, so P V
-// runs on the held values, and only l has to take it out again. A row of Q
-// is scaled by a power of two into [1, 2) before it is rounded to f16, which
-// keeps bf16's 8 bits down to 2^-24 of the row's largest value. P is f16 at
+// runs on the held values, and only l has to take it out again. P is f16 at
 // up to 2^15 (2^7 for t = m, and m is only moved when t passes it by 8), so
 // weights down to 2^-31 of the largest count; sums and maxima are fp32.
+//
+// Both products are computed transposed, keys (or head dims) as the 16 rows
+// of an mma and query rows as its 8 columns: the few query rows of a step
+// then fill it, where as the 16-row operand they would leave most of it idle.
+//   S^T = K Q^T   K as it is held (e4m3), Q in two e4m3 terms, q = hi + lo,
+//                 each row scaled by a power of two into e4m3's range: bf16's
+//                 8 bits exactly, down to 2^-18 of the row's largest value
+//   O^T = V^T P^T V as f16 (exact), P^T by an 8 x 8 transpose of P
+// The order of the head dims inside a product is free, so every lane reads
+// whole 16-byte pieces of a row.
 //
 // Bound by HBM: 2 hd bytes a key. Long caches are split over CTAs; the last
 // CTA of a row tile to finish joins their partial sums in order, so results
@@ -79,12 +85,38 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return r;
 }
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+// D (+)= A B, 16 x 8 x 16, f16 in, fp32 accumulate.
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                        uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// D (+)= A B, 16 x 8 x 32, e4m3 in, fp32 accumulate.
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, "
+      "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// An 8 x 8 matrix of 16-bit values held two a lane, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// Four scaled values into their two e4m3 terms.
+__device__ __forceinline__ void split_e4m3(const float (&x)[4], uint32_t& hi, uint32_t& lo) {
+  hi = cvt_e4m3x2(x[0], x[1]) | (cvt_e4m3x2(x[2], x[3]) << 16);
+  float back[4];
+  e4m3x4_to_f32(hi, back);
+  lo = cvt_e4m3x2(x[0] - back[0], x[1] - back[1]) |
+       (cvt_e4m3x2(x[2] - back[2], x[3] - back[3]) << 16);
 }
 
 constexpr float kKv8Shift = 7.f;  // P's f16 exponent for t = m
@@ -97,34 +129,51 @@ __device__ __forceinline__ float kv8_log2(float s) {
   return fminf(fmaxf(y, -100.f), 120.f);
 }
 
-// HDP: head_dim padded to 64, 128, 256 or 512. VS warps share a stretch of
-// keys, each with 128 of the output columns (and all of Q K^T).
-template <int HDP>
+// HDP: head_dim padded to 64, 128, 256 or 512. NR: query rows of a CTA, 8 or
+// 16 (head_dim <= 128). At head_dim 512 two warps share a stretch of keys,
+// each with half of the output columns and all of S.
+template <int HDP_, int NR_>
 struct RowsCfg {
-  static constexpr int VS = HDP <= 128 ? 1 : HDP / 128;
-  static constexpr int kWarps = 8;
+  static constexpr int HDP = HDP_, NR = NR_;
+  static constexpr int VS = HDP == 512 ? 2 : 1;
+  static constexpr int kWarps = HDP == 512 ? 8 : HDP == 256 || NR == 16 ? 12 : 16;
+  static constexpr int kThreads = 32 * kWarps;
   static constexpr int kGroups = kWarps / VS;           // key-walking groups
-  static constexpr int VC = HDP / VS;                   // output columns of a warp (64 or 128)
-  static constexpr int KU = HDP / 64;                   // 16-byte pieces of a K row per lane
-  static constexpr int kQBytes = 16 * HDP * 2;          // f16 fragments of the 16 rows
-  static constexpr int kOBytes = kGroups * 16 * HDP * 4;
-  static constexpr int kOffML = kQBytes + kOBytes;
-  static constexpr int kSmem = kOffML + kGroups * 2 * 16 * 4 + 64;
-  // Chunks in registers: one being used and, where they fit, one in flight.
-  static constexpr int kBufs = HDP <= 256 ? 2 : 1;
+  static constexpr int ST = HDP <= 128 ? (NR == 8 ? 3 : 4) : 2;  // chunks of a warp's ring
+  static constexpr int KC = (HDP + 127) / 128;          // 128-byte columns of K
+  static constexpr int VC = (KC + VS - 1) / VS;         // ... and of a warp's part of V
+  static constexpr int kCol = 16 * 128;                 // bytes of such a column of a chunk
+  static constexpr int kStage = (KC + VC) * kCol;
+  static constexpr int kWarpBytes = ST * kStage;        // later the warp's partial O
+  static constexpr int kOffBar = kWarps * kWarpBytes;
+  static constexpr int kOffML = kOffBar + (kWarps * ST * 8 + 15) / 16 * 16;
+  static constexpr int kOffMisc = kOffML + kGroups * 2 * NR * 4;
+  static constexpr int kSmem = kOffMisc + 16;
+  static constexpr int OC = HDP / VS;                   // output columns of a warp
+  static constexpr int LC = HDP == 64 ? 8 : 16;         // columns a lane has of each 128
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+  static_assert(NR * OC * 4 <= kWarpBytes, "a warp's sums fit its ring");
 };
 
-template <int HDP>
-__global__ void __launch_bounds__(256, 1) attn_kv8_rows_kernel(const Kv8AttnParams p) {
-  using C = RowsCfg<HDP>;
+template <class C>
+__global__ void __launch_bounds__(C::kThreads, 1)
+    attn_kv8_rows_kernel(const __grid_constant__ CUtensorMap tm_k,
+                         const __grid_constant__ CUtensorMap tm_v, const Kv8AttnParams p) {
+  constexpr int HDP = C::HDP, NR = C::NR, ST = C::ST;
+  constexpr int NT = NR / 8;             // 8-row tiles
+  constexpr int KU = HDP / 64;           // 16-byte pieces of a K row per lane
+  constexpr int VB = C::OC / (8 * C::LC);  // 128-byte columns (one half-filled at 64) of V
+  constexpr int MT = VB * C::LC / 2;     // 16-dim tiles of O^T
   extern __shared__ __align__(1024) uint8_t smem[];
-  uint32_t* sq = reinterpret_cast<uint32_t*>(smem);
-  float* so = reinterpret_cast<float*>(smem + C::kQBytes);
+  if ((smem_u32(smem) & 1023u) != 0) {
+    if (threadIdx.x == 0) atomicExch(p.err ? p.err : &g_device_error, kErrLayout);
+    return;
+  }
   float* sml = reinterpret_cast<float*>(smem + C::kOffML);
-  int* smisc = reinterpret_cast<int*>(smem + C::kOffML + C::kGroups * 2 * 16 * 4);
+  int* smisc = reinterpret_cast<int*>(smem + C::kOffMisc);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int grp = warp / C::VS, vb = warp % C::VS;
+  const int grp = warp / C::VS, vs = warp % C::VS;
   const int split = blockIdx.x % p.splits, tile = blockIdx.x / p.splits;
   const int kvh = blockIdx.y, b = blockIdx.z;
   const int hd = p.c.hd;
@@ -132,36 +181,46 @@ __global__ void __launch_bounds__(256, 1) attn_kv8_rows_kernel(const Kv8AttnPara
   const int q_beg = p.cu_q ? p.cu_q[b] : b * p.sq;
   const int q_len = p.cu_q ? p.cu_q[b + 1] - q_beg : p.sq;
   const long long n_rows = static_cast<long long>(q_len) * p.G;
-  const long long row0 = static_cast<long long>(tile) * 16;
+  const long long row0 = static_cast<long long>(tile) * NR;
   if (row0 >= n_rows) return;
-  const int rows = static_cast<int>(min(16ll, n_rows - row0));
+  const int rows = static_cast<int>(min(static_cast<long long>(NR), n_rows - row0));
   const int len = p.kv_len ? min(max(p.kv_len[b], 0), p.c.n_total) : p.c.n_total;
+  const int prefix = p.seq_prefix ? p.seq_prefix[b] : p.causal_prefix;
+  const unsigned G = static_cast<unsigned>(p.G);
 
-  // Rows g and g + 8 of this lane: interval, and the tile's hull.
-  int lo[2], hi[2];
+  // Lane (g, t) has query rows 2 t and 2 t + 1 of each 8: what they see, the
+  // hull of what any row sees, and what every row sees.
+  int lo[NT][2], hi[NT][2];
+  int k_lo = 0, k_hi = len, f_lo = 0, f_hi = len;
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int r = g + 8 * x;
-    lo[x] = hi[x] = 0;
-    if (r < rows) {
-      const int tok = static_cast<int>((row0 + r) / p.G);
-      const int pos = p.q_pos ? p.q_pos[q_beg + tok] : len - q_len + tok;
-      kv8_interval(pos, len, p.window, p.seq_prefix ? p.seq_prefix[b] : p.causal_prefix, lo[x],
-                   hi[x]);
-    }
+  for (int x = 0; x < NT; ++x) lo[x][0] = lo[x][1] = 0, hi[x][0] = hi[x][1] = len;
+  if (p.window != kNoWindow || prefix >= 0) {
+    k_lo = f_hi = INT_MAX;
+    k_hi = f_lo = 0;
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int r = 8 * x + 2 * t + y;
+        if (r < rows) {
+          const int tok = static_cast<int>(static_cast<unsigned>(row0 + r) / G);
+          const int pos = p.q_pos ? __ldg(p.q_pos + q_beg + tok) : len - q_len + tok;
+          kv8_interval(pos, len, p.window, prefix, lo[x][y], hi[x][y]);
+          // A row that sees nothing does not widen the hull.
+          if (lo[x][y] < hi[x][y]) {
+            k_lo = min(k_lo, lo[x][y]);
+            k_hi = max(k_hi, hi[x][y]);
+          }
+          f_lo = max(f_lo, lo[x][y]);
+          f_hi = min(f_hi, hi[x][y]);
+        }
+      }
+    k_lo = __reduce_min_sync(0xffffffffu, k_lo);
+    k_hi = __reduce_max_sync(0xffffffffu, k_hi);
+    f_lo = __reduce_max_sync(0xffffffffu, f_lo);
+    f_hi = __reduce_min_sync(0xffffffffu, f_hi);
   }
-  // Rows that see nothing do not widen the hull; rows past the end neither.
-  const int any0 = lo[0] < hi[0], any1 = lo[1] < hi[1];
-  int k_lo = min(any0 ? lo[0] : INT_MAX, any1 ? lo[1] : INT_MAX);
-  int k_hi = max(any0 ? hi[0] : 0, any1 ? hi[1] : 0);
-  const bool r0 = g < rows, r1 = g + 8 < rows;
-  int f_lo = max(r0 ? lo[0] : 0, r1 ? lo[1] : 0);
-  int f_hi = min(r0 ? hi[0] : INT_MAX, r1 ? hi[1] : INT_MAX);
-  k_lo = __reduce_min_sync(0xffffffffu, k_lo);
-  k_hi = __reduce_max_sync(0xffffffffu, k_hi);
-  f_lo = __reduce_max_sync(0xffffffffu, f_lo);  // every row sees [f_lo, f_hi)
-  f_hi = __reduce_min_sync(0xffffffffu, f_hi);
-  // This CTA's chunks of 16 keys.
+  // This group's chunks: c_beg + grp, + kGroups, ...
   int c_beg = 0, c_end = 0;
   if (k_lo < k_hi) {
     const int first = k_lo >> 4, n = ((k_hi + 15) >> 4) - first;
@@ -169,266 +228,316 @@ __global__ void __launch_bounds__(256, 1) attn_kv8_rows_kernel(const Kv8AttnPara
     c_beg = first + min(n, split * per);
     c_end = first + min(n, (split + 1) * per);
   }
+  const int c0 = c_beg + grp;
 
-  // Q: each row scaled by a power of two, rounded to f16, in fragment order
-  // [k-step][lane][4]: step 4 i + c of lane (g, t) takes head dims
-  // (t + 4 i) 16 + 4 c .. + 3 of rows g and g + 8.
-  float qs[2];
-  {
-    __shared__ int s_exp[16];
-    for (int r = warp; r < 16; r += C::kWarps) {
-      float amax = 0.f;
-      const __nv_bfloat16* src = nullptr;
-      if (r < rows) {
-        const long long rr = row0 + r;
-        src = p.q + (q_beg + rr / p.G) * p.q_row_stride + (kvh * p.G + rr % p.G) * hd;
-        for (int e = lane * 4; e < hd; e += 128) {
-          const uint2 w = __ldg(reinterpret_cast<const uint2*>(src + e));
-          amax = fmaxf(amax, fmaxf(fmaxf(fabsf(__uint_as_float(w.x << 16)),
-                                         fabsf(__uint_as_float(w.x & 0xffff0000u))),
-                                   fmaxf(fabsf(__uint_as_float(w.y << 16)),
-                                         fabsf(__uint_as_float(w.y & 0xffff0000u)))));
-        }
-      }
-      const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));
-      const int ex = min(max(static_cast<int>(top >> 23) - 127, -100), 120);
-      if (lane == 0) s_exp[r] = ex;
-      const float inv = exp2_int(-ex);
-      for (int e = lane * 4; e < HDP; e += 128) {
-        uint32_t w0 = 0u, w1 = 0u;
-        if (r < rows && e < hd) {
-          const uint2 w = __ldg(reinterpret_cast<const uint2*>(src + e));
-          w0 = pack_f16(__uint_as_float(w.x << 16) * inv, __uint_as_float(w.x & 0xffff0000u) * inv);
-          w1 = pack_f16(__uint_as_float(w.y << 16) * inv, __uint_as_float(w.y & 0xffff0000u) * inv);
-        }
-        const int piece = e >> 4, c = (e >> 2) & 3;
-        const int step = (piece >> 2) * 4 + c, tt = piece & 3;
-        uint32_t* d = sq + (step * 32 + (r & 7) * 4 + tt) * 4 + (r >> 3);
-        d[0] = w0;
-        d[2] = w1;
-      }
-    }
-    __syncthreads();
-    qs[0] = exp2_int(s_exp[g]);
-    qs[1] = exp2_int(s_exp[g + 8]);
+  const uint32_t ring = smem_u32(smem + warp * C::kWarpBytes);
+  const uint32_t bar0 = smem_u32(smem + C::kOffBar) + warp * ST * 8;
+  const int tok0 = b * p.c.n_total;
+  auto fetch = [&](int ch, int s) {  // lane 0
+    const uint32_t dst = ring + s * C::kStage, bar = bar0 + 8 * s;
+    mbar_arrive_expect_tx(bar, C::kStage);
+#pragma unroll
+    for (int c = 0; c < C::KC; ++c)
+      tma_load_3d(dst + c * C::kCol, &tm_k, bar, c * 128, kvh, tok0 + ch * 16);
+#pragma unroll
+    for (int c = 0; c < C::VC; ++c)
+      tma_load_3d(dst + (C::KC + c) * C::kCol, &tm_v, bar, (vs * C::VC + c) * 128, kvh,
+                  tok0 + ch * 16);
+  };
+  if (lane == 0) {
+    for (int s = 0; s < ST; ++s) mbar_init(bar0 + 8 * s, 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
+    for (int s = 0; s < ST; ++s)
+      if (c0 + s * C::kGroups < c_end) fetch(c0 + s * C::kGroups, s);
   }
+  __syncwarp();
 
-  const uint8_t* kb = p.c.k + static_cast<long long>(b) * p.c.n_total * p.c.row_stride +
-                      static_cast<long long>(kvh) * hd;
-  const uint8_t* vbase = p.c.v + static_cast<long long>(b) * p.c.n_total * p.c.row_stride +
-                         static_cast<long long>(kvh) * hd;
   const float* ksc = p.c.k_scale + static_cast<long long>(b) * p.c.n_blocks * p.c.Hkv + kvh;
   const float* vsc = p.c.v_scale + static_cast<long long>(b) * p.c.n_blocks * p.c.Hkv + kvh;
   const int shift = 31 - __clz(p.c.T);
-
-  constexpr int NT = C::VC / 8;  // 8-column tiles of O
-  float o[NT][4];
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int x = 0; x < 4; ++x) o[j][x] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  const float cap_l2 = p.softcap * 1.4426950408889634f;
-  const float inv_cap = p.softcap != 0.f ? p.scale / p.softcap : 0.f;
-
-  // K piece i of key n: 16 bytes at head dim (t + 4 i) 16. V: keys 2 t,
-  // 2 t + 1, 2 t + 8, 2 t + 9 of the chunk, columns g 16 (g 8 at 64) on.
-  uint4 kr[C::kBufs][2][C::KU];
-  uint4 vr[C::kBufs][4];
-  float sc[C::kBufs][2];
-  auto load = [&](int ch, int buf) {
-    const int key0 = ch * 16;
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int key = key0 + 8 * n + g;
-      const uint8_t* a = kb + static_cast<long long>(key) * p.c.row_stride;
-#pragma unroll
-      for (int i = 0; i < C::KU; ++i) {
-        const int e = (t + 4 * i) * 16;
-        kr[buf][n][i] = key < k_hi && e < hd ? __ldg(reinterpret_cast<const uint4*>(a + e))
-                                            : make_uint4(0u, 0u, 0u, 0u);
-      }
+  float nk = 0.f, nv = 1.f;  // the next chunk's scales
+  auto scales = [&](int ch) {
+    if (ch < c_end) {
+      const long long blk = static_cast<long long>((ch * 16) >> shift) * p.c.Hkv;
+      nk = __ldg(ksc + blk);
+      nv = __ldg(vsc + blk);
     }
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int key = key0 + 2 * t + (x & 1) + 8 * (x >> 1);
-      const uint8_t* a = vbase + static_cast<long long>(key) * p.c.row_stride;
-      if constexpr (C::VC == 64) {
-        const int e = g * 8;
-        const uint2 w = key >= k_lo && key < k_hi && e < hd ? __ldg(reinterpret_cast<const uint2*>(a + e))
-                                            : make_uint2(0u, 0u);
-        vr[buf][x] = make_uint4(w.x, w.y, 0u, 0u);
-      } else {
-        const int e = vb * 128 + g * 16;
-        vr[buf][x] = key >= k_lo && key < k_hi && e < hd ? __ldg(reinterpret_cast<const uint4*>(a + e))
-                                         : make_uint4(0u, 0u, 0u, 0u);
-      }
-    }
-    const long long blk = static_cast<long long>(key0 >> shift) * p.c.Hkv;
-    sc[buf][0] = __ldg(ksc + blk);
-    sc[buf][1] = __ldg(vsc + blk);
   };
+  scales(c0);
 
-  auto chunk = [&](int ch, int buf) {
-    float s[2][4];
+  // Q as the products' B operand: lane (g, t) has of row g the head dims
+  // (t + 4 i) 16 .. + 15, two steps of 32 for each i.
+  uint32_t qf[NT][2][KU][4];
+  float qs[NT][2];  // the scale of rows 2 t, 2 t + 1
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+  for (int x = 0; x < NT; ++x) {
+    uint4 raw[KU][2];
+    const int r = 8 * x + g;
+    const unsigned rr = static_cast<unsigned>(row0 + r), tok = rr / G;
+    const __nv_bfloat16* src = p.q + (q_beg + static_cast<long long>(tok)) * p.q_row_stride +
+                               (kvh * p.G + static_cast<int>(rr - tok * G)) *
+                                   static_cast<long long>(hd);
+    float amax = 0.f;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) s[n][x] = 0.f;
+    for (int i = 0; i < KU; ++i) {
+      const int e = (t + 4 * i) * 16;
+      raw[i][0] = raw[i][1] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < rows && e < hd) {
+        raw[i][0] = __ldg(reinterpret_cast<const uint4*>(src + e));
+        raw[i][1] = __ldg(reinterpret_cast<const uint4*>(src + e) + 1);
+      }
+    }
 #pragma unroll
-    for (int i = 0; i < C::KU; ++i) {
+    for (int i = 0; i < KU; ++i)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint4 a = *reinterpret_cast<const uint4*>(sq + ((i * 4 + c) * 32 + lane) * 4);
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t w4[4] = {raw[i][h].x, raw[i][h].y, raw[i][h].z, raw[i][h].w};
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const uint4& w4 = kr[buf][n][i];
-          const uint32_t w = c == 0 ? w4.x : c == 1 ? w4.y : c == 2 ? w4.z : w4.w;
-          uint32_t b0, b1;
-          e4m3x4_to_f16(w, b0, b1);
-          mma_f16(s[n], a.x, a.y, a.z, a.w, b0, b1);
+        for (int k = 0; k < 4; ++k)
+          amax = fmax3(amax, fabsf(__uint_as_float(w4[k] << 16)),
+                       fabsf(__uint_as_float(w4[k] & 0xffff0000u)));
+      }
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const int ex = e4m3_exp(fminf(amax, __uint_as_float(0x7f7f0000u)), -120, 120);
+    const float inv = exp2_int(-ex);
+#pragma unroll
+    for (int i = 0; i < KU; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t w4[4] = {raw[i][h].x, raw[i][h].y, raw[i][h].z, raw[i][h].w};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float v[4] = {__uint_as_float(w4[2 * k] << 16) * inv,
+                              __uint_as_float(w4[2 * k] & 0xffff0000u) * inv,
+                              __uint_as_float(w4[2 * k + 1] << 16) * inv,
+                              __uint_as_float(w4[2 * k + 1] & 0xffff0000u) * inv};
+          split_e4m3(v, qf[x][0][i][2 * h + k], qf[x][1][i][2 * h + k]);
+        }
+      }
+    const float mine = exp2_int(ex);
+#pragma unroll
+    for (int y = 0; y < 2; ++y) qs[x][y] = __shfl_sync(0xffffffffu, mine, (2 * t + y) * 4);
+  }
+
+  float o[NT][MT][4];
+#pragma unroll
+  for (int x = 0; x < NT; ++x)
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) o[x][j][y] = 0.f;
+  float m[NT][2], l[NT][2];
+#pragma unroll
+  for (int x = 0; x < NT; ++x) m[x][0] = m[x][1] = -INFINITY, l[x][0] = l[x][1] = 0.f;
+  const bool capped = p.softcap != 0.f;
+  const float score = capped ? p.scale / p.softcap : p.scale_log2;
+  const float cap_l2 = p.softcap * 1.4426950408889634f;
+  bool dead = false;
+
+  int it = 0;
+  for (int ch = c0; ch < c_end; ch += C::kGroups, ++it) {
+    const int s = it % ST;
+    const float ks = nk, L = kv8_log2(nv);
+    scales(ch + C::kGroups);
+    mbar_wait(bar0 + 8 * s, (it / ST) & 1, dead, p.err);
+    if (__any_sync(0xffffffffu, dead)) break;
+    const uint32_t kb = ring + s * C::kStage, vb = kb + C::KC * C::kCol;
+    // S^T: keys g and g + 8 of the chunk as rows, query rows as columns.
+    float st[NT][4];
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) st[x][y] = 0.f;
+#pragma unroll
+    for (int i = 0; i < KU; ++i) {
+      const int u = t + 4 * (i & 1);
+      uint32_t a[4], c[4];
+      const uint32_t at = kb + (i >> 1) * C::kCol + g * 128 + ((u ^ g) << 4);
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(at));
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(at + 8 * 128));
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int term = 0; term < 2; ++term)
+            mma_e4m3(st[x], a[2 * h], c[2 * h], a[2 * h + 1], c[2 * h + 1],
+                     qf[x][term][i][2 * h], qf[x][term][i][2 * h + 1]);
+    }
+    // V: keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9, LC columns of each 128.
+    uint32_t vw[4][VB][C::LC / 4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int key = 2 * t + (k & 1) + 8 * (k >> 1);
+#pragma unroll
+      for (int c = 0; c < VB; ++c) {
+        if constexpr (C::LC == 8) {
+          asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                       : "=r"(vw[k][c][0]), "=r"(vw[k][c][1])
+                       : "r"(vb + key * 128 + (((g >> 1) ^ (key & 7)) << 4) + (g & 1) * 8));
+        } else {
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(vw[k][c][0]), "=r"(vw[k][c][1]), "=r"(vw[k][c][2]),
+                         "=r"(vw[k][c][3])
+                       : "r"(vb + c * C::kCol + key * 128 + ((g ^ (key & 7)) << 4)));
         }
       }
     }
-    // Logits in log2 units, plus the V scale's log2.
-    const float L = kv8_log2(sc[buf][1]);
-    const int key0 = ch * 16 + 2 * t;
-    const bool full = ch * 16 >= f_lo && ch * 16 + 16 <= f_hi;
+    const int key0 = ch * 16;
+    const bool full = key0 >= f_lo && key0 + 16 <= f_hi;
+    if (!full) {
+      // Keys that no row sees are zeros: what lies there is not data.
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+      for (int k = 0; k < 4; ++k) {
+        const int key = key0 + 2 * t + (k & 1) + 8 * (k >> 1);
+        if (key < k_lo || key >= k_hi) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float raw = s[n][x] * (qs[x >> 1] * sc[buf][0]);
-        float y;
-        if (p.softcap != 0.f) y = fmaf(cap_l2, tanh_via_exp2(raw * inv_cap), L);
-        else y = fmaf(raw, p.scale_log2, L);
-        const int key = key0 + 8 * n + (x & 1);
-        s[n][x] = full || (key >= lo[x >> 1] && key < hi[x >> 1]) ? y : -INFINITY;
+          for (int c = 0; c < VB; ++c)
+#pragma unroll
+            for (int w = 0; w < C::LC / 4; ++w) vw[k][c][w] = 0u;
+        }
       }
-    float mx[2];
+    }
+    // Every lane has read the stage: the next chunk may take its place.
+    __syncwarp();
+    if (lane == 0 && ch + ST * C::kGroups < c_end) fetch(ch + ST * C::kGroups, s);
+
+    // Logits in log2 units, plus the V scale's log2.
+    bool raise = false;
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
-      mx[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
-    if (__any_sync(0xffffffffu, mx[0] > m[0] + kKv8Lazy || mx[1] > m[1] + kKv8Lazy)) {
+    for (int x = 0; x < NT; ++x) {
+      const float a[2] = {qs[x][0] * ks * score, qs[x][1] * ks * score};
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-        if (mx[r] > m[r] + kKv8Lazy) {
-          const float corr = ex2_approx(m[r] - mx[r]);
-          m[r] = mx[r];
-          l[r] *= corr;
+      for (int y = 0; y < 4; ++y) {
+        float v = st[x][y] * a[y & 1];
+        v = capped ? fmaf(cap_l2, tanh_via_exp2(v), L) : v + L;
+        if (!full) {
+          const int key = key0 + g + 8 * (y >> 1);
+          v = key >= lo[x][y & 1] && key < hi[x][y & 1] ? v : -INFINITY;
+        }
+        st[x][y] = v;
+      }
+      raise |= fmaxf(st[x][0], st[x][2]) > m[x][0] + kKv8Lazy ||
+               fmaxf(st[x][1], st[x][3]) > m[x][1] + kKv8Lazy;
+    }
+    if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            o[j][2 * r] *= corr;
-            o[j][2 * r + 1] *= corr;
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          float mx = fmaxf(st[x][y], st[x][2 + y]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          if (mx > m[x][y] + kKv8Lazy) {
+            const float corr = ex2_approx(m[x][y] - mx);
+            m[x][y] = mx;
+            l[x][y] *= corr;
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+              o[x][j][y] *= corr;
+              o[x][j][2 + y] *= corr;
+            }
           }
         }
-      }
-    }
-    const float mu0 = m[0] == -INFINITY ? 0.f : m[0] - kKv8Shift;
-    const float mu1 = m[1] == -INFINITY ? 0.f : m[1] - kKv8Shift;
-    float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      s[n][0] = ex2_approx(s[n][0] - mu0);
-      s[n][1] = ex2_approx(s[n][1] - mu0);
-      s[n][2] = ex2_approx(s[n][2] - mu1);
-      s[n][3] = ex2_approx(s[n][3] - mu1);
-      sum0 += s[n][0] + s[n][1];
-      sum1 += s[n][2] + s[n][3];
     }
     const float unscale = ex2_approx(-L);
-    l[0] = fmaf(sum0, unscale, l[0]);
-    l[1] = fmaf(sum1, unscale, l[1]);
-    const uint32_t a0 = pack_f16(s[0][0], s[0][1]), a1 = pack_f16(s[0][2], s[0][3]);
-    const uint32_t a2 = pack_f16(s[1][0], s[1][1]), a3 = pack_f16(s[1][2], s[1][3]);
+    uint32_t pb[NT][2];
 #pragma unroll
-    for (int w = 0; w < NT / 4; ++w) {
-      auto word = [&](int x) -> uint32_t {
-        const uint4& v4 = vr[buf][x];
-        return w == 0 ? v4.x : w == 1 ? v4.y : w == 2 ? v4.z : v4.w;
-      };
-      const uint32_t p01 = word(0), q01 = word(1), p89 = word(2), q89 = word(3);
-      uint32_t b0[4], b1[4];
-      e4m3x4_to_f16(__byte_perm(p01, q01, 0x5140), b0[0], b0[1]);
-      e4m3x4_to_f16(__byte_perm(p01, q01, 0x7362), b0[2], b0[3]);
-      e4m3x4_to_f16(__byte_perm(p89, q89, 0x5140), b1[0], b1[1]);
-      e4m3x4_to_f16(__byte_perm(p89, q89, 0x7362), b1[2], b1[3]);
+    for (int x = 0; x < NT; ++x) {
+      const float mu0 = m[x][0] == -INFINITY ? 0.f : m[x][0] - kKv8Shift;
+      const float mu1 = m[x][1] == -INFINITY ? 0.f : m[x][1] - kKv8Shift;
+      const float p0 = ex2_approx(st[x][0] - mu0), p1 = ex2_approx(st[x][1] - mu1);
+      const float p2 = ex2_approx(st[x][2] - mu0), p3 = ex2_approx(st[x][3] - mu1);
+      l[x][0] = fmaf(p0 + p2, unscale, l[x][0]);
+      l[x][1] = fmaf(p1 + p3, unscale, l[x][1]);
+      pb[x][0] = transpose8(pack_f16(p0, p1));
+      pb[x][1] = transpose8(pack_f16(p2, p3));
+    }
+    // O^T: tile j of column c has dims LC g + 2 j (rows 0-7) and + 1 (8-15).
 #pragma unroll
-      for (int j = 0; j < 4; ++j) mma_f16(o[4 * w + j], a0, a1, a2, a3, b0[j], b1[j]);
-    }
-  };
-
-  if constexpr (C::kBufs == 2) {
-    int ch = c_beg + grp;
-    if (ch < c_end) load(ch, 0);
-    while (ch < c_end) {
-      const int nx = ch + C::kGroups;
-      if (nx < c_end) load(nx, 1);
-      chunk(ch, 0);
-      if (nx >= c_end) break;
-      const int nn = nx + C::kGroups;
-      if (nn < c_end) load(nn, 0);
-      chunk(nx, 1);
-      ch = nn;
-    }
-  } else {
-    for (int ch = c_beg + grp; ch < c_end; ch += C::kGroups) {
-      load(ch, 0);
-      chunk(ch, 0);
-    }
+    for (int c = 0; c < VB; ++c)
+#pragma unroll
+      for (int w = 0; w < C::LC / 4; ++w) {
+        uint32_t lo2[4], hi2[4];  // tiles 2 w and 2 w + 1
+        e4m3x4_to_f16(__byte_perm(vw[0][c][w], vw[1][c][w], 0x5140), lo2[0], lo2[1]);
+        e4m3x4_to_f16(__byte_perm(vw[2][c][w], vw[3][c][w], 0x5140), lo2[2], lo2[3]);
+        e4m3x4_to_f16(__byte_perm(vw[0][c][w], vw[1][c][w], 0x7362), hi2[0], hi2[1]);
+        e4m3x4_to_f16(__byte_perm(vw[2][c][w], vw[3][c][w], 0x7362), hi2[2], hi2[3]);
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+          const int j = c * C::LC / 2 + 2 * w;
+          mma_f16(o[x][j], lo2, pb[x][0], pb[x][1]);
+          mma_f16(o[x][j + 1], hi2, pb[x][0], pb[x][1]);
+        }
+      }
   }
 
-  // The groups' sums meet in shared memory. Lane (g, t) holds, of rows g and
-  // g + 8, columns 2 t NT .. + 2 NT - 1 of its warp's VC: tile j's first
-  // column is 2 t NT + j, its second NT further.
+  // The warps' sums meet in shared memory, each in its own ring.
+  float* so = reinterpret_cast<float*>(smem);
+  constexpr int kSo = C::kWarpBytes / 4;
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    if (t == 0 && vb == 0) {
-      sml[(grp * 2 + 0) * 16 + g + 8 * r] = m[r];
-      sml[(grp * 2 + 1) * 16 + g + 8 * r] = l[r];
-    }
-    float* d = so + (grp * 16 + g + 8 * r) * HDP + vb * C::VC + 2 * t * NT;
+  for (int x = 0; x < NT; ++x)
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      d[j] = o[j][2 * r];
-      d[NT + j] = o[j][2 * r + 1];
+    for (int y = 0; y < 2; ++y) {
+      const int r = 8 * x + 2 * t + y;
+      float sum = l[x][y];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+      if (g == 0 && vs == 0) {
+        sml[(grp * 2 + 0) * NR + r] = m[x][y];
+        sml[(grp * 2 + 1) * NR + r] = sum;
+      }
+      if (r < rows) {
+        float* d = so + warp * kSo + r * C::OC + g * C::LC;
+#pragma unroll
+        for (int c = 0; c < VB; ++c)
+#pragma unroll
+          for (int j = 0; j < C::LC / 2; j += 2)
+            *reinterpret_cast<float4*>(d + c * 128 + 2 * j) =
+                make_float4(o[x][c * C::LC / 2 + j][y], o[x][c * C::LC / 2 + j][2 + y],
+                            o[x][c * C::LC / 2 + j + 1][y], o[x][c * C::LC / 2 + j + 1][2 + y]);
+      }
     }
-  }
   __syncthreads();
   const long long cell = (static_cast<long long>(b) * p.c.Hkv + kvh) * p.tiles + tile;
   auto write_out = [&](int r, int e, float v) {
-    const long long rr = row0 + r;
-    const long long at = (q_beg + rr / p.G) * p.out_row_stride + (kvh * p.G + rr % p.G) * hd + e;
+    const unsigned rr = static_cast<unsigned>(row0 + r), tok = rr / G;
+    const long long at = (q_beg + static_cast<long long>(tok)) * p.out_row_stride +
+                         (kvh * p.G + static_cast<int>(rr - tok * G)) * static_cast<long long>(hd) +
+                         e;
     if (p.out_f32) static_cast<float*>(p.out)[at] = v;
     else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
   };
-  float* po = p.part_o + (cell * p.splits + split) * 16 * hd;
-  float* pml = p.part_ml + (cell * p.splits + split) * 32;
-  for (int i = threadIdx.x; i < rows * hd; i += 256) {
-    const int r = i / hd, e = i - r * hd;
+  float* po = p.part_o + (cell * p.splits + split) * NR * hd;
+  float* pml = p.part_ml + (cell * p.splits + split) * 2 * NR;
+  for (int i = threadIdx.x; i < rows * HDP; i += C::kThreads) {
+    const int r = i / HDP, e = i % HDP;
+    if (e >= hd) continue;
     float mt = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < C::kGroups; ++k) mt = fmaxf(mt, sml[k * 32 + r]);
+    for (int k = 0; k < C::kGroups; ++k) mt = fmaxf(mt, sml[k * 2 * NR + r]);
     float lt = 0.f, ot = 0.f;
     if (mt != -INFINITY) {
 #pragma unroll
       for (int k = 0; k < C::kGroups; ++k) {
-        const float w = ex2_approx(sml[k * 32 + r] - mt);
-        lt = fmaf(sml[k * 32 + 16 + r], w, lt);
-        ot = fmaf(so[(k * 16 + r) * HDP + e], w, ot);
+        const float w = ex2_approx(sml[k * 2 * NR + r] - mt);
+        lt = fmaf(sml[(k * 2 + 1) * NR + r], w, lt);
+        ot = fmaf(so[(k * C::VS + e / C::OC) * kSo + r * C::OC + e % C::OC], w, ot);
       }
     }
     if (p.splits == 1) {
       write_out(r, e, __fdiv_rn(ot, lt));
     } else {
-      po[i] = ot;
+      po[r * hd + e] = ot;
       if (e == 0) {
         pml[r] = mt;
-        pml[16 + r] = lt;
+        pml[NR + r] = lt;
       }
     }
   }
@@ -443,18 +552,20 @@ __global__ void __launch_bounds__(256, 1) attn_kv8_rows_kernel(const Kv8AttnPara
   __syncthreads();
   if (!smisc[0]) return;
   __threadfence();
-  po = p.part_o + cell * p.splits * 16 * hd;
-  pml = p.part_ml + cell * p.splits * 32;
-  for (int i = threadIdx.x; i < rows * hd; i += 256) {
-    const int r = i / hd, e = i - r * hd;
+  po = p.part_o + cell * p.splits * NR * hd;
+  pml = p.part_ml + cell * p.splits * 2 * NR;
+  for (int i = threadIdx.x; i < rows * HDP; i += C::kThreads) {
+    const int r = i / HDP, e = i % HDP;
+    if (e >= hd) continue;
     float mt = -INFINITY;
-    for (int k = 0; k < p.splits; ++k) mt = fmaxf(mt, __ldcg(pml + k * 32 + r));
+    for (int k = 0; k < p.splits; ++k) mt = fmaxf(mt, __ldcg(pml + k * 2 * NR + r));
     float lt = 0.f, ot = 0.f;
     if (mt != -INFINITY) {
+#pragma unroll 4
       for (int k = 0; k < p.splits; ++k) {
-        const float w = ex2_approx(__ldcg(pml + k * 32 + r) - mt);
-        lt = fmaf(__ldcg(pml + k * 32 + 16 + r), w, lt);
-        ot = fmaf(__ldcg(po + static_cast<long long>(k) * 16 * hd + i), w, ot);
+        const float w = ex2_approx(__ldcg(pml + k * 2 * NR + r) - mt);
+        lt = fmaf(__ldcg(pml + (k * 2 + 1) * NR + r), w, lt);
+        ot = fmaf(__ldcg(po + (static_cast<long long>(k) * NR + r) * hd + e), w, ot);
       }
     }
     write_out(r, e, __fdiv_rn(ot, lt));

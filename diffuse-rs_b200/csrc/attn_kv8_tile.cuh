@@ -291,11 +291,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                               __uint_as_float(w8[2 * k] & 0xffff0000u) * inv,
                               __uint_as_float(w8[2 * k + 1] << 16) * inv,
                               __uint_as_float(w8[2 * k + 1] & 0xffff0000u) * inv};
-          hi[k] = cvt_e4m3x2(x[0], x[1]) | (cvt_e4m3x2(x[2], x[3]) << 16);
-          float back[4];
-          e4m3x4_to_f32(hi[k], back);
-          lo[k] = cvt_e4m3x2(x[0] - back[0], x[1] - back[1]) |
-                  (cvt_e4m3x2(x[2] - back[2], x[3] - back[3]) << 16);
+          split_e4m3(x, hi[k], lo[k]);
         }
         const uint32_t at = sQ + (un >> 3) * 128 * 128 + qr * 128 + (((un & 7) ^ (qr & 7)) << 4);
         st_shared_v4(at, hi[0], hi[1], hi[2], hi[3]);

@@ -91,7 +91,7 @@ int kv8_load_impl(const ca_kv8_load_args* a, cudaStream_t st) {
 
 // How a call is laid out: which kernel, row tiles and splits of the keys.
 struct Kv8Plan {
-  bool tile;  // the 128-row tensor-core kernel, else 16 rows a CTA
+  int nr;  // query rows of a CTA: 128 (attn_kv8_tile.cuh), 16 or 8
   int tiles, splits;
   int64_t ws_bytes;
 };
@@ -104,18 +104,18 @@ int kv8_plan(const ca_attn_kv8_args* a, const Kv8View& c, bool split_ok, Kv8Plan
   const int64_t max_sq = a->cu_q ? a->max_sq : a->sq;
   const int64_t G = a->n_head / c.Hkv;
   const int64_t rows = max_sq * G;
-  pl->tile = rows > CA_KV8_TILE_ROWS && c.hd <= 256 &&
-             static_cast<int64_t>(c.batch) * c.n_total <= INT_MAX;
-  const int tr = pl->tile ? 128 : 16;
+  if (static_cast<int64_t>(c.batch) * c.n_total > INT_MAX) return CA_ERR_UNSUPPORTED;
+  const int tr = rows > CA_KV8_TILE_ROWS && c.hd <= 256 ? 128 : rows > 8 && c.hd <= 128 ? 16 : 8;
+  pl->nr = tr;
   const int64_t tiles = (rows + tr - 1) / tr;
   if (tiles > INT_MAX / 1024) return CA_ERR_UNSUPPORTED;
   const int64_t cells = tiles * c.Hkv * c.batch;
   // A key axis is split where the row tiles alone would leave SMs idle, into
-  // stretches of at least 256 keys (16-row kernel: two chunks a warp) or 512.
+  // stretches of at least 256 keys (one chunk a warp) or 512.
   int64_t splits = 1;
   if (split_ok && cells > 0 && cells < kSms) {
     splits = kSms / cells;
-    splits = std::max<int64_t>(1, std::min<int64_t>(splits, c.n_total / (pl->tile ? 512 : 256)));
+    splits = std::max<int64_t>(1, std::min<int64_t>(splits, c.n_total / (tr == 128 ? 512 : 256)));
   }
   pl->tiles = static_cast<int>(tiles);
   pl->splits = static_cast<int>(splits);
@@ -137,23 +137,6 @@ int attn_kv8_check(const ca_attn_kv8_args* a, Kv8View* c) {
   return CA_OK;
 }
 
-template <int HDP>
-int launch_rows(const Kv8AttnParams& p, cudaStream_t st) {
-  static bool attr_done[kMaxDevices] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return CA_ERR_CUDA;
-  if (!attr_done[dev]) {
-    if (cudaFuncSetAttribute(attn_kv8_rows_kernel<HDP>,
-                             cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             RowsCfg<HDP>::kSmem) != cudaSuccess)
-      return CA_ERR_CUDA;
-    attr_done[dev] = true;
-  }
-  const dim3 grid(p.tiles * p.splits, p.c.Hkv, p.c.batch);
-  attn_kv8_rows_kernel<HDP><<<grid, 256, RowsCfg<HDP>::kSmem, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
-}
-
 // e4m3 rows [tokens][kv heads][head_dim] in boxes of 128 bytes x 1 head x
 // `keys` tokens, 128-byte swizzle; what lies outside reads as zero.
 int make_tmap_kv8(CUtensorMap* m, const uint8_t* base, const Kv8View& c, uint32_t keys) {
@@ -169,6 +152,26 @@ int make_tmap_kv8(CUtensorMap* m, const uint8_t* base, const Kv8View& c, uint32_
          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? CA_OK : CA_ERR_INVALID;
+}
+
+template <class C>
+int launch_rows(const Kv8AttnParams& p, cudaStream_t st) {
+  static bool attr_done[kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return CA_ERR_CUDA;
+  CUtensorMap tk, tv;
+  int rc;
+  if ((rc = make_tmap_kv8(&tk, p.c.k, p.c, 16)) != CA_OK) return rc;
+  if ((rc = make_tmap_kv8(&tv, p.c.v, p.c, 16)) != CA_OK) return rc;
+  if (!attr_done[dev]) {
+    if (cudaFuncSetAttribute(attn_kv8_rows_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             C::kSmem) != cudaSuccess)
+      return CA_ERR_CUDA;
+    attr_done[dev] = true;
+  }
+  const dim3 grid(p.tiles * p.splits, p.c.Hkv, p.c.batch);
+  attn_kv8_rows_kernel<C><<<grid, C::kThreads, C::kSmem, st>>>(tk, tv, p);
+  return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
 }
 
 template <int HDP>
@@ -235,17 +238,19 @@ int attn_kv8_impl(const ca_attn_kv8_args* a, cudaStream_t st) {
     const int64_t cells = static_cast<int64_t>(pl.tiles) * p.c.Hkv * p.c.batch;
     p.tickets = static_cast<int*>(a->workspace);
     p.part_ml = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + CA_KV8_TICKET_BYTES);
-    p.part_o = p.part_ml + cells * pl.splits * 2 * (pl.tile ? 128 : 16);
+    p.part_o = p.part_ml + cells * pl.splits * 2 * pl.nr;
   }
-  if (pl.tile) {
+  if (pl.nr == 128) {
     if (hd <= 64) return launch_tile<64>(p, st);
     if (hd <= 128) return launch_tile<128>(p, st);
     return launch_tile<256>(p, st);
   }
-  if (hd <= 64) return launch_rows<64>(p, st);
-  if (hd <= 128) return launch_rows<128>(p, st);
-  if (hd <= 256) return launch_rows<256>(p, st);
-  return launch_rows<512>(p, st);
+  if (pl.nr == 16)
+    return hd <= 64 ? launch_rows<RowsCfg<64, 16>>(p, st) : launch_rows<RowsCfg<128, 16>>(p, st);
+  if (hd <= 64) return launch_rows<RowsCfg<64, 8>>(p, st);
+  if (hd <= 128) return launch_rows<RowsCfg<128, 8>>(p, st);
+  if (hd <= 256) return launch_rows<RowsCfg<256, 8>>(p, st);
+  return launch_rows<RowsCfg<512, 8>>(p, st);
 }
 
 }  // namespace
