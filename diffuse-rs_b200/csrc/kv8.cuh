@@ -96,22 +96,57 @@ __device__ __forceinline__ float exp2_int(int k) {  // 2^k, -126 <= k <= 127
   return __int_as_float((k + 127) << 23);
 }
 
-// One warp writes the rows of one (block, kv head) of K or of V: the largest
+// Magnitudes of two bf16 into a running pair of maxima (NaN has no part).
+__device__ __forceinline__ void amax_bf16x2(uint32_t& m, uint32_t w) {
+  asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w & 0x7fff7fffu));
+}
+
+// The larger of such a pair, infinities as the largest finite value.
+__device__ __forceinline__ float amax_of(uint32_t m) {
+  const float x = fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+  return fminf(x, __uint_as_float(0x7f7f0000u));
+}
+
+// Sixteen bf16 times inv as e4m3.
+__device__ __forceinline__ uint4 quantise16(const uint4 (&raw)[2], float inv) {
+  uint32_t o[4];
+#pragma unroll
+  for (int y = 0; y < 4; ++y) {
+    const uint4& v = raw[y >> 1];
+    const uint32_t a = (y & 1) ? v.z : v.x, c = (y & 1) ? v.w : v.y;
+    o[y] = cvt_e4m3x2(__uint_as_float(a << 16) * inv, __uint_as_float(a & 0xffff0000u) * inv) |
+           (cvt_e4m3x2(__uint_as_float(c << 16) * inv, __uint_as_float(c & 0xffff0000u) * inv)
+            << 16);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// W warps write the rows of one (block, kv head) of K or of V: the largest
 // magnitude of its new rows, the scale, the rounded rows, and, if the scale
-// grew, the rows that stay. A warp's job is rows_per_job consecutive entries
-// of the active list, for one head of K or V; it takes on the blocks whose
-// first active row lies among them and follows each into the next job's
-// entries, so every block has exactly one writer.
+// grew, the rows that stay. A job is rows_per_job consecutive entries of the
+// active list, for one head of K or V; it takes on the blocks whose first
+// active row lies among them and follows each into the next job's entries,
+// so every block has exactly one writer. A lane has U 16-value units (two
+// 16-byte loads) in flight; where W x 32 x U units are all of the block's
+// rows, they stay in registers between the maximum and the rounding.
 //
-// Bound by HBM (2 bytes read and 1 written for each value) on full passes and
-// by latency on a step's few rows.
-__global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreParams p) {
+// Bound by HBM (2 bytes read and 1 written for each value) on passes over
+// many rows: four warps with 8 units a lane there (4 x 8192 rows of 8 heads
+// x 256: 94 us with one warp and 8 units, 114 with 4 or 2). By latency on a
+// step's few rows: one warp and 2 units, whose code is short (4 rows of 4
+// heads x 128: 4.3 us, 6.0 with 4 units, most of it instruction fetch).
+template <int W, int U>
+__global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_store_kernel(const Kv8StoreParams p) {
+  constexpr int kJobs = W == 1 ? 8 : 1;  // jobs of a CTA at a time
+  __shared__ uint32_t s_max[W];
   const int lane = threadIdx.x & 31;
-  const long long warp = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int jt = W == 1 ? lane : threadIdx.x;  // thread of the job
+  const long long first = static_cast<long long>(blockIdx.x) * kJobs + (W == 1 ? threadIdx.x >> 5 : 0);
   const int heads2 = 2 * p.c.Hkv;
   const long long jobs = (p.rows + p.rows_per_job - 1) / p.rows_per_job * heads2;
-  const int T = p.c.T, hd = p.c.hd, upr = hd / 8;  // 8-value units of a row
-  for (long long job = warp; job < jobs; job += static_cast<long long>(gridDim.x) * 8) {
+  const int T = p.c.T, hd = p.c.hd, upr = hd / 16;  // 16-value units of a row
+  const unsigned magic = ((1u << 20) + upr - 1) / upr;  // u / upr for u < 2^12
+  for (long long job = first; job < jobs; job += static_cast<long long>(gridDim.x) * kJobs) {
     const int hh = static_cast<int>(job % heads2);
     const bool is_v = hh >= p.c.Hkv;
     const int h = is_v ? hh - p.c.Hkv : hh;
@@ -192,63 +227,165 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreParams p) 
         const uint32_t want = bits == 32 ? 0xffffffffu : (1u << bits) - 1u;
         stays |= (want & ~act[w]) != 0u;
       }
+      // The old scale is on its way while the rows are read.
+      float* sp = scales + (static_cast<long long>(b) * p.c.n_blocks + blk) * p.c.Hkv + h;
+      const float was = *sp;
       // Largest magnitude of the new rows. An infinity counts as the largest
       // finite value, a NaN not at all.
       const int units = n * upr;
-      float amax = 0.f;
-      for (int u = lane; u < units; u += 32) {
-        const int r = u / upr, e = (u - r * upr) * 8;
-        const uint4 raw =
-            __ldg(reinterpret_cast<const uint4*>(src + ((i + r) * p.c.Hkv + h) * hd + e));
-        const uint32_t w4[4] = {raw.x, raw.y, raw.z, raw.w};
+      uint4 raw[U][2];
+      auto row_of = [&](int u) -> int { return static_cast<int>((u * magic) >> 20); };
+      auto read = [&](int u0) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          amax = fmaxf(amax, fabsf(__uint_as_float(w4[k] << 16)));
-          amax = fmaxf(amax, fabsf(__uint_as_float(w4[k] & 0xffff0000u)));
+        for (int k = 0; k < U; ++k) {
+          const int u = u0 + 32 * W * k + jt;
+          raw[k][0] = raw[k][1] = make_uint4(0u, 0u, 0u, 0u);
+          if (u < units) {
+            const int r = row_of(u), e = (u - r * upr) * 16;
+            const uint4* from =
+                reinterpret_cast<const uint4*>(src + ((i + r) * p.c.Hkv + h) * hd + e);
+            raw[k][0] = __ldg(from);
+            raw[k][1] = __ldg(from + 1);
+          }
         }
+      };
+      uint32_t pair = 0u;
+      for (int u0 = 0; u0 < units; u0 += 32 * W * U) {
+        read(u0);
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            amax_bf16x2(pair, raw[k][x].x);
+            amax_bf16x2(pair, raw[k][x].y);
+            amax_bf16x2(pair, raw[k][x].z);
+            amax_bf16x2(pair, raw[k][x].w);
+          }
       }
-      amax = fminf(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax))),
-                   __uint_as_float(0x7f7f0000u));
-      const float need = exp2_int(e4m3_exp(amax, kKv8MinExp, kKv8MaxExp));
-      float* sp = scales + (static_cast<long long>(b) * p.c.n_blocks + blk) * p.c.Hkv + h;
-      const float was = *sp;
+      uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(amax_of(pair)));
+      if constexpr (W > 1) {
+        __syncthreads();  // the last block's maxima were read
+        if (lane == 0) s_max[threadIdx.x >> 5] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; ++w) top = max(top, s_max[w]);
+      }
+      const float need = exp2_int(e4m3_exp(__uint_as_float(top), kKv8MinExp, kKv8MaxExp));
       const bool keep = stays && was > 0.f;
       const float now = keep ? fmaxf(was, need) : need;
       __syncwarp();
-      if (lane == 0) *sp = now;
+      if (jt == 0) *sp = now;
       const float inv = __fdiv_rn(1.f, now);
       uint8_t* base = dst + (static_cast<long long>(b) * p.c.n_total) * p.c.row_stride +
                       static_cast<long long>(h) * hd;
-      for (int u = lane; u < units; u += 32) {
-        const int r = u / upr, e = (u - r * upr) * 8;
-        const uint4 raw =
-            __ldg(reinterpret_cast<const uint4*>(src + ((i + r) * p.c.Hkv + h) * hd + e));
-        const uint32_t w4[4] = {raw.x, raw.y, raw.z, raw.w};
-        uint32_t o[4];
+      for (int u0 = 0; u0 < units; u0 += 32 * W * U) {
+        if (units > 32 * W * U) read(u0);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          o[k] = cvt_e4m3x2(__uint_as_float(w4[k] << 16) * inv,
-                            __uint_as_float(w4[k] & 0xffff0000u) * inv);
-        const int q = __ldg(p.pos + i + r);
-        *reinterpret_cast<uint2*>(base + q * p.c.row_stride + e) =
-            make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
+        for (int k = 0; k < U; ++k) {
+          const int u = u0 + 32 * W * k + jt;
+          if (u < units) {
+            const int r = row_of(u), e = (u - r * upr) * 16;
+            const int q = __ldg(p.pos + i + r);
+            *reinterpret_cast<uint4*>(base + q * p.c.row_stride + e) = quantise16(raw[k], inv);
+          }
+        }
       }
       if (keep && now > was) {
         const float ratio = __fdiv_rn(was, now);
-        for (int u = lane; u < in_block * upr; u += 32) {
-          const int r = u / upr, e = (u - r * upr) * 8;
+        for (int u = jt; u < in_block * upr; u += 32 * W) {
+          const int r = row_of(u), e = (u - r * upr) * 16;
           if ((act[r >> 5] >> (r & 31)) & 1u) continue;
-          uint2* at = reinterpret_cast<uint2*>(base + (static_cast<long long>(blk) * T + r) *
+          uint4* at = reinterpret_cast<uint4*>(base + (static_cast<long long>(blk) * T + r) *
                                                           p.c.row_stride + e);
-          const uint2 old = *at;
-          float x[4], y[4];
-          e4m3x4_to_f32(old.x, x);
-          e4m3x4_to_f32(old.y, y);
-          *at = make_uint2(cvt_e4m3x2(x[0] * ratio, x[1] * ratio) |
-                               (cvt_e4m3x2(x[2] * ratio, x[3] * ratio) << 16),
-                           cvt_e4m3x2(y[0] * ratio, y[1] * ratio) |
-                               (cvt_e4m3x2(y[2] * ratio, y[3] * ratio) << 16));
+          const uint4 old = *at;
+          uint32_t w4[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            float x[4];
+            e4m3x4_to_f32(w4[y], x);
+            w4[y] = cvt_e4m3x2(x[0] * ratio, x[1] * ratio) |
+                    (cvt_e4m3x2(x[2] * ratio, x[3] * ratio) << 16);
+          }
+          *at = make_uint4(w4[0], w4[1], w4[2], w4[3]);
         }
+      }
+    }
+  }
+}
+
+// Every position of every sequence at once (as many active rows as
+// positions: in order, they can only be 0, 1, 2, ...): a block is its T rows,
+// there is nothing to look up and nothing that stays. Four warps take a block
+// of a kv head of K or V, 8 units a thread in flight. A block whose entries
+// are not those positions is left as it was and reported.
+__global__ void __launch_bounds__(128) kv8_store_all_kernel(const Kv8StoreParams p) {
+  constexpr int U = 8;
+  __shared__ uint32_t s_max[4];
+  const int lane = threadIdx.x & 31;
+  const int T = p.c.T, hd = p.c.hd, upr = hd / 16, heads2 = 2 * p.c.Hkv;
+  const unsigned magic = ((1u << 20) + upr - 1) / upr;
+  const unsigned hh = blockIdx.x % heads2;
+  const int blk = blockIdx.x / heads2, b = blockIdx.y;
+  const bool is_v = hh >= static_cast<unsigned>(p.c.Hkv);
+  const int h = is_v ? hh - p.c.Hkv : hh;
+  const int pos0 = blk * T, n = min(T, p.c.n_total - pos0);
+  const long long row0 = static_cast<long long>(b) * p.c.n_total + pos0;
+  const __nv_bfloat16* src = (is_v ? p.v : p.k) + (row0 * p.c.Hkv + h) * hd;
+  const int src_stride = p.c.Hkv * hd;
+  uint8_t* dst = (is_v ? p.c.v : p.c.k) + row0 * p.c.row_stride + static_cast<long long>(h) * hd;
+  const int units = n * upr;
+  uint4 raw[U][2];
+  auto read = [&](int u0) {
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const unsigned u = u0 + 128 * k + threadIdx.x;
+      raw[k][0] = raw[k][1] = make_uint4(0u, 0u, 0u, 0u);
+      if (u < static_cast<unsigned>(units)) {
+        const unsigned r = (u * magic) >> 20;
+        const uint4* from = reinterpret_cast<const uint4*>(
+            src + static_cast<long long>(r) * src_stride + (u - r * upr) * 16);
+        raw[k][0] = __ldg(from);
+        raw[k][1] = __ldg(from + 1);
+      }
+    }
+  };
+  uint32_t pair = 0u;
+  for (int u0 = 0; u0 < units; u0 += 128 * U) {
+    read(u0);
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        amax_bf16x2(pair, raw[k][x].x);
+        amax_bf16x2(pair, raw[k][x].y);
+        amax_bf16x2(pair, raw[k][x].z);
+        amax_bf16x2(pair, raw[k][x].w);
+      }
+  }
+  const bool bad = static_cast<int>(threadIdx.x) < n &&
+                   __ldg(p.pos + row0 + threadIdx.x) != pos0 + static_cast<int>(threadIdx.x);
+  uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(amax_of(pair)));
+  if (lane == 0) s_max[threadIdx.x >> 5] = top;
+  if (__syncthreads_or(bad)) {
+    if (threadIdx.x == 0 && p.err) atomicExch(p.err, kErrInvalidRow);
+    return;
+  }
+#pragma unroll
+  for (int w = 0; w < 4; ++w) top = max(top, s_max[w]);
+  const int ex = e4m3_exp(__uint_as_float(top), kKv8MinExp, kKv8MaxExp);
+  const float inv = exp2_int(-ex);
+  if (threadIdx.x == 0)
+    (is_v ? p.c.v_scale : p.c.k_scale)[(static_cast<long long>(b) * p.c.n_blocks + blk) * p.c.Hkv +
+                                       h] = exp2_int(ex);
+  for (int u0 = 0; u0 < units; u0 += 128 * U) {
+    if (units > 128 * U) read(u0);
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const unsigned u = u0 + 128 * k + threadIdx.x;
+      if (u < static_cast<unsigned>(units)) {
+        const unsigned r = (u * magic) >> 20;
+        *reinterpret_cast<uint4*>(dst + r * p.c.row_stride + (u - r * upr) * 16) =
+            quantise16(raw[k], inv);
       }
     }
   }
@@ -261,7 +398,6 @@ struct Kv8LoadParams {
   int out_f32;
   const int* pos;  // [batch, n_pos] or null (positions 0 .. n_pos - 1)
   int n_pos;
-  long long rows;  // batch * n_pos
   int* err;
 };
 
@@ -269,18 +405,18 @@ struct Kv8LoadParams {
 // load, two (four) 16-byte stores. Bound by HBM: 1 byte read and 2 (4)
 // written for each value.
 __global__ void __launch_bounds__(256) kv8_load_kernel(const Kv8LoadParams p) {
-  const int upr = p.c.Hkv * p.c.hd / 16;  // 16-value units of a row
-  const long long units = p.rows * upr;
+  const unsigned upr = p.c.Hkv * p.c.hd / 16;  // 16-value units of a row
   const uint8_t* src = blockIdx.y ? p.c.v : p.c.k;
   const float* scales = blockIdx.y ? p.c.v_scale : p.c.k_scale;
   void* dst = blockIdx.y ? p.v_out : p.k_out;
   if (!dst) return;
-  for (long long u = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; u < units;
-       u += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const long long row = u / upr;
-    const int e = static_cast<int>(u - row * upr) * 16;
-    const int b = static_cast<int>(row / p.n_pos);
-    const int pos = p.pos ? __ldg(p.pos + row) : static_cast<int>(row - static_cast<long long>(b) * p.n_pos);
+  const int b = blockIdx.z;
+  const unsigned units = p.n_pos * upr;
+  for (unsigned u = blockIdx.x * blockDim.x + threadIdx.x; u < units; u += gridDim.x * blockDim.x) {
+    const unsigned i = u / upr;
+    const int e = static_cast<int>(u - i * upr) * 16;
+    const long long row = static_cast<long long>(b) * p.n_pos + i;
+    const int pos = p.pos ? __ldg(p.pos + row) : static_cast<int>(i);
     if (pos < 0 || pos >= p.c.n_total) {
       if (p.err) atomicExch(p.err, kErrInvalidRow);
       continue;

@@ -55,14 +55,26 @@ int kv8_store_impl(const ca_kv8_store_args* a, cudaStream_t st) {
   p.kv_len = a->kv_len;
   p.na = a->n_active;
   p.err = a->status;
-  // Entries of the active list a warp looks through: one where that leaves
+  if (!p.cu_active && a->n_active == p.c.n_total && p.c.batch <= 65535) {
+    const dim3 grid(p.c.n_blocks * 2 * p.c.Hkv, p.c.batch);
+    kv8_store_all_kernel<<<grid, 128, 0, st>>>(p);
+    return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
+  }
+  // Entries of the active list a job looks through: one where that leaves
   // every warp slot of the GPU at most one job, 32 (a lane each) at most.
+  // From 8 on, rows are many and mostly side by side: four warps a job.
   const int64_t slots = static_cast<int64_t>(kSms) * 64;
   const int64_t one = p.rows * 2 * p.c.Hkv;
   p.rows_per_job = static_cast<int>(std::min<int64_t>(32, (one + slots - 1) / slots));
+  const bool many = p.rows_per_job >= 8;
+  if (many) p.rows_per_job = 32;
   const int64_t jobs = (p.rows + p.rows_per_job - 1) / p.rows_per_job * 2 * p.c.Hkv;
-  const int blocks = static_cast<int>(std::min<int64_t>((jobs + 7) / 8, kSms * 64));
-  kv8_store_kernel<<<blocks, 256, 0, st>>>(p);
+  if (many)
+    kv8_store_kernel<4, 8>
+        <<<static_cast<int>(std::min<int64_t>(jobs, kSms * 1024)), 128, 0, st>>>(p);
+  else
+    kv8_store_kernel<1, 1>
+        <<<static_cast<int>(std::min<int64_t>((jobs + 7) / 8, kSms * 64)), 256, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
 }
 
@@ -75,16 +87,17 @@ int kv8_load_impl(const ca_kv8_load_args* a, cudaStream_t st) {
     return CA_ERR_INVALID;
   if ((a->k_out && !aligned16(a->k_out)) || (a->v_out && !aligned16(a->v_out)))
     return CA_ERR_INVALID;
-  p.rows = static_cast<int64_t>(p.c.batch) * a->n_pos;
-  if (p.rows == 0) return CA_OK;
+  if (a->n_pos == 0 || p.c.batch == 0) return CA_OK;
+  const int64_t units = static_cast<int64_t>(a->n_pos) * (static_cast<int64_t>(p.c.Hkv) * p.c.hd / 16);
+  if (p.c.batch > 65535 || units > INT_MAX) return CA_ERR_UNSUPPORTED;
   p.k_out = a->k_out;
   p.v_out = a->v_out;
   p.out_f32 = a->out_f32 ? 1 : 0;
   p.pos = a->pos;
   p.n_pos = a->n_pos;
   p.err = a->status;
-  const int64_t units = p.rows * (static_cast<int64_t>(p.c.Hkv) * p.c.hd / 16);
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((units + 255) / 256, kSms * 32)), 2);
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((units + 255) / 256, kSms * 32)), 2,
+                  p.c.batch);
   kv8_load_kernel<<<grid, 256, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
 }
@@ -113,10 +126,9 @@ int kv8_plan(const ca_attn_kv8_args* a, const Kv8View& c, bool split_ok, Kv8Plan
   // A key axis is split where the row tiles alone would leave SMs idle, into
   // stretches of at least 256 keys (one chunk a warp) or 512.
   int64_t splits = 1;
-  if (split_ok && cells > 0 && cells < kSms) {
-    splits = kSms / cells;
-    splits = std::max<int64_t>(1, std::min<int64_t>(splits, c.n_total / (tr == 128 ? 512 : 256)));
-  }
+  if (split_ok && cells > 0 && cells < kSms)
+    splits = std::max<int64_t>(
+        1, std::min<int64_t>(kSms / cells, c.n_total / (tr == 128 ? 512 : 256)));
   pl->tiles = static_cast<int>(tiles);
   pl->splits = static_cast<int>(splits);
   pl->ws_bytes = splits == 1 ? 0
