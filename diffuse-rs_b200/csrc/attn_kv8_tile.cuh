@@ -17,39 +17,42 @@
 // f16 in shared memory by four warps of its own, which keep out of the
 // softmax warps' issue slots.
 //
-// Warp roles (one CTA per SM; head_dim <= 128: 768 threads, 256: 512):
-//   warp 0       K tiles, TMA into a ring (lane 0)
+// Warp roles (one CTA per SM):
+//   warp 0       K tiles of 64 keys, TMA into a ring (lane 0)
 //   warp 1       TMEM, tcgen05.mma issue (lane 0)
 //   warp 2       V tiles, TMA into a ring (lane 0)
-//   warps 4 on   softmax. head_dim <= 128: two tile groups take alternate key
-//                tiles, each with its own S and O in TMEM, merged at the end;
-//                256: one group, 64-key tiles, three S buffers, one O. In a
-//                group two warps share 32 rows, each with half of a tile's
-//                keys and of O's columns; they exchange row maxima through
+//   warps 4 on   softmax. head_dim <= 128: two tile groups take alternate
+//                tiles, each with an O of its own, merged at the end; 256: one
+//                group. CH warps share 32 rows of a tile, each with a part of
+//                its keys and of O's columns; they exchange row maxima through
 //                shared memory and a barrier of their own.
 //   last 4       V tile -> f16
-// The softmax is a chain of latencies (TMEM load, maximum, exponentials, TMEM
-// store), so it wants warps: with one warp for whole 128-key rows a tile took
-// a group about 3100 clocks besides its MMAs.
+// S and P have TMEM columns of their own, so that S of tile j + 2 is computed
+// while tile j is exponentiated: the softmax is a chain of latencies (TMEM
+// load, maximum, exponentials, TMEM store), and its own next S is not one of
+// them.
 #pragma once
 
 #include "attn_kv8_rows.cuh"
 
 namespace ca {
 
-template <int HDP_>
+template <int HDP_, int CH_>
 struct TileCfg {
   static constexpr int HDP = HDP_;                       // 64, 128 or 256
-  static constexpr bool ALT = HDP <= 128;
-  static constexpr int BN = ALT ? 128 : 64;              // keys of a tile
-  static constexpr int TG = ALT ? 2 : 1;                 // tile groups
-  static constexpr int SC = BN / 2;                      // keys of a softmax thread's half row
-  static constexpr int kSoftWarps = 8 * TG;
+  static constexpr int CH = CH_;                         // warps that share 32 rows of a tile
+  static constexpr int TG = HDP <= 128 ? 2 : 1;          // tile groups, each with its own O
+  static constexpr int BN = TG == 2 ? 128 : 64;          // keys of a tile
+  // P has TMEM columns of its own (one group), or takes S's place (two: their
+  // two O's leave no room).
+  static constexpr bool PSEP = TG == 1;
+  static constexpr int SC = BN / CH;                     // keys of a softmax thread's part
+  static constexpr int kSoftWarps = 4 * TG * CH;
   static constexpr int kSoftThreads = 32 * kSoftWarps;
   static constexpr int kThreads = 256 + kSoftThreads;
   static constexpr int kConvWarp0 = 4 + kSoftWarps;
-  static constexpr int STK = 3, STV = 2;                 // stages: K, V as held; V as f16 has 2
-  static constexpr int SB = ALT ? 2 : 3;                 // S buffers
+  // Stages of K and V as held (V in f16 has two).
+  static constexpr int STK = 3, STV = 2;
   static constexpr int kChunks = (HDP + 127) / 128;      // 128-byte columns of an e4m3 tile
   static constexpr int kSteps = HDP / 32;                // k-steps of S
   static constexpr int kQTerm = kChunks * 128 * 128;     // one term of Q
@@ -65,19 +68,27 @@ struct TileCfg {
   static constexpr int kBarKE = kBarK + STK;    // [STK] K free
   static constexpr int kBarV8 = kBarKE + STK;   // [STV] V landed
   static constexpr int kBarV8E = kBarV8 + STV;  // [STV] V free
-  static constexpr int kBarV = kBarV8E + STV;   // [2] V in f16
-  static constexpr int kBarVE = kBarV + 2;      // [2] free
-  static constexpr int kBarS = kBarVE + 2;      // [SB]
-  static constexpr int kBarP = kBarS + SB;      // [2] P written (per group)
-  static constexpr int kBarO = kBarP + 2;       // [2] P V done (per O)
+  static constexpr int kBarS = kBarV8E + STV;   // [2] S of an (even, odd) tile
+  static constexpr int kBarSE = kBarS + 2;      // [2] read
+  static constexpr int kBarP = kBarSE + 2;      // [2] P written and V in f16
+  static constexpr int kBarO = kBarP + 2;       // [2] P V done
   static constexpr int kBarF = kBarO + 2;       // every MMA done
   static constexpr int kNumBars = kBarF + 1;
   static constexpr int kOffQs = kOffBar + (kNumBars * 8 + 15) / 16 * 16;  // float [128]
-  static constexpr int kOffXch = kOffQs + 128 * 4;       // float [2 TG][2][128]
-  static constexpr int kOffSc = kOffXch + 2 * TG * 2 * 128 * 4;  // float [warp][2][3][4]
-  static constexpr int kOffMisc = kOffSc + kSoftWarps * 2 * 3 * 4 * 4;
+  static constexpr int kOffXch = kOffQs + 128 * 4;       // float [TG CH][2][128]
+  static constexpr int kOffSc = kOffXch + TG * CH * 2 * 128 * 4;  // float [warp][2][3][NC]
+  static constexpr int NC = SC / 16;                     // 16-key pieces of a part
+  static constexpr int kOffRow = kOffSc + kSoftWarps * 2 * 3 * NC * 4;  // int64 [128]
+  static constexpr int kOffMisc = kOffRow + 128 * 8;
   static constexpr int kSmem = kOffMisc + 64;
-  static constexpr int kOCol = SB * BN;
+  // TMEM: S of two tiles, P, O.
+  static constexpr int kPCol = PSEP ? 2 * BN : 0;        // P of an (even, odd) tile
+  static constexpr int kPStep = PSEP ? 8 : 16;           // columns of 16 keys
+  static constexpr int kOCol = PSEP ? 3 * BN : 2 * BN;
+  // Registers (CH 1, two groups: 512 threads launched with 128 each): two
+  // warpgroups with whole rows of 128 keys at 192, the other two at 64, are
+  // those 4 x 128.
+  static constexpr bool REGS = SC == 128;
   static constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(BN >> 3) << 17) |
                                       (128u >> 4 << 24);  // e4m3 x e4m3, fp32
   static constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) |
@@ -85,7 +96,13 @@ struct TileCfg {
                                       (128u >> 4 << 24);  // f16 x f16 (MN-major), fp32
   static_assert(kOCol + TG * HDP <= 512, "TMEM");
   static_assert(kSmem <= 227 * 1024, "shared memory");
+  static_assert(kSoftWarps * 4096 <= STK * kTile8 + STV * kTile8, "output staging");
 };
+
+#ifndef CA_KV8_POLY
+#define CA_KV8_POLY 0
+#endif
+constexpr int kTilePoly = CA_KV8_POLY;
 
 // D[tmem] (+)= A[smem] x B[smem]^T, kind::f8f6f4 (e4m3 in, fp32 accumulate).
 __device__ __forceinline__ void umma_ss_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
@@ -107,16 +124,12 @@ __device__ __forceinline__ void reg_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// Registers at head_dim <= 128: 768 threads are launched with 80 each; four
-// softmax warpgroups at 96 and the other two at 48 are those 6 x 80.
-constexpr int kTileSoftRegs = 96, kTileOtherRegs = 48;
-
 template <class C>
 __global__ void __launch_bounds__(C::kThreads, 1)
     attn_kv8_tile_kernel(const __grid_constant__ CUtensorMap tm_k,
                          const __grid_constant__ CUtensorMap tm_v, const Kv8AttnParams p) {
   constexpr int BN = C::BN, HDP = C::HDP, SC = C::SC;
-  constexpr bool ALT = C::ALT;
+  constexpr int TG = C::TG, CH = C::CH;
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023u) != 0) {
     if (threadIdx.x == 0) atomicExch(p.err ? p.err : &g_device_error, kErrLayout);
@@ -223,12 +236,11 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   } else if (warp == 3) {
     if (lane == 0) {
       for (int s = 0; s < 2; ++s) {
-        mbar_init(bar(C::kBarV + s), 4);
-        mbar_init(bar(C::kBarVE + s), 1);
-        mbar_init(bar(C::kBarP + s), 8);
+        mbar_init(bar(C::kBarS + s), 1);
+        mbar_init(bar(C::kBarSE + s), 4 * CH);
+        mbar_init(bar(C::kBarP + s), 4 * CH + 4);
         mbar_init(bar(C::kBarO + s), 1);
       }
-      for (int s = 0; s < C::SB; ++s) mbar_init(bar(C::kBarS + s), 1);
       mbar_init(bar(C::kBarF), 1);
       fence_barrier_init();
       fence_proxy_async_smem();
@@ -313,7 +325,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   bool dead = false;
 
   if (warp < 4) {
-    if constexpr (ALT) reg_dec<kTileOtherRegs>();
+    if constexpr (C::REGS) reg_dec<64>();
     if (warp == 0 || warp == 2) {
       // ---------------------------------------------------------- producers
       if (lane == 0) {
@@ -330,71 +342,67 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         for (int u = max(0, n - NS); u < n; ++u)
           mbar_wait(bar(full + u % NS), (u / NS) & 1, d2, p.err);
       }
-    } else if (warp == 1) {
+    } else if (warp == 1 && lane == 0) {
       // ---------------------------------------------------------- MMA issue
-      if (lane == 0) {
-        auto og = [&](int i) -> int { return ALT ? (i & 1) : 0; };
-        auto ouse = [&](int i) -> int { return ALT ? (i >> 1) : i; };
-        auto issue_s = [&](int j) -> bool {
-          const int s = j % C::STK, sb = j % C::SB;
-          if (!mbar_wait(bar(C::kBarK + s), (j / C::STK) & 1, dead, p.err)) return false;
-          // The buffer last held P[j - SB]: P V[j - SB] has read it. (With one
-          // group S[j] is issued after P V[j - 2], whose issue waited for
-          // P V[j - 3].)
-          if (ALT && j >= C::SB &&
-              !mbar_wait(bar(C::kBarO + og(j - C::SB)), ouse(j - C::SB) & 1, dead, p.err))
-            return false;
-          tc_fence_after();
-          const uint32_t kbase = sK + s * C::kTile8;
+      // One thread: an issuing thread is held while its MMAs run, and two (S
+      // from one, P V from another) interleave them, so that both of a pair
+      // end late: a 2 x 4096 canvas took 389 us that way. A descriptor's
+      // address field counts 16-byte units: offsets add.
+      const uint64_t dq = umma_desc_sw128(sQ, 16, 1024), dk0 = umma_desc_sw128(sK, 16, 1024);
+      const uint64_t dv0 = umma_desc_sw128(sV, BN * 128, 1024);
+      auto issue_s = [&](int j) -> bool {
+        const int s = j % C::STK, x = j & 1;
+        if (!mbar_wait(bar(C::kBarK + s), (j / C::STK) & 1, dead, p.err)) return false;
+        // The buffer is free once S[j - 2] was read (or, with P in its place,
+        // once P V[j - 2] is done).
+        if (j >= 2 &&
+            !mbar_wait(bar((C::PSEP ? C::kBarSE : C::kBarO) + x), ((j >> 1) - 1) & 1, dead, p.err))
+          return false;
+        tc_fence_after();
+        const uint64_t dk = dk0 + s * (C::kTile8 >> 4);
 #pragma unroll
-          for (int term = 0; term < 2; ++term)
+        for (int term = 0; term < 2; ++term)
 #pragma unroll
-            for (int kk = 0; kk < C::kSteps; ++kk) {
-              const uint64_t a = umma_desc_sw128(
-                  sQ + term * C::kQTerm + (kk >> 2) * 128 * 128 + (kk & 3) * 32, 16, 1024);
-              const uint64_t bd =
-                  umma_desc_sw128(kbase + (kk >> 2) * BN * 128 + (kk & 3) * 32, 16, 1024);
-              umma_ss_f8(tmem + sb * BN, a, bd, C::kIdescS, term + kk > 0 ? 1u : 0u);
-            }
-          umma_commit(bar(C::kBarS + sb));
-          umma_commit(bar(C::kBarKE + s));
-          return true;
-        };
-        auto issue_pv = [&](int i) -> bool {
-          const int g = og(i), use = ouse(i), s = i & 1;
-          if (!mbar_wait(bar(C::kBarV + s), (i >> 1) & 1, dead, p.err)) return false;
-          if (!mbar_wait(bar(C::kBarP + g), use & 1, dead, p.err)) return false;
-          if (!ALT && i > 0 && !mbar_wait(bar(C::kBarO), (i - 1) & 1, dead, p.err)) return false;
-          tc_fence_after();
-          const uint32_t vbase = sV + s * C::kTile16;
-          const uint32_t pcol = tmem + (i % C::SB) * BN;
-          const uint32_t dst = tmem + C::kOCol + g * HDP;
+          for (int kk = 0; kk < C::kSteps; ++kk)
+            umma_ss_f8(tmem + x * BN,
+                       dq + ((term * C::kQTerm + (kk >> 2) * 128 * 128 + (kk & 3) * 32) >> 4),
+                       dk + (((kk >> 2) * BN * 128 + (kk & 3) * 32) >> 4), C::kIdescS,
+                       term + kk > 0 ? 1u : 0u);
+        umma_commit(bar(C::kBarS + x));
+        return true;
+      };
+      auto issue_pv = [&](int j) -> bool {
+        const int x = j & 1;
+        if (!mbar_wait(bar(C::kBarP + x), (j >> 1) & 1, dead, p.err)) return false;
+        tc_fence_after();
+        const uint64_t dv = dv0 + x * (C::kTile16 >> 4);
+        const uint32_t pcol = tmem + C::kPCol + x * (BN / 16 * C::kPStep);
+        const uint32_t dst = tmem + C::kOCol + (TG == 2 ? x * HDP : 0);
 #pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk) {
-            const uint64_t bd = umma_desc_sw128(vbase + kk * 2048, BN * 128, 1024);
-            umma_ts(dst, pcol + kk * 16, bd, C::kIdescO, use > 0 || kk > 0 ? 1u : 0u);
-          }
-          umma_commit(bar(C::kBarO + g));
-          umma_commit(bar(C::kBarVE + s));
-          return true;
-        };
-        if (n > 0) {
-          bool ok = issue_s(0) && (n < 2 || issue_s(1));
-          for (int j = 0; ok && j < n; ++j) ok = issue_pv(j) && (j + 2 >= n || issue_s(j + 2));
-        }
-        umma_commit(bar(C::kBarF));
-        bool d2 = false;
-        mbar_wait(bar(C::kBarF), 0, d2, p.err);
+        for (int kk = 0; kk < BN / 16; ++kk)
+          umma_ts(dst, pcol + kk * C::kPStep, dv + ((kk * 2048) >> 4), C::kIdescO,
+                  j >= TG || kk > 0 ? 1u : 0u);
+        umma_commit(bar(C::kBarO + x));
+        return true;
+      };
+      bool ok = n > 0 && issue_s(0) && (n < 2 || issue_s(1));
+      for (int j = 0; ok && j < n; ++j) {
+        if (C::PSEP) ok = (j + 2 >= n || issue_s(j + 2)) && issue_pv(j);
+        else ok = issue_pv(j) && (j + 2 >= n || issue_s(j + 2));
       }
+      // Every MMA issued is done before the role ends.
+      umma_commit(bar(C::kBarF));
+      bool d2 = false;
+      mbar_wait(bar(C::kBarF), 0, d2, p.err);
     }
   } else if (warp >= C::kConvWarp0) {
     // ------------------------------------------------------------ V to f16
-    if constexpr (ALT) reg_dec<kTileOtherRegs>();
+    if constexpr (C::REGS) reg_dec<64>();
     const int cw = warp - C::kConvWarp0;
     for (int j = 0; j < n; ++j) {
       const int s8 = j % C::STV, s = j & 1;
       mbar_wait(bar(C::kBarV8 + s8), (j / C::STV) & 1, dead, p.err);
-      if (j >= 2) mbar_wait(bar(C::kBarVE + s), ((j >> 1) - 1) & 1, dead, p.err);
+      if (j >= 2) mbar_wait(bar(C::kBarO + s), ((j >> 1) - 1) & 1, dead, p.err);
       dead = __any_sync(0xffffffffu, dead);
       if (dead) break;
       const uint32_t src = sV8 + s8 * C::kTile8, dst = sV + s * C::kTile16;
@@ -432,22 +440,29 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(bar(C::kBarV + s));
+        mbar_arrive(bar(C::kBarP + s));
         mbar_arrive(bar(C::kBarV8E + s8));
       }
     }
   } else {
     // ------------------------------------------------------------ softmax
-    if constexpr (ALT) reg_inc<kTileSoftRegs>();
-    const int wg = (warp - 4) >> 2;       // warpgroup: tile group, half of the row
-    const int grp = wg >> 1, half = wg & 1;
+    if constexpr (C::REGS) reg_inc<192>();
+    const int wg = (warp - 4) >> 2;       // warpgroup: tile group, part of the row
+    const int grp = wg / CH, part = wg % CH;
     const int wq = warp & 3;
     const int r = wq * 32 + lane;
     const int st = tid - 128;  // softmax thread
     const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
-    const int pair_bar = 2 + grp * 4 + wq;  // the two warps of these rows
+    const int row_bar = 2 + grp * 4 + wq;  // the warps that share these rows
     float* xch = reinterpret_cast<float*>(smem + C::kOffXch);
 
+    // Where a row goes in the output.
+    long long* row_at = reinterpret_cast<long long*>(smem + C::kOffRow);
+    if (wg == 0 && r < rows) {
+      const unsigned rr = static_cast<unsigned>(row0 + r), tok = rr / static_cast<unsigned>(p.G);
+      row_at[r] = (q_beg + static_cast<long long>(tok)) * p.out_row_stride +
+                  (kvh * p.G + static_cast<int>(rr - tok * p.G)) * static_cast<long long>(hd);
+    }
     int lo = 0, hi = INT_MAX;  // rows past the end see everything: they slow nothing down
     if (r < rows) interval(r, lo, hi);
     const float qs = sQs[r];
@@ -460,54 +475,64 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     const int shift = 31 - __clz(p.c.T);
     const float* ksc = p.c.k_scale + static_cast<long long>(b) * p.c.n_blocks * p.c.Hkv + kvh;
     const float* vsc = p.c.v_scale + static_cast<long long>(b) * p.c.n_blocks * p.c.Hkv + kvh;
-    // Lane c < SC / 16 takes the scales of this half's keys 16 c .. 16 c + 15,
+    // Lane c < SC / 16 takes the scales of this part's keys 16 c .. 16 c + 15,
     // loaded a tile ahead; they reach the other lanes through shared memory.
-    constexpr int NC = SC / 16;
+    constexpr int NC = C::NC;
     float nk = 0.f, nv = 1.f;
     auto scales = [&](int j) {
       if (j < n) {
-        const int key = (kt0 + j) * BN + half * SC + (lane % NC) * 16;
+        const int key = (kt0 + j) * BN + part * SC + (lane % NC) * 16;
         const long long at = static_cast<long long>(min(key >> shift, p.c.n_blocks - 1)) * p.c.Hkv;
         nk = __ldg(ksc + at);
         nv = __ldg(vsc + at);
       }
     };
-    float* my_sc = reinterpret_cast<float*>(smem + C::kOffSc) + (warp - 4) * 24;
+    float* my_sc = reinterpret_cast<float*>(smem + C::kOffSc) + (warp - 4) * 6 * NC;
     float m = -INFINITY, l = 0.f;
     int used = 0;
     scales(grp);
-    for (int j = grp; j < n; j += C::TG) {
-      const int sb = j % C::SB;
-      float* tab = my_sc + (used & 1) * 12;  // [k scale, L, 2^-L][4]
+    for (int j = grp; j < n; j += TG) {
+      const int x2 = j & 1, use = j >> 1;
+      float* tab = my_sc + (used & 1) * 3 * NC;  // [k scale, L, 2^-L][NC]
       if (lane < NC) {
         const float L = kv8_log2(nv);
         tab[lane] = nk;
-        tab[4 + lane] = L;
-        tab[8 + lane] = ex2_approx(-L);
+        tab[NC + lane] = L;
+        tab[2 * NC + lane] = ex2_approx(-L);
       }
-      scales(j + C::TG);
+      scales(j + TG);
       __syncwarp();
-      mbar_wait(bar(C::kBarS + sb), (j / C::SB) & 1, dead, p.err);
+      mbar_wait(bar(C::kBarS + x2), use & 1, dead, p.err);
       dead = __any_sync(0xffffffffu, dead);
-      // A pair ends together: neither warp waits for the other below.
+      if (st == grp * 128 * CH) mbar_arrive(bar(C::kBarKE + j % C::STK));  // K[j] was read
+      if (CH == 1 && dead) break;
+      // (The warps of a row end together, so that none waits for another.)
       tc_fence_after();
-      const uint32_t s_addr = tmem + lane_off + sb * BN + half * SC;
-      const int key0 = (kt0 + j) * BN + half * SC;
+      const uint32_t s_addr = tmem + lane_off + x2 * BN + part * SC;
+      const int key0 = (kt0 + j) * BN + part * SC;
       const bool full = key0 >= f_lo && key0 + SC <= f_hi;
-      // Column i of the half is visible iff (unsigned)(i - v0) < v1.
+      // Column i of the part is visible iff (unsigned)(i - v0) < v1.
       const int v0 = lo - key0;
       const uint32_t v1 = static_cast<uint32_t>(hi) - static_cast<uint32_t>(lo);
       float sr[SC];
+      if constexpr (SC >= 32) {
 #pragma unroll
-      for (int cb = 0; cb < SC / 32; ++cb)
-        tmem_ld32(s_addr + cb * 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[cb * 32]));
+        for (int cb = 0; cb < SC / 32; ++cb)
+          tmem_ld32(s_addr + cb * 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[cb * 32]));
+      } else {
+        tmem_ld16(s_addr, *reinterpret_cast<uint32_t(*)[16]>(&sr[0]));
+      }
       float a16[NC], L16[NC];
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         a16[c] = row_c * tab[c];
-        L16[c] = tab[4 + c];
+        L16[c] = tab[NC + c];
       }
       tmem_wait_ld();
+      if constexpr (C::PSEP) {
+        tc_fence_before();
+        if (lane == 0) mbar_arrive(bar(C::kBarSE + x2));
+      }
       if (!full) {
 #pragma unroll
         for (int i = 0; i < SC; ++i)
@@ -540,15 +565,20 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         }
         cmax = fmaxf(cmax, m0);
       }
-      // The other half's maximum (and whether its warp gave up).
-      {
-        float* mine = xch + ((wg * 2 + (used & 1)) * 128) + r;
-        *mine = dead ? __int_as_float(0x7fc00000) : cmax;  // a maximum is never NaN
-        named_bar_sync(pair_bar, 64);
-        const float other = xch[((wg ^ 1) * 2 + (used & 1)) * 128 + r];
-        dead = __any_sync(0xffffffffu, dead || other != other);
+      if constexpr (CH > 1) {
+        // The other parts' maxima (and whether a warp gave up: a NaN, which a
+        // maximum never is).
+        xch[(wg * 2 + (used & 1)) * 128 + r] = dead ? __int_as_float(0x7fc00000) : cmax;
+        named_bar_sync(row_bar, 32 * CH);
+#pragma unroll
+        for (int k = 1; k < CH; ++k) {
+          const int o = grp * CH + (part + k) % CH;
+          const float other = xch[(o * 2 + (used & 1)) * 128 + r];
+          dead |= other != other;
+          cmax = fmaxf(cmax, other);
+        }
+        dead = __any_sync(0xffffffffu, dead);
         if (dead) break;
-        cmax = fmaxf(cmax, other);
       }
       const bool resc = cmax > m + kKv8Lazy;
       float corr = 1.f;
@@ -558,6 +588,15 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       }
       const float mu = m == -INFINITY ? 0.f : m - kKv8Shift;
       const bool poly = capped && __all_sync(0xffffffffu, umax <= kTanhPolyMax);
+      // P of tile j - 2 must have been read before P[j] takes its place. (P in
+      // S's place: S[j] waited for that, and this group's O is at rest.)
+      if (C::PSEP && j >= 2) {
+        mbar_wait(bar(C::kBarO + x2), (use - 1) & 1, dead, p.err);
+        dead = __any_sync(0xffffffffu, dead);
+        tc_fence_after();
+      }
+      const uint32_t p_addr =
+          tmem + lane_off + C::kPCol + x2 * (BN / 16 * C::kPStep) + part * (SC / 16 * C::kPStep);
       float sum = 0.f;
       auto pass2 = [&](auto cap_c) {
         constexpr int CAP = decltype(cap_c)::value;  // 0 none, 1 tanh, 2 its polynomial
@@ -585,30 +624,36 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 y.y = x1 == -INFINITY ? x1 : y.y;
               }
             }
-            const float p0 = ex2_approx(y.x), p1 = ex2_approx(y.y);
+            float p0, p1;
+            if (CAP == 0 && kTilePoly > 0 && full && q % (kTilePoly + 1) == kTilePoly) {
+              const float2 e = ex2_poly3x2(y.x, y.y);
+              p0 = e.x;
+              p1 = e.y;
+            } else {
+              p0 = ex2_approx(y.x);
+              p1 = ex2_approx(y.y);
+            }
             s2 = __fadd2_rn(s2, make_float2(p0, p1));
             w[q] = pack_f16(p0, p1);
           }
-          tmem_st8(s_addr + c * 16, w);
-          sum = fmaf(s2.x + s2.y, tab[8 + c], sum);
+          tmem_st8(p_addr + c * C::kPStep, w);
+          sum = fmaf(s2.x + s2.y, tab[2 * NC + c], sum);
         }
       };
       if (!capped) pass2(std::integral_constant<int, 0>{});
       else if (!poly) pass2(std::integral_constant<int, 1>{});
       else pass2(std::integral_constant<int, 2>{});
       l = fmaf(l, corr, sum);
-      // One group: the previous P V may still add to O, and its end shows
-      // that the MMA warp has taken P[j - 1].
-      if (!ALT && used > 0) {
-        mbar_wait(bar(C::kBarO), (j - 1) & 1, dead, p.err);
-        dead = __any_sync(0xffffffffu, dead);
-        tc_fence_after();
-      }
-      if (used > 0 && __any_sync(0xffffffffu, resc)) {
+      if (j >= TG && __any_sync(0xffffffffu, resc)) {
+        if (TG == 1) {  // the previous P V may still add to O
+          mbar_wait(bar(C::kBarO + (x2 ^ 1)), ((j - 1) >> 1) & 1, dead, p.err);
+          dead = __any_sync(0xffffffffu, dead);
+          tc_fence_after();
+        }
 #pragma unroll 1
-        for (int c = 0; c < HDP / 64; ++c) {
+        for (int c = 0; c < HDP / CH / 32; ++c) {
           uint32_t o[32];
-          const uint32_t ta = tmem + lane_off + C::kOCol + grp * HDP + half * (HDP / 2) + c * 32;
+          const uint32_t ta = tmem + lane_off + C::kOCol + grp * HDP + part * (HDP / CH) + c * 32;
           tmem_ld32(ta, o);
           tmem_wait_ld();
 #pragma unroll
@@ -619,7 +664,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(C::kBarP + grp));
+      if (lane == 0) mbar_arrive(bar(C::kBarP + x2));
       ++used;
     }
 
@@ -629,24 +674,29 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       dead = __any_sync(0xffffffffu, dead);
       tc_fence_after();
     }
-    // Maxima and sums of all halves: [warpgroup][l, m][128]. A pair has one
-    // maximum.
+    // Maxima and sums of all parts: [warpgroup][l, m][128]. The parts of a
+    // group have one maximum.
     named_bar_sync(1, C::kSoftThreads);
     xch[wg * 256 + r] = l;
     xch[wg * 256 + 128 + r] = m;
     named_bar_sync(1, C::kSoftThreads);
-    float s_me = 1.f, s_ot = 0.f, mt = m;
-    float lt = xch[(grp * 2) * 256 + r] + xch[(grp * 2 + 1) * 256 + r];
-    if constexpr (ALT) {
-      const float l_ot = xch[((grp ^ 1) * 2) * 256 + r] + xch[((grp ^ 1) * 2 + 1) * 256 + r];
-      const float m_ot = xch[((grp ^ 1) * 2) * 256 + 128 + r];
+    auto group_sum = [&](int k) -> float {
+      float y = 0.f;
+#pragma unroll
+      for (int h = 0; h < CH; ++h) y += xch[(k * CH + h) * 256 + r];
+      return y;
+    };
+    float s_me = 1.f, s_ot = 0.f, mt = m, lt = group_sum(grp);
+    if constexpr (TG == 2) {
+      const float l_ot = group_sum(grp ^ 1);
+      const float m_ot = xch[((grp ^ 1) * CH) * 256 + 128 + r];
       mt = fmaxf(m, m_ot);
       const float ref = mt == -INFINITY ? 0.f : mt;
       s_me = ex2_approx(m - ref);
       s_ot = ex2_approx(m_ot - ref);
       lt = grp == 0 ? fmaf(lt, s_me, l_ot * s_ot) : fmaf(l_ot, s_ot, lt * s_me);
     }
-    const int n_me = ALT ? (grp == 0 ? (n + 1) / 2 : n / 2) : n;
+    const int n_me = TG == 2 ? (grp == 0 ? (n + 1) / 2 : n / 2) : n;
     const int n_ot = n - n_me;
     const bool final_out = p.splits == 1;
     const float inv = final_out ? __fdiv_rn(1.f, lt) : 1.f;
@@ -656,7 +706,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     // row, so that global stores are whole 64- or 128-byte pieces.
     const bool f32 = !final_out || p.out_f32;
     const uint32_t stage = sK + (warp - 4) * 4096;
-    constexpr int WC = HDP / (2 * C::TG);  // columns a warp writes
+    constexpr int WC = HDP / (CH * TG);  // columns a warp writes
     constexpr int PC = WC < 32 ? WC : 32;  // ... at a time
 #pragma unroll 1
     for (int c = 0; c < WC / PC; ++c) {
@@ -671,7 +721,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = u2f(o[i]) * s_me;
       }
-      if (ALT && n_ot > 0 && !dead) {
+      if (TG == 2 && n_ot > 0 && !dead) {
         tmem_ld32(tmem + lane_off + C::kOCol + (grp ^ 1) * HDP + col0, o);
         tmem_wait_ld();
 #pragma unroll
@@ -680,7 +730,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = dead ? __int_as_float(0x7fc00000) : v[i] * inv;
       // Units of 16 bytes: 4 fp32 or 8 bf16.
-      const int units = f32 ? PC / 4 : PC / 8;
+      const int units = f32 ? PC / 4 : PC / 8, sh = 31 - __clz(units);
       const uint32_t my_row = stage + lane * (units * 16);
 #pragma unroll
       for (int u = 0; u < PC / 4; ++u) {
@@ -696,22 +746,17 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       __syncwarp();
 #pragma unroll 1
       for (int i = lane; i < 32 * units; i += 32) {
-        const int wr = i / units, u = i - wr * units;
+        const int wr = i >> sh, u = i & (units - 1);
         const int gr = wq * 32 + wr, col = col0 + u * (f32 ? 4 : 8);
         if (gr < rows && col < hd) {
           uint32_t w[4];
           asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                        : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
                        : "r"(stage + wr * (units * 16) + ((u ^ (wr & (units - 1))) << 4)));
-          const unsigned rr = static_cast<unsigned>(row0 + gr);
-          const unsigned tok = rr / static_cast<unsigned>(p.G);
-          const long long at = (q_beg + static_cast<long long>(tok)) * p.out_row_stride +
-                               (kvh * p.G + static_cast<int>(rr - tok * p.G)) *
-                                   static_cast<long long>(hd) + col;
           char* d = !final_out
                         ? reinterpret_cast<char*>(
                               p.part_o + ((cell * p.splits + split) * 128 + gr) * hd + col)
-                        : static_cast<char*>(p.out) + at * (f32 ? 4 : 2);
+                        : static_cast<char*>(p.out) + (row_at[gr] + col) * (f32 ? 4 : 2);
           *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
@@ -755,9 +800,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             }
           }
           const float ij = __fdiv_rn(1.f, lj);
-          const long long gr = row0 + jr;
-          const long long d = (q_beg + gr / p.G) * p.out_row_stride +
-                              (kvh * p.G + gr % p.G) * static_cast<long long>(hd) + e;
+          const long long d = row_at[jr] + e;
           if (p.out_f32)
             *reinterpret_cast<float4*>(static_cast<float*>(p.out) + d) =
                 make_float4(oj.x * ij, oj.y * ij, oj.z * ij, oj.w * ij);

@@ -401,52 +401,87 @@ struct Kv8LoadParams {
   int* err;
 };
 
-// Rows of the cache as bf16 or fp32. One thread turns 16 values: one 16-byte
-// load, two (four) 16-byte stores. Bound by HBM: 1 byte read and 2 (4)
-// written for each value.
+// Eight 32-bit words to a 32-byte aligned address in one store.
+__device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]),
+               "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+// Rows of the cache as bf16 or fp32. A thread has 16 values of a row (one
+// 16-byte load, one 32-byte store in bf16) and keeps its column from row to
+// row, so that indices cost it next to nothing; U rows are in flight. Bound
+// by HBM: 1 byte read and 2 (4) written for each value.
+template <int U>
 __global__ void __launch_bounds__(256) kv8_load_kernel(const Kv8LoadParams p) {
-  const unsigned upr = p.c.Hkv * p.c.hd / 16;  // 16-value units of a row
+  const int upr = p.c.Hkv * p.c.hd / 16;  // 16-value units of a row
   const uint8_t* src = blockIdx.y ? p.c.v : p.c.k;
   const float* scales = blockIdx.y ? p.c.v_scale : p.c.k_scale;
   void* dst = blockIdx.y ? p.v_out : p.k_out;
   if (!dst) return;
   const int b = blockIdx.z;
-  const unsigned units = p.n_pos * upr;
-  for (unsigned u = blockIdx.x * blockDim.x + threadIdx.x; u < units; u += gridDim.x * blockDim.x) {
-    const unsigned i = u / upr;
-    const int e = static_cast<int>(u - i * upr) * 16;
-    const long long row = static_cast<long long>(b) * p.n_pos + i;
-    const int pos = p.pos ? __ldg(p.pos + row) : static_cast<int>(i);
-    if (pos < 0 || pos >= p.c.n_total) {
-      if (p.err) atomicExch(p.err, kErrInvalidRow);
-      continue;
-    }
-    const float s = __ldg(scales + (static_cast<long long>(b) * p.c.n_blocks + pos / p.c.T) * p.c.Hkv +
-                          e / p.c.hd);
-    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(
-        src + (static_cast<long long>(b) * p.c.n_total + pos) * p.c.row_stride + e));
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    float x[16];
+  const int shift = 31 - __clz(p.c.T);
+  const int rows = upr < 256 ? 256 / upr : 1;  // rows a CTA has at a time
+  const int mine = upr < 256 ? static_cast<int>(threadIdx.x) / upr : 0;
+  if (mine >= rows) return;
+  const int* pos = p.pos ? p.pos + static_cast<long long>(b) * p.n_pos : nullptr;
+  const bool v8 = (reinterpret_cast<uintptr_t>(dst) & 31u) == 0;
+  const int step = rows;  // a CTA's U x rows rows lie side by side
+  for (int un = upr < 256 ? static_cast<int>(threadIdx.x) - mine * upr : threadIdx.x; un < upr;
+       un += 256) {
+    const uint8_t* from = src + static_cast<long long>(b) * p.c.n_total * p.c.row_stride + un * 16;
+    const float* sc = scales + static_cast<long long>(b) * p.c.n_blocks * p.c.Hkv + un * 16 / p.c.hd;
+    const long long out0 = static_cast<long long>(b) * p.n_pos * upr + un;
+    for (long long at = static_cast<long long>(blockIdx.x) * U * rows + mine; at < p.n_pos;
+         at += static_cast<long long>(gridDim.x) * U * rows) {
+      const int i0 = static_cast<int>(at);
+      uint4 raw[U];
+      float s[U];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float y[4];
-      e4m3x4_to_f32(w[k], y);
+      for (int k = 0; k < U; ++k) {
+        const int i = i0 + k * step;
+        s[k] = -1.f;
+        if (i < p.n_pos && i >= i0) {
+          const int q = pos ? __ldg(pos + i) : i;
+          if (q >= 0 && q < p.c.n_total) {
+            raw[k] = __ldg(reinterpret_cast<const uint4*>(from + q * p.c.row_stride));
+            s[k] = __ldg(sc + (q >> shift) * p.c.Hkv);
+          } else if (p.err) {
+            atomicExch(p.err, kErrInvalidRow);
+          }
+        }
+      }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[4 * k + j] = y[j] * s;
-    }
-    const long long o = row * p.c.Hkv * p.c.hd + e;
-    if (p.out_f32) {
-      float4* d = reinterpret_cast<float4*>(static_cast<float*>(dst) + o);
+      for (int k = 0; k < U; ++k) {
+        if (s[k] == -1.f) continue;
+        const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+        float x[16];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        d[k] = make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
-    } else {
-      uint4* d = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(dst) + o);
+        for (int y = 0; y < 4; ++y) {
+          float v[4];
+          e4m3x4_to_f32(w[y], v);
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-        d[k] = make_uint4(pack_bf16(x[8 * k], x[8 * k + 1]), pack_bf16(x[8 * k + 2], x[8 * k + 3]),
-                          pack_bf16(x[8 * k + 4], x[8 * k + 5]),
-                          pack_bf16(x[8 * k + 6], x[8 * k + 7]));
+          for (int j = 0; j < 4; ++j) x[4 * y + j] = v[j] * s[k];
+        }
+        const long long o = (out0 + static_cast<long long>(i0 + k * step) * upr) * 16;
+        if (p.out_f32) {
+          float4* d = reinterpret_cast<float4*>(static_cast<float*>(dst) + o);
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            d[y] = make_float4(x[4 * y], x[4 * y + 1], x[4 * y + 2], x[4 * y + 3]);
+        } else {
+          uint32_t h[8];
+#pragma unroll
+          for (int y = 0; y < 8; ++y) h[y] = pack_bf16(x[2 * y], x[2 * y + 1]);
+          __nv_bfloat16* d = static_cast<__nv_bfloat16*>(dst) + o;
+          if (v8) {
+            st_global_v8(d, h);
+          } else {
+            reinterpret_cast<uint4*>(d)[0] = make_uint4(h[0], h[1], h[2], h[3]);
+            reinterpret_cast<uint4*>(d)[1] = make_uint4(h[4], h[5], h[6], h[7]);
+          }
+        }
+      }
     }
   }
 }

@@ -61,9 +61,9 @@ int kv8_store_impl(const ca_kv8_store_args* a, cudaStream_t st) {
     return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
   }
   // Entries of the active list a job looks through: one where that leaves
-  // every warp slot of the GPU at most one job, 32 (a lane each) at most.
+  // half the GPU's warp slots at most one job each, 32 (a lane each) at most.
   // From 8 on, rows are many and mostly side by side: four warps a job.
-  const int64_t slots = static_cast<int64_t>(kSms) * 64;
+  const int64_t slots = static_cast<int64_t>(kSms) * 32;
   const int64_t one = p.rows * 2 * p.c.Hkv;
   p.rows_per_job = static_cast<int>(std::min<int64_t>(32, (one + slots - 1) / slots));
   const bool many = p.rows_per_job >= 8;
@@ -88,17 +88,24 @@ int kv8_load_impl(const ca_kv8_load_args* a, cudaStream_t st) {
   if ((a->k_out && !aligned16(a->k_out)) || (a->v_out && !aligned16(a->v_out)))
     return CA_ERR_INVALID;
   if (a->n_pos == 0 || p.c.batch == 0) return CA_OK;
-  const int64_t units = static_cast<int64_t>(a->n_pos) * (static_cast<int64_t>(p.c.Hkv) * p.c.hd / 16);
-  if (p.c.batch > 65535 || units > INT_MAX) return CA_ERR_UNSUPPORTED;
+  if (p.c.batch > 65535) return CA_ERR_UNSUPPORTED;
   p.k_out = a->k_out;
   p.v_out = a->v_out;
   p.out_f32 = a->out_f32 ? 1 : 0;
   p.pos = a->pos;
   p.n_pos = a->n_pos;
   p.err = a->status;
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((units + 255) / 256, kSms * 32)), 2,
-                  p.c.batch);
-  kv8_load_kernel<<<grid, 256, 0, st>>>(p);
+  // Four rows in flight where that still gives each SM its eight CTAs.
+  const int upr = p.c.Hkv * p.c.hd / 16;
+  const int rows = upr < 256 ? 256 / upr : 1;
+  const int64_t pieces = (static_cast<int64_t>(a->n_pos) + rows - 1) / rows;
+  const int64_t tensors = 2ll * p.c.batch;
+  const bool many = pieces * tensors >= 4 * 8 * kSms;
+  const int64_t blocks =
+      many ? std::min<int64_t>((pieces + 3) / 4, std::max<int64_t>(1, 8 * kSms / tensors)) : pieces;
+  const dim3 grid(static_cast<unsigned>(blocks), 2, p.c.batch);
+  if (many) kv8_load_kernel<4><<<grid, 256, 0, st>>>(p);
+  else kv8_load_kernel<1><<<grid, 256, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
 }
 
@@ -186,9 +193,14 @@ int launch_rows(const Kv8AttnParams& p, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
 }
 
-template <int HDP>
+#ifndef CA_KV8_CH
+#define CA_KV8_CH 1
+#endif
+#ifndef CA_KV8_CH256
+#define CA_KV8_CH256 2
+#endif
+template <class C>
 int launch_tile(const Kv8AttnParams& p, cudaStream_t st) {
-  using C = TileCfg<HDP>;
   static bool attr_done[kMaxDevices] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return CA_ERR_CUDA;
@@ -253,9 +265,9 @@ int attn_kv8_impl(const ca_attn_kv8_args* a, cudaStream_t st) {
     p.part_o = p.part_ml + cells * pl.splits * 2 * pl.nr;
   }
   if (pl.nr == 128) {
-    if (hd <= 64) return launch_tile<64>(p, st);
-    if (hd <= 128) return launch_tile<128>(p, st);
-    return launch_tile<256>(p, st);
+    if (hd <= 64) return launch_tile<TileCfg<64, CA_KV8_CH>>(p, st);
+    if (hd <= 128) return launch_tile<TileCfg<128, CA_KV8_CH>>(p, st);
+    return launch_tile<TileCfg<256, CA_KV8_CH256>>(p, st);
   }
   if (pl.nr == 16)
     return hd <= 64 ? launch_rows<RowsCfg<64, 16>>(p, st) : launch_rows<RowsCfg<128, 16>>(p, st);
