@@ -171,7 +171,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
 
   // Warps 0, 2 and 3 find the keys: the hull of what the rows see, what
   // every row sees, and this CTA's tiles kt0 .. kt0 + n - 1. The producers
-  // set up their own barriers and start at once, while warps 4-11 split Q.
+  // set up their own barriers and ask for their first tiles at once, while
+  // warps 4-11 split Q.
   int k_lo = 0, k_hi = 0, f_lo = 0, f_hi = 0, kt0 = 0, n = 0;
   auto find_keys = [&]() {
     k_lo = 0;
@@ -219,8 +220,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       fence_proxy_async_smem();
     }
     find_keys();
-    if (lane == 0)
-      for (int u = 0; u < min(n, C::STK); ++u) load_tile(&tm_k, sK, C::kBarK, u, u);
+    if (lane == 0 && n > 0) load_tile(&tm_k, sK, C::kBarK, 0, 0);
   } else if (warp == 2) {
     if (lane == 0) {
       for (int s = 0; s < C::STV; ++s) {
@@ -231,8 +231,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       fence_proxy_async_smem();
     }
     find_keys();
-    if (lane == 0)
-      for (int u = 0; u < min(n, C::STV); ++u) load_tile(&tm_v, sV8, C::kBarV8, u, u);
+    if (lane == 0 && n > 0) load_tile(&tm_v, sV8, C::kBarV8, 0, 0);
   } else if (warp == 3) {
     if (lane == 0) {
       for (int s = 0; s < 2; ++s) {
@@ -260,7 +259,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   } else if (warp < 12) {
     // Q into its two terms: a lane takes 16 values, HDP / 16 lanes a row.
     constexpr int LPR = HDP / 16, RPW = 32 / LPR, NP = 128 / (8 * RPW);
-    constexpr int NB = NP < 4 ? NP : 4;  // rows a lane has in flight
+    constexpr int NB = NP < 8 ? NP : 8;  // rows a lane has in flight
     const int un = lane % LPR, e = un * 16;
 #pragma unroll 1
     for (int p0 = 0; p0 < NP; p0 += NB) {
@@ -333,9 +332,11 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         const int full = is_k ? C::kBarK : C::kBarV8;
         const int empty = is_k ? C::kBarKE : C::kBarV8E;
         const int NS = is_k ? C::STK : C::STV;
-        for (int u = NS; u < n; ++u) {
+        // The first tiles were asked for before Q; the rest of the rings only
+        // now, so as not to stand in Q's way.
+        for (int u = 1; u < n; ++u) {
           const int s = u % NS;
-          if (!mbar_wait(bar(empty + s), ((u / NS) - 1) & 1, dead, p.err)) break;
+          if (u >= NS && !mbar_wait(bar(empty + s), ((u / NS) - 1) & 1, dead, p.err)) break;
           load_tile(is_k ? &tm_k : &tm_v, is_k ? sK : sV8, full, u, s);
         }
         bool d2 = false;  // leave no copy in flight
@@ -399,6 +400,14 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     // ------------------------------------------------------------ V to f16
     if constexpr (C::REGS) reg_dec<64>();
     const int cw = warp - C::kConvWarp0;
+    constexpr int UPR = HDP == 64 ? 4 : 8;  // units of a row within a 128-byte column
+    constexpr int RPW = 32 / UPR;           // rows a warp covers at once
+    static_assert((4 * RPW) % 8 == 0, "one swizzle a lane");
+    const int u = lane % UPR, r0 = cw * RPW + lane / UPR;
+    const bool swap = UPR == 8 && u >= 4;
+    const uint32_t from = r0 * 128 + ((u ^ (r0 & 7)) << 4);
+    const uint32_t to0 = (u >> 2) * BN * 128 + r0 * 128 + (((2 * (u & 3)) ^ (r0 & 7)) << 4);
+    const uint32_t to1 = (u >> 2) * BN * 128 + r0 * 128 + (((2 * (u & 3) + 1) ^ (r0 & 7)) << 4);
     for (int j = 0; j < n; ++j) {
       const int s8 = j % C::STV, s = j & 1;
       mbar_wait(bar(C::kBarV8 + s8), (j / C::STV) & 1, dead, p.err);
@@ -410,33 +419,37 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       // A row's 16-byte unit u (16 values) becomes two units of its atom.
       // Eight lanes take a row's units; those of the upper half write their
       // second unit first, so that each store of eight lanes covers all banks.
-      constexpr int UPR = HDP == 64 ? 4 : 8;  // units of a row within a 128-byte column
-      constexpr int RPW = 32 / UPR;           // rows a warp covers at once
-      const int u = lane % UPR;
+      // A lane's rows are 4 RPW apart, so its swizzle is the same in all.
+      auto turn = [&](auto edge_c) {
+        constexpr bool EDGE = decltype(edge_c)::value;
 #pragma unroll
-      for (int c = 0; c < C::kChunks; ++c) {
-#pragma unroll 4
-        for (int r0 = cw * RPW; r0 < BN; r0 += 4 * RPW) {
-          const int r = r0 + lane / UPR;
-          uint32_t w[4], o[8];
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                       : "r"(src + c * BN * 128 + r * 128 + ((u ^ (r & 7)) << 4)));
-          // Keys that no row sees are zeros: what lies there is not data.
-          if (key0 + r < k_lo || key0 + r >= k_hi) w[0] = w[1] = w[2] = w[3] = 0u;
+        for (int c = 0; c < C::kChunks; ++c) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) e4m3x4_to_f16(w[i], o[2 * i], o[2 * i + 1]);
-          const uint32_t row = dst + (c * 2 + (u >> 2)) * BN * 128 + r * 128;
-          const int d = 2 * (u & 3), first = UPR == 8 ? u >> 2 : 0;
-          if (first == 0) {
-            st_shared_v4(row + ((d ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
-            st_shared_v4(row + (((d + 1) ^ (r & 7)) << 4), o[4], o[5], o[6], o[7]);
-          } else {
-            st_shared_v4(row + (((d + 1) ^ (r & 7)) << 4), o[4], o[5], o[6], o[7]);
-            st_shared_v4(row + ((d ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
+          for (int i = 0; i < BN / (4 * RPW); ++i) {
+            uint32_t w[4], o[8];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(src + from + c * BN * 128 + i * 4 * RPW * 128));
+            if (EDGE) {
+              // Keys that no row sees are zeros: what lies there is not data.
+              const int key = key0 + r0 + i * 4 * RPW;
+              if (key < k_lo || key >= k_hi) w[0] = w[1] = w[2] = w[3] = 0u;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) e4m3x4_to_f16(w[k], o[2 * k], o[2 * k + 1]);
+            const uint32_t at = dst + c * 2 * BN * 128 + i * 4 * RPW * 128;
+            if (swap) {
+              st_shared_v4(at + to1, o[4], o[5], o[6], o[7]);
+              st_shared_v4(at + to0, o[0], o[1], o[2], o[3]);
+            } else {
+              st_shared_v4(at + to0, o[0], o[1], o[2], o[3]);
+              st_shared_v4(at + to1, o[4], o[5], o[6], o[7]);
+            }
           }
         }
-      }
+      };
+      if (key0 < k_lo || key0 + BN > k_hi) turn(std::true_type{});
+      else turn(std::false_type{});
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -538,7 +551,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         for (int i = 0; i < SC; ++i)
           sr[i] = static_cast<uint32_t>(i - v0) < v1 ? sr[i] : -INFINITY;
       }
-      float cmax = -INFINITY, umax = 0.f;
+      float cmax = -INFINITY;
+      float m16[NC];  // each piece's largest score
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         const float* x = &sr[c * 16];
@@ -548,22 +562,39 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         m0 = fmax3(m0, x[10], x[11]);
         m1 = fmax3(m1, x[12], x[13]);
         m0 = fmax3(m0, x[14], x[15]);
-        m0 = fmaxf(m0, m1);
-        if (capped) {
-          // The largest magnitude: of the visible scores' two ends.
-          float n0 = INFINITY, n1 = INFINITY;
+        m16[c] = fmaxf(m0, m1);
+      }
+      bool poly = false;
+      if (capped) {
+        // Whether every argument of tanh is in the polynomial's range: the
+        // largest magnitude (masked scores, -inf, count as 0).
+        float umax = 0.f;
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            n0 = fminf(n0, x[i] == -INFINITY ? INFINITY : x[i]);
-            n1 = fminf(n1, x[i + 1] == -INFINITY ? INFINITY : x[i + 1]);
+        for (int c = 0; c < NC; ++c) {
+          const float* x = &sr[c * 16];
+          float u0 = 0.f, u1 = 0.f;
+          if (full) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+              u0 = fmax3(u0, fabsf(x[i]), fabsf(x[i + 1]));
+              u1 = fmax3(u1, fabsf(x[i + 2]), fabsf(x[i + 3]));
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) u0 = fmaxf(u0, x[i] == -INFINITY ? 0.f : fabsf(x[i]));
           }
-          n0 = fminf(n0, n1);
-          if (m0 != -INFINITY) umax = fmax3(umax, fabsf(m0) * a16[c], fabsf(n0) * a16[c]);
-          m0 = m0 == -INFINITY ? m0 : fmaf(cap_l2, tanh_via_exp2(m0 * a16[c]), L16[c]);
-        } else {
-          m0 = fmaf(m0, a16[c], L16[c]);
+          umax = fmaxf(umax, fmaxf(u0, u1) * a16[c]);
         }
-        cmax = fmaxf(cmax, m0);
+        poly = __all_sync(0xffffffffu, umax <= kTanhPolyMax);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const float u = m16[c] * a16[c];
+          const float t = poly ? tanh_poly(u) : tanh_via_exp2(u);
+          cmax = fmaxf(cmax, m16[c] == -INFINITY ? m16[c] : fmaf(cap_l2, t, L16[c]));
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) cmax = fmaxf(cmax, fmaf(m16[c], a16[c], L16[c]));
       }
       if constexpr (CH > 1) {
         // The other parts' maxima (and whether a warp gave up: a NaN, which a
@@ -587,7 +618,6 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         m = cmax;
       }
       const float mu = m == -INFINITY ? 0.f : m - kKv8Shift;
-      const bool poly = capped && __all_sync(0xffffffffu, umax <= kTanhPolyMax);
       // P of tile j - 2 must have been read before P[j] takes its place. (P in
       // S's place: S[j] waited for that, and this group's O is at rest.)
       if (C::PSEP && j >= 2) {
@@ -598,51 +628,77 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       const uint32_t p_addr =
           tmem + lane_off + C::kPCol + x2 * (BN / 16 * C::kPStep) + part * (SC / 16 * C::kPStep);
       float sum = 0.f;
-      auto pass2 = [&](auto cap_c) {
+      auto pass2 = [&](auto cap_c, auto full_c) {
         constexpr int CAP = decltype(cap_c)::value;  // 0 none, 1 tanh, 2 its polynomial
+        constexpr bool FULL = decltype(full_c)::value;
+        // Two pieces of 16 keys at a time, operation by operation: the chain
+        // of one element is long, so many are kept in flight.
+        constexpr int PP = NC < 2 ? 1 : 2;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const float off = L16[c] - mu;
-          uint32_t w[8];
-          float2 s2 = make_float2(0.f, 0.f);
+        for (int c0 = 0; c0 < NC; c0 += PP) {
+          float2 y[PP][8];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const float x0 = sr[c * 16 + 2 * q], x1 = sr[c * 16 + 2 * q + 1];
-            float2 y;
-            if constexpr (CAP == 0) {
-              y = __ffma2_rn(make_float2(x0, x1), make_float2(a16[c], a16[c]),
-                             make_float2(off, off));
-            } else if constexpr (CAP == 1) {
-              y.x = x0 == -INFINITY ? x0 : fmaf(cap_l2, tanh_via_exp2(x0 * a16[c]), off);
-              y.y = x1 == -INFINITY ? x1 : fmaf(cap_l2, tanh_via_exp2(x1 * a16[c]), off);
-            } else {
-              const float2 t = tanh_poly2(__fmul2_rn(make_float2(x0, x1),
-                                                     make_float2(a16[c], a16[c])));
-              y = __ffma2_rn(make_float2(cap_l2, cap_l2), t, make_float2(off, off));
-              if (!full) {
-                y.x = x0 == -INFINITY ? x0 : y.x;
-                y.y = x1 == -INFINITY ? x1 : y.y;
+          for (int h = 0; h < PP; ++h) {
+            const int c = c0 + h;
+            const float off = L16[c] - mu;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const float x0 = sr[c * 16 + 2 * q], x1 = sr[c * 16 + 2 * q + 1];
+              if constexpr (CAP == 0) {
+                y[h][q] = __ffma2_rn(make_float2(x0, x1), make_float2(a16[c], a16[c]),
+                                     make_float2(off, off));
+              } else if constexpr (CAP == 1) {
+                y[h][q].x = x0 == -INFINITY ? x0 : fmaf(cap_l2, tanh_via_exp2(x0 * a16[c]), off);
+                y[h][q].y = x1 == -INFINITY ? x1 : fmaf(cap_l2, tanh_via_exp2(x1 * a16[c]), off);
+              } else {
+                const float2 t = tanh_poly2(__fmul2_rn(make_float2(x0, x1),
+                                                       make_float2(a16[c], a16[c])));
+                y[h][q] = __ffma2_rn(make_float2(cap_l2, cap_l2), t, make_float2(off, off));
+                if (!FULL) {
+                  y[h][q].x = x0 == -INFINITY ? x0 : y[h][q].x;
+                  y[h][q].y = x1 == -INFINITY ? x1 : y[h][q].y;
+                }
               }
             }
-            float p0, p1;
-            if (CAP == 0 && kTilePoly > 0 && full && q % (kTilePoly + 1) == kTilePoly) {
-              const float2 e = ex2_poly3x2(y.x, y.y);
-              p0 = e.x;
-              p1 = e.y;
-            } else {
-              p0 = ex2_approx(y.x);
-              p1 = ex2_approx(y.y);
-            }
-            s2 = __fadd2_rn(s2, make_float2(p0, p1));
-            w[q] = pack_f16(p0, p1);
           }
-          tmem_st8(p_addr + c * C::kPStep, w);
-          sum = fmaf(s2.x + s2.y, tab[2 * NC + c], sum);
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+#pragma unroll
+            for (int h = 0; h < PP; ++h) {
+              if (CAP == 0 && FULL && kTilePoly > 0 && q % kTilePoly == kTilePoly - 1) {
+                y[h][q] = ex2_poly3x2(y[h][q].x, y[h][q].y);
+              } else {
+                y[h][q].x = ex2_approx(y[h][q].x);
+                y[h][q].y = ex2_approx(y[h][q].y);
+              }
+            }
+#pragma unroll
+          for (int h = 0; h < PP; ++h) {
+            uint32_t w[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) w[q] = pack_f16(y[h][q].x, y[h][q].y);
+            tmem_st8(p_addr + (c0 + h) * C::kPStep, w);
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1)
+#pragma unroll
+              for (int q = 0; q < o; ++q) y[h][q] = __fadd2_rn(y[h][q], y[h][q + o]);
+            sum = fmaf(y[h][0].x + y[h][0].y, tab[2 * NC + c0 + h], sum);
+          }
         }
       };
-      if (!capped) pass2(std::integral_constant<int, 0>{});
-      else if (!poly) pass2(std::integral_constant<int, 1>{});
-      else pass2(std::integral_constant<int, 2>{});
+      using Cap0 = std::integral_constant<int, 0>;
+      using Cap1 = std::integral_constant<int, 1>;
+      using Cap2 = std::integral_constant<int, 2>;
+      if (!capped) {
+        if (full) pass2(Cap0{}, std::true_type{});
+        else pass2(Cap0{}, std::false_type{});
+      } else if (!poly) {
+        pass2(Cap1{}, std::false_type{});
+      } else if (full) {
+        pass2(Cap2{}, std::true_type{});
+      } else {
+        pass2(Cap2{}, std::false_type{});
+      }
       l = fmaf(l, corr, sum);
       if (j >= TG && __any_sync(0xffffffffu, resc)) {
         if (TG == 1) {  // the previous P V may still add to O
