@@ -46,6 +46,8 @@ struct TileCfg {
   // P has TMEM columns of its own (one group), or takes S's place (two: their
   // two O's leave no room).
   static constexpr bool PSEP = TG == 1;
+  // P V of a tile's first half starts while the second is exponentiated.
+  static constexpr bool HALVES = TG == 2 && CH == 1;
   static constexpr int SC = BN / CH;                     // keys of a softmax thread's part
   static constexpr int kSoftWarps = 4 * TG * CH;
   static constexpr int kSoftThreads = 32 * kSoftWarps;
@@ -70,8 +72,9 @@ struct TileCfg {
   static constexpr int kBarV8E = kBarV8 + STV;  // [STV] V free
   static constexpr int kBarS = kBarV8E + STV;   // [2] S of an (even, odd) tile
   static constexpr int kBarSE = kBarS + 2;      // [2] read
-  static constexpr int kBarP = kBarSE + 2;      // [2] P written and V in f16
-  static constexpr int kBarO = kBarP + 2;       // [2] P V done
+  static constexpr int kBarP = kBarSE + 2;      // [2] P (its first half) written and V in f16
+  static constexpr int kBarP2 = kBarP + 2;      // [2] P's second half
+  static constexpr int kBarO = kBarP2 + 2;      // [2] P V done
   static constexpr int kBarF = kBarO + 2;       // every MMA done
   static constexpr int kNumBars = kBarF + 1;
   static constexpr int kOffQs = kOffBar + (kNumBars * 8 + 15) / 16 * 16;  // float [128]
@@ -238,6 +241,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         mbar_init(bar(C::kBarS + s), 1);
         mbar_init(bar(C::kBarSE + s), 4 * CH);
         mbar_init(bar(C::kBarP + s), 4 * CH + 4);
+        mbar_init(bar(C::kBarP2 + s), 4 * CH);
         mbar_init(bar(C::kBarO + s), 1);
       }
       mbar_init(bar(C::kBarF), 1);
@@ -380,9 +384,14 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         const uint32_t pcol = tmem + C::kPCol + x * (BN / 16 * C::kPStep);
         const uint32_t dst = tmem + C::kOCol + (TG == 2 ? x * HDP : 0);
 #pragma unroll
-        for (int kk = 0; kk < BN / 16; ++kk)
+        for (int kk = 0; kk < BN / 16; ++kk) {
+          if (C::HALVES && kk == BN / 32) {
+            if (!mbar_wait(bar(C::kBarP2 + x), (j >> 1) & 1, dead, p.err)) return false;
+            tc_fence_after();
+          }
           umma_ts(dst, pcol + kk * C::kPStep, dv + ((kk * 2048) >> 4), C::kIdescO,
                   j >= TG || kk > 0 ? 1u : 0u);
+        }
         umma_commit(bar(C::kBarO + x));
         return true;
       };
@@ -627,6 +636,24 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       }
       const uint32_t p_addr =
           tmem + lane_off + C::kPCol + x2 * (BN / 16 * C::kPStep) + part * (SC / 16 * C::kPStep);
+      // O follows a moved maximum before any of this tile's P V.
+      if (j >= TG && __any_sync(0xffffffffu, resc)) {
+        if (TG == 1) {  // the previous P V may still add to O
+          mbar_wait(bar(C::kBarO + (x2 ^ 1)), ((j - 1) >> 1) & 1, dead, p.err);
+          dead = __any_sync(0xffffffffu, dead);
+          tc_fence_after();
+        }
+#pragma unroll 1
+        for (int c = 0; c < HDP / CH / 32; ++c) {
+          uint32_t o[32];
+          const uint32_t ta = tmem + lane_off + C::kOCol + grp * HDP + part * (HDP / CH) + c * 32;
+          tmem_ld32(ta, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = f2u(u2f(o[i]) * corr);
+          tmem_st32(ta, o);
+        }
+      }
       float sum = 0.f;
       auto pass2 = [&](auto cap_c, auto full_c) {
         constexpr int CAP = decltype(cap_c)::value;  // 0 none, 1 tanh, 2 its polynomial
@@ -636,6 +663,12 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         constexpr int PP = NC < 2 ? 1 : 2;
 #pragma unroll
         for (int c0 = 0; c0 < NC; c0 += PP) {
+          if (C::HALVES && c0 == NC / 2) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(C::kBarP + x2));
+          }
           float2 y[PP][8];
 #pragma unroll
           for (int h = 0; h < PP; ++h) {
@@ -700,27 +733,10 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         pass2(Cap2{}, std::false_type{});
       }
       l = fmaf(l, corr, sum);
-      if (j >= TG && __any_sync(0xffffffffu, resc)) {
-        if (TG == 1) {  // the previous P V may still add to O
-          mbar_wait(bar(C::kBarO + (x2 ^ 1)), ((j - 1) >> 1) & 1, dead, p.err);
-          dead = __any_sync(0xffffffffu, dead);
-          tc_fence_after();
-        }
-#pragma unroll 1
-        for (int c = 0; c < HDP / CH / 32; ++c) {
-          uint32_t o[32];
-          const uint32_t ta = tmem + lane_off + C::kOCol + grp * HDP + part * (HDP / CH) + c * 32;
-          tmem_ld32(ta, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = f2u(u2f(o[i]) * corr);
-          tmem_st32(ta, o);
-        }
-      }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(C::kBarP + x2));
+      if (lane == 0) mbar_arrive(bar((C::HALVES ? C::kBarP2 : C::kBarP) + x2));
       ++used;
     }
 
