@@ -147,7 +147,7 @@ struct RowsCfg {
   static constexpr int kWarpBytes = ST * kStage;        // later the warp's partial O
   static constexpr int kOffBar = kWarps * kWarpBytes;
   static constexpr int kOffML = kOffBar + (kWarps * ST * 8 + 15) / 16 * 16;
-  static constexpr int kOffMisc = kOffML + kGroups * 2 * NR * 4;
+  static constexpr int kOffMisc = kOffML + (kGroups * 3 + 1) * NR * 4;
   static constexpr int kSmem = kOffMisc + 16;
   static constexpr int OC = HDP / VS;                   // output columns of a warp
   static constexpr int LC = HDP == 64 ? 8 : 16;         // columns a lane has of each 128
@@ -184,9 +184,37 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   const long long row0 = static_cast<long long>(tile) * NR;
   if (row0 >= n_rows) return;
   const int rows = static_cast<int>(min(static_cast<long long>(NR), n_rows - row0));
+  const unsigned G = static_cast<unsigned>(p.G);
+
+  // What needs nothing but the arguments comes first: the ring's barriers,
+  // and Q, whose way from HBM is as long as that of kv_len.
+  const uint32_t ring = smem_u32(smem + warp * C::kWarpBytes);
+  const uint32_t bar0 = smem_u32(smem + C::kOffBar) + warp * ST * 8;
+  if (lane == 0) {
+    for (int s = 0; s < ST; ++s) mbar_init(bar0 + 8 * s, 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  uint4 raw[NT][KU][2];
+#pragma unroll
+  for (int x = 0; x < NT; ++x) {
+    const int r = 8 * x + g;
+    const unsigned rr = static_cast<unsigned>(row0 + r), tok = rr / G;
+    const __nv_bfloat16* src = p.q + (q_beg + static_cast<long long>(tok)) * p.q_row_stride +
+                               (kvh * p.G + static_cast<int>(rr - tok * G)) *
+                                   static_cast<long long>(hd);
+#pragma unroll
+    for (int i = 0; i < KU; ++i) {
+      const int e = (t + 4 * i) * 16;
+      raw[x][i][0] = raw[x][i][1] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < rows && e < hd) {
+        raw[x][i][0] = __ldg(reinterpret_cast<const uint4*>(src + e));
+        raw[x][i][1] = __ldg(reinterpret_cast<const uint4*>(src + e) + 1);
+      }
+    }
+  }
   const int len = p.kv_len ? min(max(p.kv_len[b], 0), p.c.n_total) : p.c.n_total;
   const int prefix = p.seq_prefix ? p.seq_prefix[b] : p.causal_prefix;
-  const unsigned G = static_cast<unsigned>(p.G);
 
   // Lane (g, t) has query rows 2 t and 2 t + 1 of each 8: what they see, the
   // hull of what any row sees, and what every row sees.
@@ -230,8 +258,6 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   }
   const int c0 = c_beg + grp;
 
-  const uint32_t ring = smem_u32(smem + warp * C::kWarpBytes);
-  const uint32_t bar0 = smem_u32(smem + C::kOffBar) + warp * ST * 8;
   const int tok0 = b * p.c.n_total;
   auto fetch = [&](int ch, int s) {  // lane 0
     const uint32_t dst = ring + s * C::kStage, bar = bar0 + 8 * s;
@@ -245,9 +271,6 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                   tok0 + ch * 16);
   };
   if (lane == 0) {
-    for (int s = 0; s < ST; ++s) mbar_init(bar0 + 8 * s, 1);
-    fence_barrier_init();
-    fence_proxy_async_smem();
     for (int s = 0; s < ST; ++s)
       if (c0 + s * C::kGroups < c_end) fetch(c0 + s * C::kGroups, s);
   }
@@ -272,27 +295,12 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   float qs[NT][2];  // the scale of rows 2 t, 2 t + 1
 #pragma unroll
   for (int x = 0; x < NT; ++x) {
-    uint4 raw[KU][2];
-    const int r = 8 * x + g;
-    const unsigned rr = static_cast<unsigned>(row0 + r), tok = rr / G;
-    const __nv_bfloat16* src = p.q + (q_beg + static_cast<long long>(tok)) * p.q_row_stride +
-                               (kvh * p.G + static_cast<int>(rr - tok * G)) *
-                                   static_cast<long long>(hd);
     float amax = 0.f;
-#pragma unroll
-    for (int i = 0; i < KU; ++i) {
-      const int e = (t + 4 * i) * 16;
-      raw[i][0] = raw[i][1] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < rows && e < hd) {
-        raw[i][0] = __ldg(reinterpret_cast<const uint4*>(src + e));
-        raw[i][1] = __ldg(reinterpret_cast<const uint4*>(src + e) + 1);
-      }
-    }
 #pragma unroll
     for (int i = 0; i < KU; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t w4[4] = {raw[i][h].x, raw[i][h].y, raw[i][h].z, raw[i][h].w};
+        const uint32_t w4[4] = {raw[x][i][h].x, raw[x][i][h].y, raw[x][i][h].z, raw[x][i][h].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           amax = fmax3(amax, fabsf(__uint_as_float(w4[k] << 16)),
@@ -306,7 +314,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     for (int i = 0; i < KU; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t w4[4] = {raw[i][h].x, raw[i][h].y, raw[i][h].z, raw[i][h].w};
+        const uint32_t w4[4] = {raw[x][i][h].x, raw[x][i][h].y, raw[x][i][h].z, raw[x][i][h].w};
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const float v[4] = {__uint_as_float(w4[2 * k] << 16) * inv,
@@ -505,38 +513,64 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       }
     }
   __syncthreads();
+  // Each group's weight for each row, its sum times that, and the row's
+  // maximum.
+  float* row_m = sml + C::kGroups * 2 * NR;
+  float* sw = row_m + NR;
+  for (int i = threadIdx.x; i < NR * C::kGroups; i += C::kThreads) {
+    const int r = i % NR, k = i / NR;
+    float mt = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < C::kGroups; ++x) mt = fmaxf(mt, sml[x * 2 * NR + r]);
+    const float w = mt == -INFINITY ? 0.f : ex2_approx(sml[k * 2 * NR + r] - mt);
+    const float part = sml[(k * 2 + 1) * NR + r] * w;
+    if (k == 0) row_m[r] = mt;
+    sml[(k * 2 + 1) * NR + r] = mt == -INFINITY ? 0.f : part;
+    sw[i] = w;
+  }
+  __syncthreads();
   const long long cell = (static_cast<long long>(b) * p.c.Hkv + kvh) * p.tiles + tile;
-  auto write_out = [&](int r, int e, float v) {
+  auto row_base = [&](int r) -> long long {
     const unsigned rr = static_cast<unsigned>(row0 + r), tok = rr / G;
-    const long long at = (q_beg + static_cast<long long>(tok)) * p.out_row_stride +
-                         (kvh * p.G + static_cast<int>(rr - tok * G)) * static_cast<long long>(hd) +
-                         e;
-    if (p.out_f32) static_cast<float*>(p.out)[at] = v;
-    else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+    return (q_beg + static_cast<long long>(tok)) * p.out_row_stride +
+           (kvh * p.G + static_cast<int>(rr - tok * G)) * static_cast<long long>(hd);
+  };
+  auto write_out = [&](int r, int e, float4 v, float inv) {
+    const long long at = row_base(r) + e;
+    if (p.out_f32)
+      *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) =
+          make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    else
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at) =
+          make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+  };
+  auto fma4 = [](float4& a, const float4& x, float w) {
+    a.x = fmaf(x.x, w, a.x);
+    a.y = fmaf(x.y, w, a.y);
+    a.z = fmaf(x.z, w, a.z);
+    a.w = fmaf(x.w, w, a.w);
   };
   float* po = p.part_o + (cell * p.splits + split) * NR * hd;
   float* pml = p.part_ml + (cell * p.splits + split) * 2 * NR;
-  for (int i = threadIdx.x; i < rows * HDP; i += C::kThreads) {
-    const int r = i / HDP, e = i % HDP;
+  for (int i = threadIdx.x; i < rows * (HDP / 4); i += C::kThreads) {
+    const int r = i / (HDP / 4), e = i % (HDP / 4) * 4;
     if (e >= hd) continue;
-    float mt = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < C::kGroups; ++k) mt = fmaxf(mt, sml[k * 2 * NR + r]);
-    float lt = 0.f, ot = 0.f;
-    if (mt != -INFINITY) {
-#pragma unroll
-      for (int k = 0; k < C::kGroups; ++k) {
-        const float w = ex2_approx(sml[k * 2 * NR + r] - mt);
-        lt = fmaf(sml[(k * 2 + 1) * NR + r], w, lt);
-        ot = fmaf(so[(k * C::VS + e / C::OC) * kSo + r * C::OC + e % C::OC], w, ot);
-      }
+    float lt = 0.f;
+    float4 ot = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k < C::kGroups; ++k) {
+      const float w = sw[k * NR + r];
+      lt += sml[(k * 2 + 1) * NR + r];
+      // A group without a chunk left nothing: its sums are zeros.
+      fma4(ot, *reinterpret_cast<const float4*>(so + (k * C::VS + e / C::OC) * kSo + r * C::OC +
+                                                e % C::OC), w);
     }
     if (p.splits == 1) {
-      write_out(r, e, __fdiv_rn(ot, lt));
+      write_out(r, e, ot, __fdiv_rn(1.f, lt));
     } else {
-      po[r * hd + e] = ot;
+      *reinterpret_cast<float4*>(po + r * hd + e) = ot;
       if (e == 0) {
-        pml[r] = mt;
+        pml[r] = row_m[r];
         pml[NR + r] = lt;
       }
     }
@@ -552,23 +586,33 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   __syncthreads();
   if (!smisc[0]) return;
   __threadfence();
+  // The last CTA joins the splits: weights first, as above, then the sums.
   po = p.part_o + cell * p.splits * NR * hd;
   pml = p.part_ml + cell * p.splits * 2 * NR;
-  for (int i = threadIdx.x; i < rows * HDP; i += C::kThreads) {
-    const int r = i / HDP, e = i % HDP;
-    if (e >= hd) continue;
+  float* jm = so;                      // [splits][2][NR], then the weights
+  float* jw = so + p.splits * 2 * NR;  // [splits][NR]
+  for (int i = threadIdx.x; i < p.splits * 2 * NR; i += C::kThreads) jm[i] = __ldcg(pml + i);
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.splits * NR; i += C::kThreads) {
+    const int r = i % NR, k = i / NR;
     float mt = -INFINITY;
-    for (int k = 0; k < p.splits; ++k) mt = fmaxf(mt, __ldcg(pml + k * 2 * NR + r));
-    float lt = 0.f, ot = 0.f;
-    if (mt != -INFINITY) {
-#pragma unroll 4
-      for (int k = 0; k < p.splits; ++k) {
-        const float w = ex2_approx(__ldcg(pml + k * 2 * NR + r) - mt);
-        lt = fmaf(__ldcg(pml + (k * 2 + 1) * NR + r), w, lt);
-        ot = fmaf(__ldcg(po + (static_cast<long long>(k) * NR + r) * hd + e), w, ot);
-      }
+    for (int x = 0; x < p.splits; ++x) mt = fmaxf(mt, jm[x * 2 * NR + r]);
+    jw[i] = mt == -INFINITY ? 0.f : ex2_approx(jm[k * 2 * NR + r] - mt);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * (HDP / 4); i += C::kThreads) {
+    const int r = i / (HDP / 4), e = i % (HDP / 4) * 4;
+    if (e >= hd) continue;
+    float lt = 0.f;
+    float4 ot = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int k = 0; k < p.splits; ++k) {
+      const float w = jw[k * NR + r];
+      lt = fmaf(jm[(k * 2 + 1) * NR + r], w, lt);
+      fma4(ot, __ldcg(reinterpret_cast<const float4*>(
+                   po + (static_cast<long long>(k) * NR + r) * hd + e)), w);
     }
-    write_out(r, e, __fdiv_rn(ot, lt));
+    write_out(r, e, ot, __fdiv_rn(1.f, lt));
   }
 }
 

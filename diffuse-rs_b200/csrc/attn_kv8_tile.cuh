@@ -512,9 +512,26 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     float* my_sc = reinterpret_cast<float*>(smem + C::kOffSc) + (warp - 4) * 6 * NC;
     float m = -INFINITY, l = 0.f;
     int used = 0;
+    // Nothing but padding in this warp's 32 rows: their P stays as it is.
+    const bool idle = wq * 32 >= rows;
     scales(grp);
     for (int j = grp; j < n; j += TG) {
       const int x2 = j & 1, use = j >> 1;
+      if (idle) {
+        mbar_wait(bar(C::kBarS + x2), use & 1, dead, p.err);
+        if (C::PSEP) {
+          if (lane == 0) mbar_arrive(bar(C::kBarSE + x2));
+          // As below: P[j] counts only once P[j - 2] was read.
+          if (j >= 2) mbar_wait(bar(C::kBarO + x2), (use - 1) & 1, dead, p.err);
+        }
+        dead = __any_sync(0xffffffffu, dead);
+        if (dead) break;
+        if (lane == 0) {
+          mbar_arrive(bar(C::kBarP + x2));
+          if (C::HALVES) mbar_arrive(bar(C::kBarP2 + x2));
+        }
+        continue;
+      }
       float* tab = my_sc + (used & 1) * 3 * NC;  // [k scale, L, 2^-L][NC]
       if (lane < NC) {
         const float L = kv8_log2(nv);
