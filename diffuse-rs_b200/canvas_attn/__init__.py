@@ -57,6 +57,7 @@ EXPORTED_SYMBOLS = (
     "ca_kv8_load",
     "ca_attention_kv8_dev",
     "ca_attention_kv8_workspace",
+    "ca_attention_block_kv8_dev",
 )
 
 

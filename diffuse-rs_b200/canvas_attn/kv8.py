@@ -4,6 +4,7 @@ with a scale for each block of positions and kv head.
   store      K and V rows are quantised as they are written   (ca_kv8_store)
   load       rows are read back as bf16 or fp32               (ca_kv8_load)
   attention  attention over the cache as it is held           (ca_attention_kv8_dev)
+  attention_block  norms, RoPE, store and attention of a step (ca_attention_block_kv8_dev)
 
 Each call has a `make_*_args` form for programs that keep their buffers: the
 argument block is built once and `*_args(a, stream)` launches it. All calls
@@ -56,8 +57,26 @@ class CaAttnKv8Args(ctypes.Structure):
                 ("workspace_bytes", ctypes.c_int64)]
 
 
+class CaBlockKv8Args(ctypes.Structure):
+    _fields_ = [("cache", CaKv8Cache), ("q", ctypes.c_void_p), ("k", ctypes.c_void_p),
+                ("v", ctypes.c_void_p), ("n_head", ctypes.c_int32), ("n_active", ctypes.c_int32),
+                ("active_pos", ctypes.c_void_p), ("cu_active", ctypes.c_void_p),
+                ("max_active", ctypes.c_int32), ("total_active", ctypes.c_int64),
+                ("held", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
+                ("q_norm_w", ctypes.c_void_p), ("k_norm_w", ctypes.c_void_p),
+                ("v_norm", ctypes.c_int32), ("rms_eps", ctypes.c_float),
+                ("rope", ctypes.c_void_p), ("rope_len", ctypes.c_int32),
+                ("rope_dim", ctypes.c_int32), ("work", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("out_f32", ctypes.c_int32), ("out_row_stride", ctypes.c_int64),
+                ("sliding_window", ctypes.c_int64), ("causal_prefix", ctypes.c_int64),
+                ("seq_prefix", ctypes.c_void_p), ("scale", ctypes.c_float),
+                ("softcap", ctypes.c_float), ("status", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)]
+
+
 for _name, _args in (("ca_kv8_store", CaKv8StoreArgs), ("ca_kv8_load", CaKv8LoadArgs),
-                     ("ca_attention_kv8_dev", CaAttnKv8Args)):
+                     ("ca_attention_kv8_dev", CaAttnKv8Args),
+                     ("ca_attention_block_kv8_dev", CaBlockKv8Args)):
     _f = getattr(lib, _name)
     _f.argtypes = [ctypes.POINTER(_args), ctypes.c_void_p]
     _f.restype = ctypes.c_int
@@ -250,3 +269,58 @@ def attention_args(a: CaAttnKv8Args, stream=None) -> None:
 def attention(q, cache: Kv8Cache, out, *, stream=None, **kw) -> None:
     """ca_attention_kv8_dev: attention over the cache (see make_attention_args)."""
     attention_args(make_attention_args(q, cache, out, **kw), stream)
+
+
+def make_block_args(q, k, v, cache: Kv8Cache, out, *, active_pos, rope, rope_len: int,
+                    rope_dim: int, work=None, cu_active=None, max_active=0, held=None, kv_len=None,
+                    q_norm_w=None, k_norm_w=None, v_norm=False, rms_eps=1e-6,
+                    sliding_window: Optional[int] = None, causal_prefix: Optional[int] = None,
+                    seq_prefix=None, scale=1.0, softcap=0.0, status=None,
+                    workspace=None) -> CaBlockKv8Args:
+    """q, k, v: post-projection bf16 [batch, n_active, heads, head_dim], or
+    [rows, heads, head_dim] with cu_active and max_active; out: q's shape, bf16
+    or fp32. rope: the table of build_rope_cache on the device. work (bf16
+    scratch) and workspace: made here and kept with the arguments when None."""
+    c = cache.to_c()
+    heads = int(q.shape[-2])
+    rows = _rows("q", q, ("torch.bfloat16",), heads, c.head_dim)
+    for name, x in (("k", k), ("v", v)):
+        if _rows(name, x, ("torch.bfloat16",), c.n_head_kv, c.head_dim) != rows:
+            raise ValueError(f"{name} must have q's rows")
+    if cu_active is None and c.batch and rows % c.batch:
+        raise ValueError("rows must be the same for every sequence (or pass cu_active)")
+    if str(rope.dtype) != "torch.float32" or rope.numel() < rope_len * (rope_dim // 2) * 2:
+        raise ValueError("rope must be float32 [rope_len, rope_dim / 2, 2]")
+    _i32("active_pos", active_pos, rows)
+    _i32("cu_active", cu_active, c.batch + 1)
+    _i32("held", held, c.batch)
+    need = rows * (heads + 2 * c.n_head_kv) * c.head_dim
+    if work is None:
+        import torch
+        work = torch.empty(need, dtype=torch.bfloat16, device=q.device)
+    if str(work.dtype) != "torch.bfloat16" or work.numel() < need:
+        raise ValueError(f"work must be bfloat16 with at least {need} elements")
+    # The attention's own checks and workspace.
+    t = make_attention_args(q, cache, out, q_pos=active_pos, kv_len=kv_len, cu_q=cu_active,
+                            max_sq=max_active, sliding_window=sliding_window,
+                            causal_prefix=causal_prefix, seq_prefix=seq_prefix, scale=scale,
+                            softcap=softcap, status=status, workspace=workspace)
+    a = CaBlockKv8Args(c, _ptr(q), _ptr(k), _ptr(v), heads, t.sq, _ptr(active_pos),
+                       _ptr(cu_active), int(max_active), t.total_q, _ptr(held), _ptr(kv_len),
+                       _ptr(q_norm_w), _ptr(k_norm_w), 1 if v_norm else 0, float(rms_eps),
+                       _ptr(rope), int(rope_len), int(rope_dim), _ptr(work), _ptr(out), t.out_f32,
+                       t.out_row_stride, t.sliding_window, t.causal_prefix, _ptr(seq_prefix),
+                       float(scale), float(softcap), _ptr(status), t.workspace, t.workspace_bytes)
+    a._keep = (t, k, v, active_pos, cu_active, held, q_norm_w, k_norm_w, rope, work, status)
+    return a
+
+
+def block_args(a: CaBlockKv8Args, stream=None) -> None:
+    _check(lib.ca_attention_block_kv8_dev(ctypes.byref(a), _stream(stream)),
+           "ca_attention_block_kv8_dev")
+
+
+def attention_block(q, k, v, cache: Kv8Cache, out, *, stream=None, **kw) -> None:
+    """ca_attention_block_kv8_dev: one layer's step over the cache (see
+    make_block_args)."""
+    block_args(make_block_args(q, k, v, cache, out, **kw), stream)

@@ -102,11 +102,6 @@ struct TileCfg {
   static_assert(kSoftWarps * 4096 <= STK * kTile8 + STV * kTile8, "output staging");
 };
 
-#ifndef CA_KV8_POLY
-#define CA_KV8_POLY 0
-#endif
-constexpr int kTilePoly = CA_KV8_POLY;
-
 // D[tmem] (+)= A[smem] x B[smem]^T, kind::f8f6f4 (e4m3 in, fp32 accumulate).
 __device__ __forceinline__ void umma_ss_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
                                            uint32_t idesc, uint32_t accumulate) {
@@ -715,12 +710,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
           for (int q = 0; q < 8; ++q)
 #pragma unroll
             for (int h = 0; h < PP; ++h) {
-              if (CAP == 0 && FULL && kTilePoly > 0 && q % kTilePoly == kTilePoly - 1) {
-                y[h][q] = ex2_poly3x2(y[h][q].x, y[h][q].y);
-              } else {
-                y[h][q].x = ex2_approx(y[h][q].x);
-                y[h][q].y = ex2_approx(y[h][q].y);
-              }
+              y[h][q].x = ex2_approx(y[h][q].x);
+              y[h][q].y = ex2_approx(y[h][q].y);
             }
 #pragma unroll
           for (int h = 0; h < PP; ++h) {
@@ -736,19 +727,10 @@ __global__ void __launch_bounds__(C::kThreads, 1)
           }
         }
       };
-      using Cap0 = std::integral_constant<int, 0>;
-      using Cap1 = std::integral_constant<int, 1>;
-      using Cap2 = std::integral_constant<int, 2>;
-      if (!capped) {
-        if (full) pass2(Cap0{}, std::true_type{});
-        else pass2(Cap0{}, std::false_type{});
-      } else if (!poly) {
-        pass2(Cap1{}, std::false_type{});
-      } else if (full) {
-        pass2(Cap2{}, std::true_type{});
-      } else {
-        pass2(Cap2{}, std::false_type{});
-      }
+      if (!capped) pass2(std::integral_constant<int, 0>{}, std::true_type{});
+      else if (!poly) pass2(std::integral_constant<int, 1>{}, std::true_type{});
+      else if (full) pass2(std::integral_constant<int, 2>{}, std::true_type{});
+      else pass2(std::integral_constant<int, 2>{}, std::false_type{});
       l = fmaf(l, corr, sum);
       tmem_wait_st();
       tc_fence_before();

@@ -335,59 +335,12 @@ bool block_vec(const ca_block_args* a) {
          a->rope_dim % 16 == 0;
 }
 
-int block_impl(const ca_block_args* a, cudaStream_t st) {
-  if (!a || !a->q || !a->k || !a->v || !a->active_pos || !a->rope || !a->cache_k ||
-      !a->cache_v || !a->q_work || !a->out)
-    return CA_ERR_INVALID;
-  const int H = a->n_head, Hkv = a->n_head_kv, hd = a->head_dim;
-  const bool varlen = a->cu_active != nullptr;
-  if (a->batch < 0 || H <= 0 || Hkv <= 0 || hd <= 0 || H % Hkv) return CA_ERR_INVALID;
-  if (varlen ? (!a->cu_total || a->total_active < 0 || a->total_cache < 0 || a->max_active < 0)
-             : (a->n_active < 0 || a->n_total < a->n_active))
-    return CA_ERR_INVALID;
-  if (a->rope_dim < 0 || a->rope_dim > hd || a->rope_dim % 2 || a->rope_len <= 0)
-    return CA_ERR_INVALID;
-  if (a->batch == 0 || (varlen ? a->total_active == 0 : a->n_active == 0)) return CA_OK;
-  if (varlen && (a->total_active > INT_MAX || a->total_cache > INT_MAX)) return CA_ERR_UNSUPPORTED;
-  PrepParams pp{};
-  pp.q = static_cast<const __nv_bfloat16*>(a->q);
-  pp.k = static_cast<const __nv_bfloat16*>(a->k);
-  pp.v = static_cast<const __nv_bfloat16*>(a->v);
-  pp.pos = a->active_pos;
-  pp.q_norm_w = a->q_norm_w;
-  pp.k_norm_w = a->k_norm_w;
-  pp.v_norm = a->v_norm;
-  pp.eps = a->rms_eps;
-  pp.rope = a->rope;
-  pp.rope_len = a->rope_len;
-  pp.rope_dim = a->rope_dim;
-  pp.q_out = static_cast<__nv_bfloat16*>(a->q_work);
-  pp.cache_k = static_cast<__nv_bfloat16*>(a->cache_k);
-  pp.cache_v = static_cast<__nv_bfloat16*>(a->cache_v);
-  pp.batch = a->batch;
-  pp.na = a->n_active;
-  pp.n_total = a->n_total;
-  pp.cu_active = a->cu_active;
-  pp.cu_total = a->cu_total;
-  pp.total_active = varlen ? a->total_active : 0;
-  const bool vec = block_vec(a);
-  // head_dim 128 with rotation over the whole head: the attention kernel
-  // normalises and rotates its own Q tile (each Q row belongs to exactly one
-  // CTA), so the pre-ops pass covers K and V only and Q never round-trips
-  // through HBM; q_work is then unused.
-  // The in-kernel pass lengthens every CTA's prologue, paid once per wave of
-  // CTAs and not amortised over few key tiles: measured on B200 (bench.py
-  // steps, same box) c2 (7 waves, 8 key tiles) -2.7%, c4 (1 wave, 33 tiles)
-  // -1%, c1 (1 key tile) +7%, c3 (28 waves) +3%.
-  const bool fuse_q = block_fuses_q(a, vec);
-  const int Hp = fuse_q ? 0 : H;  // Q rows handled by the pre-ops pass
-  pp.H = Hp;
-  pp.Hkv = Hkv;
-  pp.hd = hd;
-  const long long toks =
-      varlen ? a->total_active : static_cast<long long>(a->batch) * a->n_active;
+// Launches the pre-ops pass over `toks` active tokens (pp.H query rows, 0
+// where the attention kernel does its own, and 2 pp.Hkv K and V rows each).
+// `vec`: every pointer is 16-byte aligned and rope_dim % 16 == 0.
+int launch_prep(PrepParams pp, long long toks, bool vec, cudaStream_t st) {
+  const int Hp = pp.H, Hkv = pp.Hkv, hd = pp.hd;
   const long long jobs = toks * (Hp + 2 * Hkv);
-  pp.err = a->status;
   const long long stage = static_cast<long long>(Hp + 2 * Hkv) * hd * 2;
   const size_t bulk_smem = kPrepStages * stage + 16 * kPrepStages;
   // Bulk-copy pre-ops (a shared-memory ring per CTA) at head_dim 256: c5's
@@ -401,7 +354,7 @@ int block_impl(const ca_block_args* a, cudaStream_t st) {
   // Short passes (c2's 32K and c4's 8K rows of K and V) measured 3-5 us
   // faster on the token kernel, whose many small jobs start at once.
   int ring_t = 0;
-  if (vec && a->rope_dim == hd && (hd == 64 || hd == 128 || hd == 256) &&
+  if (vec && pp.rope_dim == hd && (hd == 64 || hd == 128 || hd == 256) &&
       jobs >= 256LL * 1024) {
     const long long tok_bytes = static_cast<long long>(Hp + 2 * Hkv) * hd * 2;
     ring_t = static_cast<int>(std::min<long long>(16, 48 * 1024 / tok_bytes));
@@ -463,7 +416,7 @@ int block_impl(const ca_block_args* a, cudaStream_t st) {
     const int blocks = static_cast<int>(std::min<long long>((pjobs + 7) / 8, 148LL * 8));
     // head_dim 256 with full rotation: every NeoX pair inside one lane
     // (measured faster there; at 64 / 128 the partner-exchange form is).
-    if (hd == 256 && a->rope_dim == hd) prep_pair_kernel<32><<<blocks, 256, 0, st>>>(pp);
+    if (hd == 256 && pp.rope_dim == hd) prep_pair_kernel<32><<<blocks, 256, 0, st>>>(pp);
     else if (hd == 64) prep_token_kernel<8><<<blocks, 256, 0, st>>>(pp);
     else if (hd == 128) prep_token_kernel<16><<<blocks, 256, 0, st>>>(pp);
     else prep_token_kernel<32><<<blocks, 256, 0, st>>>(pp);
@@ -471,7 +424,63 @@ int block_impl(const ca_block_args* a, cudaStream_t st) {
     const int blocks = static_cast<int>(std::min<long long>((jobs + 7) / 8, 148LL * 16));
     prep_block_kernel<<<blocks, 256, 8 * hd * sizeof(float), st>>>(pp);
   }
-  if (cudaGetLastError() != cudaSuccess) return CA_ERR_CUDA;
+  return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
+}
+
+int block_impl(const ca_block_args* a, cudaStream_t st) {
+  if (!a || !a->q || !a->k || !a->v || !a->active_pos || !a->rope || !a->cache_k ||
+      !a->cache_v || !a->q_work || !a->out)
+    return CA_ERR_INVALID;
+  const int H = a->n_head, Hkv = a->n_head_kv, hd = a->head_dim;
+  const bool varlen = a->cu_active != nullptr;
+  if (a->batch < 0 || H <= 0 || Hkv <= 0 || hd <= 0 || H % Hkv) return CA_ERR_INVALID;
+  if (varlen ? (!a->cu_total || a->total_active < 0 || a->total_cache < 0 || a->max_active < 0)
+             : (a->n_active < 0 || a->n_total < a->n_active))
+    return CA_ERR_INVALID;
+  if (a->rope_dim < 0 || a->rope_dim > hd || a->rope_dim % 2 || a->rope_len <= 0)
+    return CA_ERR_INVALID;
+  if (a->batch == 0 || (varlen ? a->total_active == 0 : a->n_active == 0)) return CA_OK;
+  if (varlen && (a->total_active > INT_MAX || a->total_cache > INT_MAX)) return CA_ERR_UNSUPPORTED;
+  PrepParams pp{};
+  pp.q = static_cast<const __nv_bfloat16*>(a->q);
+  pp.k = static_cast<const __nv_bfloat16*>(a->k);
+  pp.v = static_cast<const __nv_bfloat16*>(a->v);
+  pp.pos = a->active_pos;
+  pp.q_norm_w = a->q_norm_w;
+  pp.k_norm_w = a->k_norm_w;
+  pp.v_norm = a->v_norm;
+  pp.eps = a->rms_eps;
+  pp.rope = a->rope;
+  pp.rope_len = a->rope_len;
+  pp.rope_dim = a->rope_dim;
+  pp.q_out = static_cast<__nv_bfloat16*>(a->q_work);
+  pp.cache_k = static_cast<__nv_bfloat16*>(a->cache_k);
+  pp.cache_v = static_cast<__nv_bfloat16*>(a->cache_v);
+  pp.batch = a->batch;
+  pp.na = a->n_active;
+  pp.n_total = a->n_total;
+  pp.cu_active = a->cu_active;
+  pp.cu_total = a->cu_total;
+  pp.total_active = varlen ? a->total_active : 0;
+  const bool vec = block_vec(a);
+  // head_dim 128 with rotation over the whole head: the attention kernel
+  // normalises and rotates its own Q tile (each Q row belongs to exactly one
+  // CTA), so the pre-ops pass covers K and V only and Q never round-trips
+  // through HBM; q_work is then unused.
+  // The in-kernel pass lengthens every CTA's prologue, paid once per wave of
+  // CTAs and not amortised over few key tiles: measured on B200 (bench.py
+  // steps, same box) c2 (7 waves, 8 key tiles) -2.7%, c4 (1 wave, 33 tiles)
+  // -1%, c1 (1 key tile) +7%, c3 (28 waves) +3%.
+  const bool fuse_q = block_fuses_q(a, vec);
+  const int Hp = fuse_q ? 0 : H;  // Q rows handled by the pre-ops pass
+  pp.H = Hp;
+  pp.Hkv = Hkv;
+  pp.hd = hd;
+  const long long toks =
+      varlen ? a->total_active : static_cast<long long>(a->batch) * a->n_active;
+  pp.err = a->status;
+  const int rc = launch_prep(pp, toks, vec, st);
+  if (rc != CA_OK) return rc;
 
   ca_dev_args d{};
   d.q = fuse_q ? a->q : a->q_work;

@@ -116,16 +116,12 @@ struct Kv8Plan {
   int64_t ws_bytes;
 };
 
-#ifndef CA_KV8_TILE_ROWS
-#define CA_KV8_TILE_ROWS 16
-#endif
-
 int kv8_plan(const ca_attn_kv8_args* a, const Kv8View& c, bool split_ok, Kv8Plan* pl) {
   const int64_t max_sq = a->cu_q ? a->max_sq : a->sq;
   const int64_t G = a->n_head / c.Hkv;
   const int64_t rows = max_sq * G;
   if (static_cast<int64_t>(c.batch) * c.n_total > INT_MAX) return CA_ERR_UNSUPPORTED;
-  const int tr = rows > CA_KV8_TILE_ROWS && c.hd <= 256 ? 128 : rows > 8 && c.hd <= 128 ? 16 : 8;
+  const int tr = rows > 16 && c.hd <= 256 ? 128 : rows > 8 && c.hd <= 128 ? 16 : 8;
   pl->nr = tr;
   const int64_t tiles = (rows + tr - 1) / tr;
   if (tiles > INT_MAX / 1024) return CA_ERR_UNSUPPORTED;
@@ -194,12 +190,6 @@ int launch_rows(const Kv8AttnParams& p, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
 }
 
-#ifndef CA_KV8_CH
-#define CA_KV8_CH 1
-#endif
-#ifndef CA_KV8_CH256
-#define CA_KV8_CH256 2
-#endif
 template <class C>
 int launch_tile(const Kv8AttnParams& p, cudaStream_t st) {
   static bool attr_done[kMaxDevices] = {};
@@ -220,7 +210,8 @@ int launch_tile(const Kv8AttnParams& p, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
 }
 
-int attn_kv8_impl(const ca_attn_kv8_args* a, cudaStream_t st) {
+// `check_only`: says whether the call would be taken, and launches nothing.
+int attn_kv8_impl(const ca_attn_kv8_args* a, cudaStream_t st, bool check_only = false) {
   Kv8AttnParams p{};
   int rc = attn_kv8_check(a, &p.c);
   if (rc != CA_OK) return rc;
@@ -239,6 +230,7 @@ int attn_kv8_impl(const ca_attn_kv8_args* a, cudaStream_t st) {
   if ((rc = kv8_plan(a, p.c, a->workspace != nullptr, &pl)) != CA_OK) return rc;
   if (a->workspace && (!aligned16(a->workspace) || a->workspace_bytes < pl.ws_bytes))
     return CA_ERR_INVALID;
+  if (check_only) return CA_OK;
   p.q = static_cast<const __nv_bfloat16*>(a->q);
   p.out = a->out;
   p.out_f32 = a->out_f32 ? 1 : 0;
@@ -266,9 +258,9 @@ int attn_kv8_impl(const ca_attn_kv8_args* a, cudaStream_t st) {
     p.part_o = p.part_ml + cells * pl.splits * 2 * pl.nr;
   }
   if (pl.nr == 128) {
-    if (hd <= 64) return launch_tile<TileCfg<64, CA_KV8_CH>>(p, st);
-    if (hd <= 128) return launch_tile<TileCfg<128, CA_KV8_CH>>(p, st);
-    return launch_tile<TileCfg<256, CA_KV8_CH256>>(p, st);
+    if (hd <= 64) return launch_tile<TileCfg<64, 1>>(p, st);
+    if (hd <= 128) return launch_tile<TileCfg<128, 1>>(p, st);
+    return launch_tile<TileCfg<256, 2>>(p, st);
   }
   if (pl.nr == 16)
     return hd <= 64 ? launch_rows<RowsCfg<64, 16>>(p, st) : launch_rows<RowsCfg<128, 16>>(p, st);
@@ -278,10 +270,98 @@ int attn_kv8_impl(const ca_attn_kv8_args* a, cudaStream_t st) {
   return launch_rows<RowsCfg<512, 8>>(p, st);
 }
 
+int block_kv8_impl(const ca_block_kv8_args* a, cudaStream_t st) {
+  if (!a || !a->q || !a->k || !a->v || !a->active_pos || !a->rope || !a->work || !a->out)
+    return CA_ERR_INVALID;
+  Kv8View c;
+  int rc = kv8_view(a->cache, &c);
+  if (rc != CA_OK) return rc;
+  const int H = a->n_head;
+  if (H <= 0 || H % c.Hkv || !aligned16(a->work)) return CA_ERR_INVALID;
+  if (a->cu_active ? (a->total_active < 0 || a->max_active < 0) : a->n_active < 0)
+    return CA_ERR_INVALID;
+  if (a->rope_dim < 0 || a->rope_dim > c.hd || a->rope_dim % 2 || a->rope_len < c.n_total)
+    return CA_ERR_INVALID;
+  const int64_t rows = a->cu_active ? a->total_active : static_cast<int64_t>(c.batch) * a->n_active;
+  if (rows > INT_MAX) return CA_ERR_UNSUPPORTED;
+  // The three parts are checked before the first is launched.
+  __nv_bfloat16* wq = static_cast<__nv_bfloat16*>(a->work);
+  __nv_bfloat16* wk = wq + rows * H * c.hd;
+  __nv_bfloat16* wv = wk + rows * c.Hkv * c.hd;
+  ca_kv8_store_args s{};
+  s.cache = a->cache;
+  s.k = wk;
+  s.v = wv;
+  s.n_active = a->n_active;
+  s.active_pos = a->active_pos;
+  s.cu_active = a->cu_active;
+  s.total_active = a->total_active;
+  s.kv_len = a->held;
+  s.status = a->status;
+  ca_attn_kv8_args t{};
+  t.cache = a->cache;
+  t.q = wq;
+  t.out = a->out;
+  t.out_f32 = a->out_f32;
+  t.out_row_stride = a->out_row_stride;
+  t.n_head = H;
+  t.sq = a->n_active;
+  t.cu_q = a->cu_active;
+  t.max_sq = a->max_active;
+  t.total_q = a->total_active;
+  t.q_pos = a->active_pos;
+  t.kv_len = a->kv_len;
+  t.sliding_window = a->sliding_window;
+  t.causal_prefix = a->causal_prefix;
+  t.seq_prefix = a->seq_prefix;
+  t.scale = a->scale;
+  t.softcap = a->softcap;
+  t.status = a->status;
+  t.workspace = a->workspace;
+  t.workspace_bytes = a->workspace_bytes;
+  if ((rc = attn_kv8_impl(&t, st, true)) != CA_OK) return rc;
+  if (c.batch == 0 || rows == 0) return CA_OK;
+  PrepParams pp{};
+  pp.q = static_cast<const __nv_bfloat16*>(a->q);
+  pp.k = static_cast<const __nv_bfloat16*>(a->k);
+  pp.v = static_cast<const __nv_bfloat16*>(a->v);
+  pp.pos = a->active_pos;
+  pp.q_norm_w = a->q_norm_w;
+  pp.k_norm_w = a->k_norm_w;
+  pp.v_norm = a->v_norm;
+  pp.eps = a->rms_eps;
+  pp.rope = a->rope;
+  pp.rope_len = a->rope_len;
+  pp.rope_dim = a->rope_dim;
+  pp.q_out = wq;
+  pp.cache_k = wk;
+  pp.cache_v = wv;
+  pp.kv_rows = 1;
+  pp.batch = c.batch;
+  pp.na = a->n_active;
+  pp.n_total = c.n_total;
+  pp.cu_active = a->cu_active;
+  pp.total_active = a->total_active;
+  pp.err = a->status;
+  pp.H = H;
+  pp.Hkv = c.Hkv;
+  pp.hd = c.hd;
+  const bool vec = aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->rope) &&
+                   (!a->q_norm_w || aligned16(a->q_norm_w)) &&
+                   (!a->k_norm_w || aligned16(a->k_norm_w)) && a->rope_dim % 16 == 0;
+  if ((rc = launch_prep(pp, rows, vec, st)) != CA_OK) return rc;
+  if ((rc = kv8_store_impl(&s, st)) != CA_OK) return rc;
+  return attn_kv8_impl(&t, st);
+}
+
 }  // namespace
 }  // namespace ca
 
 extern "C" {
+
+int ca_attention_block_kv8_dev(const ca_block_kv8_args* a, void* stream) {
+  return ca::block_kv8_impl(a, static_cast<cudaStream_t>(stream));
+}
 
 int ca_kv8_store(const ca_kv8_store_args* a, void* stream) {
   return ca::kv8_store_impl(a, static_cast<cudaStream_t>(stream));

@@ -43,6 +43,7 @@ struct PrepParams {
   const int* cu_total;
   long long total_active;
   int* err;  // status word of the call (null: the device-wide word)
+  int kv_rows;  // 1: K and V go to row `token` of cache_k / cache_v, not to a position
 };
 
 // Active tokens of the whole call.
@@ -52,6 +53,7 @@ __device__ __forceinline__ long long prep_tokens(const PrepParams& p) {
 
 // Cache row (sequence base + position) of active token `tok`.
 __device__ __forceinline__ long long cache_row(const PrepParams& p, long long tok, int pos) {
+  if (p.kv_rows) return tok;
   if (!p.cu_active) return static_cast<long long>(tok / p.na) * p.n_total + pos;
   int lo = 0, hi = p.batch - 1;  // last b with cu_active[b] <= tok
   while (lo < hi) {

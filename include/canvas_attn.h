@@ -485,6 +485,53 @@ typedef struct {
  */
 int ca_attention_kv8_dev(const ca_attn_kv8_args* a, void* stream);
 
+/* Arguments of the fused block over the 8-bit cache. Rows are those of
+ * ca_block_args: uniform (n_active rows a sequence), or ragged with cu_active. */
+typedef struct {
+    ca_kv8_cache cache;
+    const void* q;             /* bf16 [rows, n_head, head_dim], post-projection, pre-norm */
+    const void* k;             /* bf16 [rows, n_head_kv, head_dim] */
+    const void* v;
+    int32_t n_head;
+    int32_t n_active;
+    const int32_t* active_pos; /* int32 [rows], 0 .. n_total - 1, ascending within a sequence */
+    const int32_t* cu_active;  /* int32 [batch + 1] or NULL */
+    int32_t max_active;        /* with cu_active: largest per-sequence row count */
+    int64_t total_active;      /* with cu_active: cu_active[batch] */
+    const int32_t* held;       /* int32 [batch]: positions held before the call; NULL = n_total */
+    const int32_t* kv_len;     /* int32 [batch]: positions held after it; NULL = n_total */
+    const float* q_norm_w;     /* as ca_block_args, from here to rope_dim */
+    const float* k_norm_w;
+    int32_t v_norm;
+    float rms_eps;
+    const float* rope;         /* fp32 [rope_len, rope_dim/2, 2]; rope_len >= n_total */
+    int32_t rope_len;
+    int32_t rope_dim;
+    void* work;                /* bf16 scratch of rows * (n_head + 2 * n_head_kv) * head_dim
+                                  elements, 16-byte aligned (caller-owned) */
+    void* out;                 /* [rows, n_head, head_dim] */
+    int32_t out_f32;
+    int64_t out_row_stride;
+    int64_t sliding_window;
+    int64_t causal_prefix;
+    const int32_t* seq_prefix;
+    float scale;
+    float softcap;
+    int32_t* status;
+    void* workspace;           /* as ca_attn_kv8_args */
+    int64_t workspace_bytes;
+} ca_block_kv8_args;
+
+/*
+ * ca_attention_block_kv8_dev -- ca_attention_block_dev over the 8-bit cache
+ * (src/model/forward.rs:296-343): per-head norms and RoPE of the active rows
+ * in the pre-ops kernels of that call, ca_kv8_store of the post-RoPE K and V
+ * (bf16, as the bf16 cache would hold them), and ca_attention_kv8_dev of the
+ * rotated queries over every held position, the active ones included.
+ * Asynchronous on `stream`; allocates nothing.
+ */
+int ca_attention_block_kv8_dev(const ca_block_kv8_args* a, void* stream);
+
 /* Bytes of workspace a call with these arguments uses (pointers are not
  * read), or a negative ca_status. */
 int64_t ca_attention_kv8_workspace(const ca_attn_kv8_args* a);

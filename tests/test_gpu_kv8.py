@@ -420,6 +420,69 @@ def test_load_reports_bad_positions():
     assert bool((out[0, 1:] == 7.0).all()) and not bool((out[0, 0] == 7.0).any())
 
 
+# ------------------------------------------------------------------ block
+@pytest.mark.parametrize("hd,rope_dim,ragged", [(64, 64, False), (128, 64, False), (128, 128, True),
+                                                (256, 256, False), (80, 32, True)])
+def test_block_is_its_parts(hd, rope_dim, ragged):
+    # Norms and RoPE as the bf16 block leaves them (its cache and q_work), the
+    # store and the attention of this cache: the same bits in one call.
+    g = torch.Generator().manual_seed(hd)
+    B, n, H, Hkv, T = 3, 300, 4, 2, 32
+    counts = [50, 1, 23] if ragged else [40] * B
+    total = sum(counts)
+    bf = torch.bfloat16
+    q, k, v = (torch.randn(total, h, hd, generator=g).to(bf).cuda() for h in (H, Hkv, Hkv))
+    pos = torch.cat([torch.randperm(n, generator=g)[:c].sort().values for c in counts])
+    pos = pos.to(torch.int32).cuda()
+    wq, wk = (torch.rand(hd, generator=g).cuda() + 0.5 for _ in range(2))
+    rope = torch.from_numpy(ca.build_rope_cache(n, rope_dim, 1e4)).cuda()
+    kw = dict(active_pos=pos, rope=rope, rope_len=n, rope_dim=rope_dim, q_norm_w=wq, k_norm_w=wk,
+              v_norm=True, rms_eps=1e-6, scale=hd ** -0.5)
+    at = [0]
+    for c in counts:
+        at.append(at[-1] + c)
+    cu = torch.tensor(at, dtype=torch.int32).cuda()
+    k16 = torch.zeros(B * n, Hkv, hd, dtype=bf, device="cuda")
+    v16 = torch.zeros_like(k16)
+    q_work, out16 = torch.empty_like(q), torch.empty_like(q)
+    ca.attention_block_dev(q, k, v, batch=B, n_active=0, cache_k=k16, cache_v=v16, n_total=0,
+                           q_work=q_work, out=out16, n_head=H, n_head_kv=Hkv, head_dim=hd,
+                           cu_active=cu, cu_total=(torch.arange(B + 1, dtype=torch.int32) * n).cuda(),
+                           max_active=max(counts), total_active=total, total_cache=B * n, **kw)
+    rows = torch.cat([pos[a:b].long() + i * n for i, (a, b) in enumerate(zip(at, at[1:]))])
+    parts = cache_of(g, B, n, Hkv, hd, T)
+    whole = kv8.Kv8Cache(parts.k.clone(), parts.v.clone(), parts.k_scale.clone(),
+                         parts.v_scale.clone(), T)
+    kv8.store(parts, k16[rows], v16[rows], pos, cu_active=cu)
+    want = torch.full((total, H, hd), 7.0, device="cuda")
+    kv8.attention(q_work, parts, want, cu_q=cu, max_sq=max(counts), q_pos=pos, scale=hd ** -0.5,
+                  sliding_window=100)
+    got = torch.full_like(want, 8.0)
+    if ragged:
+        kv8.attention_block(q, k, v, whole, got, cu_active=cu, max_active=max(counts),
+                            sliding_window=100, **kw)
+    else:
+        four = lambda x: x.view((B, counts[0]) + x.shape[1:])  # noqa: E731
+        kv8.attention_block(four(q), four(k), four(v), whole, four(got), sliding_window=100, **kw)
+    torch.cuda.synchronize()
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert torch.equal(getattr(whole, name), getattr(parts, name)), name
+    assert torch.equal(got, want)
+
+
+def test_example_runs():
+    import importlib.util
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    spec = importlib.util.spec_from_file_location(
+        "kv8_denoise", os.path.join(root, "examples", "kv8_denoise.py"))
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    far, same = m.main(["--batch", "2", "--total", "256", "--steps", "3", "--layers", "2"])
+    # A value of 4 significant bits is within 2^-4 of what it stands for.
+    assert max(far) < 2.0 ** -4 and min(same) > 0.5
+
+
 def test_offsets_past_32_bits():
     # A cache of more than 2^32 bytes: the last sequence's rows.
     B, n, Hkv, d, T = 17, 131072, 16, 128, 128

@@ -101,6 +101,32 @@ def test_attention_arguments(kw, status):
     assert attn_call(**kw) == status
 
 
+def block_call(cache=None, **kw):
+    d = dict(q=FAKE, k=FAKE, v=FAKE, n_head=4, n_active=3, active_pos=FAKE, rope=FAKE, rope_len=100,
+             rope_dim=128, work=FAKE, out=FAKE, sliding_window=-1, causal_prefix=-1, scale=1.0)
+    d.update(kw)
+    a = kv8.CaBlockKv8Args(cache=cache or c_cache(), **d)
+    return ca.lib.ca_attention_block_kv8_dev(ctypes.byref(a), None)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(q=None), ca.CA_ERR_INVALID), (dict(work=None), ca.CA_ERR_INVALID),
+    (dict(work=FAKE + 8), ca.CA_ERR_INVALID), (dict(active_pos=None), ca.CA_ERR_INVALID),
+    (dict(rope_len=99), ca.CA_ERR_INVALID), (dict(rope_dim=130), ca.CA_ERR_INVALID),
+    (dict(rope_dim=3), ca.CA_ERR_INVALID), (dict(n_head=3), ca.CA_ERR_INVALID),
+    (dict(n_active=-1), ca.CA_ERR_INVALID), (dict(out=FAKE + 4), ca.CA_ERR_INVALID),
+    (dict(cu_active=FAKE, total_active=3, max_active=-1), ca.CA_ERR_INVALID),
+    (dict(out_row_stride=8), ca.CA_ERR_INVALID), (dict(n_active=0), ca.CA_OK),
+])
+def test_block_arguments(kw, status):
+    assert block_call(**kw) == status
+
+
+@pytest.mark.parametrize("kw,status", BAD_CACHES)
+def test_block_refuses_bad_caches(kw, status):
+    assert block_call(c_cache(**kw)) == status
+
+
 def test_workspace_is_checked_and_sized():
     long = c_cache(batch=1, n_total=8192)
     a = attn_args(long, sq=1)
