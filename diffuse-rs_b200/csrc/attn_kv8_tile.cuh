@@ -37,9 +37,12 @@
 
 namespace ca {
 
-template <int HDP_, int CH_>
+// CAPPED: the soft-cap's arithmetic (a kernel of its own: the softmax loop is
+// long, and instruction fetch is some of its time).
+template <int HDP_, int CH_, bool CAPPED_>
 struct TileCfg {
   static constexpr int HDP = HDP_;                       // 64, 128 or 256
+  static constexpr bool CAPPED = CAPPED_;
   static constexpr int CH = CH_;                         // warps that share 32 rows of a tile
   static constexpr int TG = HDP <= 128 ? 2 : 1;          // tile groups, each with its own O
   static constexpr int BN = TG == 2 ? 128 : 64;          // keys of a tile
@@ -483,7 +486,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     int lo = 0, hi = INT_MAX;  // rows past the end see everything: they slow nothing down
     if (r < rows) interval(r, lo, hi);
     const float qs = sQs[r];
-    const bool capped = p.softcap != 0.f;
+    constexpr bool capped = C::CAPPED;
     // Score factor without the block's K scale: log2 units, or for the
     // soft-cap the argument of tanh.
     const float row_c =
@@ -586,7 +589,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         m16[c] = fmaxf(m0, m1);
       }
       bool poly = false;
-      if (capped) {
+      if constexpr (capped) {
         // Whether every argument of tanh is in the polynomial's range: the
         // largest magnitude (masked scores, -inf, count as 0).
         float umax = 0.f;
@@ -727,10 +730,13 @@ __global__ void __launch_bounds__(C::kThreads, 1)
           }
         }
       };
-      if (!capped) pass2(std::integral_constant<int, 0>{}, std::true_type{});
-      else if (!poly) pass2(std::integral_constant<int, 1>{}, std::true_type{});
-      else if (full) pass2(std::integral_constant<int, 2>{}, std::true_type{});
-      else pass2(std::integral_constant<int, 2>{}, std::false_type{});
+      if constexpr (!capped) {
+        pass2(std::integral_constant<int, 0>{}, std::true_type{});
+      } else {
+        if (!poly) pass2(std::integral_constant<int, 1>{}, std::true_type{});
+        else if (full) pass2(std::integral_constant<int, 2>{}, std::true_type{});
+        else pass2(std::integral_constant<int, 2>{}, std::false_type{});
+      }
       l = fmaf(l, corr, sum);
       tmem_wait_st();
       tc_fence_before();

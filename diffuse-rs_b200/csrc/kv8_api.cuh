@@ -258,9 +258,14 @@ int attn_kv8_impl(const ca_attn_kv8_args* a, cudaStream_t st, bool check_only = 
     p.part_o = p.part_ml + cells * pl.splits * 2 * pl.nr;
   }
   if (pl.nr == 128) {
-    if (hd <= 64) return launch_tile<TileCfg<64, 1>>(p, st);
-    if (hd <= 128) return launch_tile<TileCfg<128, 1>>(p, st);
-    return launch_tile<TileCfg<256, 2>>(p, st);
+    if (p.softcap != 0.f) {
+      if (hd <= 64) return launch_tile<TileCfg<64, 1, true>>(p, st);
+      if (hd <= 128) return launch_tile<TileCfg<128, 1, true>>(p, st);
+      return launch_tile<TileCfg<256, 2, true>>(p, st);
+    }
+    if (hd <= 64) return launch_tile<TileCfg<64, 1, false>>(p, st);
+    if (hd <= 128) return launch_tile<TileCfg<128, 1, false>>(p, st);
+    return launch_tile<TileCfg<256, 2, false>>(p, st);
   }
   if (pl.nr == 16)
     return hd <= 64 ? launch_rows<RowsCfg<64, 16>>(p, st) : launch_rows<RowsCfg<128, 16>>(p, st);
