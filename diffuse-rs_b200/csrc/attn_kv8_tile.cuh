@@ -92,8 +92,9 @@ struct TileCfg {
   static constexpr int kPStep = PSEP ? 8 : 16;           // columns of 16 keys
   static constexpr int kOCol = PSEP ? 3 * BN : 2 * BN;
   // Registers (CH 1, two groups: 512 threads launched with 128 each): two
-  // warpgroups with whole rows of 128 keys at 192, the other two at 64, are
-  // those 4 x 128.
+  // warpgroups with whole rows of 128 keys at 200, the other two at 56, are
+  // those 4 x 128. (192 and 64: 3% slower; 208 and 48: no different.)
+  static constexpr int kSoftRegs = 200, kOtherRegs = 56;
   static constexpr bool REGS = SC == 128;
   static constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(BN >> 3) << 17) |
                                       (128u >> 4 << 24);  // e4m3 x e4m3, fp32
@@ -326,7 +327,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   bool dead = false;
 
   if (warp < 4) {
-    if constexpr (C::REGS) reg_dec<64>();
+    if constexpr (C::REGS) reg_dec<C::kOtherRegs>();
     if (warp == 0 || warp == 2) {
       // ---------------------------------------------------------- producers
       if (lane == 0) {
@@ -405,7 +406,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     }
   } else if (warp >= C::kConvWarp0) {
     // ------------------------------------------------------------ V to f16
-    if constexpr (C::REGS) reg_dec<64>();
+    if constexpr (C::REGS) reg_dec<C::kOtherRegs>();
     const int cw = warp - C::kConvWarp0;
     constexpr int UPR = HDP == 64 ? 4 : 8;  // units of a row within a 128-byte column
     constexpr int RPW = 32 / UPR;           // rows a warp covers at once
@@ -466,7 +467,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     }
   } else {
     // ------------------------------------------------------------ softmax
-    if constexpr (C::REGS) reg_inc<192>();
+    if constexpr (C::REGS) reg_inc<C::kSoftRegs>();
     const int wg = (warp - 4) >> 2;       // warpgroup: tile group, part of the row
     const int grp = wg / CH, part = wg % CH;
     const int wq = warp & 3;
@@ -515,7 +516,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     scales(grp);
     for (int j = grp; j < n; j += TG) {
       const int x2 = j & 1, use = j >> 1;
-      if (idle) {
+      if (__builtin_expect(idle, 0)) {
         mbar_wait(bar(C::kBarS + x2), use & 1, dead, p.err);
         if (C::PSEP) {
           if (lane == 0) mbar_arrive(bar(C::kBarSE + x2));
@@ -570,7 +571,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         tc_fence_before();
         if (lane == 0) mbar_arrive(bar(C::kBarSE + x2));
       }
-      if (!full) {
+      if (__builtin_expect(!full, 0)) {
 #pragma unroll
         for (int i = 0; i < SC; ++i)
           sr[i] = static_cast<uint32_t>(i - v0) < v1 ? sr[i] : -INFINITY;
@@ -652,7 +653,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       const uint32_t p_addr =
           tmem + lane_off + C::kPCol + x2 * (BN / 16 * C::kPStep) + part * (SC / 16 * C::kPStep);
       // O follows a moved maximum before any of this tile's P V.
-      if (j >= TG && __any_sync(0xffffffffu, resc)) {
+      if (__builtin_expect(j >= TG && __any_sync(0xffffffffu, resc), 0)) {
         if (TG == 1) {  // the previous P V may still add to O
           mbar_wait(bar(C::kBarO + (x2 ^ 1)), ((j - 1) >> 1) & 1, dead, p.err);
           dead = __any_sync(0xffffffffu, dead);
