@@ -130,11 +130,10 @@ __device__ __forceinline__ uint4 quantise16(const uint4 (&raw)[2], float inv) {
 // 16-byte loads) in flight; where W x 32 x U units are all of the block's
 // rows, they stay in registers between the maximum and the rounding.
 //
-// Bound by HBM (2 bytes read and 1 written for each value) on passes over
-// many rows: four warps with 8 units a lane there (4 x 8192 rows of 8 heads
-// x 256: 94 us with one warp and 8 units, 114 with 4 or 2). By latency on a
-// step's few rows: one warp and 2 units, whose code is short (4 rows of 4
-// heads x 128: 4.3 us, 6.0 with 4 units, most of it instruction fetch).
+// Bound by latency on a step's few rows: one warp and one unit a lane, whose
+// code is short (4 rows of 4 heads x 128: 4.2 us, 6.0 with four units, most of
+// the difference instruction fetch; 16 x 32 scattered rows of 8 x 128: 8.2 us).
+// Passes over many rows: four warps, 8 units (4 x 8192 x 8 x 256: 105 us).
 template <int W, int U>
 __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_store_kernel(const Kv8StoreParams p) {
   constexpr int kJobs = W == 1 ? 8 : 1;  // jobs of a CTA at a time
@@ -317,7 +316,9 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_store_kernel(const 
 // positions: in order, they can only be 0, 1, 2, ...): a block is its T rows,
 // there is nothing to look up and nothing that stays. Four warps take a block
 // of a kv head of K or V, 8 units a thread in flight. A block whose entries
-// are not those positions is left as it was and reported.
+// are not those positions is left as it was and reported. Bound by HBM: 2
+// bytes read and 1 written for each value, 4 x 8192 x 8 x 256 in 61.5 us,
+// 6.5 TB/s.
 __global__ void __launch_bounds__(128) kv8_store_all_kernel(const Kv8StoreParams p) {
   constexpr int U = 8;
   __shared__ uint32_t s_max[4];
