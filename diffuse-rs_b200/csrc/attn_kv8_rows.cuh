@@ -327,7 +327,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
           split_e4m3(v, qf[x][0][i][2 * h + k], qf[x][1][i][2 * h + k]);
         }
       }
-    const float mine = exp2_int(ex);
+    // A row with an infinity has scores that are none: NaN comes out.
+    const float mine = amax == INFINITY ? INFINITY : exp2_int(ex);
 #pragma unroll
     for (int y = 0; y < 2; ++y) qs[x][y] = __shfl_sync(0xffffffffu, mine, (2 * t + y) * 4);
   }

@@ -304,7 +304,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         const int ex = e4m3_exp(fminf(amax, __uint_as_float(0x7f7f0000u)), -120, 120);
         // A negative scale turns Q's sign, so that the scores' factor is not.
         const float inv = p.scale < 0.f ? -exp2_int(-ex) : exp2_int(-ex);
-        if (un == 0) sQs[qr] = exp2_int(ex);
+        // A row with an infinity has scores that are none: NaN comes out.
+        if (un == 0) sQs[qr] = amax == INFINITY ? INFINITY : exp2_int(ex);
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {

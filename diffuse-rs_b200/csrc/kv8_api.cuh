@@ -121,6 +121,10 @@ int kv8_plan(const ca_attn_kv8_args* a, const Kv8View& c, bool split_ok, Kv8Plan
   const int64_t G = a->n_head / c.Hkv;
   const int64_t rows = max_sq * G;
   if (static_cast<int64_t>(c.batch) * c.n_total > INT_MAX) return CA_ERR_UNSUPPORTED;
+  // Measured with 16 sequences of 4128 positions, 4 query heads a kv head, in
+  // us, rows kernel against tile kernel: 8 rows 31 and 45 at head_dim 128, 35
+  // and 51 at 256, 23 and 40 at 64; 16 rows 47 and 45, 49 and 55, 33 and 39;
+  // 20 rows (a tile of 16 more) 89 and 46, 92 and 57, 60 and 40.
   const int tr = rows > 16 && c.hd <= 256 ? 128 : rows > 8 && c.hd <= 128 ? 16 : 8;
   pl->nr = tr;
   const int64_t tiles = (rows + tr - 1) / tr;

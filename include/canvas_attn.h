@@ -479,7 +479,7 @@ typedef struct {
  * positions 0 .. kv_len - 1 of each sequence, masks as in ca_attention_dev
  * (no sequence ids: every sequence has its own cache). Products and sums in
  * fp32, softmax weights in f16 (11 bits). Scales may be any positive finite
- * values. A query row with no visible key gets NaN. A NaN held in V may reach
+ * values, those of V in one sequence within 2^80 of one another. A query row with no visible key gets NaN. A NaN held in V may reach
  * the rows of its sequence and kv head that do not see it. Asynchronous on
  * `stream`; allocates nothing.
  */

@@ -185,6 +185,25 @@ def test_attention_loud_and_quiet_queries():
             run_attention(1, sq, 8, 2, 128, 200, 32, qscale=qscale, scale=0.1 / qscale)
 
 
+def test_attention_nan_and_infinite_queries():
+    # Such a row is NaN, its neighbours are not touched.
+    g = torch.Generator().manual_seed(12)
+    for sq, d in ((1, 128), (40, 128), (40, 256), (2, 512)):
+        cache = cache_of(g, 1, 200, 2, d, 32)
+        q = torch.randn(1, sq, 4, d, generator=g).to(torch.bfloat16).cuda()
+        clean = torch.empty(1, sq, 4, d, device="cuda")
+        kv8.attention(q, cache, clean, scale=0.1)
+        for bad in (float("nan"), float("inf"), float("-inf")):
+            q2, out = q.clone(), torch.empty_like(clean)
+            q2[0, sq - 1, 1, 3] = bad
+            kv8.attention(q2, cache, out, scale=0.1)
+            torch.cuda.synchronize()
+            assert ca.device_status() == ca.CA_OK
+            assert bool(torch.isnan(out[0, sq - 1, 1]).all()), (sq, d, bad)
+            out[0, sq - 1, 1] = clean[0, sq - 1, 1]
+            assert torch.equal(out, clean), (sq, d, bad)
+
+
 def test_attention_sink_and_flat_tail():
     # One key with nearly all the weight of a row, and thousands whose weights
     # are 2^-20 of it but add up.
