@@ -181,6 +181,18 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   const int kvh = blockIdx.y, b = blockIdx.z;
   const int hd = p.c.hd;
 
+  // What needs nothing but the arguments comes first.
+  const uint32_t ring = smem_u32(smem + warp * C::kWarpBytes);
+  const uint32_t bar0 = smem_u32(smem + C::kOffBar) + warp * ST * 8;
+  if (lane == 0) {
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+    for (int s = 0; s < ST; ++s) mbar_init(bar0 + 8 * s, 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  dependency_wait();
+
   const int q_beg = p.cu_q ? p.cu_q[b] : b * p.sq;
   const int q_len = p.cu_q ? p.cu_q[b + 1] - q_beg : p.sq;
   const long long n_rows = static_cast<long long>(q_len) * p.G;
@@ -189,15 +201,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   const int rows = static_cast<int>(min(static_cast<long long>(NR), n_rows - row0));
   const unsigned G = static_cast<unsigned>(p.G);
 
-  // What needs nothing but the arguments comes first: the ring's barriers,
-  // and Q, whose way from HBM is as long as that of kv_len.
-  const uint32_t ring = smem_u32(smem + warp * C::kWarpBytes);
-  const uint32_t bar0 = smem_u32(smem + C::kOffBar) + warp * ST * 8;
-  if (lane == 0) {
-    for (int s = 0; s < ST; ++s) mbar_init(bar0 + 8 * s, 1);
-    fence_barrier_init();
-    fence_proxy_async_smem();
-  }
+  // Q's way from HBM is as long as that of kv_len: both at once.
   uint4 raw[NT][KU][2];
 #pragma unroll
   for (int x = 0; x < NT; ++x) {

@@ -149,6 +149,11 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   const int kvh = blockIdx.y, b = blockIdx.z;
   const int hd = p.c.hd;
 
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  dependency_wait();
   const int q_beg = p.cu_q ? p.cu_q[b] : b * p.sq;
   const int q_len = p.cu_q ? p.cu_q[b + 1] - q_beg : p.sq;
   const long long n_rows = static_cast<long long>(q_len) * p.G;

@@ -46,6 +46,15 @@ struct Kv8StoreParams {
   int* err;
 };
 
+// These kernels are launched so that they may start while the kernel before
+// them in the stream ends (programmatic dependent launch): until
+// dependency_wait returns, which is when that kernel is complete and its
+// writes are visible, they touch nothing in memory but their arguments. Each
+// lets its own successor come up right away in the same manner.
+__device__ __forceinline__ void dependency_wait() {
+  asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
+}
+
 // Two fp32 to two e4m3 (round to nearest even, saturating, NaN kept): lo in
 // the low byte.
 __device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
@@ -137,6 +146,7 @@ __device__ __forceinline__ uint4 quantise16(const uint4 (&raw)[2], float inv) {
 template <int W, int U>
 __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_store_kernel(const Kv8StoreParams p) {
   constexpr int kJobs = W == 1 ? 8 : 1;  // jobs of a CTA at a time
+  dependency_wait();
   __shared__ uint32_t s_max[W];
   const int lane = threadIdx.x & 31;
   const int jt = W == 1 ? lane : threadIdx.x;  // thread of the job
@@ -322,6 +332,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_store_kernel(const 
 __global__ void __launch_bounds__(128) kv8_store_all_kernel(const Kv8StoreParams p) {
   constexpr int U = 8;
   __shared__ uint32_t s_max[4];
+  dependency_wait();
   const int lane = threadIdx.x & 31;
   const int T = p.c.T, hd = p.c.hd, upr = hd / 16, heads2 = 2 * p.c.Hkv;
   const unsigned magic = ((1u << 20) + upr - 1) / upr;
@@ -415,6 +426,7 @@ __device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&w)[8]) {
 // by HBM: 1 byte read and 2 (4) written for each value.
 template <int U>
 __global__ void __launch_bounds__(256) kv8_load_kernel(const Kv8LoadParams p) {
+  dependency_wait();
   const int upr = p.c.Hkv * p.c.hd / 16;  // 16-value units of a row
   const uint8_t* src = blockIdx.y ? p.c.v : p.c.k;
   const float* scales = blockIdx.y ? p.c.v_scale : p.c.k_scale;

@@ -12,6 +12,27 @@ namespace {
 
 constexpr int kSms = 148;
 
+// A launch that may overlap the end of the kernel before it (dependency_wait).
+template <class... P, class... A>
+int launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st,
+                 A... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
+    cudaGetLastError();
+    return CA_ERR_CUDA;
+  }
+  return CA_OK;
+}
+
 // The cache as the kernels see it, or why not.
 int kv8_view(const ca_kv8_cache& c, Kv8View* v) {
   if (!c.k || !c.v || !c.k_scale || !c.v_scale) return CA_ERR_INVALID;
@@ -57,8 +78,7 @@ int kv8_store_impl(const ca_kv8_store_args* a, cudaStream_t st) {
   p.err = a->status;
   if (!p.cu_active && a->n_active == p.c.n_total && p.c.batch <= 65535) {
     const dim3 grid(p.c.n_blocks * 2 * p.c.Hkv, p.c.batch);
-    kv8_store_all_kernel<<<grid, 128, 0, st>>>(p);
-    return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
+    return launch_after(kv8_store_all_kernel, grid, 128, 0, st, p);
   }
   // Entries of the active list a job looks through: one where that leaves
   // half the GPU's warp slots at most one job each, 32 (a lane each) at most.
@@ -70,12 +90,12 @@ int kv8_store_impl(const ca_kv8_store_args* a, cudaStream_t st) {
   if (many) p.rows_per_job = 32;
   const int64_t jobs = (p.rows + p.rows_per_job - 1) / p.rows_per_job * 2 * p.c.Hkv;
   if (many)
-    kv8_store_kernel<4, 8>
-        <<<static_cast<int>(std::min<int64_t>(jobs, kSms * 1024)), 128, 0, st>>>(p);
-  else
-    kv8_store_kernel<1, 1>
-        <<<static_cast<int>(std::min<int64_t>((jobs + 7) / 8, kSms * 64)), 256, 0, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
+    return launch_after(kv8_store_kernel<4, 8>,
+                        dim3(static_cast<unsigned>(std::min<int64_t>(jobs, kSms * 1024))), 128, 0,
+                        st, p);
+  return launch_after(kv8_store_kernel<1, 1>,
+                      dim3(static_cast<unsigned>(std::min<int64_t>((jobs + 7) / 8, kSms * 64))),
+                      256, 0, st, p);
 }
 
 int kv8_load_impl(const ca_kv8_load_args* a, cudaStream_t st) {
@@ -104,9 +124,8 @@ int kv8_load_impl(const ca_kv8_load_args* a, cudaStream_t st) {
   const int64_t blocks =
       many ? std::min<int64_t>((pieces + 3) / 4, std::max<int64_t>(1, 8 * kSms / tensors)) : pieces;
   const dim3 grid(static_cast<unsigned>(blocks), 2, p.c.batch);
-  if (many) kv8_load_kernel<4><<<grid, 256, 0, st>>>(p);
-  else kv8_load_kernel<1><<<grid, 256, 0, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
+  return many ? launch_after(kv8_load_kernel<4>, grid, 256, 0, st, p)
+              : launch_after(kv8_load_kernel<1>, grid, 256, 0, st, p);
 }
 
 // How a call is laid out: which kernel, row tiles and splits of the keys.
@@ -190,8 +209,7 @@ int launch_rows(const Kv8AttnParams& p, cudaStream_t st) {
     attr_done[dev] = true;
   }
   const dim3 grid(p.tiles * p.splits, p.c.Hkv, p.c.batch);
-  attn_kv8_rows_kernel<C><<<grid, C::kThreads, C::kSmem, st>>>(tk, tv, p);
-  return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
+  return launch_after(attn_kv8_rows_kernel<C>, grid, C::kThreads, C::kSmem, st, tk, tv, p);
 }
 
 template <class C>
@@ -210,8 +228,7 @@ int launch_tile(const Kv8AttnParams& p, cudaStream_t st) {
     attr_done[dev] = true;
   }
   const dim3 grid(p.tiles * p.splits, p.c.Hkv, p.c.batch);
-  attn_kv8_tile_kernel<C><<<grid, C::kThreads, C::kSmem, st>>>(tk, tv, p);
-  return cudaGetLastError() == cudaSuccess ? CA_OK : CA_ERR_CUDA;
+  return launch_after(attn_kv8_tile_kernel<C>, grid, C::kThreads, C::kSmem, st, tk, tv, p);
 }
 
 // `check_only`: says whether the call would be taken, and launches nothing.
