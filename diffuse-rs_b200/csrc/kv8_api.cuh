@@ -139,7 +139,8 @@ int kv8_plan(const ca_attn_kv8_args* a, const Kv8View& c, bool split_ok, Kv8Plan
   const int64_t max_sq = a->cu_q ? a->max_sq : a->sq;
   const int64_t G = a->n_head / c.Hkv;
   const int64_t rows = max_sq * G;
-  if (static_cast<int64_t>(c.batch) * c.n_total > INT_MAX) return CA_ERR_UNSUPPORTED;
+  // Rows of the tensor maps are int32, a tile's last ones past the end too.
+  if (static_cast<int64_t>(c.batch) * c.n_total > INT_MAX - 128) return CA_ERR_UNSUPPORTED;
   // Measured with 16 sequences of 4128 positions, 4 query heads a kv head, in
   // us, rows kernel against tile kernel: 8 rows 31 and 45 at head_dim 128, 35
   // and 51 at 256, 23 and 40 at 64; 16 rows 47 and 45, 49 and 55, 33 and 39;

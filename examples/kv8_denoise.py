@@ -33,6 +33,7 @@ class Layer:
         self.cache8 = kv8.Kv8Cache.alloc(batch, n_total, KV, HD, block_tokens=32, device=dev)
         self.k16 = torch.zeros(batch, n_total, KV, HD, dtype=torch.bfloat16, device=dev)
         self.v16 = torch.zeros_like(self.k16)
+        self.kept = {}  # by rows of a sequence: q, k, v, out, positions, the step's arguments
 
 
 def linear(x, w, residual=None, dtype=torch.bfloat16):
@@ -49,16 +50,22 @@ def forward(layers, x, pos, rope, n_total, eight):
     x = x.reshape(b * n, e)
     for ly in layers:
         h = (x.float() * torch.rsqrt(x.float().square().mean(-1, keepdim=True) + 1e-6)).bfloat16()
-        q, k, v = (y.reshape(b, n, -1, HD).contiguous()
-                   for y in linear(h, ly.wqkv).split([HEADS * HD, KV * HD, KV * HD], dim=-1))
-        out = torch.empty_like(q)
         kw = dict(rope=rope, rope_len=n_total, rope_dim=HD, q_norm_w=ly.qn, k_norm_w=ly.kn,
-                  active_pos=pos, scale=HD ** -0.5)
+                  scale=HD ** -0.5)
+        if n not in ly.kept:
+            mk = lambda heads: torch.empty(b, n, heads, HD, dtype=x.dtype, device=x.device)  # noqa: E731
+            q, k, v, out, at = mk(HEADS), mk(KV), mk(KV), mk(HEADS), torch.empty_like(pos)
+            ly.kept[n] = (q, k, v, out, at, torch.empty_like(q),
+                          kv8.make_block_args(q, k, v, ly.cache8, out, active_pos=at, **kw))
+        q, k, v, out, at, q_work, step8 = ly.kept[n]
+        for buf, y in zip((q, k, v), linear(h, ly.wqkv).split([HEADS * HD, KV * HD, KV * HD], -1)):
+            buf.copy_(y.reshape(buf.shape))
+        at.copy_(pos)
         if eight:
-            kv8.attention_block(q, k, v, ly.cache8, out, **kw)
+            kv8.block_args(step8)
         else:
-            ca.attention_block_dev(q, k, v, batch=b, n_active=n, cache_k=ly.k16, cache_v=ly.v16,
-                                   n_total=n_total, q_work=torch.empty_like(q), out=out,
+            ca.attention_block_dev(q, k, v, batch=b, n_active=n, active_pos=at, cache_k=ly.k16,
+                                   cache_v=ly.v16, n_total=n_total, q_work=q_work, out=out,
                                    n_head=HEADS, n_head_kv=KV, head_dim=HD, **kw)
         x = linear(out.view(b * n, e), ly.wo, residual=x)
     return x.view(b, n, e)

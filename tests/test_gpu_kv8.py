@@ -404,6 +404,24 @@ def test_store_reports_bad_positions():
     assert seen <= {0, 3, 4, 5, 7, 9, 20} and {0, 3, 4, 5, 7, 20} <= seen
 
 
+def test_store_of_every_row_checks_its_positions():
+    # As many rows as positions, but one of them elsewhere: its block is left
+    # as it was and reported, the others are written.
+    n, T = 100, 32
+    cache = kv8.Kv8Cache.alloc(2, n, 3, 64, block_tokens=T)
+    x = torch.ones(2, n, 3, 64, dtype=torch.bfloat16, device="cuda")
+    pos = torch.arange(n, dtype=torch.int32).repeat(2, 1)
+    pos[1, 40] = 39
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    kv8.store(cache, x, 2 * x, pos.cuda(), status=status)
+    torch.cuda.synchronize()
+    assert int(status) == ca.CA_ERR_INVALID
+    for held, scale, want in ((cache.k, cache.k_scale, 1.0), (cache.v, cache.v_scale, 2.0)):
+        y = held_values(held, scale, T)
+        assert bool((y[0] == want).all()) and bool((y[1, 64:] == want).all())
+        assert bool((y[1, :32] == want).all()) and bool((y[1, 32:64] == 0).all())
+
+
 # ------------------------------------------------------------------ load
 @pytest.mark.parametrize("B,n,Hkv,d,T,n_pos,dtype", [
     (1, 1, 1, 16, 16, 1, torch.bfloat16), (2, 100, 2, 128, 32, 100, torch.bfloat16),

@@ -101,6 +101,11 @@ def test_attention_arguments(kw, status):
     assert attn_call(**kw) == status
 
 
+def test_caches_past_int32_rows_are_refused():
+    big = c_cache(batch=2, n_total=(1 << 30) - 20)
+    assert attn_call(big) == ca.CA_ERR_UNSUPPORTED
+
+
 def block_call(cache=None, **kw):
     d = dict(q=FAKE, k=FAKE, v=FAKE, n_head=4, n_active=3, active_pos=FAKE, rope=FAKE, rope_len=100,
              rope_dim=128, work=FAKE, out=FAKE, sliding_window=-1, causal_prefix=-1, scale=1.0)
