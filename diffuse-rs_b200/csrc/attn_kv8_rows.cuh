@@ -122,6 +122,14 @@ __device__ __forceinline__ void split_e4m3(const float (&x)[4], uint32_t& hi, ui
        (cvt_e4m3x2(x[2] - back[2], x[3] - back[3]) << 16);
 }
 
+// tanh(x) = 1 - 2 / (2^(2 x log2 e) + 1), good to 2e-7 (the soft-cap's logits
+// to 1e-5 of a unit); the infinities come out as 1 and -1.
+__device__ __forceinline__ float kv8_tanh(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(ex2_approx(x * 2.8853900817779268f) + 1.f));
+  return fmaf(-2.f, r, 1.f);
+}
+
 constexpr float kKv8Shift = 7.f;  // P's f16 exponent for t = m
 constexpr float kKv8Lazy = 8.f;   // how far t may pass m before m moves
 
@@ -430,7 +438,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         float v = st[x][y] * a[y & 1];
-        v = capped ? fmaf(cap_l2, tanh_via_exp2(v), L) : v + L;
+        v = capped ? fmaf(cap_l2, kv8_tanh(v), L) : v + L;
         if (!full) {
           const int key = key0 + g + 8 * (y >> 1);
           v = key >= lo[x][y & 1] && key < hi[x][y & 1] ? v : -INFINITY;

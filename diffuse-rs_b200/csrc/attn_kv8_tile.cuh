@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           const float u = m16[c] * a16[c];
-          const float t = poly ? tanh_poly(u) : tanh_via_exp2(u);
+          const float t = poly ? tanh_poly(u) : kv8_tanh(u);
           cmax = fmaxf(cmax, m16[c] == -INFINITY ? m16[c] : fmaf(cap_l2, t, L16[c]));
         }
       } else {
@@ -710,8 +710,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 y[h][q] = __ffma2_rn(make_float2(x0, x1), make_float2(a16[c], a16[c]),
                                      make_float2(off, off));
               } else if constexpr (CAP == 1) {
-                y[h][q].x = x0 == -INFINITY ? x0 : fmaf(cap_l2, tanh_via_exp2(x0 * a16[c]), off);
-                y[h][q].y = x1 == -INFINITY ? x1 : fmaf(cap_l2, tanh_via_exp2(x1 * a16[c]), off);
+                y[h][q].x = x0 == -INFINITY ? x0 : fmaf(cap_l2, kv8_tanh(x0 * a16[c]), off);
+                y[h][q].y = x1 == -INFINITY ? x1 : fmaf(cap_l2, kv8_tanh(x1 * a16[c]), off);
               } else {
                 const float2 t = tanh_poly2(__fmul2_rn(make_float2(x0, x1),
                                                        make_float2(a16[c], a16[c])));
