@@ -110,7 +110,10 @@ struct TileCfg {
                                       (128u >> 4 << 24);  // f16 x f16 (MN-major), fp32
   static_assert(kOCol + TG * HDP <= 512, "TMEM");
   static_assert(kSmem <= 227 * 1024, "shared memory");
-  static_assert(kSoftWarps * 4096 <= STK * kTile8 + STV * kTile8, "output staging");
+  static constexpr int kRings = STK * kTile8 + STV * kTile8;
+  static_assert(kSoftWarps * 4096 <= kRings, "output staging");
+  static constexpr int kMaxSplits = kRings / 512;  // a join's weights: float [splits][128]
+  static_assert(kMaxSplits >= 148, "weights of a join");
 };
 
 // D[tmem] (+)= A[smem] x B[smem]^T, kind::f8f6f4 (e4m3 in, fp32 accumulate).
@@ -871,33 +874,59 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         __threadfence();
         pml = p.part_ml + cell * p.splits * 256;
         const float* po = p.part_o + cell * p.splits * 128 * static_cast<long long>(hd);
-        const int upr = hd / 4;
-        for (int i = st; i < rows * upr; i += C::kSoftThreads) {
-          const int jr = i / upr, e = (i - jr * upr) * 4;
-          float mj = -INFINITY;
+        // Each split's weight in each row, divided by the row's sum, first (in
+        // the idle rings); then the sums, eight loads of a thread in flight.
+        float* jw = reinterpret_cast<float*>(smem + C::kOffK);
+        for (int jr = st; jr < rows; jr += C::kSoftThreads) {
+          float mj = -INFINITY, lj = 0.f;
+#pragma unroll 8
           for (int k = 0; k < p.splits; ++k) mj = fmaxf(mj, __ldcg(pml + k * 256 + jr));
-          float lj = 0.f;
-          float4 oj = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (mj != -INFINITY) {
-            for (int k = 0; k < p.splits; ++k) {
-              const float w = ex2_approx(__ldcg(pml + k * 256 + jr) - mj);
-              lj = fmaf(__ldcg(pml + k * 256 + 128 + jr), w, lj);
+#pragma unroll 8
+          for (int k = 0; k < p.splits; ++k) {
+            const float w = mj == -INFINITY ? 0.f : ex2_approx(__ldcg(pml + k * 256 + jr) - mj);
+            lj = fmaf(__ldcg(pml + k * 256 + 128 + jr), w, lj);
+            jw[k * 128 + jr] = w;
+          }
+          // A row that sees nothing: 0 / 0.
+          const float ij = mj == -INFINITY ? __int_as_float(0x7fc00000) : __fdiv_rn(1.f, lj);
+          for (int k = 0; k < p.splits; ++k) jw[k * 128 + jr] *= ij;
+        }
+        named_bar_sync(1, C::kSoftThreads);
+        const int upr = hd / 4, total = rows * upr;
+        constexpr int U = 4;
+#pragma unroll 1
+        for (int i0 = st; i0 < total; i0 += U * C::kSoftThreads) {
+          float4 acc[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+          for (int k = 0; k < p.splits; ++k) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              const int i = min(i0 + u * C::kSoftThreads, total - 1);
+              const float w = jw[k * 128 + i / upr];
+              // Rows lie hd apart: element i of the tile is float4 i of the split's.
               const float4 x = __ldcg(reinterpret_cast<const float4*>(
-                  po + (static_cast<long long>(k) * 128 + jr) * hd + e));
-              oj.x = fmaf(x.x, w, oj.x);
-              oj.y = fmaf(x.y, w, oj.y);
-              oj.z = fmaf(x.z, w, oj.z);
-              oj.w = fmaf(x.w, w, oj.w);
+                  po + static_cast<long long>(k) * 128 * hd) + i);
+              acc[u].x = fmaf(x.x, w, acc[u].x);
+              acc[u].y = fmaf(x.y, w, acc[u].y);
+              acc[u].z = fmaf(x.z, w, acc[u].z);
+              acc[u].w = fmaf(x.w, w, acc[u].w);
             }
           }
-          const float ij = __fdiv_rn(1.f, lj);
-          const long long d = row_at[jr] + e;
-          if (p.out_f32)
-            *reinterpret_cast<float4*>(static_cast<float*>(p.out) + d) =
-                make_float4(oj.x * ij, oj.y * ij, oj.z * ij, oj.w * ij);
-          else
-            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + d) =
-                make_uint2(pack_bf16(oj.x * ij, oj.y * ij), pack_bf16(oj.z * ij, oj.w * ij));
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * C::kSoftThreads;
+            if (i < total) {
+              const int jr = i / upr;
+              const long long d = row_at[jr] + (i - jr * upr) * 4;
+              if (p.out_f32)
+                *reinterpret_cast<float4*>(static_cast<float*>(p.out) + d) = acc[u];
+              else
+                *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + d) =
+                    make_uint2(pack_bf16(acc[u].x, acc[u].y), pack_bf16(acc[u].z, acc[u].w));
+            }
+          }
         }
       }
     }
