@@ -40,6 +40,8 @@
 // their fixed part, exponentials on the FMA pipe to their issue slots.
 #pragma once
 
+#include <cfloat>
+
 #include "attn_kv8_rows.cuh"
 
 namespace ca {
@@ -591,6 +593,13 @@ __global__ void __launch_bounds__(C::kThreads, 1)
 #pragma unroll
         for (int i = 0; i < SC; ++i)
           sr[i] = static_cast<uint32_t>(i - v0) < v1 ? sr[i] : -INFINITY;
+        // A masked score has to stay -inf times its piece's factor. That one
+        // is no number above zero where nothing was written (scale 0, or
+        // whatever the allocation held), where scale is 0, or where it
+        // underflowed (a row of zeros over a block of zeros): the smallest
+        // normal number stands in, which adds nothing to a visible score.
+#pragma unroll
+        for (int c = 0; c < NC; ++c) a16[c] = fmaxf(a16[c], FLT_MIN);
       }
       float cmax = -INFINITY;
       float m16[NC];  // each piece's largest score
