@@ -8,11 +8,16 @@ with a scale for each block of positions and kv head.
 
 Each call has a `make_*_args` form for programs that keep their buffers: the
 argument block is built once and `*_args(a, stream)` launches it. All calls
-are asynchronous on `stream` and allocate nothing, except that
-`make_attention_args` makes the workspace when none is passed.
+are asynchronous on `stream` (None: the legacy default stream) and allocate
+nothing, except for scratch that is not passed: `attention` and
+`attention_block` make it on the stream that they launch on, `make_*_args` on
+torch's current stream, which the first launch on another stream waits for.
+Like every tensor of a call, the arguments are to be kept until the work that
+was launched with them is done.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from dataclasses import dataclass
 from typing import Any, Optional
@@ -82,6 +87,59 @@ for _name, _args in (("ca_kv8_store", CaKv8StoreArgs), ("ca_kv8_load", CaKv8Load
     _f.restype = ctypes.c_int
 lib.ca_attention_kv8_workspace.argtypes = [ctypes.POINTER(CaAttnKv8Args)]
 lib.ca_attention_kv8_workspace.restype = ctypes.c_int64
+
+
+def _torch_stream(stream, device):
+    """torch's object for the stream that a launch with `stream` goes to."""
+    import torch
+    handle = _stream(stream)
+    if not handle:
+        return torch.cuda.default_stream(device)
+    return torch.cuda.ExternalStream(handle, device=device)
+
+
+def _scratch_on(stream, x, needed):
+    """A context in which torch allocates on the stream of a launch, so that
+    scratch is cleared before its kernels run there and, once dropped, goes to
+    none but later work of that stream."""
+    if not needed or not x.is_cuda:
+        return contextlib.nullcontext()
+    import torch
+    return torch.cuda.stream(_torch_stream(stream, x.device))
+
+
+class _Made:
+    """Scratch that a make_*_args call made on torch's current stream: where
+    and when, for launches on other streams."""
+
+    def __init__(self, device):
+        import torch
+        here = torch.cuda.current_stream(device)
+        self.device, self.ordered = device, {here.cuda_stream}
+        # In a capture the scratch belongs to the graph, as its launches do.
+        self.event = None if torch.cuda.is_current_stream_capturing() else here.record_event()
+
+    def before(self, stream):
+        """Orders what is launched on `stream` next after the scratch."""
+        handle = _stream(stream) or 0
+        if handle in self.ordered or self.event is None:
+            return
+        import torch
+        to = _torch_stream(stream, self.device)
+        with torch.cuda.stream(to):
+            # A capture cannot wait for work outside it; beginning one after
+            # the scratch was cleared is the caller's part (torch.cuda.graph
+            # waits for the device).
+            if torch.cuda.is_current_stream_capturing():
+                return
+        to.wait_event(self.event)
+        self.ordered.add(handle)
+
+
+def _after_scratch(a, stream):
+    made = getattr(a, "_made", None)
+    if made is not None:
+        made.before(stream)
 
 
 @dataclass
@@ -250,11 +308,13 @@ def make_attention_args(q, cache: Kv8Cache, out, *, q_pos=None, kv_len=None, cu_
                       _ptr(kv_len), -1 if sliding_window is None else int(sliding_window),
                       -1 if causal_prefix is None else int(causal_prefix), _ptr(seq_prefix),
                       float(scale), float(softcap), _ptr(status), None, 0)
+    a._made = None
     if workspace is None:
         n = workspace_bytes(a)
         if n:
             import torch
             workspace = torch.zeros(n, dtype=torch.uint8, device=q.device)
+            a._made = _Made(q.device) if q.is_cuda else None
     if workspace is not None and workspace is not False:
         a.workspace, a.workspace_bytes = _ptr(workspace), workspace.numel() * \
             workspace.element_size()
@@ -263,12 +323,15 @@ def make_attention_args(q, cache: Kv8Cache, out, *, q_pos=None, kv_len=None, cu_
 
 
 def attention_args(a: CaAttnKv8Args, stream=None) -> None:
+    _after_scratch(a, stream)
     _check(lib.ca_attention_kv8_dev(ctypes.byref(a), _stream(stream)), "ca_attention_kv8_dev")
 
 
 def attention(q, cache: Kv8Cache, out, *, stream=None, **kw) -> None:
     """ca_attention_kv8_dev: attention over the cache (see make_attention_args)."""
-    attention_args(make_attention_args(q, cache, out, **kw), stream)
+    with _scratch_on(stream, q, kw.get("workspace") is None):
+        a = make_attention_args(q, cache, out, **kw)
+    attention_args(a, stream)
 
 
 def make_block_args(q, k, v, cache: Kv8Cache, out, *, active_pos, rope, rope_len: int,
@@ -295,7 +358,8 @@ def make_block_args(q, k, v, cache: Kv8Cache, out, *, active_pos, rope, rope_len
     _i32("cu_active", cu_active, c.batch + 1)
     _i32("held", held, c.batch)
     need = rows * (heads + 2 * c.n_head_kv) * c.head_dim
-    if work is None:
+    made = work is None
+    if made:
         import torch
         work = torch.empty(need, dtype=torch.bfloat16, device=q.device)
     if str(work.dtype) != "torch.bfloat16" or work.numel() < need:
@@ -312,10 +376,14 @@ def make_block_args(q, k, v, cache: Kv8Cache, out, *, active_pos, rope, rope_len
                        t.out_row_stride, t.sliding_window, t.causal_prefix, _ptr(seq_prefix),
                        float(scale), float(softcap), _ptr(status), t.workspace, t.workspace_bytes)
     a._keep = (t, k, v, active_pos, cu_active, held, q_norm_w, k_norm_w, rope, work, status)
+    a._made = t._made
+    if made and a._made is None and q.is_cuda:
+        a._made = _Made(q.device)
     return a
 
 
 def block_args(a: CaBlockKv8Args, stream=None) -> None:
+    _after_scratch(a, stream)
     _check(lib.ca_attention_block_kv8_dev(ctypes.byref(a), _stream(stream)),
            "ca_attention_block_kv8_dev")
 
@@ -323,4 +391,6 @@ def block_args(a: CaBlockKv8Args, stream=None) -> None:
 def attention_block(q, k, v, cache: Kv8Cache, out, *, stream=None, **kw) -> None:
     """ca_attention_block_kv8_dev: one layer's step over the cache (see
     make_block_args)."""
-    block_args(make_block_args(q, k, v, cache, out, **kw), stream)
+    with _scratch_on(stream, q, kw.get("workspace") is None or kw.get("work") is None):
+        a = make_block_args(q, k, v, cache, out, **kw)
+    block_args(a, stream)
