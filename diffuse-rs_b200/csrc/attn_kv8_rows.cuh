@@ -223,8 +223,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       const int e = (t + 4 * i) * 16;
       raw[x][i][0] = raw[x][i][1] = make_uint4(0u, 0u, 0u, 0u);
       if (r < rows && e < hd) {
-        raw[x][i][0] = __ldg(reinterpret_cast<const uint4*>(src + e));
-        raw[x][i][1] = __ldg(reinterpret_cast<const uint4*>(src + e) + 1);
+        raw[x][i][0] = reinterpret_cast<const uint4*>(src + e)[0];
+        raw[x][i][1] = reinterpret_cast<const uint4*>(src + e)[1];
       }
     }
   }
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         const int r = 8 * x + 2 * t + y;
         if (r < rows) {
           const int tok = static_cast<int>(static_cast<unsigned>(row0 + r) / G);
-          const int pos = p.q_pos ? __ldg(p.q_pos + q_beg + tok) : len - q_len + tok;
+          const int pos = p.q_pos ? p.q_pos[q_beg + tok] : len - q_len + tok;
           kv8_interval(pos, len, p.window, prefix, lo[x][y], hi[x][y]);
           // A row that sees nothing does not widen the hull.
           if (lo[x][y] < hi[x][y]) {
@@ -298,8 +298,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   auto scales = [&](int ch) {
     if (ch < c_end) {
       const long long blk = static_cast<long long>((ch * 16) >> shift) * p.c.Hkv;
-      nk = __ldg(ksc + blk);
-      nv = __ldg(vsc + blk);
+      nk = ksc[blk];
+      nv = vsc[blk];
     }
   };
   scales(c0);

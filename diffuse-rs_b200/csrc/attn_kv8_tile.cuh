@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     hi = len;
     if (!masked) return;
     const int tok = static_cast<int>((row0 + r) / p.G);
-    const int pos = p.q_pos ? __ldg(p.q_pos + q_beg + tok) : len - q_len + tok;
+    const int pos = p.q_pos ? p.q_pos[q_beg + tok] : len - q_len + tok;
     kv8_interval(pos, len, p.window, prefix, lo, hi);
   };
   const int tok0 = b * p.c.n_total;  // the sequence's first row of the tensor maps
@@ -294,8 +294,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
           const uint4* src = reinterpret_cast<const uint4*>(
               p.q + (q_beg + static_cast<long long>(tok)) * p.q_row_stride +
               (kvh * p.G + static_cast<int>(rr - tok * p.G)) * static_cast<long long>(hd) + e);
-          raw[i][0] = __ldg(src);
-          raw[i][1] = __ldg(src + 1);
+          raw[i][0] = src[0];
+          raw[i][1] = src[1];
         }
       }
 #pragma unroll
@@ -522,8 +522,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       if (j < n) {
         const int key = (kt0 + j) * BN + part * SC + (lane % NC) * 16;
         const long long at = static_cast<long long>(min(key >> shift, p.c.n_blocks - 1)) * p.c.Hkv;
-        nk = __ldg(ksc + at);
-        nv = __ldg(vsc + at);
+        nk = ksc[at];
+        nv = vsc[at];
       }
     };
     float* my_sc = reinterpret_cast<float*>(smem + C::kOffSc) + (warp - 4) * 6 * NC;

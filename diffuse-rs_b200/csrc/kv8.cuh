@@ -50,7 +50,10 @@ struct Kv8StoreParams {
 // them in the stream ends (programmatic dependent launch): until
 // dependency_wait returns, which is when that kernel is complete and its
 // writes are visible, they touch nothing in memory but their arguments. Each
-// lets its own successor come up right away in the same manner.
+// lets its own successor come up right away in the same manner. What the
+// kernel before may have written is read with plain loads: read-only ones
+// (__ldg, ld.global.nc) are defined only for data that does not change from
+// the start of the kernel that reads it, and that start is before the wait.
 __device__ __forceinline__ void dependency_wait() {
   asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
 }
@@ -176,19 +179,19 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_store_kernel(const 
         int lo = 0, hi = p.c.batch - 1;
         while (lo < hi) {
           const int mid = (lo + hi + 1) >> 1;
-          if (__ldg(p.cu_active + mid) <= mine) lo = mid;
+          if (p.cu_active[mid] <= mine) lo = mid;
           else hi = mid - 1;
         }
         my_b = lo;
-        s0 = __ldg(p.cu_active + lo);
-        my_end = min(static_cast<long long>(__ldg(p.cu_active + lo + 1)), p.rows);
+        s0 = p.cu_active[lo];
+        my_end = min(static_cast<long long>(p.cu_active[lo + 1]), p.rows);
       } else {
         my_b = static_cast<int>(mine / p.na);
         s0 = static_cast<long long>(my_b) * p.na;
         my_end = s0 + p.na;
       }
-      my_pos = __ldg(p.pos + mine);
-      const int before = mine > s0 ? __ldg(p.pos + mine - 1) : -1;
+      my_pos = p.pos[mine];
+      const int before = mine > s0 ? p.pos[mine - 1] : -1;
       if (my_pos < 0 || my_pos >= p.c.n_total || my_pos <= before || mine >= my_end) {
         if (p.err) atomicExch(p.err, kErrInvalidRow);
       } else {
@@ -211,7 +214,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_store_kernel(const 
       for (int c = 0; c < 4; ++c) {
         if (more && c * 32 < T) {
           const long long j = i + c * 32 + lane;
-          const int q = j < s1 ? __ldg(p.pos + j) : -1;
+          const int q = j < s1 ? p.pos[j] : -1;
           int prev = __shfl_up_sync(0xffffffffu, q, 1);
           if (lane == 0) prev = last;
           last = __shfl_sync(0xffffffffu, q, 31);
@@ -228,7 +231,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_store_kernel(const 
         }
       }
       const int in_block = min(T, p.c.n_total - blk * T);
-      const int held = p.kv_len ? min(max(__ldg(p.kv_len + b) - blk * T, 0), in_block) : in_block;
+      const int held = p.kv_len ? min(max(p.kv_len[b] - blk * T, 0), in_block) : in_block;
       bool stays = false;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -253,8 +256,8 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_store_kernel(const 
             const int r = row_of(u), e = (u - r * upr) * 16;
             const uint4* from =
                 reinterpret_cast<const uint4*>(src + ((i + r) * p.c.Hkv + h) * hd + e);
-            raw[k][0] = __ldg(from);
-            raw[k][1] = __ldg(from + 1);
+            raw[k][0] = from[0];
+            raw[k][1] = from[1];
           }
         }
       };
@@ -289,13 +292,18 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_store_kernel(const 
                       static_cast<long long>(h) * hd;
       for (int u0 = 0; u0 < units; u0 += 32 * W * U) {
         if (units > 32 * W * U) read(u0);
+        int to[U];  // positions, before the first store
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          const int u = u0 + 32 * W * k + jt;
+          to[k] = u < units ? p.pos[i + row_of(u)] : 0;
+        }
 #pragma unroll
         for (int k = 0; k < U; ++k) {
           const int u = u0 + 32 * W * k + jt;
           if (u < units) {
             const int r = row_of(u), e = (u - r * upr) * 16;
-            const int q = __ldg(p.pos + i + r);
-            *reinterpret_cast<uint4*>(base + q * p.c.row_stride + e) = quantise16(raw[k], inv);
+            *reinterpret_cast<uint4*>(base + to[k] * p.c.row_stride + e) = quantise16(raw[k], inv);
           }
         }
       }
@@ -356,8 +364,8 @@ __global__ void __launch_bounds__(128) kv8_store_all_kernel(const Kv8StoreParams
         const unsigned r = (u * magic) >> 20;
         const uint4* from = reinterpret_cast<const uint4*>(
             src + static_cast<long long>(r) * src_stride + (u - r * upr) * 16);
-        raw[k][0] = __ldg(from);
-        raw[k][1] = __ldg(from + 1);
+        raw[k][0] = from[0];
+        raw[k][1] = from[1];
       }
     }
   };
@@ -375,7 +383,7 @@ __global__ void __launch_bounds__(128) kv8_store_all_kernel(const Kv8StoreParams
       }
   }
   const bool bad = static_cast<int>(threadIdx.x) < n &&
-                   __ldg(p.pos + row0 + threadIdx.x) != pos0 + static_cast<int>(threadIdx.x);
+                   p.pos[row0 + threadIdx.x] != pos0 + static_cast<int>(threadIdx.x);
   uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(amax_of(pair)));
   if (lane == 0) s_max[threadIdx.x >> 5] = top;
   if (__syncthreads_or(bad)) {
@@ -448,25 +456,30 @@ __global__ void __launch_bounds__(256) kv8_load_kernel(const Kv8LoadParams p) {
     for (long long at = static_cast<long long>(blockIdx.x) * U * rows + mine; at < p.n_pos;
          at += static_cast<long long>(gridDim.x) * U * rows) {
       const int i0 = static_cast<int>(at);
+      int q[U];  // positions; -1: no row
+      bool bad = false;
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int i = i0 + k * step;
+        const bool row = i < p.n_pos && i >= i0;
+        q[k] = row ? (pos ? pos[i] : i) : -1;
+        const bool held = q[k] >= 0 && q[k] < p.c.n_total;
+        bad |= row && !held;
+        q[k] = held ? q[k] : -1;
+      }
       uint4 raw[U];
       float s[U];
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        const int i = i0 + k * step;
-        s[k] = -1.f;
-        if (i < p.n_pos && i >= i0) {
-          const int q = pos ? __ldg(pos + i) : i;
-          if (q >= 0 && q < p.c.n_total) {
-            raw[k] = __ldg(reinterpret_cast<const uint4*>(from + q * p.c.row_stride));
-            s[k] = __ldg(sc + (q >> shift) * p.c.Hkv);
-          } else if (p.err) {
-            atomicExch(p.err, kErrInvalidRow);
-          }
+        if (q[k] >= 0) {
+          raw[k] = *reinterpret_cast<const uint4*>(from + q[k] * p.c.row_stride);
+          s[k] = sc[(q[k] >> shift) * p.c.Hkv];
         }
       }
+      if (bad && p.err) atomicExch(p.err, kErrInvalidRow);
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        if (s[k] == -1.f) continue;
+        if (q[k] < 0) continue;
         const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
         float x[16];
 #pragma unroll
