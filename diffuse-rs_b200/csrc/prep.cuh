@@ -64,6 +64,12 @@ __device__ __forceinline__ long long cache_row(const PrepParams& p, long long to
   return static_cast<long long>(__ldg(p.cu_total + lo)) + pos;
 }
 
+// Row of the (sin, cos) table of a position. One out of range (the 8-bit
+// cache's store, which follows this pass, reports it) takes the last row.
+__device__ __forceinline__ long long rope_row(const PrepParams& p, int pos) {
+  return min(static_cast<unsigned>(pos), static_cast<unsigned>(p.rope_len - 1));
+}
+
 __device__ __forceinline__ uint32_t pack2_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -123,8 +129,8 @@ __global__ void __launch_bounds__(256) prep_block_kernel(const PrepParams p) {
     }
     const int half = rope ? p.rope_dim / 2 : 0;
     for (int i = lane; i < half; i += 32) {
-      const float sn = p.rope[2 * (static_cast<long long>(pos) * half + i)];
-      const float cs = p.rope[2 * (static_cast<long long>(pos) * half + i) + 1];
+      const float sn = p.rope[2 * (rope_row(p, pos) * half + i)];
+      const float cs = p.rope[2 * (rope_row(p, pos) * half + i) + 1];
       const float a = buf[i], bb = buf[i + half];
       dst[i] = __float2bfloat16_rn(__fsub_rn(__fmul_rn(a, cs), __fmul_rn(bb, sn)));
       dst[i + half] = __float2bfloat16_rn(__fadd_rn(__fmul_rn(a, sn), __fmul_rn(bb, cs)));
@@ -171,7 +177,7 @@ __global__ void __launch_bounds__(256) prep_token_kernel(const PrepParams p) {
     const bool rot = e0 < 2 * half;
     {
       const int idx = e0 < half ? e0 : e0 - half;
-      const float4* t4 = reinterpret_cast<const float4*>(p.rope + 2 * (static_cast<long long>(pos) * half + idx));
+      const float4* t4 = reinterpret_cast<const float4*>(p.rope + 2 * (rope_row(p, pos) * half + idx));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float4 v = rot ? __ldg(t4 + i) : make_float4(0.f, 1.f, 0.f, 1.f);
@@ -322,7 +328,7 @@ __global__ void __launch_bounds__(256) prep_pair_kernel(const PrepParams p) {
     float sn[4], cs[4];
     {
       const float4* t4 =
-          reinterpret_cast<const float4*>(p.rope + 2 * (static_cast<long long>(pos) * HALF + e0));
+          reinterpret_cast<const float4*>(p.rope + 2 * (rope_row(p, pos) * HALF + e0));
       const float4 a = __ldg(t4), c = __ldg(t4 + 1);
       sn[0] = a.x; cs[0] = a.y; sn[1] = a.z; cs[1] = a.w;
       sn[2] = c.x; cs[2] = c.y; sn[3] = c.z; cs[3] = c.w;
@@ -470,7 +476,7 @@ __global__ void __launch_bounds__(kPrepThreads) prep_bulk_kernel(const PrepParam
     {
       const int idx = e0 < half ? e0 : e0 - half;
       const float4* t4 =
-          reinterpret_cast<const float4*>(p.rope + 2 * (static_cast<long long>(pos) * half + idx));
+          reinterpret_cast<const float4*>(p.rope + 2 * (rope_row(p, pos) * half + idx));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float4 v = rot ? __ldg(t4 + i) : make_float4(0.f, 1.f, 0.f, 1.f);
@@ -670,7 +676,7 @@ __global__ void __launch_bounds__(kRingThreads) prep_ring_kernel(const PrepParam
         for (int t = 0; t < nt; ++t) {
           const int pos = __ldg(p.pos + tok0 + t);
           pos_s[t] = pos;  // ordered before the consumers' reads by the stage barrier
-          bulk_load(dst + tab_off + t * HD * 4, p.rope + static_cast<long long>(pos) * HD,
+          bulk_load(dst + tab_off + t * HD * 4, p.rope + rope_row(p, pos) * HD,
                     HD * 4, bars + 8 * s);
         }
       }
