@@ -298,6 +298,8 @@ def make_attention_args(q, cache: Kv8Cache, out, *, q_pos=None, kv_len=None, cu_
             raise ValueError(f"{name}: only the stride between tokens may differ from dense")
         strides.append(rs if x.shape[-3] > 1 or (want == 4 and c.batch > 1) else 0)
     total = int(q.shape[0]) if want == 3 else int(q.shape[0]) * int(q.shape[1])
+    if cu_q is not None and total > c.batch * int(max_sq):
+        raise ValueError("max_sq must be the largest query count of a sequence")
     _i32("q_pos", q_pos, total)
     _i32("kv_len", kv_len, c.batch)
     _i32("cu_q", cu_q, c.batch + 1)
@@ -352,6 +354,8 @@ def make_block_args(q, k, v, cache: Kv8Cache, out, *, active_pos, rope, rope_len
             raise ValueError(f"{name} must have q's rows")
     if cu_active is None and c.batch and rows % c.batch:
         raise ValueError("rows must be the same for every sequence (or pass cu_active)")
+    if cu_active is not None and rows > c.batch * int(max_active):
+        raise ValueError("max_active must be the largest row count of a sequence")
     if str(rope.dtype) != "torch.float32" or rope.numel() < rope_len * (rope_dim // 2) * 2:
         raise ValueError("rope must be float32 [rope_len, rope_dim / 2, 2]")
     _i32("active_pos", active_pos, rows)

@@ -174,6 +174,8 @@ int attn_kv8_check(const ca_attn_kv8_args* a, Kv8View* c) {
   if (c->batch > 65535 || c->Hkv > 65535) return CA_ERR_UNSUPPORTED;
   const int64_t total_q = a->cu_q ? a->total_q : static_cast<int64_t>(c->batch) * a->sq;
   if (total_q > INT_MAX) return CA_ERR_UNSUPPORTED;
+  // Rows that no sequence could hold would be left unwritten.
+  if (a->cu_q && total_q > static_cast<int64_t>(c->batch) * a->max_sq) return CA_ERR_INVALID;
   return CA_OK;
 }
 

@@ -452,8 +452,9 @@ typedef struct {
     int32_t n_head;
     int32_t sq;               /* query rows of each sequence (cu_q NULL) */
     const int32_t* cu_q;      /* int32 [batch + 1] row offsets, or NULL */
-    int32_t max_sq;           /* with cu_q: largest per-sequence query count */
-    int64_t total_q;          /* with cu_q: cu_q[batch] */
+    int32_t max_sq;           /* with cu_q: largest per-sequence query count (rows past it
+                                 are not written) */
+    int64_t total_q;          /* with cu_q: cu_q[batch], at most batch * max_sq */
     const int32_t* q_pos;     /* int32 [total_q] positions; NULL: the last held ones,
                                  kv_len - sq + row */
     const int32_t* kv_len;    /* int32 [batch]: positions held (clamped to 0 .. n_total);
@@ -497,7 +498,7 @@ typedef struct {
     const int32_t* active_pos; /* int32 [rows], 0 .. n_total - 1, ascending within a sequence */
     const int32_t* cu_active;  /* int32 [batch + 1] or NULL */
     int32_t max_active;        /* with cu_active: largest per-sequence row count */
-    int64_t total_active;      /* with cu_active: cu_active[batch] */
+    int64_t total_active;      /* with cu_active: cu_active[batch], at most batch * max_active */
     const int32_t* held;       /* int32 [batch]: positions held before the call; NULL = n_total */
     const int32_t* kv_len;     /* int32 [batch]: positions held after it; NULL = n_total */
     const float* q_norm_w;     /* as ca_block_args, from here to rope_dim */

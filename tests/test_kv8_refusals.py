@@ -175,3 +175,30 @@ def test_python_checks():
         kv8.Kv8Cache(cache.k, cache.v, cache.k_scale, cache.v_scale, 32).to_c()
     with pytest.raises(ValueError):
         kv8.Kv8Cache(cache.k, cache.v, cache.k_scale, cache.v_scale, 24).to_c()
+
+
+def test_ragged_rows_need_their_largest_count():
+    # With the count left at 0, or too small for the rows, rows would be left
+    # unwritten: refused by the C entries before anything is launched ...
+    ragged = dict(cu_q=FAKE, total_q=9)
+    for max_sq, status in ((0, ca.CA_ERR_INVALID), (4, ca.CA_ERR_INVALID)):
+        assert attn_call(max_sq=max_sq, **ragged) == status
+        a = attn_args(max_sq=max_sq, **ragged)
+        assert ca.lib.ca_attention_kv8_workspace(ctypes.byref(a)) == status
+        assert block_call(cu_active=FAKE, total_active=9, max_active=max_sq) == status
+    assert kv8.workspace_bytes(attn_args(max_sq=5, **ragged)) >= 0
+    # ... and by Python, where it has a default.
+    cache = kv8.Kv8Cache.alloc(2, 40, 2, 64, block_tokens=16, device="cpu")
+    q = torch.zeros(3, 4, 64, dtype=torch.bfloat16)
+    kv = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    cu = torch.tensor([0, 1, 3], dtype=torch.int32)
+    kv8.make_attention_args(q, cache, q.clone(), cu_q=cu, max_sq=2, workspace=False)
+    for kw in (dict(), dict(max_sq=1)):
+        with pytest.raises(ValueError, match="max_sq"):
+            kv8.make_attention_args(q, cache, q.clone(), cu_q=cu, workspace=False, **kw)
+    block = dict(active_pos=torch.zeros(3, dtype=torch.int32), rope=torch.zeros(40, 2), rope_len=40,
+                 rope_dim=0, cu_active=cu, workspace=False)
+    kv8.make_block_args(q, kv, kv, cache, q.clone(), max_active=2, **block)
+    for kw in (dict(), dict(max_active=1)):
+        with pytest.raises(ValueError, match="max_active"):
+            kv8.make_block_args(q, kv, kv, cache, q.clone(), **kw, **block)
