@@ -183,7 +183,8 @@ class Kv8Cache:
                     or not x.is_contiguous():
                 raise ValueError(f"{name} must be contiguous float32 of shape {(b, n_blocks, h)}")
         return CaKv8Cache(_ptr(self.k), _ptr(self.v), _ptr(self.k_scale), _ptr(self.v_scale), b, n,
-                          h, d, int(self.block_tokens), int(self.k.stride(1)) if n > 1 else 0)
+                          h, d, int(self.block_tokens),
+                          int(self.k.stride(1)) if n > 1 or b > 1 else 0)
 
 
 def _rows(name, x, dtypes, heads, head_dim):

@@ -202,3 +202,13 @@ def test_ragged_rows_need_their_largest_count():
     for kw in (dict(), dict(max_active=1)):
         with pytest.raises(ValueError, match="max_active"):
             kv8.make_block_args(q, kv, kv, cache, q.clone(), **kw, **block)
+
+
+@pytest.mark.parametrize("batch,n,stride", [(3, 5, 256), (3, 1, 256), (1, 5, 256), (1, 1, 0)])
+def test_stride_of_a_cache_in_wider_rows(batch, n, stride):
+    # The first 2 of 4 heads; with one position a sequence the stride is still
+    # what lies between the sequences.
+    wide = kv8.Kv8Cache.alloc(batch, n, 4, 64, block_tokens=16, device="cpu")
+    cut = kv8.Kv8Cache(wide.k[:, :, :2], wide.v[:, :, :2], wide.k_scale[:, :, :2].contiguous(),
+                       wide.v_scale[:, :, :2].contiguous(), 16)
+    assert cut.to_c().row_stride == stride
