@@ -366,7 +366,25 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     const float ks = nk, L = kv8_log2(nv);
     scales(ch + C::kGroups);
     mbar_wait(bar0 + 8 * s, (it / ST) & 1, dead, p.err);
-    if (__any_sync(0xffffffffu, dead)) break;
+    if (__builtin_expect(__any_sync(0xffffffffu, dead), 0)) {
+      // A wait ran out: leave no copy of this warp's in flight (the ring is
+      // about to hold its sums, and shared memory ends with the CTA), and
+      // make its rows NaN.
+      if (lane == 0) {
+        bool d2 = false;
+        for (int k = 0; k < ST && ch + k * C::kGroups < c_end; ++k)
+          mbar_wait(bar0 + 8 * ((it + k) % ST), ((it + k) / ST) & 1, d2, p.err);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          m[x][y] = 0.f;  // a maximum, so that the joins take the sum in
+          l[x][y] = __int_as_float(0x7fc00000);
+        }
+      break;
+    }
     const uint32_t kb = ring + s * C::kStage, vb = kb + C::KC * C::kCol;
     // S^T: keys g and g + 8 of the chunk as rows, query rows as columns.
     float st[NT][4];
