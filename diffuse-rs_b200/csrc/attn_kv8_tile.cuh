@@ -355,14 +355,17 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         const int NS = is_k ? C::STK : C::STV;
         // The first tiles were asked for before Q; the rest of the rings only
         // now, so as not to stand in Q's way.
-        for (int u = 1; u < n; ++u) {
+        int u = 1;
+        for (; u < n; ++u) {
           const int s = u % NS;
           if (u >= NS && !mbar_wait(bar(empty + s), ((u / NS) - 1) & 1, dead, p.err)) break;
           load_tile(is_k ? &tm_k : &tm_v, is_k ? sK : sV8, full, u, s);
         }
-        bool d2 = false;  // leave no copy in flight
-        for (int u = max(0, n - NS); u < n; ++u)
-          mbar_wait(bar(full + u % NS), (u / NS) & 1, d2, p.err);
+        // Leave no copy in flight: those of the last tiles asked for.
+        const int end = n > 0 ? u : 0;
+        bool d2 = false;
+        for (int w = max(0, end - NS); w < end; ++w)
+          mbar_wait(bar(full + w % NS), (w / NS) & 1, d2, p.err);
       }
     } else if (warp == 1 && lane == 0) {
       // ---------------------------------------------------------- MMA issue
