@@ -138,7 +138,9 @@ __device__ __forceinline__ uint4 quantise16(const uint4 (&raw)[2], float inv) {
 // grew, the rows that stay. A job is rows_per_job consecutive entries of the
 // active list, for one head of K or V; it takes on the blocks whose first
 // active row lies among them and follows each into the next job's entries,
-// so every block has exactly one writer. A lane has U 16-value units (two
+// so every block has exactly one writer (where a sequence's positions do not
+// ascend, which is reported, a block may have two: its contents are then
+// unspecified). A lane has U 16-value units (two
 // 16-byte loads) in flight; where W x 32 x U units are all of the block's
 // rows, they stay in registers between the maximum and the rounding.
 //

@@ -405,8 +405,10 @@ typedef struct {
     int64_t total_active;      /* with cu_active: cu_active[batch] */
     const int32_t* kv_len;     /* int32 [batch]: positions held before this call, or NULL */
     int32_t* status;           /* device int32 or NULL: set to CA_ERR_INVALID by a position
-                                  out of range or out of order (its row, and later rows
-                                  of the same block, may be skipped) */
+                                  out of range or out of order. Rows out of range are
+                                  skipped, others of their block may be; where a
+                                  sequence's positions do not ascend, what the blocks that
+                                  its rows fall in hold afterwards is unspecified */
 } ca_kv8_store_args;
 
 /*
@@ -479,10 +481,13 @@ typedef struct {
  * the 8-bit cache: bf16 queries, K and V taken as they are held, keys at
  * positions 0 .. kv_len - 1 of each sequence, masks as in ca_attention_dev
  * (no sequence ids: every sequence has its own cache). Products and sums in
- * fp32, softmax weights in f16 (11 bits). Scales may be any positive finite
- * values, those of V in one sequence within 2^80 of one another. A query row with no visible key gets NaN. A NaN held in V may reach
- * the rows of its sequence and kv head that do not see it. Asynchronous on
- * `stream`; allocates nothing.
+ * fp32, softmax weights in f16 (11 bits); queries in two e4m3 terms, which
+ * hold bf16's bits down to 2^-10 of a row's largest element and 2^-18 of that
+ * element below. Scales of held positions may be any positive finite values,
+ * those of V from 2^-80 to 2^120 and, in one sequence, within 2^80 of one
+ * another; blocks past kv_len may hold anything. A query row with no visible
+ * key gets NaN. A NaN held in V may reach the rows of its sequence and kv head
+ * that do not see it. Asynchronous on `stream`; allocates nothing.
  */
 int ca_attention_kv8_dev(const ca_attn_kv8_args* a, void* stream);
 
