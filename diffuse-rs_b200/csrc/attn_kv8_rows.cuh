@@ -26,11 +26,11 @@
 // whole 16-byte pieces of a row.
 //
 // Bound by HBM: 2 hd bytes a key. One token over 131072 positions of 8 kv
-// heads x 128: 51 us, 5.2 TB/s, of which about 8 us are start and join (the
+// heads x 128: 53 us, 5.1 TB/s, of which about 8 us are start and join (the
 // 16-row form of both products, with K and V turned in registers, took 90);
-// 1001 positions of 4 kv heads: 10.4 us, all latency. Long caches are split over CTAs; the last
-// CTA of a row tile to finish joins their partial sums in order, so results
-// do not depend on which that was.
+// 1001 positions of 4 kv heads: 9.4 us, all latency. Long caches are split
+// over CTAs; the last CTA of a row tile to finish joins their partial sums in
+// order, so results do not depend on which that was.
 #pragma once
 
 #include <climits>
@@ -58,9 +58,10 @@ struct Kv8AttnParams {
   int H, G;
   float scale, scale_log2, softcap;
   int splits;
-  float* part_o;       // [tile][split][16][hd]
-  float* part_ml;      // [tile][split][2][16]
-  int* tickets;        // [tile], zero between calls
+  // A cell is a row tile of a (sequence, kv head), of nr = 8, 16 or 128 rows.
+  float* part_o;       // [cell][split][nr][hd]
+  float* part_ml;      // [cell][split][2][nr]
+  int* tickets;        // [cell], zero between calls
   int tiles;           // row tiles of a (sequence, kv head)
   int* err;
 };

@@ -31,13 +31,15 @@
 // (they exchange row maxima through shared memory and a barrier of their
 // own), one O; P has columns of its own, so S runs two tiles ahead.
 //
-// Bound, measured on B200: 2 sequences x 4096 x 4096, 16 heads of 128: 289 us,
-// 953 TFLOP/s (tensor pipe busy 44%): the chain S -> TMEM load -> maximum ->
-// exponentials -> TMEM store -> P V of a group, about 4100 clocks for 128
-// keys, two groups in turn; P V and S are 1072 of them. 16 x 32 queries over
-// 4128 positions, 32/8 heads: 49 us. head_dim 256, window 512, soft-cap,
-// 2048 rows: 78 us, about 2900 clocks a 64-key tile. Small tiles lose to
-// their fixed part, exponentials on the FMA pipe to their issue slots.
+// Bound, measured on B200: 2 sequences x 4096 x 4096, 16 heads of 128: 320 us,
+// 860 TFLOP/s in runs of half a second (296 us, 929 TFLOP/s in runs of
+// milliseconds, at a higher clock; tensor pipe busy 44%): the chain S -> TMEM
+// load -> maximum -> exponentials -> TMEM store -> P V of a group, about 4100
+// clocks for 128 keys, two groups in turn; P V and S are 1072 of them. 16 x 32
+// queries over 4128 positions, 32/8 heads: 54 us (51 in short runs). head_dim
+// 256, window 512, soft-cap, 2048 rows: 76 us, about 2900 clocks a 64-key
+// tile. Small tiles lose to their fixed part, exponentials on the FMA pipe to
+// their issue slots.
 #pragma once
 
 #include <cfloat>
@@ -371,7 +373,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       // ---------------------------------------------------------- MMA issue
       // One thread: an issuing thread is held while its MMAs run, and two (S
       // from one, P V from another) interleave them, so that both of a pair
-      // end late: a 2 x 4096 canvas took 389 us that way. A descriptor's
+      // end late: a 2 x 4096 canvas took 5% longer that way. A descriptor's
       // address field counts 16-byte units: offsets add.
       const uint64_t dq = umma_desc_sw128(sQ, 16, 1024), dk0 = umma_desc_sw128(sK, 16, 1024);
       const uint64_t dv0 = umma_desc_sw128(sV, BN * 128, 1024);

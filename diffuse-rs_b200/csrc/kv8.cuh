@@ -140,14 +140,17 @@ __device__ __forceinline__ uint4 quantise16(const uint4 (&raw)[2], float inv) {
 // active row lies among them and follows each into the next job's entries,
 // so every block has exactly one writer (where a sequence's positions do not
 // ascend, which is reported, a block may have two: its contents are then
-// unspecified). A lane has U 16-value units (two
-// 16-byte loads) in flight; where W x 32 x U units are all of the block's
-// rows, they stay in registers between the maximum and the rounding.
+// unspecified). A lane has U 16-value units (two 16-byte loads) in flight;
+// where W x 32 x U units are all of the block's rows, they stay in registers
+// between the maximum and the rounding.
 //
 // Bound by latency on a step's few rows: one warp and one unit a lane, whose
-// code is short (4 rows of 4 heads x 128: 4.2 us, 6.0 with four units, most of
-// the difference instruction fetch; 16 x 32 scattered rows of 8 x 128: 8.2 us).
-// Passes over many rows: four warps, 8 units (4 x 8192 x 8 x 256: 105 us).
+// code is short (4 rows of 4 heads x 128: 4.3 us; four units a lane took 1.8
+// us more, most of it instruction fetch; 16 x 32 scattered rows of 8 x 128:
+// 6.6 us). Passes over many rows: four warps, 8 units; a block after the
+// other, each found through its entries, which is well short of HBM's rate (4
+// x 7000 of 8192 positions, 8 x 256: 104 us, 3.3 TB/s; 8 x 3000 of 4096, 8 x
+// 128, blocks of 32: 105 us, 1.4 TB/s).
 template <int W, int U>
 __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_store_kernel(const Kv8StoreParams p) {
   constexpr int kJobs = W == 1 ? 8 : 1;  // jobs of a CTA at a time
@@ -337,8 +340,8 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) kv8_store_kernel(const 
 // there is nothing to look up and nothing that stays. Four warps take a block
 // of a kv head of K or V, 8 units a thread in flight. A block whose entries
 // are not those positions is left as it was and reported. Bound by HBM: 2
-// bytes read and 1 written for each value, 4 x 8192 x 8 x 256 in 61.5 us,
-// 6.5 TB/s.
+// bytes read and 1 written for each value, 4 x 8192 x 8 x 256 in 62.4 us,
+// 6.4 TB/s.
 __global__ void __launch_bounds__(128) kv8_store_all_kernel(const Kv8StoreParams p) {
   constexpr int U = 8;
   __shared__ uint32_t s_max[4];
@@ -433,7 +436,8 @@ __device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&w)[8]) {
 // Rows of the cache as bf16 or fp32. A thread has 16 values of a row (one
 // 16-byte load, one 32-byte store in bf16) and keeps its column from row to
 // row, so that indices cost it next to nothing; U rows are in flight. Bound
-// by HBM: 1 byte read and 2 (4) written for each value.
+// by HBM: 1 byte read and 2 (4) written for each value; 8 x 4096 x 16 x 128 in
+// bf16 in 68.9 us, 5.8 TB/s.
 template <int U>
 __global__ void __launch_bounds__(256) kv8_load_kernel(const Kv8LoadParams p) {
   dependency_wait();
