@@ -118,3 +118,26 @@ def test_block_in_one_call_on_another_stream():
     check_attention(q, cache, out, pos, [n], scale=0.1)
     torch.cuda.synchronize()
     del keep
+
+
+@pytest.mark.parametrize("sq", [1, 40])
+def test_one_call_in_a_graph(sq):
+    # The workspace is the graph's, cleared in each replay; arguments made
+    # before the capture go into it as they are.
+    cache, q, out, pos = setup(sq=sq)
+    kept = torch.full_like(out, 7.0)
+    a = kv8.make_attention_args(q, cache, kept, scale=0.1)
+    kv8.attention(q, cache, out, scale=0.1)
+    torch.cuda.synchronize()
+    want = out.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kv8.attention(q, cache, out, scale=0.1, stream=torch.cuda.current_stream())
+        kv8.attention_args(a, torch.cuda.current_stream())
+    for _ in range(3):
+        out.zero_()
+        kept.zero_()
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(kept, want)
+    check_attention(q, cache, out, pos, [3000], scale=0.1)
