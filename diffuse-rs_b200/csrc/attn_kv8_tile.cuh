@@ -107,6 +107,8 @@ struct TileCfg {
   // those 4 x 128. (192 and 64: 3% slower; 208 and 48: no different.)
   static constexpr int kSoftRegs = 200, kOtherRegs = 56;
   static constexpr bool REGS = SC == 128;
+  static constexpr int kRegsAsked =
+      kSoftThreads * kSoftRegs + (kThreads - kSoftThreads) * kOtherRegs;
   static constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(BN >> 3) << 17) |
                                       (128u >> 4 << 24);  // e4m3 x e4m3, fp32
   static constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) |

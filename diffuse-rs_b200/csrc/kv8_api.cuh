@@ -225,6 +225,14 @@ int launch_tile(const Kv8AttnParams& p, cudaStream_t st) {
   if ((rc = make_tmap_kv8(&tk, p.c.k, p.c, C::BN)) != CA_OK) return rc;
   if ((rc = make_tmap_kv8(&tv, p.c.v, p.c, C::BN)) != CA_OK) return rc;
   if (!attr_done[dev]) {
+    if (C::REGS) {
+      // The warpgroups' shares come out of the block's registers at launch
+      // (eight a thread at a time): a build with fewer would wait for good.
+      cudaFuncAttributes fa;
+      if (cudaFuncGetAttributes(&fa, attn_kv8_tile_kernel<C>) != cudaSuccess ||
+          (fa.numRegs + 7) / 8 * 8 * C::kThreads < C::kRegsAsked)
+        return CA_ERR_CUDA;
+    }
     if (cudaFuncSetAttribute(attn_kv8_tile_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              C::kSmem) != cudaSuccess)
       return CA_ERR_CUDA;
