@@ -58,6 +58,10 @@ EXPORTED_SYMBOLS = (
     "ca_attention_kv8_dev",
     "ca_attention_kv8_workspace",
     "ca_attention_block_kv8_dev",
+    "ca_rms_norm",
+    "ca_linear_q8",
+    "ca_gated_linear",
+    "ca_sample",
 )
 
 

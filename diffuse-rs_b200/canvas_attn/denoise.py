@@ -9,10 +9,11 @@ candidate come back to the host, where ranking and commit run as in the
 reference (update_credit :597-609, rank_candidates :613-656, commit
 :658-671, tokens_to_unmask :115-132 through the C ABI in f32).
 
-Sampling at temperature > 0 (Gumbel / nucleus, pick_token :766-806) draws
-from the reference's own RNG stream and is not part of this path; neither is
-Remasking::Random's shuffle with the reference's StdRng (this mirror takes a
-numpy Generator for it, so its order is not the reference's).
+At temperature > 0 (pick_token :766-806) the tokens come from ca_sample, in a
+second launch over the same logits: temperature, top-k, top-p and min-p, one
+random number a candidate. Those numbers come from a numpy Generator, so the
+draws are not the reference's own RNG stream; neither is Remasking::Random's
+shuffle, which takes the same Generator in place of the reference's StdRng.
 """
 from __future__ import annotations
 
@@ -22,7 +23,7 @@ from typing import Optional, Sequence
 
 import numpy as np
 
-from . import CaError, _ptr, _stream, lib
+from . import CaError, _check, _ptr, _stream, lib
 
 COSINE, LINEAR = 0, 1
 ENTROPY_EXIT, LOW_CONFIDENCE, MARGIN, CONFIDENCE, ENTROPY_BOUND, RANDOM = range(6)
@@ -67,6 +68,88 @@ def candidate_stats(logits, rows, token, entropy=None, margin=None, prob=None, *
         raise CaError(rc, "ca_candidate_stats")
 
 
+class CaSampleArgs(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("logits_bf16", ctypes.c_int32),
+                ("n_rows", ctypes.c_int64), ("n_vocab", ctypes.c_int64),
+                ("row_stride", ctypes.c_int64), ("rows", ctypes.c_void_p),
+                ("n_cand", ctypes.c_int32), ("mask_id", ctypes.c_int32),
+                ("suppress", ctypes.c_void_p), ("n_suppress", ctypes.c_int32),
+                ("u", ctypes.c_void_p), ("temperature", ctypes.c_float),
+                ("top_k", ctypes.c_int32), ("top_p", ctypes.c_float), ("min_p", ctypes.c_float),
+                ("temperature_row", ctypes.c_void_p), ("top_k_row", ctypes.c_void_p),
+                ("top_p_row", ctypes.c_void_p), ("min_p_row", ctypes.c_void_p),
+                ("token", ctypes.c_void_p), ("prob", ctypes.c_void_p)]
+
+
+lib.ca_sample.argtypes = [ctypes.POINTER(CaSampleArgs), ctypes.c_void_p]
+lib.ca_sample.restype = ctypes.c_int
+
+
+def make_sample_args(logits, rows, u, token, prob=None, *, n_vocab: Optional[int] = None,
+                     temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask_id: int = -1,
+                     suppress=None) -> CaSampleArgs:
+    """logits: fp32 or bf16 [n_rows, >= n_vocab], rows of any stride; rows: int32
+    [n_cand] (None: row i); u: fp32 [n_cand] in [0, 1); token: int32 [n_cand]
+    out; prob: fp32 [n_cand] out or None. temperature, top_k, top_p and min_p
+    are numbers, or tensors with an entry for each candidate (fp32; top_k
+    int32). suppress: int32 token ids. Kept for programs that keep their
+    buffers; sample_args launches it."""
+    kind = {"torch.float32": 0, "torch.bfloat16": 1}.get(str(logits.dtype))
+    if kind is None or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be float32 or bfloat16 [rows, vocab]")
+    v = int(logits.shape[1]) if n_vocab is None else int(n_vocab)
+    if v > logits.shape[1]:
+        raise ValueError("n_vocab exceeds the logits' columns")
+    n = int(token.numel())
+
+    def check(name, x, dtype, count=None):
+        if str(x.dtype) != dtype or not x.is_contiguous() or \
+                (count is not None and x.numel() != count):
+            raise ValueError(f"{name} must be contiguous {dtype}"
+                             + ("" if count is None else f" with {count} entries"))
+
+    check("token", token, "torch.int32")
+    check("u", u, "torch.float32", n)
+    for name, x, dtype in (("rows", rows, "torch.int32"), ("prob", prob, "torch.float32")):
+        if x is not None:
+            check(name, x, dtype, n)
+    if suppress is not None:
+        check("suppress", suppress, "torch.int32")
+    scalars, tensors = [], []
+    for name, x, dtype in (("temperature", temperature, "torch.float32"),
+                           ("top_k", top_k, "torch.int32"), ("top_p", top_p, "torch.float32"),
+                           ("min_p", min_p, "torch.float32")):
+        each = hasattr(x, "data_ptr")
+        if each:
+            check(name, x, dtype, n)
+        tensors.append(x if each else None)
+        scalars.append((int if name == "top_k" else float)(0 if each else x))
+    if rows is None and n > logits.shape[0]:
+        raise ValueError("more candidates than rows")
+    kept = (logits, rows, u, token, prob, suppress, *tensors)
+    if len({x.device for x in kept if x is not None}) > 1:
+        raise ValueError("tensors of one call are on several devices")
+    n_sup = 0 if suppress is None else int(suppress.numel())
+    a = CaSampleArgs(_ptr(logits), kind, int(logits.shape[0]), v,
+                     int(logits.stride(0)) if logits.shape[0] > 1 else 0, _ptr(rows), n,
+                     int(mask_id), _ptr(suppress) if n_sup else None, n_sup, _ptr(u),
+                     scalars[0], max(min(scalars[1], 0x7fffffff), -1), scalars[2], scalars[3],
+                     _ptr(tensors[0]), _ptr(tensors[1]), _ptr(tensors[2]), _ptr(tensors[3]),
+                     _ptr(token), _ptr(prob))
+    a._keep = kept
+    return a
+
+
+def sample_args(a: CaSampleArgs, stream=None) -> None:
+    _check(lib.ca_sample(ctypes.byref(a), _stream(stream)), "ca_sample")
+
+
+def sample(logits, rows, u, token, prob=None, *, stream=None, **kw) -> None:
+    """ca_sample: a token for each candidate row of device logits (see
+    make_sample_args and include/canvas_attn.h)."""
+    sample_args(make_sample_args(logits, rows, u, token, prob, **kw), stream)
+
+
 @dataclass
 class Candidate:
     pos: int
@@ -86,6 +169,10 @@ class StepParams:
     eb_entropy_bound: float = 0.0
     credit_steps: int = 0
     suppress_ids: Sequence[int] = field(default_factory=list)
+    temperature: float = 0.0  # 0: the greedy pick
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
 
 
 class DenoiseState:
@@ -102,10 +189,13 @@ class DenoiseState:
 
 
 def collect_candidates(state: DenoiseState, logits, n_vocab: int, rng: range, shift: int,
-                       params: StepParams, stream=None):
+                       params: StepParams, stream=None,
+                       draw_rng: Optional[np.random.Generator] = None):
     """collect_candidates (sampler.rs:720-749) with the row reductions on the
     GPU. `logits`: device fp32 [len(seq), n_vocab]; its suppressed entries of
-    the candidate rows are set to -inf, as process_logits does."""
+    the candidate rows are set to -inf, as process_logits does. At
+    params.temperature > 0 token and prob are those of the draw, entropy and
+    margin the row's; draw_rng gives the random numbers."""
     import torch
     pos = [p for p in rng if state.is_masked[p]]
     if not pos:
@@ -122,6 +212,12 @@ def collect_candidates(state: DenoiseState, logits, n_vocab: int, rng: range, sh
     candidate_stats(logits, rows, tok, vals[0], vals[1], vals[2], n_vocab=n_vocab,
                     mask_id=state.mask_id, suppress=sup, want_entropy=needs_entropy,
                     want_prob=needs_prob, stream=stream)
+    if params.temperature > 0:
+        g = draw_rng or np.random.default_rng()
+        u = torch.from_numpy(g.random(n, dtype=np.float32)).to(dev)
+        sample(logits, rows, u, tok, vals[2], n_vocab=n_vocab, temperature=params.temperature,
+               top_k=params.top_k, top_p=params.top_p, min_p=params.min_p, mask_id=state.mask_id,
+               suppress=sup, stream=stream)
     tok_h = tok.cpu().numpy()
     ent, mar, prob = vals.cpu().numpy()
     return [Candidate(p, int(tok_h[i]), float(ent[i]), float(mar[i]), float(prob[i]))
@@ -209,8 +305,10 @@ def process_logits(state: DenoiseState, logits, n_vocab: int, rng: range, shift:
                    local_step: int, block_steps: int, params: StepParams,
                    stream=None, shuffle_rng=None) -> int:
     """process_logits (sampler.rs:581-593) after the forward: suppress,
-    collect, credit, rank, commit. Returns the number of committed tokens."""
-    cands = collect_candidates(state, logits, n_vocab, rng, shift, params, stream)
+    collect, credit, rank, commit. Returns the number of committed tokens.
+    shuffle_rng: the random numbers of Remasking::Random and of the draws at
+    params.temperature > 0."""
+    cands = collect_candidates(state, logits, n_vocab, rng, shift, params, stream, shuffle_rng)
     update_credit(state, cands, params)
     n_unmask = rank_candidates(cands, params, local_step, block_steps, shuffle_rng)
     return commit(state, cands, n_unmask, params)

@@ -17,6 +17,7 @@
 #include "host_round.h"
 
 #include "canvas_attn.h"
+#include "host_util.cuh"
 #include "attn_fwd.cuh"
 #include "prep.cuh"
 #include "sampler.cuh"
@@ -25,28 +26,6 @@
 
 namespace ca {
 namespace {
-
-constexpr int kMaxDevices = 64;
-
-// ---------------------------------------------------------------- driver entry
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
-}
 
 // 3-D bf16 view [tokens][heads][hd] (innermost first in TMA order), boxes of
 // 64 x box_heads x box_tokens with 128-byte swizzle; out-of-range reads fill 0.
@@ -65,8 +44,6 @@ int make_tmap(CUtensorMap* m, const void* base, int64_t hd, int64_t heads, int64
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? CA_OK : CA_ERR_INVALID;
 }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // 4-D view of the output [batch][tokens][heads][hd] (uniform batch), bf16 or
 // fp32, boxes of one 128-byte column chunk x box_heads x box_tokens, 128-byte
@@ -1329,7 +1306,7 @@ int ca_device_status(void* stream) {
   int derr = 0;
   if (cudaMemcpyFromSymbol(&derr, ca::g_device_error, sizeof(int)) != cudaSuccess)
     return CA_ERR_CUDA;
-  if (derr == 0) return CA_OK;
+  if (derr == 0) return ca::layer_device_error();
   const int zero = 0;
   cudaMemcpyToSymbol(ca::g_device_error, &zero, sizeof(int));
   return derr;

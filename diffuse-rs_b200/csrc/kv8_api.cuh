@@ -10,29 +10,6 @@
 namespace ca {
 namespace {
 
-constexpr int kSms = 148;
-
-// A launch that may overlap the end of the kernel before it (dependency_wait).
-template <class... P, class... A>
-int launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st,
-                 A... args) {
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
-    cudaGetLastError();
-    return CA_ERR_CUDA;
-  }
-  return CA_OK;
-}
-
 // The cache as the kernels see it, or why not.
 int kv8_view(const ca_kv8_cache& c, Kv8View* v) {
   if (!c.k || !c.v || !c.k_scale || !c.v_scale) return CA_ERR_INVALID;

@@ -1,0 +1,256 @@
+// layer.cu -- what a layer does around its attention block: ca_rms_norm,
+// ca_linear_q8, ca_gated_linear (include/canvas_attn.h).
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+
+#include "canvas_attn.h"
+#include "host_util.cuh"
+#include "rows.cuh"
+#include "skinny.cuh"
+
+namespace ca {
+
+int layer_device_error() {
+  int e = 0;
+  if (cudaMemcpyFromSymbol(&e, g_device_error, sizeof(int)) != cudaSuccess) return CA_ERR_CUDA;
+  if (e != 0) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
+  }
+  return e;
+}
+
+namespace {
+
+int type_size(int t) {
+  return t == CA_TYPE_BF16 ? 2 : t == CA_TYPE_F32 ? 4 : t == CA_TYPE_E4M3 ? 1 : 0;
+}
+
+bool aligned_to(const void* p, int bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & static_cast<uintptr_t>(bytes - 1)) == 0;
+}
+
+template <int NT, int C>
+int launch_rows_as(const RowsParams& p, bool vec, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(p.rows));
+  return vec ? launch_after(rows_kernel<NT, C, true>, grid, NT, 0, st, p)
+             : launch_after(rows_kernel<NT, C, false>, grid, NT, 0, st, p);
+}
+
+int rms_norm_impl(const ca_rms_norm_args* a, cudaStream_t st) {
+  if (!a || a->rows < 0 || a->cols <= 0) return CA_ERR_INVALID;
+  // No rows: there is nothing that a pointer could point to.
+  if (a->rows > 0 && (!a->x || !a->out)) return CA_ERR_INVALID;
+  if (a->x_type != CA_TYPE_BF16 && a->x_type != CA_TYPE_F32) return CA_ERR_INVALID;
+  if (type_size(a->out_type) == 0) return CA_ERR_INVALID;
+  if (a->rows == 0) return CA_OK;
+  if (a->residual && ((a->residual_type != CA_TYPE_BF16 && a->residual_type != CA_TYPE_F32) ||
+                      !a->sum_out))
+    return CA_ERR_INVALID;
+  if (!a->residual && a->sum_out) return CA_ERR_INVALID;
+  if (a->out_type == CA_TYPE_E4M3 && !a->out_scale) return CA_ERR_INVALID;
+  if (a->norm && !(a->eps >= 0.f)) return CA_ERR_INVALID;
+  RowsParams p{};
+  auto stride = [&](int64_t s) { return s ? s : a->cols; };
+  p.x_stride = stride(a->x_stride);
+  p.res_stride = stride(a->residual_stride);
+  p.sum_stride = stride(a->sum_stride);
+  p.out_stride = stride(a->out_stride);
+  if (p.x_stride < a->cols || p.res_stride < a->cols || p.sum_stride < a->cols ||
+      p.out_stride < a->cols)
+    return CA_ERR_INVALID;
+  const int xs = type_size(a->x_type), os = type_size(a->out_type);
+  const int rs = a->residual ? type_size(a->residual_type) : 4;
+  if (!aligned_to(a->x, xs) || !aligned_to(a->out, os) || !aligned_to(a->w, 4) ||
+      !aligned_to(a->residual, rs) || !aligned_to(a->sum_out, rs) || !aligned_to(a->out_scale, 4))
+    return CA_ERR_INVALID;
+  if (a->cols > 32768 || a->rows > INT_MAX) return CA_ERR_UNSUPPORTED;
+  p.x = a->x;
+  p.res = a->residual;
+  p.sum = a->sum_out;
+  p.w = a->w;
+  p.out = a->out;
+  p.out_scale = a->out_type == CA_TYPE_E4M3 ? a->out_scale : nullptr;
+  p.rows = a->rows;
+  p.cols = static_cast<int>(a->cols);
+  p.x_f32 = a->x_type == CA_TYPE_F32;
+  p.res_f32 = a->residual_type == CA_TYPE_F32;
+  p.out_type = a->out_type;
+  p.norm = a->norm ? 1 : 0;
+  p.eps = a->eps;
+  auto rows16 = [](const void* q, int64_t bytes) { return !q || (aligned16(q) && bytes % 16 == 0); };
+  const bool vec = p.cols % 8 == 0 && rows16(p.x, p.x_stride * xs) &&
+                   rows16(p.res, p.res_stride * rs) && rows16(p.sum, p.sum_stride * rs) &&
+                   aligned16(p.w) &&
+                   (os == 1 ? aligned_to(p.out, 8) && p.out_stride % 8 == 0
+                            : rows16(p.out, p.out_stride * os));
+  if (p.rows < 4 * kSms && p.cols <= 8192) {
+    if (p.cols <= 1024) return launch_rows_as<128, 1>(p, vec, st);
+    if (p.cols <= 2048) return launch_rows_as<256, 1>(p, vec, st);
+    if (p.cols <= 4096) return launch_rows_as<512, 1>(p, vec, st);
+    return launch_rows_as<1024, 1>(p, vec, st);
+  }
+  if (p.cols <= 1024) return launch_rows_as<128, 1>(p, vec, st);
+  if (p.cols <= 4096) return launch_rows_as<128, 4>(p, vec, st);
+  if (p.cols <= 8192) return launch_rows_as<256, 4>(p, vec, st);
+  if (p.cols <= 16384) return launch_rows_as<512, 4>(p, vec, st);
+  return launch_rows_as<1024, 4>(p, vec, st);
+}
+
+// A row-major matrix of 1- or 2-byte elements in boxes of 128 bytes of
+// box_rows rows, 128-byte swizzle; what lies outside reads as zero.
+int make_tmap_2d(CUtensorMap* m, const void* base, int kind, int64_t cols, int64_t rows,
+                 int64_t stride, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return CA_ERR_CUDA;
+  const int es = kind == kKindBf16 ? 2 : 1;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * es};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / es), box_rows};
+  cuuint32_t elem[2] = {1, 1};
+  const CUresult r =
+      fn(m, kind == kKindBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2,
+         const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? CA_OK : CA_ERR_INVALID;
+}
+
+// A product as both entry points ask for it.
+struct Product {
+  const void* act;
+  const void* w;
+  const void* up;  // gated: the second matrix
+  int64_t act_stride, cols;
+  LinearParams p;
+};
+
+template <int KIND, int G, int NT>
+int launch_skinny(const Product& q, cudaStream_t st) {
+  using C = SkinnyCfg<KIND, G, NT>;
+  static bool attr_done[kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return CA_ERR_CUDA;
+  CUtensorMap tw, tu, tx;
+  int rc;
+  if ((rc = make_tmap_2d(&tw, q.w, KIND, q.cols, q.p.rows, q.cols, 128)) != CA_OK) return rc;
+  tu = tw;
+  if (G == 2 && (rc = make_tmap_2d(&tu, q.up, KIND, q.cols, q.p.rows, q.cols, 128)) != CA_OK)
+    return rc;
+  if ((rc = make_tmap_2d(&tx, q.act, KIND, q.cols, q.p.n, q.act_stride, NT)) != CA_OK) return rc;
+  if (!attr_done[dev]) {
+    if (cudaFuncSetAttribute(skinny_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             C::kSmem) != cudaSuccess)
+      return CA_ERR_CUDA;
+    attr_done[dev] = true;
+  }
+  const int64_t tiles = (q.p.rows + 127) / 128, tok = (q.p.n + NT - 1) / NT;
+  if (tiles > INT_MAX / 8 || tok > 65535) return CA_ERR_UNSUPPORTED;
+  // Columns are split while that fills SMs (two CTAs fit on one) and leaves a
+  // CTA at least four stages of work.
+  int S = 1;
+  while (S < 8 && tiles * tok * S * 2 <= 2 * kSms && q.p.kblocks >= 8 * S) S *= 2;
+  return launch_cluster_after(skinny_kernel<C>,
+                              dim3(static_cast<unsigned>(tiles * S), static_cast<unsigned>(tok)),
+                              C::kThreads, C::kSmem, S, st, tw, tu, tx, q.p);
+}
+
+template <int KIND, int G>
+int launch_product(const Product& q, cudaStream_t st) {
+  if (q.p.n <= 16) return launch_skinny<KIND, G, 16>(q, st);
+  if (q.p.n <= 32) return launch_skinny<KIND, G, 32>(q, st);
+  return launch_skinny<KIND, G, 64>(q, st);
+}
+
+// Shapes, strides and alignment of a product; es: bytes of an operand's element.
+int check_product(Product* q, int es, int out_f32) {
+  LinearParams& p = q->p;
+  if (!q->w || p.n < 0 || p.rows <= 0 || q->cols <= 0) return CA_ERR_INVALID;
+  if (p.n > 0 && (!q->act || !p.out)) return CA_ERR_INVALID;
+  if (!q->act_stride) q->act_stride = q->cols;
+  if (!p.out_stride) p.out_stride = p.rows;
+  if (!p.res_stride) p.res_stride = p.rows;
+  if (q->act_stride < q->cols || p.out_stride < p.rows || p.res_stride < p.rows ||
+      q->act_stride * es % 16 || !aligned16(q->act) || !aligned16(q->w) ||
+      (q->up && !aligned16(q->up)))
+    return CA_ERR_INVALID;
+  const int os = out_f32 ? 4 : 2;
+  if (!aligned_to(p.out, os) || !aligned_to(p.residual, os)) return CA_ERR_INVALID;
+  if (q->cols * es % 16) return CA_ERR_UNSUPPORTED;
+  if (p.n > INT_MAX - 256 || p.rows > INT_MAX - 256 || q->cols > INT_MAX - 256)
+    return CA_ERR_UNSUPPORTED;
+  p.kblocks = static_cast<int>((q->cols * es + 127) / 128);
+  p.out_f32 = out_f32 ? 1 : 0;
+  return CA_OK;
+}
+
+int linear_q8_impl(const ca_linear_q8_args* a, cudaStream_t st) {
+  if (!a) return CA_ERR_INVALID;
+  Product q{};
+  q.act = a->act;
+  q.w = a->w;
+  q.act_stride = a->act_stride;
+  q.cols = a->cols;
+  q.p.act_scale = a->act_scale;
+  q.p.w_scale = a->w_scale;
+  q.p.bias = a->bias;
+  q.p.residual = a->residual;
+  q.p.out = a->out;
+  q.p.out_stride = a->out_stride;
+  q.p.res_stride = a->residual_stride;
+  q.p.n = a->n;
+  q.p.rows = a->rows;
+  q.p.err = a->status;
+  const int rc = check_product(&q, 1, a->out_f32);
+  if (rc != CA_OK || q.p.n == 0) return rc;
+  return launch_product<kKindE4m3, 1>(q, st);
+}
+
+int gated_linear_impl(const ca_gated_linear_args* a, cudaStream_t st) {
+  if (!a || !a->w_up) return CA_ERR_INVALID;
+  if (a->type != CA_TYPE_BF16 && a->type != CA_TYPE_E4M3) return CA_ERR_INVALID;
+  if (a->activation != CA_ACT_SILU && a->activation != CA_ACT_GELU) return CA_ERR_INVALID;
+  if (a->type == CA_TYPE_BF16 && (a->act_scale || a->gate_scale || a->up_scale))
+    return CA_ERR_INVALID;
+  Product q{};
+  q.act = a->act;
+  q.w = a->w_gate;
+  q.up = a->w_up;
+  q.act_stride = a->act_stride;
+  q.cols = a->cols;
+  q.p.act_scale = a->act_scale;
+  q.p.w_scale = a->gate_scale;
+  q.p.up_scale = a->up_scale;
+  q.p.act = a->activation;
+  q.p.out = a->out;
+  q.p.out_stride = a->out_stride;
+  q.p.n = a->n;
+  q.p.rows = a->rows;
+  q.p.err = a->status;
+  const int rc = check_product(&q, type_size(a->type), a->out_f32);
+  if (rc != CA_OK || q.p.n == 0) return rc;
+  return a->type == CA_TYPE_BF16 ? launch_product<kKindBf16, 2>(q, st)
+                                 : launch_product<kKindE4m3, 2>(q, st);
+}
+
+}  // namespace
+}  // namespace ca
+
+extern "C" {
+
+int ca_rms_norm(const ca_rms_norm_args* a, void* stream) {
+  return ca::rms_norm_impl(a, static_cast<cudaStream_t>(stream));
+}
+
+int ca_linear_q8(const ca_linear_q8_args* a, void* stream) {
+  return ca::linear_q8_impl(a, static_cast<cudaStream_t>(stream));
+}
+
+int ca_gated_linear(const ca_gated_linear_args* a, void* stream) {
+  return ca::gated_linear_impl(a, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

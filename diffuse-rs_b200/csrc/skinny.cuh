@@ -1,0 +1,276 @@
+// skinny.cuh -- act . W^T for few rows of act, alone or gated, on tcgen05.
+//
+//   out[t, r] = sa[t] sw[r] sum_c act[t, c] W[r, c] (+ bias[r]) (+ residual[t, r])
+//   out[t, r] = f(sa[t] sg[r] act . Wg[r]) * (sa[t] su[r] act . Wu[r])
+//
+// The weights are the M operand: a CTA takes 128 of their rows (for the gated
+// form of both matrices) and the tokens are the N columns, 16 to 64 of them,
+// so one token costs the tensor core no more than 16. What bounds it is the
+// weights' way from HBM: each is read once. A stage holds 128 bytes of each
+// row; the ring of stages (about 100 KB, so that two CTAs share an SM) keeps
+// the loads in flight. Where 128 rows a CTA would leave SMs idle, the S CTAs
+// of a cluster split the columns between them and add their parts through
+// distributed shared memory, in the order of their ranks: no workspace, no
+// atomics, the same bits every time.
+//
+// Lane = weight row, TMEM column = token, so that a warp's 32 threads store 32
+// neighbours of an output row.
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+
+#include "cluster.cuh"
+#include "sm100.cuh"
+
+namespace ca {
+
+constexpr int kKindBf16 = 0, kKindE4m3 = 1;
+
+struct LinearParams {
+  const float* act_scale;   // [n] or null
+  const float* w_scale;     // [rows] or null
+  const float* up_scale;    // gated: [rows] or null
+  const float* bias;        // [rows] or null
+  const void* residual;     // out's type, or null
+  void* out;
+  long long out_stride, res_stride;
+  long long n, rows;
+  int kblocks;              // 128-byte pieces of a row
+  int out_f32;
+  int act;                  // CA_ACT_*
+  int n_tiles, r_tiles;     // pair.cuh: its tiles
+  int* err;
+};
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* tmap, uint32_t bar,
+                                            int32_t x, int32_t y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+
+// D[tmem] (+)= A[smem] x B[smem]^T, both K-major.
+template <int KIND>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accumulate) {
+  if constexpr (KIND == kKindBf16) {
+    umma_ss(d, a, b, idesc, accumulate);
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+
+// Instruction descriptor: e4m3 (formats 0) or bf16 operands, fp32 D.
+__host__ __device__ constexpr uint32_t linear_idesc(int kind, int M, int N) {
+  return kind == kKindBf16 ? umma_idesc_bf16(M, N, 0, 0)
+                           : (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) |
+                                 (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void st_shared_f32(uint32_t addr, float v) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+// The gate's activation, in fp32: g / (1 + e^-g), and with y = sqrt(2/pi) (g +
+// 0.044715 g^3), 0.5 g (1 + tanh y) = g / (1 + e^-2y). Exponentials that run to
+// infinity give 0.
+__device__ __forceinline__ float activate(float g, int act) {
+  if (act == 0) return __fdividef(g, 1.f + __expf(-g));
+  const float y = 0.7978845608028654f * (g + 0.044715f * g * g * g);
+  return __fdividef(g, 1.f + __expf(-2.f * y));
+}
+
+// What a product of one token and weight row becomes.
+template <int G>
+__device__ __forceinline__ void linear_store(const LinearParams& p, float d0, float d1, float w0,
+                                             float w1, float bias, long long t, long long r) {
+  const float sa = p.act_scale ? p.act_scale[t] : 1.f;
+  float v;
+  if constexpr (G == 2) {
+    v = activate(d0 * sa * w0, p.act) * (d1 * sa * w1);
+  } else {
+    v = d0 * sa * w0 + bias;
+    if (p.residual) {
+      const long long i = t * p.res_stride + r;
+      v += p.out_f32 ? static_cast<const float*>(p.residual)[i]
+                     : __bfloat162float(static_cast<const __nv_bfloat16*>(p.residual)[i]);
+    }
+  }
+  const long long o = t * p.out_stride + r;
+  if (p.out_f32)
+    static_cast<float*>(p.out)[o] = v;
+  else
+    static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(v);
+}
+
+template <int KIND_, int G_, int NT_>
+struct SkinnyCfg {
+  static constexpr int KIND = KIND_;  // operands
+  static constexpr int G = G_;        // weight matrices
+  static constexpr int NT = NT_;      // tokens of a CTA
+  static constexpr int kStage = G * 16384 + NT * 128;
+  static constexpr int kStages = 104 * 1024 / kStage;
+  static constexpr int kRing = kStages * kStage;
+  static_assert(kRing >= G * NT * 512, "the parts of a sum are laid over the ring");
+  static constexpr int kThreads = 192;
+  static constexpr int kBars = 2 * kStages + 1;
+  static constexpr int kSmem = 1024 + kRing + 8 * kBars + 16;
+  static constexpr int kTmemCols = G * NT < 32 ? 32 : G * NT;
+  static constexpr int kElems = KIND == kKindBf16 ? 64 : 128;  // of 128 bytes
+};
+
+template <class C>
+__global__ void __launch_bounds__(C::kThreads)
+    skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_u,
+                  const __grid_constant__ CUtensorMap tm_x, const LinearParams p) {
+  extern __shared__ uint8_t raw_smem[];
+  const uint32_t base = (smem_u32(raw_smem) + 1023u) & ~1023u;
+  const uint32_t bars = base + C::kRing, slot = bars + 8 * C::kBars;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  auto full = [&](int s) { return bars + 8 * s; };
+  auto empty = [&](int s) { return bars + 8 * (C::kStages + s); };
+  const uint32_t done = bars + 8 * (2 * C::kStages);
+  const uint32_t S = cluster_size(), rank = cluster_rank();
+  const int r0 = static_cast<int>(blockIdx.x / S) * 128;
+  const int t0 = static_cast<int>(blockIdx.y) * C::NT;
+  const int kb0 = static_cast<int>(static_cast<long long>(p.kblocks) * rank / S);
+  const int kb1 = static_cast<int>(static_cast<long long>(p.kblocks) * (rank + 1) / S);
+
+  if (tid == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    mbar_init(done, 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  // TMEM is taken only once the kernel before is complete, and the next one
+  // let in only then: neither can hold columns that the other waits for.
+  wait_prior_kernel();
+  if (warp == 1) {
+    tmem_alloc(slot, C::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  let_next_kernel();
+  uint32_t tmem;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
+  bool dead = false;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int i = 0;
+      for (int kb = kb0; kb < kb1; ++kb, ++i) {
+        const int s = i % C::kStages;
+        if (i >= C::kStages && !mbar_wait(empty(s), ((i / C::kStages) - 1) & 1, dead, p.err)) break;
+        const uint32_t dst = base + s * C::kStage;
+        mbar_arrive_expect_tx(full(s), C::kStage);
+        tma_load_2d(dst, &tm_w, full(s), kb * C::kElems, r0);
+        if constexpr (C::G == 2) tma_load_2d(dst + 16384, &tm_u, full(s), kb * C::kElems, r0);
+        tma_load_2d(dst + C::G * 16384, &tm_x, full(s), kb * C::kElems, t0);
+      }
+      // After an expired wait the copies in flight still have to land.
+      if (dead) {
+        bool late = false;
+        for (int j = max(0, i - C::kStages); j < i; ++j)
+          mbar_wait(full(j % C::kStages), (j / C::kStages) & 1, late, p.err);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = linear_idesc(C::KIND, 128, C::NT);
+      int i = 0;
+      for (int kb = kb0; kb < kb1; ++kb, ++i) {
+        const int s = i % C::kStages;
+        if (!mbar_wait(full(s), (i / C::kStages) & 1, dead, p.err)) break;
+        tc_fence_after();
+        const uint32_t at = base + s * C::kStage;
+        const uint64_t dw = umma_desc_sw128(at, 16, 1024);
+        const uint64_t dx = umma_desc_sw128(at + C::G * 16384, 16, 1024);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          mma_ss<C::KIND>(tmem, dw + 2 * kk, dx + 2 * kk, idesc, i | kk);
+          if constexpr (C::G == 2)
+            mma_ss<C::KIND>(tmem + C::NT, dw + 1024 + 2 * kk, dx + 2 * kk, idesc, i | kk);
+        }
+        umma_commit(empty(s));
+      }
+      umma_commit(done);
+    }
+    __syncwarp();
+  }
+
+  // Warps 2 to 5: lanes 32 (warp % 4) .. + 31 of TMEM, a weight row each.
+  const int f = (warp & 3) * 32 + lane;
+  const long long r = r0 + f;
+  float w0 = 1.f, w1 = 1.f, bias = 0.f;
+  if (warp >= 2) {
+    if (r < p.rows) {
+      if (p.w_scale) w0 = p.w_scale[r];
+      if (C::G == 2 && p.up_scale) w1 = p.up_scale[r];
+      if (C::G == 1 && p.bias) bias = p.bias[r];
+    }
+    mbar_wait(done, 0, dead, p.err);
+    tc_fence_after();
+    const uint32_t col = tmem + (static_cast<uint32_t>(warp & 3) << 21);
+#pragma unroll
+    for (int j0 = 0; j0 < C::NT; j0 += 16) {
+      uint32_t d0[16], d1[16];
+      tmem_ld16(col + j0, d0);
+      if constexpr (C::G == 2) tmem_ld16(col + C::NT + j0, d1);
+      tmem_wait_ld();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float a = __uint_as_float(d0[j]), b = C::G == 2 ? __uint_as_float(d1[j]) : 0.f;
+        if (S == 1) {
+          if (t0 + j0 + j < p.n && r < p.rows)
+            linear_store<C::G>(p, a, b, w0, w1, bias, t0 + j0 + j, r);
+        } else {
+          st_shared_f32(base + ((j0 + j) * 128 + f) * 4, a);
+          if constexpr (C::G == 2) st_shared_f32(base + ((C::NT + j0 + j) * 128 + f) * 4, b);
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  if (S > 1) {
+    // Rank i joins tokens NT i / S .. NT (i + 1) / S - 1, parts in the order
+    // of the ranks.
+    __syncwarp();
+    cluster_sync_all();
+    if (warp >= 2 && r < p.rows) {
+      const int j1 = min(static_cast<long long>(C::NT * (rank + 1) / S), p.n - t0);
+      for (int j = C::NT * rank / S; j < j1; ++j) {
+        float a = 0.f, b = 0.f;
+        for (uint32_t q = 0; q < S; ++q) {
+          a += ld_cluster_f32(map_to_rank(base + (j * 128 + f) * 4, q));
+          if constexpr (C::G == 2)
+            b += ld_cluster_f32(map_to_rank(base + ((C::NT + j) * 128 + f) * 4, q));
+        }
+        linear_store<C::G>(p, a, b, w0, w1, bias, t0 + j, r);
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();  // no CTA leaves while its parts are read
+  } else {
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
+}  // namespace ca

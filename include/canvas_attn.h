@@ -295,6 +295,54 @@ typedef struct {
  */
 int ca_candidate_stats(const ca_cand_args* a, void* stream);
 
+/* Arguments of ca_sample (device pointers unless noted). */
+typedef struct {
+    const void* logits;       /* [n_rows, row_stride] fp32, or bf16 when logits_bf16: the step's
+                                 logits. Not written */
+    int32_t logits_bf16;
+    int64_t n_rows;
+    int64_t n_vocab;          /* at most 425984 fp32 or 851968 bf16 entries */
+    int64_t row_stride;       /* elements between rows; 0 = n_vocab */
+    const int32_t* rows;      /* int32 [n_cand]: logit row of each candidate, or NULL (row i).
+                                 A row out of range gets token -1, prob 0 */
+    int32_t n_cand;
+    int32_t mask_id;          /* mask token id, or < 0 for none */
+    const int32_t* suppress;  /* int32 [n_suppress] token ids never drawn, or NULL */
+    int32_t n_suppress;
+    const float* u;           /* fp32 [n_cand]: a number in [0, 1) for each candidate (others are
+                                 taken as the nearest in it, NaN as 0) */
+    float temperature;        /* <= 0 (or NaN): the maximum's first index, filters and u unused */
+    int32_t top_k;            /* <= 0: off */
+    float top_p;              /* >= 1 (or NaN): off; <= 0: the first entry alone */
+    float min_p;              /* <= 0 (or NaN): off */
+    const float* temperature_row; /* [n_cand] or NULL: each candidate's own, in place of the
+                                     value above; the same for the next three */
+    const int32_t* top_k_row;
+    const float* top_p_row;
+    const float* min_p_row;
+    int32_t* token;           /* int32 [n_cand] out */
+    float* prob;              /* fp32 [n_cand] out, or NULL */
+} ca_sample_args;
+
+/*
+ * ca_sample -- pick_token (src/model/sampler.rs:754-806) at any temperature,
+ * from random numbers that the caller gives: one launch for a step's
+ * candidates, on logits resident in HBM, asynchronous on `stream`. Over
+ * candidate i's row l, with the mask token, the suppressed ids and NaN
+ * entries taken as -inf, m its maximum and w_j = exp((l_j - m) / temperature):
+ * entries in the order of their logits, largest first and ties by index, are
+ * kept while they are among the first top_k, while the weights before an
+ * entry sum to less than top_p times the weight of those top_k, and while
+ * w_j >= min_p; the first is always kept. token is the first kept index j, in
+ * the vocabulary's order, for which the kept weights up to j sum to more than
+ * u times all kept weights. prob = softmax(l)_token, at temperature 1 and
+ * without filters: the confidence that ca_candidate_stats gives for the
+ * greedy pick. Weights are summed as 64-bit integers of steps 2^-44, so that
+ * results do not depend on any order of summation. A row with no entry above
+ * -inf gets token 0, prob 0. Allocates nothing.
+ */
+int ca_sample(const ca_sample_args* a, void* stream);
+
 /* tokens_to_unmask (src/model/sampler.rs:115-132), host, in the reference's
  * f32 arithmetic: how many of `masked` remaining tokens to commit at `step`
  * of `total_steps`. Returns the count, or CA_ERR_INVALID. */
@@ -541,6 +589,108 @@ int ca_attention_block_kv8_dev(const ca_block_kv8_args* a, void* stream);
 /* Bytes of workspace a call with these arguments uses (pointers are not
  * read), or a negative ca_status. */
 int64_t ca_attention_kv8_workspace(const ca_attn_kv8_args* a);
+
+/* Element types of the calls below. */
+#define CA_TYPE_BF16 0
+#define CA_TYPE_F32 1
+#define CA_TYPE_E4M3 2
+
+/* Arguments of ca_rms_norm (device pointers; strides in elements). */
+typedef struct {
+    const void* x;           /* [rows, cols] bf16 or fp32 */
+    int32_t x_type;
+    int64_t x_stride;        /* between rows; 0 = cols (as all strides here) */
+    const void* residual;    /* [rows, cols] bf16 or fp32, or NULL */
+    int32_t residual_type;
+    int64_t residual_stride;
+    void* sum_out;           /* [rows, cols] of residual_type, required with residual: may be
+                                the residual itself (the stream updated in place) or x where
+                                types and strides agree */
+    int64_t sum_stride;
+    const float* w;          /* fp32 [cols] gain, or NULL (none) */
+    int32_t norm;            /* 1: RMS norm; 0: rows as they are (the quantisation alone) */
+    float eps;
+    void* out;               /* [rows, cols] of out_type: bf16, fp32 or e4m3; may be x where
+                                types and strides agree */
+    int32_t out_type;
+    int64_t out_stride;
+    float* out_scale;        /* fp32 [rows], required for e4m3: the value is e4m3 * scale */
+    int64_t rows;
+    int64_t cols;
+} ca_rms_norm_args;
+
+/*
+ * ca_rms_norm -- residual_add and rms_norm_inplace (src/model/ops.rs:107-114,
+ * src/model/forward.rs:345-370) of the rows between a layer's products, in one
+ * pass: s = x + residual rounded to the residual stream's type (x itself
+ * without one), y = s * w / sqrt(sum s^2 / cols + eps), sums in fp32. e4m3
+ * output: scale = 2^k with the smallest k in [-64, 120] such that no finite
+ * |y| of the row exceeds 448 * 2^k, value = y / scale to nearest even;
+ * infinities saturate, NaN stays NaN and takes no part in the scale (the rule
+ * of ca_kv8_store, a scale for each row). With norm = 0 it quantises rows: the
+ * operands of ca_linear_q8, weights at load among them. Asynchronous on
+ * `stream`; allocates nothing.
+ */
+int ca_rms_norm(const ca_rms_norm_args* a, void* stream);
+
+/* Arguments of ca_linear_q8 (device pointers; strides in elements). */
+typedef struct {
+    const void* act;         /* e4m3 [n, cols], 16-byte aligned */
+    int64_t act_stride;      /* 0 = cols; a multiple of 16 */
+    const float* act_scale;  /* fp32 [n], or NULL (1) */
+    const void* w;           /* e4m3 [rows, cols], 16-byte aligned */
+    const float* w_scale;    /* fp32 [rows], or NULL (1) */
+    const float* bias;       /* fp32 [rows] or NULL */
+    const void* residual;    /* [n, rows] of out's type or NULL; may be the same buffer as out */
+    int64_t residual_stride; /* 0 = rows */
+    void* out;               /* [n, rows]: bf16, or fp32 when out_f32 */
+    int32_t out_f32;
+    int64_t out_stride;      /* 0 = rows */
+    int64_t n;
+    int64_t rows;
+    int64_t cols;            /* a multiple of 16 */
+    int32_t* status;         /* as ca_dev_args.status */
+} ca_linear_q8_args;
+
+/*
+ * ca_linear_q8 -- ca_linear over 8-bit operands: out = act_scale * w_scale *
+ * (act . W^T) (+ bias) (+ residual), products of e4m3 rows summed in fp32 on
+ * the tensor cores, one rounding to out's type. Asynchronous on `stream`;
+ * allocates nothing.
+ */
+int ca_linear_q8(const ca_linear_q8_args* a, void* stream);
+
+#define CA_ACT_SILU 0
+#define CA_ACT_GELU 1  /* 0.5 g (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) */
+
+/* Arguments of ca_gated_linear (device pointers; strides in elements). */
+typedef struct {
+    const void* act;         /* [n, cols] bf16 or e4m3 (type), 16-byte aligned */
+    int32_t type;            /* of act and both weights */
+    int64_t act_stride;      /* 0 = cols; a multiple of 16 bytes */
+    const float* act_scale;  /* e4m3: fp32 [n] or NULL (1); bf16: NULL */
+    const void* w_gate;      /* [rows, cols], 16-byte aligned */
+    const void* w_up;        /* [rows, cols], 16-byte aligned */
+    const float* gate_scale; /* e4m3: fp32 [rows] or NULL (1); bf16: NULL */
+    const float* up_scale;
+    int32_t activation;      /* CA_ACT_SILU or CA_ACT_GELU, of the gate */
+    void* out;               /* [n, rows]: bf16, or fp32 when out_f32 */
+    int32_t out_f32;
+    int64_t out_stride;      /* 0 = rows */
+    int64_t n;
+    int64_t rows;
+    int64_t cols;            /* a multiple of 16 bytes */
+    int32_t* status;         /* as ca_dev_args.status */
+} ca_gated_linear_args;
+
+/*
+ * ca_gated_linear -- the first half of ffn_block (src/model/forward.rs:
+ * 354-370, :439-461): out = activation(act . Wgate^T) * (act . Wup^T), both
+ * products in fp32 on the tensor cores, the activation and the product of the
+ * two in the same kernel, one rounding. Neither product goes to memory.
+ * Asynchronous on `stream`; allocates nothing.
+ */
+int ca_gated_linear(const ca_gated_linear_args* a, void* stream);
 
 /* Reads and clears the device-wide error word of the current device after
  * synchronising `stream`: CA_OK, or CA_ERR_TIMEOUT if the bounded wait of a
