@@ -9,6 +9,7 @@
 #include "canvas_attn.h"
 #include "host_util.cuh"
 #include "rows.cuh"
+#include "pair.cuh"
 #include "skinny.cuh"
 
 namespace ca {
@@ -151,15 +152,62 @@ int launch_skinny(const Product& q, cudaStream_t st) {
   if (tiles > INT_MAX / 8 || tok > 65535) return CA_ERR_UNSUPPORTED;
   // Columns are split while that fills SMs (two CTAs fit on one) and leaves a
   // CTA at least four stages of work.
+  // fp32 outputs of bf16 operands: few additions to an accumulator, too, which
+  // truncates (pair.cuh).
+  const int64_t most = KIND == kKindBf16 && q.p.out_f32 ? 16 : INT_MAX;
   int S = 1;
+  while (S < 8 && q.p.kblocks > most * S) S *= 2;
   while (S < 8 && tiles * tok * S * 2 <= 2 * kSms && q.p.kblocks >= 8 * S) S *= 2;
   return launch_cluster_after(skinny_kernel<C>,
                               dim3(static_cast<unsigned>(tiles * S), static_cast<unsigned>(tok)),
                               C::kThreads, C::kSmem, S, st, tw, tu, tx, q.p);
 }
 
+template <int KIND, int G, int NT, int CHUNK = 0>
+int launch_pair(const Product& q, cudaStream_t st) {
+  using C = PairCfg<KIND, G, NT, CHUNK>;
+  static bool attr_done[kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return CA_ERR_CUDA;
+  CUtensorMap tw, tu, tx;
+  int rc;
+  const uint32_t box = G == 2 ? 64 : 128;
+  if ((rc = make_tmap_2d(&tw, q.w, KIND, q.cols, q.p.rows, q.cols, box)) != CA_OK) return rc;
+  tu = tw;
+  if (G == 2 && (rc = make_tmap_2d(&tu, q.up, KIND, q.cols, q.p.rows, q.cols, box)) != CA_OK)
+    return rc;
+  if ((rc = make_tmap_2d(&tx, q.act, KIND, q.cols, q.p.n, q.act_stride, NT / 2)) != CA_OK)
+    return rc;
+  if (!attr_done[dev]) {
+    if (cudaFuncSetAttribute(pair_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             C::kSmem) != cudaSuccess)
+      return CA_ERR_CUDA;
+    attr_done[dev] = true;
+  }
+  LinearParams p = q.p;
+  const int64_t rt = (p.rows + C::kRows - 1) / C::kRows, tt = (p.n + NT - 1) / NT;
+  if (rt * tt > INT_MAX / 2) return CA_ERR_UNSUPPORTED;
+  p.r_tiles = static_cast<int>(rt);
+  p.t_tiles = static_cast<int>(tt);
+  const int pairs = static_cast<int>(std::min<int64_t>(rt * tt, kSms / 2));
+  return launch_after(pair_kernel<C>, dim3(2 * pairs), C::kThreads, C::kSmem, st, tw, tu, tx, p);
+}
+
 template <int KIND, int G>
 int launch_product(const Product& q, cudaStream_t st) {
+  if (q.p.n > 64) {
+    // 16 pieces of 64 bf16 are 64 additions to an accumulator.
+    if (KIND == kKindBf16 && q.p.out_f32) return launch_pair<KIND, G, 128, 16>(q, st);
+    // Tiles of 128 tokens where they take fewer rounds of the pairs: one costs
+    // about 0.6 of a tile of 256 (its operands' way out of shared memory is the
+    // bound).
+    const int64_t rt = (q.p.rows + 256 / G - 1) / (256 / G);
+    auto rounds = [&](int64_t nt) {
+      return (rt * ((q.p.n + nt - 1) / nt) + kSms / 2 - 1) / (kSms / 2);
+    };
+    if (6 * rounds(128) < 10 * rounds(256)) return launch_pair<KIND, G, 128>(q, st);
+    return launch_pair<KIND, G, 256>(q, st);
+  }
   if (q.p.n <= 16) return launch_skinny<KIND, G, 16>(q, st);
   if (q.p.n <= 32) return launch_skinny<KIND, G, 32>(q, st);
   return launch_skinny<KIND, G, 64>(q, st);

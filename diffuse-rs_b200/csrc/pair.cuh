@@ -1,0 +1,349 @@
+// pair.cuh -- act . W^T for many rows of act, alone or gated: two SMs on one
+// tile (tcgen05 with cta_group::2), persistent.
+//
+// Formulas as in skinny.cuh. The two CTAs of a cluster take 256 weight rows by
+// NT tokens: each holds 128 rows of the weights and half the tokens in its
+// shared memory and, in its TMEM, its 128 rows of the product, so that an
+// operand byte fetched from L2 serves twice the multiplications that it would
+// in one CTA. Accumulators are double buffered in TMEM: while the tensor cores
+// work on a tile, eight warps of each CTA scale, activate, round and store the
+// one before.
+//
+// Gated: of a CTA's 128 rows 64 are of Wgate and 64 of Wup, the same ones. A
+// row's gate and up are then 64 lanes apart, in two warps that pass each other
+// half their tokens through shared memory (16 tokens at a time: eight stores,
+// a barrier of the two, eight loads) and finish the other half each. Both
+// matrices as operands of their own would leave room for 128 tokens a tile
+// with two buffers, and at 128 the operands' way out of shared memory is the
+// bound (8192 tokens, 4096 -> 12288 in e4m3: 1031 us); turns of 16 rows, which
+// a shuffle could bring together, need nine loads a stage (887 us).
+//
+// CHUNK > 0: the tensor core adds to an accumulator for CHUNK pieces of 128
+// bytes at most, then the storing warps add it up in registers. It truncates
+// as it accumulates: bf16 operands of 4112 columns gave fp32 results 9e-6 off
+// in 2-norm without it (e4m3 ones, whose products are short, 2e-6 at 18944
+// columns). Only fp32 outputs of bf16 operands show that.
+//
+// Warps: 0 loads (TMA, both CTAs, completing on the even CTA's barriers), 1
+// issues (the even CTA alone), 2-9 store, half the tokens of 32 lanes each. Lane = weight row, column = token: a
+// warp's threads store 32 neighbours of an output row.
+#pragma once
+
+#include <cstdint>
+
+#include "skinny.cuh"
+
+namespace ca {
+
+// A load into this CTA's shared memory that completes on `bar`, which may be a
+// barrier of the pair's other CTA.
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap, uint32_t bar,
+                                                 int32_t x, int32_t y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile"
+      ".mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+
+template <int KIND>
+__device__ __forceinline__ void mma_ss_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                            uint32_t accumulate) {
+  if constexpr (KIND == kKindBf16) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+
+// Arrives on `bar` of both CTAs when every MMA issued so far is done.
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;" ::"r"(bar),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+               : "memory");
+}
+
+template <int KIND_, int G_, int NT_, int CHUNK_ = 0>
+struct PairCfg {
+  static constexpr int CHUNK = CHUNK_;
+  static constexpr int KIND = KIND_;
+  static constexpr int G = G_;
+  static constexpr int NT = NT_;  // tokens of a tile
+  static constexpr int kStage = 16384 + NT / 2 * 128;
+  static constexpr int kStages = 208 * 1024 / kStage < 8 ? 208 * 1024 / kStage : 8;
+  static constexpr int kRing = kStages * kStage;
+  static constexpr int kThreads = 320;
+  static constexpr int kBars = 2 * kStages + 4;
+  static constexpr int kHalf = NT / 2;  // tokens of a storing warp
+  static constexpr int kScales = 8 * kHalf * 4;
+  static constexpr int kSwap = G == 2 ? 16384 : 0;  // 8 warps x 2 buffers x 8 tokens x 32 lanes
+  static constexpr int kSmem = 1024 + kRing + kScales + kSwap + 8 * kBars + 16;
+  static constexpr int kBuf = NT;  // TMEM columns of a buffer
+  static constexpr int kRows = 256 / G;  // output rows of a tile
+  static constexpr int kTmemCols = 2 * kBuf;
+  static constexpr int kElems = KIND == kKindBf16 ? 64 : 128;
+  static_assert(kTmemCols <= 512 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM");
+};
+
+constexpr int kPairGroup = 8;  // row tiles side by side in the order of the tiles
+
+// Tile i of r_tiles x t_tiles: row tiles in groups, tokens in a group's turn,
+// so that the tiles in work at a time share what they read in both operands.
+__device__ __forceinline__ void pair_tile(const LinearParams& p, int i, int& rt, int& tt) {
+  const int g = i / (kPairGroup * p.t_tiles);
+  const int first = g * kPairGroup, size = min(kPairGroup, p.r_tiles - first);
+  const int j = i - first * p.t_tiles;
+  rt = first + j % size;
+  tt = j / size;
+}
+
+template <class C>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::kThreads)
+    pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_u,
+                const __grid_constant__ CUtensorMap tm_x, const LinearParams p) {
+  extern __shared__ uint8_t raw_smem[];
+  const uint32_t base = (smem_u32(raw_smem) + 1023u) & ~1023u;
+  const uint32_t scales = base + C::kRing, swap = scales + C::kScales;
+  const uint32_t bars = swap + C::kSwap, slot = bars + 8 * C::kBars;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  auto full = [&](int s) { return bars + 8 * s; };                      // of the even CTA
+  auto empty = [&](int s) { return bars + 8 * (C::kStages + s); };      // each CTA's
+  auto acc_full = [&](int b) { return bars + 8 * (2 * C::kStages + b); };
+  auto acc_empty = [&](int b) { return bars + 8 * (2 * C::kStages + 2 + b); };  // of the even CTA
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+  const int tiles = p.r_tiles * p.t_tiles;
+
+  if (tid == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full(b), 1);
+      mbar_init(acc_empty(b), 16);
+    }
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  wait_prior_kernel();  // before TMEM is taken, as in skinny.cuh
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot),
+                 "r"(C::kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync_all();  // the barriers of both are set
+  tc_fence_after();
+  let_next_kernel();
+  uint32_t tmem;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
+  bool dead = false;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int i = 0;  // stages filled
+      for (int tile = pair; tile < tiles && !dead; tile += n_pairs) {
+        int rt, tt;
+        pair_tile(p, tile, rt, tt);
+        const int r0 = rt * C::kRows + static_cast<int>(rank) * (C::kRows / 2);
+        const int t0 = tt * C::NT + static_cast<int>(rank) * (C::NT / 2);
+        for (int kb = 0; kb < p.kblocks; ++kb, ++i) {
+          const int s = i % C::kStages;
+          if (i >= C::kStages && !mbar_wait(empty(s), ((i / C::kStages) - 1) & 1, dead, p.err))
+            break;
+          if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * C::kStage);
+          const uint32_t dst = base + s * C::kStage, bar = map_to_rank(full(s), 0);
+          tma_load_2d_pair(dst, &tm_w, bar, kb * C::kElems, r0);
+          if constexpr (C::G == 2) tma_load_2d_pair(dst + 8192, &tm_u, bar, kb * C::kElems, r0);
+          tma_load_2d_pair(dst + 16384, &tm_x, bar, kb * C::kElems, t0);
+        }
+      }
+      // After an expired wait the copies in flight still have to land; the
+      // even CTA's barriers count those of both.
+      if (dead && rank == 0) {
+        bool late = false;
+        for (int j = max(0, i - C::kStages); j < i; ++j)
+          mbar_wait(full(j % C::kStages), (j / C::kStages) & 1, late, p.err);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = linear_idesc(C::KIND, 256, C::NT);
+      int i = 0, n = 0;  // stages taken, accumulators filled
+      for (int tile = pair; tile < tiles && !dead; tile += n_pairs, ++n) {
+        uint32_t acc = 0;
+        int first = 0;
+        for (int kb = 0; kb < p.kblocks; ++kb, ++i) {
+          if (kb == 0 || (C::CHUNK > 0 && kb % C::CHUNK == 0)) {
+            if (kb > 0) umma_commit_pair(acc_full(n++ & 1));
+            if (n >= 2 && !mbar_wait(acc_empty(n & 1), ((n >> 1) - 1) & 1, dead, p.err)) break;
+            tc_fence_after();
+            acc = tmem + (n & 1) * C::kBuf;
+            first = kb;
+          }
+          const int s = i % C::kStages;
+          if (!mbar_wait(full(s), (i / C::kStages) & 1, dead, p.err)) break;
+          tc_fence_after();
+          const uint32_t at = base + s * C::kStage;
+          const uint64_t dw = umma_desc_sw128(at, 16, 1024);
+          const uint64_t dx = umma_desc_sw128(at + 16384, 16, 1024);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_ss_pair<C::KIND>(acc, dw + 2 * kk, dx + 2 * kk, idesc, (kb - first) | kk);
+          umma_commit_pair(empty(s));
+        }
+        umma_commit_pair(acc_full(n & 1));
+      }
+    }
+  } else {
+    int n = 0;
+    const int half0 = (warp - 2) / 4 * C::kHalf;  // this warp's first token of a tile
+    // Gated: the warp that holds the other matrix's rows, its barrier.
+    const bool up = C::G == 2 && (warp & 2);
+    const int swap_bar = 1 + (warp & 1) + (warp - 2) / 4 * 2;
+    int turn = 0;
+    const uint32_t sa_at = scales + (warp - 2) * C::kHalf * 4;
+    auto take = [&]() {  // the next accumulator
+      mbar_wait(acc_full(n & 1), (n >> 1) & 1, dead, p.err);
+      __syncwarp();
+      tc_fence_after();
+      return tmem + (n & 1) * C::kBuf + half0 + (static_cast<uint32_t>(warp & 3) << 21);
+    };
+    auto give = [&]() {  // it may be written again
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_to_rank(acc_empty(n & 1), 0));
+      ++n;
+    };
+    // An expired wait (`dead`: later ones return at once) ends no warp early:
+    // warps that pass each other their parts stay in step.
+    for (int tile = pair; tile < tiles; tile += n_pairs) {
+      int rt, tt;
+      pair_tile(p, tile, rt, tt);
+      // The output row of this lane; gated: of lanes l and l + 64 of TMEM.
+      const int q = (C::G == 2 ? warp & 1 : warp & 3) * 32 + lane;
+      const long long r = static_cast<long long>(rt) * C::kRows + rank * (C::kRows / 2) + q;
+      const long long t0 = static_cast<long long>(tt) * C::NT + half0;
+      const bool ok = r < p.rows;
+      float w0 = 1.f, w1 = 1.f, bias = 0.f;
+      if (ok) {
+        if (p.w_scale) w0 = p.w_scale[r];
+        if (C::G == 2 && p.up_scale) w1 = p.up_scale[r];
+        if (C::G == 1 && p.bias) bias = p.bias[r];
+      }
+      if (p.act_scale) {
+        __syncwarp();  // the last tile's are read
+        for (int j = lane; j < C::kHalf; j += 32)
+          st_shared_f32(sa_at + 4 * j, t0 + j < p.n ? p.act_scale[t0 + j] : 1.f);
+        __syncwarp();
+      }
+      float next[16];  // residuals of the sixteen tokens to come
+      if (C::G == 1 && p.residual) load_residual(p, next, t0, r, tokens_in<16>(p, t0, ok));
+      // Sixteen tokens from t0 + j0 on.
+      auto finish = [&](float (&d)[16], int j0) {
+        if (p.act_scale) {
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            float s[4];
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(s[0]), "=f"(s[1]), "=f"(s[2]), "=f"(s[3])
+                         : "r"(sa_at + 4 * (j0 + j)));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) d[j + k] *= s[k];
+          }
+        }
+        if constexpr (C::G == 2) {
+          // Gate warps finish the first eight tokens, up warps the others.
+          const uint32_t mine = swap + (warp - 2) * 2048 + (turn & 1) * 1024 + lane * 4;
+          const uint32_t theirs = swap + ((warp - 2) ^ 2) * 2048 + (turn & 1) * 1024 + lane * 4;
+          ++turn;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) st_shared_f32(mine + j * 128, up ? d[j] : d[8 + j]);
+          named_bar_sync(swap_bar, 64);
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float other;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(theirs + j * 128) : "memory");
+            const float g = up ? other : d[j], u = up ? d[8 + j] : other;
+            v[j] = activate(g * w0, p.act) * (u * w1);
+          }
+          const long long t = t0 + j0 + (up ? 8 : 0);
+          store_tokens(p, v, t, r, tokens_in<8>(p, t, ok));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) d[j] = fmaf(d[j], w0, bias);
+          if (p.residual) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) d[j] += next[j];
+            const long long t = t0 + j0 + 16;
+            if (j0 + 16 < C::kHalf) load_residual(p, next, t, r, tokens_in<16>(p, t, ok));
+          }
+          store_tokens(p, d, t0 + j0, r, tokens_in<16>(p, t0 + j0, ok));
+        }
+      };
+      if constexpr (C::CHUNK > 0) {
+        float v[C::kHalf / 16][16];
+#pragma unroll
+        for (int j = 0; j < C::kHalf; ++j) v[j / 16][j % 16] = 0.f;
+        for (int kb = 0; kb < p.kblocks; kb += C::CHUNK) {
+          const uint32_t col = take();
+#pragma unroll
+          for (int j0 = 0; j0 < C::kHalf; j0 += 16) {
+            uint32_t d[16];
+            tmem_ld16(col + j0, d);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j0 / 16][j] += __uint_as_float(d[j]);
+          }
+          give();
+        }
+#pragma unroll
+        for (int j0 = 0; j0 < C::kHalf; j0 += 16) finish(v[j0 / 16], j0);
+      } else {
+        const uint32_t col = take();
+#pragma unroll 1
+        for (int j0 = 0; j0 < C::kHalf; j0 += 16) {
+          uint32_t d[16];
+          tmem_ld16(col + j0, d);
+          tmem_wait_ld();
+          float v[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(d[j]);
+          finish(v, j0);
+        }
+        give();
+      }
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(C::kTmemCols));
+  }
+  __syncwarp();
+  cluster_sync_all();
+}
+
+}  // namespace ca

@@ -39,7 +39,7 @@ struct LinearParams {
   int kblocks;              // 128-byte pieces of a row
   int out_f32;
   int act;                  // CA_ACT_*
-  int n_tiles, r_tiles;     // pair.cuh: its tiles
+  int r_tiles, t_tiles;     // pair.cuh: its tiles
   int* err;
 };
 
@@ -88,27 +88,52 @@ __device__ __forceinline__ float activate(float g, int act) {
   return __fdividef(g, 1.f + __expf(-2.f * y));
 }
 
-// What a product of one token and weight row becomes.
-template <int G>
-__device__ __forceinline__ void linear_store(const LinearParams& p, float d0, float d1, float w0,
-                                             float w1, float bias, long long t, long long r) {
-  const float sa = p.act_scale ? p.act_scale[t] : 1.f;
-  float v;
-  if constexpr (G == 2) {
-    v = activate(d0 * sa * w0, p.act) * (d1 * sa * w1);
+// How many of the N tokens from t on have an element r of their own.
+template <int N>
+__device__ __forceinline__ int tokens_in(const LinearParams& p, long long t, bool ok) {
+  return ok ? static_cast<int>(max(0ll, min(static_cast<long long>(N), p.n - t))) : 0;
+}
+
+// The residual's element r of the first m of N tokens from t on.
+template <int N>
+__device__ __forceinline__ void load_residual(const LinearParams& p, float (&x)[N], long long t,
+                                              long long r, int m) {
+  if (p.out_f32) {
+    const float* s = static_cast<const float*>(p.residual) + t * p.res_stride + r;
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = j < m ? s[j * p.res_stride] : 0.f;
   } else {
-    v = d0 * sa * w0 + bias;
-    if (p.residual) {
-      const long long i = t * p.res_stride + r;
-      v += p.out_f32 ? static_cast<const float*>(p.residual)[i]
-                     : __bfloat162float(static_cast<const __nv_bfloat16*>(p.residual)[i]);
+    const __nv_bfloat16* s = static_cast<const __nv_bfloat16*>(p.residual) + t * p.res_stride + r;
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = j < m ? __bfloat162float(s[j * p.res_stride]) : 0.f;
+  }
+}
+
+// Element r of the first m of N tokens from t on, rounded once.
+template <int N>
+__device__ __forceinline__ void store_tokens(const LinearParams& p, const float (&v)[N],
+                                             long long t, long long r, int m) {
+  if (p.out_f32) {
+    float* o = static_cast<float*>(p.out) + t * p.out_stride + r;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < m) o[j * p.out_stride] = v[j];
+  } else {
+    __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + t * p.out_stride + r;
+    if (m == N) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) o[j * p.out_stride] = __float2bfloat16_rn(v[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (j < m) o[j * p.out_stride] = __float2bfloat16_rn(v[j]);
     }
   }
-  const long long o = t * p.out_stride + r;
-  if (p.out_f32)
-    static_cast<float*>(p.out)[o] = v;
-  else
-    static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(v);
+}
+
+// The scales of tokens t .. t + 31, one a lane.
+__device__ __forceinline__ float act_scale_of(const LinearParams& p, long long t) {
+  return p.act_scale && t < p.n ? p.act_scale[t] : 1.f;
 }
 
 template <int KIND_, int G_, int NT_>
@@ -216,6 +241,9 @@ __global__ void __launch_bounds__(C::kThreads)
   const int f = (warp & 3) * 32 + lane;
   const long long r = r0 + f;
   float w0 = 1.f, w1 = 1.f, bias = 0.f;
+  auto combine = [&](float a, float b, float sa) {
+    return C::G == 2 ? activate(a * sa * w0, p.act) * (b * sa * w1) : a * sa * w0 + bias;
+  };
   if (warp >= 2) {
     if (r < p.rows) {
       if (p.w_scale) w0 = p.w_scale[r];
@@ -225,21 +253,34 @@ __global__ void __launch_bounds__(C::kThreads)
     mbar_wait(done, 0, dead, p.err);
     tc_fence_after();
     const uint32_t col = tmem + (static_cast<uint32_t>(warp & 3) << 21);
-#pragma unroll
+#pragma unroll 1
     for (int j0 = 0; j0 < C::NT; j0 += 16) {
       uint32_t d0[16], d1[16];
       tmem_ld16(col + j0, d0);
       if constexpr (C::G == 2) tmem_ld16(col + C::NT + j0, d1);
+      const float sa = act_scale_of(p, t0 + j0 + (lane & 15));
       tmem_wait_ld();
+      if (S == 1) {
+        const int m = tokens_in<16>(p, t0 + j0, r < p.rows);
+        // Residuals are all asked for before the first store: out may be the
+        // same memory, so the compiler may not move them up itself.
+        float v[16], x[16];
+        if (p.residual) load_residual(p, x, t0 + j0, r, m);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float a = __uint_as_float(d0[j]), b = C::G == 2 ? __uint_as_float(d1[j]) : 0.f;
-        if (S == 1) {
-          if (t0 + j0 + j < p.n && r < p.rows)
-            linear_store<C::G>(p, a, b, w0, w1, bias, t0 + j0 + j, r);
-        } else {
-          st_shared_f32(base + ((j0 + j) * 128 + f) * 4, a);
-          if constexpr (C::G == 2) st_shared_f32(base + ((C::NT + j0 + j) * 128 + f) * 4, b);
+        for (int j = 0; j < 16; ++j)
+          v[j] = combine(__uint_as_float(d0[j]), C::G == 2 ? __uint_as_float(d1[j]) : 0.f,
+                         __shfl_sync(0xffffffffu, sa, j));
+        if (p.residual) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] += x[j];
+        }
+        store_tokens(p, v, t0 + j0, r, m);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          st_shared_f32(base + ((j0 + j) * 128 + f) * 4, __uint_as_float(d0[j]));
+          if constexpr (C::G == 2)
+            st_shared_f32(base + ((C::NT + j0 + j) * 128 + f) * 4, __uint_as_float(d1[j]));
         }
       }
     }
@@ -259,7 +300,13 @@ __global__ void __launch_bounds__(C::kThreads)
           if constexpr (C::G == 2)
             b += ld_cluster_f32(map_to_rank(base + ((C::NT + j) * 128 + f) * 4, q));
         }
-        linear_store<C::G>(p, a, b, w0, w1, bias, t0 + j, r);
+        float v[1] = {combine(a, b, p.act_scale ? p.act_scale[t0 + j] : 1.f)};
+        if (p.residual) {
+          float x[1];
+          load_residual(p, x, t0 + j, r, 1);
+          v[0] += x[0];
+        }
+        store_tokens(p, v, t0 + j, r, 1);
       }
     }
     __syncwarp();
