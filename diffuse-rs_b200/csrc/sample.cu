@@ -19,21 +19,21 @@ int launch_sample(const ca_sample_args* a, SampleParams p, cudaStream_t st) {
   constexpr int most = kSampleSegBytes / sizeof(T);
   if (!attr_done[dev]) {
     if (cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kSampleSegBytes) != cudaSuccess)
+                             kSampleSegBytes + kSampleExtra) != cudaSuccess)
       return CA_ERR_CUDA;
     attr_done[dev] = true;
   }
-  // As many CTAs a row as it needs to fit, and more while SMs would idle and
-  // a thread has at least four entries.
+  // As many CTAs a row as leave two on an SM (one loads while the other
+  // computes), and more while SMs would idle and a thread has four entries.
+  constexpr int two = 80 * 1024 / sizeof(T);
   int c = 1;
-  while (c < 8 && (p.n_vocab > c * most || (a->n_cand * 2ll * c <= kSms &&
-                                            p.n_vocab >= 2 * c * 4 * kSampleThreads)))
+  while (c < 8 && (p.n_vocab > c * two || (a->n_cand * 2ll * c <= 2 * kSms &&
+                                           p.n_vocab >= 2 * c * 4 * kSampleThreads)))
     c *= 2;
   if (p.n_vocab > static_cast<int64_t>(c) * most) return CA_ERR_UNSUPPORTED;
-  p.seg = ((p.n_vocab + c - 1) / c + 15) / 16 * 16;
-  p.seg = std::min(p.seg, most);
+  p.seg = ((p.n_vocab + c - 1) / c + 127) / 128 * 128;
   return launch_cluster_after(sample_kernel<T>, dim3(static_cast<unsigned>(a->n_cand) * c),
-                              kSampleThreads, p.seg * sizeof(T), c, st, p);
+                              kSampleThreads, p.seg * sizeof(T) + kSampleExtra, c, st, p);
 }
 
 int sample_impl(const ca_sample_args* a, cudaStream_t st) {

@@ -10,29 +10,49 @@
 // Every cut is a border (key K, index I): an entry is before it if its key is
 // above K, or equal with an index of at most I. Sums decide which side of a
 // border a number falls on, so they are exact whatever their order: weights
-// are taken in 64 bits and rounded to steps of 2^-44 (a row's largest is 1),
-// and whole numbers are added.
+// are taken in 64 bits, rounded to steps of 2^-44 (a row's largest is 1), and
+// whole numbers are added.
 //
 // A cluster of 1 to 8 CTAs takes a row: its segments stay in shared memory,
 // so HBM sees the logits once, and what the CTAs have to tell each other goes
 // through distributed shared memory.
+//
+// Borders are found in two steps. A histogram over log2 w (bins of 1/32,
+// weights within a factor of 2^(1/32) of one another) tells which bins lie
+// before a border for certain and which may hold it. Then either every entry
+// up to there fits a list of the cluster's first CTA, which settles the rest
+// by itself (a top-k, a sharp nucleus), or the entries of the doubtful bins do
+// (a wide nucleus). What fits neither (thousands of entries in one bin, as
+// rows of equal logits have) is settled by bisection of the keys over the
+// whole row, 32 sums a border.
 #pragma once
 
 #include <cstdint>
 #include <cuda_bf16.h>
 
 #include "cluster.cuh"
+#include "sm100.cuh"
 
 namespace ca {
 
-constexpr int kSampleThreads = 1024;
+constexpr int kSampleThreads = 512;
 constexpr int kSampleWarps = kSampleThreads / 32;
-constexpr int kSampleSegBytes = 208 * 1024;  // of a row, a CTA
+constexpr int kSampleSegBytes = 184 * 1024;  // of a row, a CTA
+constexpr int kBins = 1536;                  // 1/32 each: beyond 2^-45 there is no weight
+constexpr int kBinsEach = kBins / kSampleThreads;
+constexpr float kBinsPerOctave = 32.f;
+constexpr int kListEach = 6;                 // entries of a thread
+constexpr int kList = kListEach * kSampleThreads;
+constexpr int kQueue = 160;                  // values a warp holds back
+constexpr int kSampleExtra = kBins * 4 + kList * 8;
+static_assert(kSampleWarps * kQueue * 4 <= kList * 8, "the queues lie over the list");
+
+typedef unsigned long long u64;
 
 struct SampleParams {
   const void* logits;
   long long row_stride, n_rows;
-  int n_vocab, seg;  // entries of a CTA
+  int n_vocab, seg;  // entries of a CTA, a multiple of 128
   const int* rows;
   int mask_id;
   const int* suppress;
@@ -48,119 +68,427 @@ struct SampleParams {
   float* prob;
 };
 
-typedef unsigned long long u64;
-
-// Keys in the order of the values.
+// Keys in the order of the values, NaN as -inf, -0 as +0.
 __device__ __forceinline__ uint32_t key_of(float l) {
-  const uint32_t u = __float_as_uint(l);
+  const uint32_t u = __float_as_uint(fmaxf(l, -INFINITY) + 0.f);
   return (u >> 31) ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float value_of(uint32_t k) {
+  return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
+}
 
-// Weights in steps of 2^-44, by the alignment of a sum with 256.
+// A weight of at most 1 in steps of 2^-44, by the alignment of a sum with 256.
 __device__ __forceinline__ u64 fixed44(double w) {
   return static_cast<u64>(__double_as_longlong(w + 256.0) - __double_as_longlong(256.0));
 }
 
+// 2^a for -1000 < a < 1000 to 2e-14: a = n + f with n the nearest whole number
+// (the low bits of a sum with 1.5 * 2^52), 2^f by the Chebyshev interpolation
+// of degree 9 on [-1/2, 1/2], n added to the exponent.
+__device__ __forceinline__ double exp2_64(double a) {
+  const double t = a + 6755399441055744.0;
+  const double f = a - (t - 6755399441055744.0);
+  double p = 1.0212097549811005e-07;
+  p = fma(p, f, 1.3259945262689143e-06);
+  p = fma(p, f, 1.5252640059770786e-05);
+  p = fma(p, f, 0.00015403432339553542);
+  p = fma(p, f, 0.001333355825801874);
+  p = fma(p, f, 0.009618129195951041);
+  p = fma(p, f, 0.05550410866428854);
+  p = fma(p, f, 0.24022650695631514);
+  p = fma(p, f, 0.6931471805599526);
+  p = fma(p, f, 1.000000000000014);
+  return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
+}
+
 struct SampleShared {
-  u64 warp_sum[kSampleWarps];
-  u64 cta_sum[2];
+  u64 warp_sum[kSampleWarps], warp_sum2[kSampleWarps];
+  u64 cta_sum[2], cta_sum2[2];
   uint32_t found[2];
   float max_v[kSampleWarps];
   float cta_max;
+  double warp_d[kSampleWarps];
+  uint32_t warp_u[kSampleWarps];
+  uint32_t bin_lo, bin_hi, n_lo, n_hi;
+  uint32_t border[2];              // key, index
+  uint32_t answer;
+  u64 list_sum[kSampleWarps];
+  u64 range_sum[8 * kSampleWarps]; // of the first CTA: kept doubtful entries of every warp
+};
+
+// What a row's weights are made of.
+struct SampleWeights {
+  float m, cut;   // entries at or below cut weigh nothing
+  double c, b;    // log2 w = c l + b
+  float bin_c;    // bin = -bin_c (l - m), to the nearest
+  double least;   // min_p
+
+  __device__ __forceinline__ bool none(float l) const { return l != m && !(l > cut); }
+  __device__ __forceinline__ double weight(float l) const {  // of an entry that is not none()
+    return l == m ? 1.0 : exp2_64(fma(static_cast<double>(l), c, b));
+  }
+  __device__ __forceinline__ u64 fixed(float l) const {
+    return none(l) ? 0 : fixed44(weight(l));
+  }
+  __device__ __forceinline__ int bin(float l) const {
+    if (l == m) return 0;
+    const float t = fmaf(l - m, -bin_c, 8388608.f);
+    return min(static_cast<int>(__float_as_uint(t) - 0x4B000000u), kBins - 1);
+  }
 };
 
 template <class T>
 struct SampleRow {
   const T* seg;
-  int len, first;  // entries of this CTA's segment, the first one's index
-  int lo, hi;      // this warp's entries in it
+  int first;   // index of the segment's first entry
+  int lo, hi;  // this warp's entries in it, multiples of 128
   int lane, warp;
   uint32_t rank, n_ranks;
   SampleShared* sh;
+  uint32_t* hist;
+  uint32_t* list_key;
+  uint32_t* list_idx;
   int turn = 0;
 
-  __device__ __forceinline__ float at(int i) const {
-    if constexpr (sizeof(T) == 4)
-      return seg[i];
-    else
-      return __uint_as_float(static_cast<uint32_t>(seg[i]) << 16);
+  __device__ __forceinline__ void load4(int i, float (&v)[4]) const {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = *reinterpret_cast<const float4*>(seg + i);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    } else {
+      const uint2 a = *reinterpret_cast<const uint2*>(seg + i);
+      v[0] = __uint_as_float(a.x << 16);
+      v[1] = __uint_as_float(a.x & 0xffff0000u);
+      v[2] = __uint_as_float(a.y << 16);
+      v[3] = __uint_as_float(a.y & 0xffff0000u);
+    }
   }
 
-  // The sum of q(value, index) over the row; `before`: over the entries of
-  // lower ranks, `mine`: over this warp's.
-  template <class Q>
-  __device__ __forceinline__ u64 total(Q q, u64& before, u64& mine) {
-    u64 s = 0;
-    for (int i = lo + lane; i < hi; i += 32) s += q(at(i), first + i);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    mine = s;
-    if (lane == 0) sh->warp_sum[warp] = s;
+  __device__ __forceinline__ static uint32_t smem_addr(const void* p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+  }
+
+  // Sums over a warp of numbers below 2^59: pieces of 27 bits (32 of them fit
+  // 32 bits), each by one reduction instruction.
+  __device__ __forceinline__ static u64 warp_total(u64 s) {
+    const uint32_t a = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(s) & 0x7ffffffu);
+    const uint32_t b = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(s >> 27) & 0x7ffffffu);
+    const uint32_t c = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(s >> 54));
+    return a + (static_cast<u64>(b) << 27) + (static_cast<u64>(c) << 54);
+  }
+
+  // The sum of the warps' `mine` over the row; `before`: over lower ranks.
+  // `second`: another sum, made that of the row.
+  __device__ __forceinline__ u64 gather(u64 mine, u64& before, u64* second = nullptr) {
+    if (lane == 0) {
+      sh->warp_sum[warp] = mine;
+      if (second) sh->warp_sum2[warp] = *second;
+    }
     __syncthreads();
     turn ^= 1;
     if (warp == 0) {
-      u64 c = sh->warp_sum[lane];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+      u64 c = lane < kSampleWarps ? sh->warp_sum[lane] : 0;
+      c = warp_total(c);
       if (lane == 0) sh->cta_sum[turn] = c;
+      if (second) {
+        c = lane < kSampleWarps ? sh->warp_sum2[lane] : 0;
+        c = warp_total(c);
+        if (lane == 0) sh->cta_sum2[turn] = c;
+      }
     }
     __syncwarp();
     cluster_sync_all();
-    u64 all = 0;
+    u64 all = 0, all2 = 0;
     before = 0;
+#pragma unroll 1
     for (uint32_t r = 0; r < n_ranks; ++r) {
       const u64 c = ld_cluster_u64(map_to_rank(smem_addr(&sh->cta_sum[turn]), r));
       if (r < rank) before += c;
       all += c;
+      if (second) all2 += ld_cluster_u64(map_to_rank(smem_addr(&sh->cta_sum2[turn]), r));
     }
+    if (second) *second = all2;
     return all;
+  }
+
+  // This warp's part of the sum of q(value, index).
+  template <class Q>
+  __device__ __forceinline__ u64 part(Q q) {
+    u64 s = 0;
+    for (int i = lo + 4 * lane; i < hi; i += 128) {
+      float v[4];
+      load4(i, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s += q(v[j], first + i + j);
+    }
+    return warp_total(s);
   }
   template <class Q>
   __device__ __forceinline__ u64 total(Q q) {
-    u64 a, b;
-    return total(q, a, b);
+    u64 before;
+    return gather(part(q), before);
   }
 
-  // The first index up to which q sums to more than target(sum over the row).
-  template <class Q, class F>
-  __device__ __forceinline__ int find(Q q, F target_of) {
-    u64 before, mine;
-    const u64 all = total(q, before, mine);
-    const u64 target = target_of(all);
+  // The first index up to which q sums to more than `target`, given this
+  // warp's part and what the lower ranks hold.
+  template <class Q>
+  __device__ __forceinline__ int find(Q q, u64 target, u64 before, u64 mine) {
     u64 s = before;
     for (int w = 0; w < warp; ++w) s += sh->warp_sum[w];
     if (s <= target && target < s + mine) {
-      for (int i0 = lo; i0 < hi; i0 += 32) {
-        const int i = i0 + lane;
-        u64 c = i < hi ? q(at(i), first + i) : 0;
+      for (int i0 = lo; i0 < hi; i0 += 128) {
+        const int i = i0 + 4 * lane;
+        float v[4];
+        load4(i, v);
+        u64 e[4], c = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c += e[j] = q(v[j], first + i + j);
+        u64 up = c;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const u64 t = __shfl_up_sync(0xffffffffu, c, o);
-          if (lane >= o) c += t;
+          const u64 t = __shfl_up_sync(0xffffffffu, up, o);
+          if (lane >= o) up += t;
         }
-        const uint32_t over = __ballot_sync(0xffffffffu, s + c > target);
+        const uint32_t over = __ballot_sync(0xffffffffu, s + up > target);
         if (over) {
-          const int k = __ffs(over) - 1;
-          if (static_cast<uint32_t>(lane) < n_ranks)
-            st_cluster_u32(map_to_rank(smem_addr(&sh->found[turn]), lane),
-                           static_cast<uint32_t>(first + i0 + k));
+          if (lane == __ffs(over) - 1) {
+            u64 t = s + up - c;
+            int k = 0;
+            while (k < 3 && t + e[k] <= target) t += e[k++];
+            for (uint32_t r = 0; r < n_ranks; ++r)
+              st_cluster_u32(map_to_rank(smem_addr(&sh->found[turn]), r),
+                             static_cast<uint32_t>(first + i + k));
+          }
           break;
         }
-        s += __shfl_sync(0xffffffffu, c, 31);
+        s += __shfl_sync(0xffffffffu, up, 31);
       }
     }
     __syncwarp();
     cluster_sync_all();
     return static_cast<int>(sh->found[turn]);
   }
+  template <class Q, class F>
+  __device__ __forceinline__ int find(Q q, F target_of) {
+    u64 before;
+    const u64 mine = part(q);
+    const u64 all = gather(mine, before);
+    return find(q, target_of(all), before, mine);
+  }
 
-  __device__ __forceinline__ static uint32_t smem_addr(const void* p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+  // The first index whose value is `m` (there is one).
+  __device__ __forceinline__ int first_of(float m) {
+    uint32_t best = 0xffffffffu;
+    for (int i0 = lo; i0 < hi; i0 += 128) {
+      const int i = i0 + 4 * lane;
+      float v[4];
+      load4(i, v);
+      const bool any = v[0] == m || v[1] == m || v[2] == m || v[3] == m;
+      const uint32_t who = __ballot_sync(0xffffffffu, any);
+      if (who) {
+        const int k = v[0] == m ? 0 : v[1] == m ? 1 : v[2] == m ? 2 : 3;
+        best = __shfl_sync(0xffffffffu, static_cast<uint32_t>(first + i + k), __ffs(who) - 1);
+        break;
+      }
+    }
+    if (lane == 0) sh->warp_u[warp] = best;
+    __syncthreads();
+    turn ^= 1;
+    if (warp == 0) {
+      best = __reduce_min_sync(0xffffffffu, lane < kSampleWarps ? sh->warp_u[lane] : 0xffffffffu);
+      if (lane == 0) sh->found[turn] = best;
+    }
+    __syncwarp();
+    cluster_sync_all();
+    best = 0xffffffffu;
+    for (uint32_t r = 0; r < n_ranks; ++r) {
+      uint32_t t;
+      asm volatile("ld.shared::cluster.u32 %0, [%1];"
+                   : "=r"(t) : "r"(map_to_rank(smem_addr(&sh->found[turn]), r)) : "memory");
+      best = min(best, t);
+    }
+    return static_cast<int>(best);
+  }
+
+  // This warp's part of the sum of q over the entries that `in` holds for:
+  // those are queued, so that a warp's lanes have one each to weigh.
+  template <class P, class Q>
+  __device__ __forceinline__ u64 part_of(P in, Q q) {
+    float* queue = reinterpret_cast<float*>(list_key) + warp * kQueue;
+    u64 s = 0;
+    int n = 0;
+    for (int i = lo + 4 * lane; i < hi; i += 128) {
+      float v[4];
+      load4(i, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool t = in(v[j]);
+        const uint32_t who = __ballot_sync(0xffffffffu, t);
+        if (t) queue[n + __popc(who & ((1u << lane) - 1))] = v[j];
+        n += __popc(who);
+      }
+      __syncwarp();
+      while (n >= 32) {
+        n -= 32;
+        s += q(queue[n + lane]);
+      }
+      __syncwarp();
+    }
+    if (lane < n) s += q(queue[lane]);
+    __syncwarp();
+    return warp_total(s);
+  }
+
+  // The entries that `in` holds for, in the order of their indices, into the
+  // first CTA's list (at most kList of them).
+  template <class P>
+  __device__ __forceinline__ int collect(P in) {
+    u64 n = 0;
+    for (int i = lo + 4 * lane; i < hi; i += 128) {
+      float v[4];
+      load4(i, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) n += in(v[j]) ? 1 : 0;
+    }
+    n = warp_total(n);
+    u64 before;
+    const int all = static_cast<int>(gather(n, before));
+    u64 at = before;
+    for (int w = 0; w < warp; ++w) at += sh->warp_sum[w];
+    if (n > 0 && all <= kList) {
+      const uint32_t keys = map_to_rank(smem_addr(list_key), 0);
+      const uint32_t idxs = map_to_rank(smem_addr(list_idx), 0);
+      for (int i0 = lo; i0 < hi; i0 += 128) {
+        const int i = i0 + 4 * lane;
+        float v[4];
+        load4(i, v);
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c += in(v[j]) ? 1 : 0;
+        if (!__any_sync(0xffffffffu, c)) continue;
+        int up = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int t = __shfl_up_sync(0xffffffffu, up, o);
+          if (lane >= o) up += t;
+        }
+        uint32_t to = static_cast<uint32_t>(at) + up - c;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (in(v[j])) {
+            st_cluster_u32(keys + 4 * to, key_of(v[j]));
+            st_cluster_u32(idxs + 4 * to, static_cast<uint32_t>(first + i + j));
+            ++to;
+          }
+        }
+        at += __shfl_sync(0xffffffffu, up, 31);
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();
+    return all;
+  }
+};
+
+// The first CTA's list: a thread holds the entries tid * kListEach and on, in
+// the order of their indices. Only the warps that have entries take part.
+struct SampleList {
+  uint32_t key[kListEach], idx[kListEach];
+  u64 w[kListEach];
+  bool in[kListEach];
+  SampleShared* sh;
+  int lane, warp, warps;
+
+  __device__ __forceinline__ void sync() const {
+    if (warps > 1)
+      named_bar_sync(1, warps * 32);
+    else
+      __syncwarp();
+  }
+
+  // Sum over the threads; of `before` over the lower threads.
+  __device__ __forceinline__ u64 sum(u64 v, u64* before = nullptr) {
+    u64 up = v;
+    if (before) {
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 t = __shfl_up_sync(0xffffffffu, up, o);
+        if (lane >= o) up += t;
+      }
+    }
+    const u64 mine = SampleRow<float>::warp_total(v);
+    u64 all = mine, low = 0;
+    if (warps > 1) {
+      sync();  // the last sum is read
+      if (lane == 0) sh->list_sum[warp] = mine;
+      sync();
+      const u64 c = lane < warps ? sh->list_sum[lane] : 0;
+      all = SampleRow<float>::warp_total(c);
+      if (before) low = SampleRow<float>::warp_total(lane < warp ? c : 0);
+    }
+    if (before) *before = low + up - v;
+    return all;
+  }
+
+  // The border at which `e` of the entries, in order, first sums to `need`
+  // (of at most the whole sum): key and index of that entry.
+  __device__ __forceinline__ void border(const u64 (&e)[kListEach], u64 need, uint32_t& K,
+                                         uint32_t& I) {
+    // Bits that all keys have in common need no sum.
+    uint32_t hi = 0, lo = 0xffffffffu;
+#pragma unroll
+    for (int j = 0; j < kListEach; ++j) {
+      if (e[j]) {
+        hi = max(hi, key[j]);
+        lo = min(lo, key[j]);
+      }
+    }
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    if (warps > 1) {
+      sync();
+      if (lane == 0) sh->list_sum[warp] = (static_cast<u64>(hi) << 32) | lo;
+      sync();
+      const u64 c = lane < warps ? sh->list_sum[lane] : 0xffffffffull;
+      hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(c >> 32));
+      lo = __reduce_min_sync(0xffffffffu, static_cast<uint32_t>(c));
+    }
+    const int bits = hi == lo ? 0 : 32 - __clz(hi ^ lo);
+    uint32_t k = bits == 32 ? 0 : hi >> bits << bits;
+#pragma unroll 1
+    for (int b = bits - 1; b >= 0; --b) {
+      const uint32_t t = k | (1u << b);
+      u64 s = 0;
+#pragma unroll
+      for (int j = 0; j < kListEach; ++j) s += key[j] >= t ? e[j] : 0;
+      if (sum(s) >= need) k = t;
+    }
+    u64 above = 0, same = 0, low;
+#pragma unroll
+    for (int j = 0; j < kListEach; ++j) {
+      above += key[j] > k ? e[j] : 0;
+      same += key[j] == k ? e[j] : 0;
+    }
+    above = sum(above);
+    sum(same, &low);
+    u64 at = above + low;
+#pragma unroll
+    for (int j = 0; j < kListEach; ++j) {
+      const u64 x = key[j] == k ? e[j] : 0;
+      if (at < need && at + x >= need) sh->border[1] = idx[j];
+      at += x;
+    }
+    sync();
+    K = k;
+    I = sh->border[1];
+    sync();
+#pragma unroll
+    for (int j = 0; j < kListEach; ++j)
+      in[j] = in[j] && (key[j] > K || (key[j] == K && idx[j] <= I));
   }
 };
 
 template <class T>
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) uint8_t raw_smem[];
   __shared__ SampleShared sh;
   T* seg = reinterpret_cast<T*>(raw_smem);
@@ -182,59 +510,74 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
   }
   row.seg = seg;
   row.first = static_cast<int>(row.rank) * p.seg;
-  row.len = max(0, min(p.seg, p.n_vocab - row.first));
+  auto len_in = [&](int rank) { return max(0, min(p.seg, p.n_vocab - rank * p.seg)); };
+  // Entries of a warp of that rank.
+  auto share_in = [&](int rank) {
+    return ((len_in(rank) + 127) / 128 + kSampleWarps - 1) / kSampleWarps * 128;
+  };
+  const int len = len_in(static_cast<int>(row.rank));
+  const int padded = (len + 127) / 128 * 128;
   row.lane = tid & 31;
   row.warp = tid >> 5;
   row.sh = &sh;
-  const int share = ((row.len + kSampleThreads - 1) / kSampleThreads) * 32;
-  row.lo = min(row.len, row.warp * share);
-  row.hi = min(row.len, row.lo + share);
+  row.hist = reinterpret_cast<uint32_t*>(raw_smem + p.seg * sizeof(T));
+  row.list_key = row.hist + kBins;
+  row.list_idx = row.list_key + kList;
+  const int share = share_in(static_cast<int>(row.rank));
+  row.lo = min(padded, row.warp * share);
+  row.hi = min(padded, row.lo + share);
 
-  // The segment, NaN as -inf and -0 as +0, so that equal values have equal keys.
+  // The segment, filled up with -inf.
   constexpr int V = 16 / sizeof(T);
   const T* src = static_cast<const T*>(p.logits) + at * p.row_stride + row.first;
-  auto clean = [](T x) -> T {
-    if constexpr (sizeof(T) == 4) {
-      return x == x ? x + 0.f : -INFINITY;
-    } else {
-      if ((x & 0x7fff) > 0x7f80) return 0xff80;
-      return x == 0x8000 ? 0 : x;
-    }
-  };
+  T nothing;
+  if constexpr (sizeof(T) == 4)
+    nothing = -INFINITY;
+  else
+    nothing = 0xff80;
   int i0 = 0;
   if ((reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
-    i0 = row.len / V * V;
-    for (int i = tid * V; i < i0; i += kSampleThreads * V) {
-      uint4 raw = *reinterpret_cast<const uint4*>(src + i);
-      T* v = reinterpret_cast<T*>(&raw);
+    i0 = len / V * V;
+    constexpr int U = 8;  // loads in flight
+    constexpr int step = kSampleThreads * V;
+    int i = tid * V;
+    for (; i + (U - 1) * step < i0; i += U * step) {
+      uint4 raw[U];
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = clean(v[j]);
-      *reinterpret_cast<uint4*>(seg + i) = raw;
+      for (int k = 0; k < U; ++k) raw[k] = *reinterpret_cast<const uint4*>(src + i + k * step);
+#pragma unroll
+      for (int k = 0; k < U; ++k) *reinterpret_cast<uint4*>(seg + i + k * step) = raw[k];
     }
+#pragma unroll 2
+    for (; i < i0; i += step)
+      *reinterpret_cast<uint4*>(seg + i) = *reinterpret_cast<const uint4*>(src + i);
   }
-  for (int i = i0 + tid; i < row.len; i += kSampleThreads) seg[i] = clean(src[i]);
+#pragma unroll 4
+  for (int i = i0 + tid; i < len; i += kSampleThreads) seg[i] = src[i];
+  for (int i = len + tid; i < padded; i += kSampleThreads) seg[i] = nothing;
+  for (int i = tid; i < kBins; i += kSampleThreads) row.hist[i] = 0;
+  for (int i = tid; i < 8 * kSampleWarps; i += kSampleThreads) sh.range_sum[i] = 0;
   __syncthreads();
   auto drop = [&](int id) {
     const int i = id - row.first;
-    if (id >= 0 && i >= 0 && i < row.len) {
-      if constexpr (sizeof(T) == 4)
-        seg[i] = -INFINITY;
-      else
-        seg[i] = 0xff80;
-    }
+    if (id >= 0 && i >= 0 && i < len) seg[i] = nothing;
   };
   if (tid == 0) drop(p.mask_id);
   for (int i = tid; i < p.n_suppress; i += kSampleThreads) drop(p.suppress[i]);
   __syncthreads();
 
   float m = -INFINITY;
-  for (int i = row.lo + row.lane; i < row.hi; i += 32) m = fmaxf(m, row.at(i));
+  for (int i = row.lo + 4 * row.lane; i < row.hi; i += 128) {
+    float v[4];
+    row.load4(i, v);
+    m = fmaxf(m, fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (row.lane == 0) sh.max_v[row.warp] = m;
   __syncthreads();
   if (row.warp == 0) {
-    m = sh.max_v[row.lane];
+    m = row.lane < kSampleWarps ? sh.max_v[row.lane] : -INFINITY;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (row.lane == 0) sh.cta_max = m;
@@ -245,86 +588,332 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
   for (uint32_t r = 0; r < row.n_ranks; ++r)
     m = fmaxf(m, ld_cluster_f32(map_to_rank(row.smem_addr(&sh.cta_max), r)));
 
-  const float T0 = p.temperature_row ? p.temperature_row[cand] : p.temperature;
-  const int k0 = p.top_k_row ? p.top_k_row[cand] : p.top_k;
-  const float tp = p.top_p_row ? p.top_p_row[cand] : p.top_p;
-  const float mp = p.min_p_row ? p.min_p_row[cand] : p.min_p;
+  const float temp = p.temperature_row ? p.temperature_row[cand] : p.temperature;
+  const int top_k = p.top_k_row ? p.top_k_row[cand] : p.top_k;
+  const float top_p = p.top_p_row ? p.top_p_row[cand] : p.top_p;
+  const float min_p = p.min_p_row ? p.min_p_row[cand] : p.min_p;
+  float u = p.u[cand];
+  u = u >= 0.f ? fminf(u, 0.99999994f) : 0.f;
+  auto share_of = [&](u64 all) -> u64 {
+    return static_cast<u64>(static_cast<double>(u) * static_cast<double>(all));
+  };
+  // The whole numbers below a share of `all`, and at least 1: an entry is kept
+  // while what is before it sums to less.
+  auto need_of = [&](float part, u64 all) -> u64 {
+    const double x = static_cast<double>(fmaxf(part, 0.f)) * static_cast<double>(all);
+    u64 n = static_cast<u64>(x);
+    if (static_cast<double>(n) < x) ++n;
+    return n ? n : 1;
+  };
 
   int token = 0;
   if (m != -INFINITY) {
-    if (!(T0 > 0.f)) {
-      token = row.find([&](float l, int) -> u64 { return l == m; }, [](u64) -> u64 { return 0; });
+    SampleWeights wt;
+    wt.m = m;
+    wt.least = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
+    if (!(temp > 0.f)) {
+      token = row.first_of(m);
     } else {
-      const double inv_t = 1.0 / static_cast<double>(T0), md = m;
-      auto weight = [&](float l) -> double {
-        if (l == m) return 1.0;
-        if (l == -INFINITY) return 0.0;
-        return exp((static_cast<double>(l) - md) * inv_t);
-      };
-      uint32_t K = 0;
-      int I = 0x7fffffff;
+      wt.c = 1.4426950408889634 / static_cast<double>(temp);
+      wt.b = isinf(m) ? 0.0 : -static_cast<double>(m) * wt.c;
+      wt.cut = isinf(m) ? m : m - static_cast<float>(46.0 / wt.c);
+      wt.bin_c = static_cast<float>(wt.c) * kBinsPerOctave;
+      uint32_t K = 0, I = 0xffffffffu;
       auto before = [&](float l, int i) {
         const uint32_t k = key_of(l);
-        return k > K || (k == K && i <= I);
+        return k > K || (k == K && static_cast<uint32_t>(i) <= I);
       };
-      if (k0 > 0 && k0 < p.n_vocab) {
-        uint32_t key = 0;  // the largest key that k0 entries reach
-        for (int b = 31; b >= 0; --b) {
-          const uint32_t t = key | (1u << b);
-          if (row.total([&](float l, int) -> u64 { return key_of(l) >= t; }) >=
-              static_cast<u64>(k0))
-            key = t;
+      auto kept_weight = [&](float l) -> u64 {
+        if (wt.none(l)) return 0;
+        const double w = wt.weight(l);
+        return w >= wt.least ? fixed44(w) : 0;
+      };
+      const bool by_k = top_k > 0 && top_k < p.n_vocab, by_p = top_p < 1.f;
+      bool done = false;
+      if (by_k || by_p) {
+        // The histogram, and where the nucleus is cut from the whole row, its weight.
+        u64 s = 0;
+        if (by_k) {
+          for (int i = row.lo + 4 * row.lane; i < row.hi; i += 128) {
+            float v[4];
+            row.load4(i, v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (!wt.none(v[j])) atomicAdd(&row.hist[wt.bin(v[j])], 1u);
+          }
+        } else {
+          for (int i = row.lo + 4 * row.lane; i < row.hi; i += 128) {
+            float v[4];
+            row.load4(i, v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (!wt.none(v[j])) {
+                atomicAdd(&row.hist[wt.bin(v[j])], 1u);
+                s += fixed44(wt.weight(v[j]));
+              }
+            }
+          }
         }
-        const u64 above = row.total([&](float l, int) -> u64 { return key_of(l) > key; });
-        const int last = row.find([&](float l, int) -> u64 { return key_of(l) == key; },
-                                  [&](u64) -> u64 { return k0 - above - 1; });
-        K = key;
-        I = last;
-      }
-      if (tp < 1.f) {
-        auto q = [&](float l, int i) -> u64 { return before(l, i) ? fixed44(weight(l)) : 0; };
-        const double share_d = static_cast<double>(fmaxf(tp, 0.f)) * static_cast<double>(row.total(q));
-        u64 need = static_cast<u64>(share_d);
-        if (static_cast<double>(need) < share_d) ++need;
-        if (need == 0) need = 1;
-        uint32_t key = 0;  // the largest key whose entries and those above weigh `need`
-        for (int b = 31; b >= 0; --b) {
-          const uint32_t t = key | (1u << b);
-          if (row.total([&](float l, int i) -> u64 { return key_of(l) >= t ? q(l, i) : 0; }) >= need)
-            key = t;
+        u64 lower;
+        const u64 all = row.gather(row.warp_total(s), lower);  // the histograms are complete
+        u64 need = by_k ? static_cast<u64>(top_k) : need_of(top_p, all);
+        // Bins kBinsEach tid and on of the whole row, and what is before them.
+        uint32_t own[kBinsEach];
+#pragma unroll
+        for (int h = 0; h < kBinsEach; ++h) own[h] = 0;
+        for (uint32_t r = 0; r < row.n_ranks; ++r) {
+          const uint32_t h0 = map_to_rank(row.smem_addr(row.hist), r) + 4 * kBinsEach * tid;
+#pragma unroll
+          for (int h = 0; h < kBinsEach; ++h) {
+            uint32_t a;
+            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(a) : "r"(h0 + 4 * h) : "memory");
+            own[h] += a;
+          }
         }
-        const u64 above =
-            row.total([&](float l, int i) -> u64 { return key_of(l) > key ? q(l, i) : 0; });
-        const int last =
-            row.find([&](float l, int i) -> u64 { return key_of(l) == key ? q(l, i) : 0; },
-                     [&](u64) -> u64 { return need - above - 1; });
-        K = key;
-        I = last;
-      }
-      const double least = mp > 0.f ? fmin(static_cast<double>(mp), 1.0) : 0.0;
-      float u = p.u[cand];
-      u = u >= 0.f ? fminf(u, 0.99999994f) : 0.f;
-      token = row.find(
-          [&](float l, int i) -> u64 {
-            if (!before(l, i)) return 0;
-            const double w = weight(l);
-            return w >= least ? fixed44(w) : 0;
-          },
-          [&](u64 all) -> u64 {
-            return static_cast<u64>(static_cast<double>(u) * static_cast<double>(all));
+        if (tid == 0) {
+          sh.bin_lo = kBins;
+          sh.bin_hi = 0;
+          sh.n_lo = sh.n_hi = 0;
+        }
+        double q = 0.0, own_q[kBinsEach];
+        uint32_t n = 0;
+#pragma unroll
+        for (int h = 0; h < kBinsEach; ++h) {
+          own_q[h] = static_cast<double>(
+                         exp2f(static_cast<float>(kBinsEach * tid + h) / -kBinsPerOctave)) *
+                     own[h];
+          q += own_q[h];
+          n += own[h];
+        }
+        double before_q = q;
+        uint32_t before_n = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double tq = __shfl_up_sync(0xffffffffu, before_q, o);
+          const uint32_t tn = __shfl_up_sync(0xffffffffu, before_n, o);
+          if (row.lane >= o) {
+            before_q += tq;
+            before_n += tn;
+          }
+        }
+        if (row.lane == 31) {
+          sh.warp_d[row.warp] = before_q;
+          sh.warp_u[row.warp] = before_n;
+        }
+        __syncthreads();
+        before_q -= q;
+        before_n -= n;
+        double base_q = 0.0;
+#pragma unroll
+        for (int w = 0; w < kSampleWarps; ++w) {
+          if (w < row.warp) {
+            before_q += sh.warp_d[w];
+            before_n += sh.warp_u[w];
+          }
+          base_q += sh.warp_d[w];
+        }
+        // Whether a bin is before the border for certain, or behind it.
+        const double total_w = static_cast<double>(all) * 0x1p-44;
+        const double need_w = static_cast<double>(need) * 0x1p-44;
+        const double more = 1.0111, less = 1.0 / 1.0111;  // 2^(1/64), and roundings
+#pragma unroll
+        for (int h = 0; h < kBinsEach; ++h) {
+          const uint32_t bin = kBinsEach * tid + h;
+          const uint32_t upto_n = before_n + own[h];
+          const double upto_q = before_q + own_q[h];
+          if (own[h]) {
+            bool sure, behind;
+            if (by_k) {
+              sure = upto_n <= need;
+              behind = before_n >= need;
+            } else {
+              sure = fmin(upto_q * more, total_w - (base_q - upto_q) * less) < need_w * (1 - 1e-6);
+              behind =
+                  fmax(before_q * less, total_w - (base_q - before_q) * more) > need_w * (1 + 1e-6);
+            }
+            if (!sure) atomicMin(&sh.bin_lo, bin);
+            if (!behind) {
+              atomicMax(&sh.bin_hi, bin);
+              atomicMax(&sh.n_hi, upto_n);
+            }
+            if (sure) atomicMax(&sh.n_lo, upto_n);
+          }
+          before_n = upto_n;
+          before_q = upto_q;
+        }
+        __syncthreads();
+        const int b_lo = static_cast<int>(sh.bin_lo), b_hi = static_cast<int>(sh.bin_hi);
+        const uint32_t n_lo = sh.n_lo, n_hi = sh.n_hi;
+        // A list of every entry up to the last bin that may be kept, or of the
+        // doubtful bins; sums of whole rows otherwise.
+        const bool whole = n_hi <= kList;
+        const bool doubt = !whole && n_hi - n_lo <= kList && !(by_k && by_p) && b_lo <= b_hi;
+        const bool thin = by_p && wt.least > 0.0;  // min_p thins out a wide nucleus
+        u64 sure_all = 0, mine = 0;
+        if (doubt) {  // what is before the border for certain
+          const float below = 8388608.f + static_cast<float>(b_lo);  // whole numbers, exact
+          mine = row.part_of(
+              [&](float l) {
+                return l == m || (l > wt.cut && fmaf(l - m, -wt.bin_c, 8388608.f) < below);
+              },
+              [&](float l) -> u64 {
+                const double w = wt.weight(l);
+                return by_k && w < wt.least ? 0 : fixed44(w);  // the nucleus is cut first
+              });
+          sure_all = row.gather(mine, lower);
+        }
+        if (whole || doubt) {
+          const int from = whole ? 0 : b_lo;
+          const int n = row.collect([&](float l) {
+            if (wt.none(l)) return false;
+            const int b = wt.bin(l);
+            return b >= from && b <= b_hi;
           });
+          if (row.rank == 0 && row.warp * 32 * kListEach < max(n, 1)) {
+            SampleList ls;
+            ls.sh = &sh;
+            ls.lane = row.lane;
+            ls.warp = row.warp;
+            ls.warps = (max(n, 1) + 32 * kListEach - 1) / (32 * kListEach);
+            u64 e[kListEach];
+#pragma unroll
+            for (int j = 0; j < kListEach; ++j) {
+              const int i = tid * kListEach + j;
+              ls.in[j] = i < n;
+              ls.key[j] = i < n ? row.list_key[i] : 0;
+              ls.idx[j] = i < n ? row.list_idx[i] : 0;
+              ls.w[j] = 0;
+              if (i < n) ls.w[j] = fixed44(wt.weight(value_of(ls.key[j])));
+            }
+            if (by_k) {
+              const u64 above = whole ? 0 : n_lo;
+              if (above + n > need) {  // otherwise all of them are kept
+#pragma unroll
+                for (int j = 0; j < kListEach; ++j) e[j] = ls.in[j];
+                ls.border(e, need - above, K, I);
+              }
+            }
+            if (by_p) {
+              u64 c = 0;
+#pragma unroll
+              for (int j = 0; j < kListEach; ++j) c += e[j] = ls.in[j] ? ls.w[j] : 0;
+              const u64 here = ls.sum(c);
+              if (by_k) need = need_of(top_p, here);
+              if (sure_all + here > need) ls.border(e, need - sure_all, K, I);
+            }
+            // min_p, and the draw: over a whole list in the order of the
+            // indices; doubtful entries join what their warps are sure of.
+            u64 c = 0, low;
+#pragma unroll
+            for (int j = 0; j < kListEach; ++j) {
+              if (ls.in[j] && wt.least > 0.0 && wt.weight(value_of(ls.key[j])) < wt.least)
+                ls.in[j] = false;
+              c += e[j] = ls.in[j] ? ls.w[j] : 0;
+            }
+            if (whole) {
+              const u64 sum = ls.sum(c, &low);
+              const u64 target = share_of(sum);
+#pragma unroll
+              for (int j = 0; j < kListEach; ++j) {
+                if (low <= target && target < low + e[j]) sh.answer = ls.idx[j];
+                low += e[j];
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < kListEach; ++j) {
+                if (e[j]) {
+                  const int rank = static_cast<int>(ls.idx[j]) / p.seg;
+                  const int w = (static_cast<int>(ls.idx[j]) - rank * p.seg) / share_in(rank);
+                  atomicAdd(&sh.range_sum[rank * kSampleWarps + w], e[j]);
+                }
+              }
+            }
+            if (tid == 0) {
+              sh.border[0] = K;
+              sh.border[1] = I;
+            }
+          }
+          __syncwarp();
+          cluster_sync_all();
+          if (whole) {
+            uint32_t t;
+            asm volatile("ld.shared::cluster.u32 %0, [%1];"
+                         : "=r"(t) : "r"(map_to_rank(row.smem_addr(&sh.answer), 0)) : "memory");
+            token = static_cast<int>(t);
+          } else {
+            const uint32_t b0 = map_to_rank(row.smem_addr(&sh.border[0]), 0);
+            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(K) : "r"(b0) : "memory");
+            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(I) : "r"(b0 + 4) : "memory");
+            if (!thin) {
+              mine += ld_cluster_u64(map_to_rank(
+                  row.smem_addr(&sh.range_sum[row.rank * kSampleWarps + row.warp]), 0));
+              const u64 kept = row.gather(mine, lower);
+              token = row.find(
+                  [&](float l, int i) -> u64 { return before(l, i) ? kept_weight(l) : 0; },
+                  share_of(kept), lower, mine);
+            }
+          }
+          done = whole || !thin;
+        } else if (b_lo <= b_hi || by_p) {  // else: fewer entries than top_k have a weight
+          if (by_k) {
+            uint32_t key = 0;  // the largest key that top_k entries reach
+            for (int b = 31; b >= 0; --b) {
+              const uint32_t t = key | (1u << b);
+              if (row.total([&](float l, int) -> u64 { return key_of(l) >= t; }) >= need) key = t;
+            }
+            const u64 above = row.total([&](float l, int) -> u64 { return key_of(l) > key; });
+            I = static_cast<uint32_t>(row.find([&](float l, int) -> u64 { return key_of(l) == key; },
+                                               [&](u64) -> u64 { return need - above - 1; }));
+            K = key;
+          }
+          if (by_p) {
+            auto q = [&](float l, int i) -> u64 { return before(l, i) ? wt.fixed(l) : 0; };
+            if (by_k) need = need_of(top_p, row.total(q));
+            uint32_t key = 0;  // the largest key whose entries and those above weigh `need`
+            for (int b = 31; b >= 0; --b) {
+              const uint32_t t = key | (1u << b);
+              if (row.total([&](float l, int i) -> u64 { return key_of(l) >= t ? q(l, i) : 0; }) >=
+                  need)
+                key = t;
+            }
+            const u64 above =
+                row.total([&](float l, int i) -> u64 { return key_of(l) > key ? q(l, i) : 0; });
+            const int last =
+                row.find([&](float l, int i) -> u64 { return key_of(l) == key ? q(l, i) : 0; },
+                         [&](u64) -> u64 { return need - above - 1; });
+            K = key;
+            I = static_cast<uint32_t>(last);
+          }
+        }
+      }
+      if (!done)
+        token = row.find(
+            [&](float l, int i) -> u64 { return before(l, i) ? kept_weight(l) : 0; }, share_of);
     }
   }
   if (p.prob) {
-    float pr = 0.f;
     if (m != -INFINITY) {
-      auto e = [&](float l) { return l == m ? 1.f : expf(l - m); };
-      const u64 all = row.total([&](float l, int) -> u64 { return fixed44(e(l)); });
+      // exp(l - m) in fp32, sums of a thread's few entries too.
+      auto e = [&](float l) {  // (NaN: as far below the maximum as counts)
+        return l == m ? 1.f : ex2_approx(fmaxf(l - m, -200.f) * 1.4426950408889634f);
+      };
+      float s = 0.f;
+      for (int i = row.lo + 4 * row.lane; i < row.hi; i += 128) {
+        float v[4];
+        row.load4(i, v);
+        s += (e(v[0]) + e(v[1])) + (e(v[2]) + e(v[3]));
+      }
+      u64 before;
+      const u64 all = row.gather(row.warp_total(static_cast<u64>(static_cast<double>(s) * 0x1p40)), before);
       const int i = token - row.first;
-      if (i >= 0 && i < row.len && tid == 0)
-        p.prob[cand] = static_cast<float>(e(row.at(i)) / (static_cast<double>(all) * 0x1p-44));
+      if (i >= 0 && i < len && tid == 0) {
+        const float l = sizeof(T) == 4 ? reinterpret_cast<const float*>(seg)[i]
+                                       : __uint_as_float(static_cast<uint32_t>(seg[i]) << 16);
+        p.prob[cand] = static_cast<float>(
+            (l == m ? 1.0 : static_cast<double>(expf(l - m))) / (static_cast<double>(all) * 0x1p-40));
+      }
     } else if (tid == 0 && row.rank == 0) {
-      p.prob[cand] = pr;
+      p.prob[cand] = 0.f;
     }
   }
   if (tid == 0 && row.rank == 0) p.token[cand] = token;

@@ -301,7 +301,7 @@ typedef struct {
                                  logits. Not written */
     int32_t logits_bf16;
     int64_t n_rows;
-    int64_t n_vocab;          /* at most 425984 fp32 or 851968 bf16 entries */
+    int64_t n_vocab;          /* at most 376832 fp32 or 753664 bf16 entries */
     int64_t row_stride;       /* elements between rows; 0 = n_vocab */
     const int32_t* rows;      /* int32 [n_cand]: logit row of each candidate, or NULL (row i).
                                  A row out of range gets token -1, prob 0 */

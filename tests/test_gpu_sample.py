@@ -230,3 +230,18 @@ def test_denoising_step_with_temperature():
     # The most confident draws are the ones committed.
     rest = [want[i][1] for i in range(L - P) if i not in done]
     assert min(want[i][1] for i in done) >= max(rest) * (1 - 2e-5)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("kw", [dict(top_p=0.9), dict(top_p=0.6, min_p=0.003),
+                                dict(top_k=9000), dict(top_k=9000, min_p=0.01),
+                                dict(top_k=40000, top_p=0.8), dict(top_k=59990)])
+def test_wide_kept_sets(kind, kw):
+    # Flat rows: tens of thousands of entries are kept, and the border falls
+    # among hundreds of nearly equal ones.
+    check(logits_of(19, 3, 60001, kind, scale=0.7), us(20, 3), **kw)
+
+
+def test_wide_kept_sets_of_many_rows():
+    # One CTA a row, and a vocabulary that leaves the last warps without entries.
+    check(logits_of(21, 300, 12289, scale=0.5), us(22, 300), top_p=0.95)

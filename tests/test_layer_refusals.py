@@ -73,7 +73,7 @@ SAMPLE = dict(logits=FAKE, n_rows=4, n_vocab=100, n_cand=2, mask_id=-1, u=FAKE, 
     (dict(n_vocab=0), INV), (dict(n_rows=-1), INV), (dict(n_suppress=-1), INV),
     (dict(n_suppress=2), INV), (dict(row_stride=99), INV), (dict(n_cand=5), INV),
     (dict(logits=FAKE + 2), INV), (dict(logits=FAKE + 1, logits_bf16=1), INV),
-    (dict(n_vocab=425985), UNS), (dict(n_vocab=851969, logits_bf16=1), UNS),
+    (dict(n_vocab=376833), UNS), (dict(n_vocab=753665, logits_bf16=1), UNS),
     (dict(n_vocab=1 << 32), UNS), (dict(n_cand=0), ca.CA_OK),
     (dict(n_cand=0, logits=None, u=None, token=None), ca.CA_OK),
 ])
