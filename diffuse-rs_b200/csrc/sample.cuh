@@ -39,8 +39,10 @@ constexpr int kSampleThreads = 512;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleSegBytes = 184 * 1024;  // of a row, a CTA
 constexpr int kBins = 1536;                  // 1/32 each: beyond 2^-45 there is no weight
-constexpr int kBinsEach = kBins / kSampleThreads;
+constexpr int kBinsEach = 4;                 // of a thread
+static_assert(kBins / kBinsEach <= kSampleThreads, "bins");
 constexpr float kBinsPerOctave = 32.f;
+constexpr float kNowhere = 8388608.f + 46.f * kBinsPerOctave;  // of SampleWeights::place
 constexpr int kListEach = 6;                 // entries of a thread
 constexpr int kList = kListEach * kSampleThreads;
 constexpr int kQueue = 160;                  // values a warp holds back
@@ -84,20 +86,19 @@ __device__ __forceinline__ u64 fixed44(double w) {
 
 // 2^a for -1000 < a < 1000 to 2e-14: a = n + f with n the nearest whole number
 // (the low bits of a sum with 1.5 * 2^52), 2^f by the Chebyshev interpolation
-// of degree 9 on [-1/2, 1/2], n added to the exponent.
+// of degree 9 on [-1/2, 1/2], n added to the exponent. The coefficients stand
+// in constant memory, where an instruction takes them from directly: as
+// immediates they cost two moves each, more than the arithmetic.
+__constant__ double kExp2[10] = {
+    1.000000000000014,      0.6931471805599526,     0.24022650695631514,    0.05550410866428854,
+    0.009618129195951041,   0.001333355825801874,   0.00015403432339553542, 1.5252640059770786e-05,
+    1.3259945262689143e-06, 1.0212097549811005e-07};
 __device__ __forceinline__ double exp2_64(double a) {
   const double t = a + 6755399441055744.0;
   const double f = a - (t - 6755399441055744.0);
-  double p = 1.0212097549811005e-07;
-  p = fma(p, f, 1.3259945262689143e-06);
-  p = fma(p, f, 1.5252640059770786e-05);
-  p = fma(p, f, 0.00015403432339553542);
-  p = fma(p, f, 0.001333355825801874);
-  p = fma(p, f, 0.009618129195951041);
-  p = fma(p, f, 0.05550410866428854);
-  p = fma(p, f, 0.24022650695631514);
-  p = fma(p, f, 0.6931471805599526);
-  p = fma(p, f, 1.000000000000014);
+  double p = kExp2[9];
+#pragma unroll
+  for (int i = 8; i >= 0; --i) p = fma(p, f, kExp2[i]);
   return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
 }
 
@@ -109,7 +110,8 @@ struct SampleShared {
   float cta_max;
   double warp_d[kSampleWarps];
   uint32_t warp_u[kSampleWarps];
-  uint32_t bin_lo, bin_hi, n_lo, n_hi;
+  uint32_t bin_lo, bin_hi, n_lo, n_hi;  // of the first CTA, and what it tells the others:
+  uint32_t told[4];
   uint32_t border[2];              // key, index
   uint32_t answer;
   u64 list_sum[kSampleWarps];
@@ -118,22 +120,25 @@ struct SampleShared {
 
 // What a row's weights are made of.
 struct SampleWeights {
-  float m, cut;   // entries at or below cut weigh nothing
+  float m;
+  float bin_c;    // place = -bin_c (l - m) + 2^23, whose low bits are the bin
   double c, b;    // log2 w = c l + b
-  float bin_c;    // bin = -bin_c (l - m), to the nearest
   double least;   // min_p
 
-  __device__ __forceinline__ bool none(float l) const { return l != m && !(l > cut); }
+  // To the nearest bin; not below kNowhere for an entry without a weight (NaN
+  // for NaN).
+  __device__ __forceinline__ float place(float l) const {
+    return fmaf(l - m, -bin_c, 8388608.f);
+  }
+  __device__ __forceinline__ bool none(float l) const { return !(place(l) < kNowhere); }
+  __device__ __forceinline__ static uint32_t bin(float place) {
+    return __float_as_uint(place) - 0x4B000000u;
+  }
   __device__ __forceinline__ double weight(float l) const {  // of an entry that is not none()
-    return l == m ? 1.0 : exp2_64(fma(static_cast<double>(l), c, b));
+    return exp2_64(fma(static_cast<double>(l), c, b));
   }
   __device__ __forceinline__ u64 fixed(float l) const {
     return none(l) ? 0 : fixed44(weight(l));
-  }
-  __device__ __forceinline__ int bin(float l) const {
-    if (l == m) return 0;
-    const float t = fmaf(l - m, -bin_c, 8388608.f);
-    return min(static_cast<int>(__float_as_uint(t) - 0x4B000000u), kBins - 1);
   }
 };
 
@@ -141,7 +146,8 @@ template <class T>
 struct SampleRow {
   const T* seg;
   int first;   // index of the segment's first entry
-  int lo, hi;  // this warp's entries in it, multiples of 128
+  int share, padded;  // entries of a warp, of the segment: multiples of 128
+  int lo, hi;         // this warp's
   int lane, warp;
   uint32_t rank, n_ranks;
   SampleShared* sh;
@@ -228,39 +234,68 @@ struct SampleRow {
     return gather(part(q), before);
   }
 
-  // The first index up to which q sums to more than `target`, given this
-  // warp's part and what the lower ranks hold.
+  // The first index up to which q sums to more than `target`, given what the
+  // lower ranks hold; the warps' parts are those of the last gather.
   template <class Q>
-  __device__ __forceinline__ int find(Q q, u64 target, u64 before, u64 mine) {
-    u64 s = before;
-    for (int w = 0; w < warp; ++w) s += sh->warp_sum[w];
-    if (s <= target && target < s + mine) {
-      for (int i0 = lo; i0 < hi; i0 += 128) {
-        const int i = i0 + 4 * lane;
+  __device__ __forceinline__ int find(Q q, u64 target, u64 before) {
+    // The warp whose entries it falls in; its CTA's warps then take a part of
+    // them each, one warp would take many rounds.
+    int owner = -1;
+    u64 s = before, at = 0;
+#pragma unroll
+    for (int w = 0; w < kSampleWarps; ++w) {
+      const u64 t = sh->warp_sum[w];
+      if (s <= target && target < s + t) {
+        owner = w;
+        at = s;
+      }
+      s += t;
+    }
+    if (owner >= 0) {  // the same for the whole CTA
+      const int lo0 = min(owner * share, padded), hi0 = min(lo0 + share, padded);
+      const int sub = (share / 128 + kSampleWarps - 1) / kSampleWarps * 128;
+      const int lo1 = min(lo0 + warp * sub, hi0), hi1 = min(lo1 + sub, hi0);
+      u64 c = 0;
+      for (int i = lo1 + 4 * lane; i < hi1; i += 128) {
         float v[4];
         load4(i, v);
-        u64 e[4], c = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) c += e[j] = q(v[j], first + i + j);
-        u64 up = c;
+        for (int j = 0; j < 4; ++j) c += q(v[j], first + i + j);
+      }
+      c = warp_total(c);
+      __syncthreads();  // the sums of whole warps are read
+      if (lane == 0) sh->warp_sum[warp] = c;
+      __syncthreads();
+      u64 s1 = at;
+      for (int w = 0; w < warp; ++w) s1 += sh->warp_sum[w];
+      if (s1 <= target && target < s1 + c) {
+        for (int i0 = lo1; i0 < hi1; i0 += 128) {
+          const int i = i0 + 4 * lane;
+          float v[4];
+          load4(i, v);
+          u64 e[4], c4 = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const u64 t = __shfl_up_sync(0xffffffffu, up, o);
-          if (lane >= o) up += t;
-        }
-        const uint32_t over = __ballot_sync(0xffffffffu, s + up > target);
-        if (over) {
-          if (lane == __ffs(over) - 1) {
-            u64 t = s + up - c;
-            int k = 0;
-            while (k < 3 && t + e[k] <= target) t += e[k++];
-            for (uint32_t r = 0; r < n_ranks; ++r)
-              st_cluster_u32(map_to_rank(smem_addr(&sh->found[turn]), r),
-                             static_cast<uint32_t>(first + i + k));
+          for (int j = 0; j < 4; ++j) c4 += e[j] = q(v[j], first + i + j);
+          u64 up = c4;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const u64 t = __shfl_up_sync(0xffffffffu, up, o);
+            if (lane >= o) up += t;
           }
-          break;
+          const uint32_t over = __ballot_sync(0xffffffffu, s1 + up > target);
+          if (over) {
+            if (lane == __ffs(over) - 1) {
+              u64 t = s1 + up - c4;
+              int k = 0;
+              while (k < 3 && t + e[k] <= target) t += e[k++];
+              for (uint32_t r = 0; r < n_ranks; ++r)
+                st_cluster_u32(map_to_rank(smem_addr(&sh->found[turn]), r),
+                               static_cast<uint32_t>(first + i + k));
+            }
+            break;
+          }
+          s1 += __shfl_sync(0xffffffffu, up, 31);
         }
-        s += __shfl_sync(0xffffffffu, up, 31);
       }
     }
     __syncwarp();
@@ -270,9 +305,8 @@ struct SampleRow {
   template <class Q, class F>
   __device__ __forceinline__ int find(Q q, F target_of) {
     u64 before;
-    const u64 mine = part(q);
-    const u64 all = gather(mine, before);
-    return find(q, target_of(all), before, mine);
+    const u64 all = gather(part(q), before);
+    return find(q, target_of(all), before);
   }
 
   // The first index whose value is `m` (there is one).
@@ -523,9 +557,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
   row.hist = reinterpret_cast<uint32_t*>(raw_smem + p.seg * sizeof(T));
   row.list_key = row.hist + kBins;
   row.list_idx = row.list_key + kList;
-  const int share = share_in(static_cast<int>(row.rank));
-  row.lo = min(padded, row.warp * share);
-  row.hi = min(padded, row.lo + share);
+  row.padded = padded;
+  row.share = share_in(static_cast<int>(row.rank));
+  row.lo = min(padded, row.warp * row.share);
+  row.hi = min(padded, row.lo + row.share);
 
   // The segment, filled up with -inf.
   constexpr int V = 16 / sizeof(T);
@@ -567,10 +602,20 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
   __syncthreads();
 
   float m = -INFINITY;
-  for (int i = row.lo + 4 * row.lane; i < row.hi; i += 128) {
-    float v[4];
-    row.load4(i, v);
-    m = fmaxf(m, fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+  if constexpr (sizeof(T) == 4) {
+    for (int i = 4 * tid; i < padded; i += 4 * kSampleThreads) {
+      float v[4];
+      row.load4(i, v);
+      m = fmaxf(m, fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+    }
+  } else {
+    uint32_t mm = 0xff80ff80u;  // two at a time; NaN has no part
+    for (int i = 8 * tid; i < padded; i += 8 * kSampleThreads) {
+      const uint4 a = *reinterpret_cast<const uint4*>(seg + i);
+      asm("max.bf16x2 %0, %0, %1;\n\tmax.bf16x2 %0, %0, %2;\n\tmax.bf16x2 %0, %0, %3;\n\t"
+          "max.bf16x2 %0, %0, %4;" : "+r"(mm) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w));
+    }
+    m = fmaxf(__uint_as_float(mm << 16), __uint_as_float(mm & 0xffff0000u));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -587,6 +632,20 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
   m = -INFINITY;
   for (uint32_t r = 0; r < row.n_ranks; ++r)
     m = fmaxf(m, ld_cluster_f32(map_to_rank(row.smem_addr(&sh.cta_max), r)));
+
+  m += 0.f;  // -0 as +0
+  if (m == INFINITY) {
+    // Infinite entries share the row: as zeros among -inf they have the same
+    // weights and no arithmetic of their own.
+    for (int i = tid; i < padded; i += kSampleThreads) {
+      if constexpr (sizeof(T) == 4)
+        seg[i] = seg[i] == INFINITY ? 0.f : -INFINITY;
+      else
+        seg[i] = seg[i] == 0x7f80 ? 0 : 0xff80;
+    }
+    m = 0.f;
+    __syncthreads();
+  }
 
   const float temp = p.temperature_row ? p.temperature_row[cand] : p.temperature;
   const int top_k = p.top_k_row ? p.top_k_row[cand] : p.top_k;
@@ -614,136 +673,146 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
     if (!(temp > 0.f)) {
       token = row.first_of(m);
     } else {
-      wt.c = 1.4426950408889634 / static_cast<double>(temp);
-      wt.b = isinf(m) ? 0.0 : -static_cast<double>(m) * wt.c;
-      wt.cut = isinf(m) ? m : m - static_cast<float>(46.0 / wt.c);
+      // (Temperatures below 2^-100 as 2^-100.)
+      wt.c = 1.4426950408889634 / static_cast<double>(fmaxf(temp, 0x1p-100f));
+      wt.b = -static_cast<double>(m) * wt.c;
       wt.bin_c = static_cast<float>(wt.c) * kBinsPerOctave;
       uint32_t K = 0, I = 0xffffffffu;
       auto before = [&](float l, int i) {
         const uint32_t k = key_of(l);
         return k > K || (k == K && static_cast<uint32_t>(i) <= I);
       };
-      auto kept_weight = [&](float l) -> u64 {
-        if (wt.none(l)) return 0;
+      auto kept_weight = [&](float l) -> u64 {  // of any entry: 0 without a weight
         const double w = wt.weight(l);
-        return w >= wt.least ? fixed44(w) : 0;
+        return wt.place(l) < kNowhere && w >= wt.least ? fixed44(w) : 0;
       };
       const bool by_k = top_k > 0 && top_k < p.n_vocab, by_p = top_p < 1.f;
       bool done = false;
       if (by_k || by_p) {
         // The histogram, and where the nucleus is cut from the whole row, its weight.
         u64 s = 0;
-        if (by_k) {
-          for (int i = row.lo + 4 * row.lane; i < row.hi; i += 128) {
-            float v[4];
-            row.load4(i, v);
+        for (int i = row.lo + 4 * row.lane; i < row.hi; i += 128) {
+          float v[4];
+          row.load4(i, v);
+          bool t[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (!wt.none(v[j])) atomicAdd(&row.hist[wt.bin(v[j])], 1u);
+          for (int j = 0; j < 4; ++j) {
+            const float at = wt.place(v[j]);
+            t[j] = at < kNowhere;
+            if (t[j]) atomicAdd(row.hist + wt.bin(at), 1u);
           }
-        } else {
-          for (int i = row.lo + 4 * row.lane; i < row.hi; i += 128) {
-            float v[4];
-            row.load4(i, v);
+          if (!by_k && (t[0] || t[1] || t[2] || t[3])) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              if (!wt.none(v[j])) {
-                atomicAdd(&row.hist[wt.bin(v[j])], 1u);
-                s += fixed44(wt.weight(v[j]));
-              }
+              const u64 w = fixed44(wt.weight(v[j]));
+              s += t[j] ? w : 0;
             }
           }
         }
         u64 lower;
         const u64 all = row.gather(row.warp_total(s), lower);  // the histograms are complete
         u64 need = by_k ? static_cast<u64>(top_k) : need_of(top_p, all);
-        // Bins kBinsEach tid and on of the whole row, and what is before them.
-        uint32_t own[kBinsEach];
+        // The first CTA joins the histograms, finds the bins and tells the others:
+        // every CTA reading all of them cost 20 us at 32 rows of 8 CTAs.
+        if (row.rank == 0) {
+          // Bins kBinsEach tid and on of the whole row, and what is before them.
+          uint32_t own[kBinsEach];
 #pragma unroll
-        for (int h = 0; h < kBinsEach; ++h) own[h] = 0;
-        for (uint32_t r = 0; r < row.n_ranks; ++r) {
-          const uint32_t h0 = map_to_rank(row.smem_addr(row.hist), r) + 4 * kBinsEach * tid;
+          for (int h = 0; h < kBinsEach; ++h) own[h] = 0;
+          if (tid < kBins / kBinsEach) {
+#pragma unroll 4
+            for (uint32_t r = 0; r < row.n_ranks; ++r) {
+              uint32_t a[4];
+              asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
+                           : "r"(map_to_rank(row.smem_addr(row.hist), r) + 4 * kBinsEach * tid)
+                           : "memory");
+#pragma unroll
+              for (int h = 0; h < kBinsEach; ++h) own[h] += a[h];
+            }
+          }
+          if (tid == 0) {
+            sh.bin_lo = kBins;
+            sh.bin_hi = 0;
+            sh.n_lo = sh.n_hi = 0;
+          }
+          double q = 0.0, own_q[kBinsEach];
+          uint32_t n = 0;
 #pragma unroll
           for (int h = 0; h < kBinsEach; ++h) {
-            uint32_t a;
-            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(a) : "r"(h0 + 4 * h) : "memory");
-            own[h] += a;
+            own_q[h] = static_cast<double>(
+                           exp2f(static_cast<float>(kBinsEach * tid + h) / -kBinsPerOctave)) *
+                       own[h];
+            q += own_q[h];
+            n += own[h];
           }
-        }
-        if (tid == 0) {
-          sh.bin_lo = kBins;
-          sh.bin_hi = 0;
-          sh.n_lo = sh.n_hi = 0;
-        }
-        double q = 0.0, own_q[kBinsEach];
-        uint32_t n = 0;
+          double before_q = q;
+          uint32_t before_n = n;
 #pragma unroll
-        for (int h = 0; h < kBinsEach; ++h) {
-          own_q[h] = static_cast<double>(
-                         exp2f(static_cast<float>(kBinsEach * tid + h) / -kBinsPerOctave)) *
-                     own[h];
-          q += own_q[h];
-          n += own[h];
-        }
-        double before_q = q;
-        uint32_t before_n = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double tq = __shfl_up_sync(0xffffffffu, before_q, o);
-          const uint32_t tn = __shfl_up_sync(0xffffffffu, before_n, o);
-          if (row.lane >= o) {
-            before_q += tq;
-            before_n += tn;
-          }
-        }
-        if (row.lane == 31) {
-          sh.warp_d[row.warp] = before_q;
-          sh.warp_u[row.warp] = before_n;
-        }
-        __syncthreads();
-        before_q -= q;
-        before_n -= n;
-        double base_q = 0.0;
-#pragma unroll
-        for (int w = 0; w < kSampleWarps; ++w) {
-          if (w < row.warp) {
-            before_q += sh.warp_d[w];
-            before_n += sh.warp_u[w];
-          }
-          base_q += sh.warp_d[w];
-        }
-        // Whether a bin is before the border for certain, or behind it.
-        const double total_w = static_cast<double>(all) * 0x1p-44;
-        const double need_w = static_cast<double>(need) * 0x1p-44;
-        const double more = 1.0111, less = 1.0 / 1.0111;  // 2^(1/64), and roundings
-#pragma unroll
-        for (int h = 0; h < kBinsEach; ++h) {
-          const uint32_t bin = kBinsEach * tid + h;
-          const uint32_t upto_n = before_n + own[h];
-          const double upto_q = before_q + own_q[h];
-          if (own[h]) {
-            bool sure, behind;
-            if (by_k) {
-              sure = upto_n <= need;
-              behind = before_n >= need;
-            } else {
-              sure = fmin(upto_q * more, total_w - (base_q - upto_q) * less) < need_w * (1 - 1e-6);
-              behind =
-                  fmax(before_q * less, total_w - (base_q - before_q) * more) > need_w * (1 + 1e-6);
+          for (int o = 1; o < 32; o <<= 1) {
+            const double tq = __shfl_up_sync(0xffffffffu, before_q, o);
+            const uint32_t tn = __shfl_up_sync(0xffffffffu, before_n, o);
+            if (row.lane >= o) {
+              before_q += tq;
+              before_n += tn;
             }
-            if (!sure) atomicMin(&sh.bin_lo, bin);
-            if (!behind) {
-              atomicMax(&sh.bin_hi, bin);
-              atomicMax(&sh.n_hi, upto_n);
-            }
-            if (sure) atomicMax(&sh.n_lo, upto_n);
           }
-          before_n = upto_n;
-          before_q = upto_q;
+          if (row.lane == 31) {
+            sh.warp_d[row.warp] = before_q;
+            sh.warp_u[row.warp] = before_n;
+          }
+          __syncthreads();
+          before_q -= q;
+          before_n -= n;
+          double base_q = 0.0;
+#pragma unroll
+          for (int w = 0; w < kSampleWarps; ++w) {
+            if (w < row.warp) {
+              before_q += sh.warp_d[w];
+              before_n += sh.warp_u[w];
+            }
+            base_q += sh.warp_d[w];
+          }
+          // Whether a bin is before the border for certain, or behind it.
+          const double total_w = static_cast<double>(all) * 0x1p-44;
+          const double need_w = static_cast<double>(need) * 0x1p-44;
+          const double more = 1.0111, less = 1.0 / 1.0111;  // 2^(1/64), and roundings
+#pragma unroll
+          for (int h = 0; h < kBinsEach; ++h) {
+            const uint32_t bin = kBinsEach * tid + h;
+            const uint32_t upto_n = before_n + own[h];
+            const double upto_q = before_q + own_q[h];
+            if (own[h]) {
+              bool sure, behind;
+              if (by_k) {
+                sure = upto_n <= need;
+                behind = before_n >= need;
+              } else {
+                sure = fmin(upto_q * more, total_w - (base_q - upto_q) * less) < need_w * (1 - 1e-6);
+                behind =
+                    fmax(before_q * less, total_w - (base_q - before_q) * more) > need_w * (1 + 1e-6);
+              }
+              if (!sure) atomicMin(&sh.bin_lo, bin);
+              if (!behind) {
+                atomicMax(&sh.bin_hi, bin);
+                atomicMax(&sh.n_hi, upto_n);
+              }
+              if (sure) atomicMax(&sh.n_lo, upto_n);
+            }
+            before_n = upto_n;
+            before_q = upto_q;
+          }
+          __syncthreads();
+          if (tid < 4 * row.n_ranks) {
+            const uint32_t* from = tid & 2 ? (tid & 1 ? &sh.n_hi : &sh.n_lo)
+                                           : (tid & 1 ? &sh.bin_hi : &sh.bin_lo);
+            st_cluster_u32(map_to_rank(row.smem_addr(&sh.told[tid & 3]), tid >> 2), *from);
+          }
         }
-        __syncthreads();
-        const int b_lo = static_cast<int>(sh.bin_lo), b_hi = static_cast<int>(sh.bin_hi);
-        const uint32_t n_lo = sh.n_lo, n_hi = sh.n_hi;
+        __syncwarp();
+        cluster_sync_all();
+        const int b_lo = static_cast<int>(sh.told[0]), b_hi = static_cast<int>(sh.told[1]);
+        const uint32_t n_lo = sh.told[2], n_hi = sh.told[3];
         // A list of every entry up to the last bin that may be kept, or of the
         // doubtful bins; sums of whole rows otherwise.
         const bool whole = n_hi <= kList;
@@ -753,9 +822,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
         if (doubt) {  // what is before the border for certain
           const float below = 8388608.f + static_cast<float>(b_lo);  // whole numbers, exact
           mine = row.part_of(
-              [&](float l) {
-                return l == m || (l > wt.cut && fmaf(l - m, -wt.bin_c, 8388608.f) < below);
-              },
+              [&](float l) { return wt.place(l) < below; },
               [&](float l) -> u64 {
                 const double w = wt.weight(l);
                 return by_k && w < wt.least ? 0 : fixed44(w);  // the nucleus is cut first
@@ -763,11 +830,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
           sure_all = row.gather(mine, lower);
         }
         if (whole || doubt) {
-          const int from = whole ? 0 : b_lo;
+          const float from = 8388608.f + static_cast<float>(whole ? 0 : b_lo);
+          const float to = 8388608.f + static_cast<float>(b_hi);
           const int n = row.collect([&](float l) {
-            if (wt.none(l)) return false;
-            const int b = wt.bin(l);
-            return b >= from && b <= b_hi;
+            const float at = wt.place(l);
+            return at >= from && at <= to;
           });
           if (row.rank == 0 && row.warp * 32 * kListEach < max(n, 1)) {
             SampleList ls;
@@ -850,7 +917,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
               const u64 kept = row.gather(mine, lower);
               token = row.find(
                   [&](float l, int i) -> u64 { return before(l, i) ? kept_weight(l) : 0; },
-                  share_of(kept), lower, mine);
+                  share_of(kept), lower);
             }
           }
           done = whole || !thin;
@@ -886,9 +953,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
           }
         }
       }
-      if (!done)
-        token = row.find(
-            [&](float l, int i) -> u64 { return before(l, i) ? kept_weight(l) : 0; }, share_of);
+      if (!done) {
+        if (by_k || by_p)
+          token = row.find(
+              [&](float l, int i) -> u64 { return before(l, i) ? kept_weight(l) : 0; }, share_of);
+        else
+          token = row.find([&](float l, int) -> u64 { return kept_weight(l); }, share_of);
+      }
     }
   }
   if (p.prob) {
