@@ -25,6 +25,12 @@
 // (a wide nucleus). What fits neither (thousands of entries in one bin, as
 // rows of equal logits have) is settled by bisection of the keys over the
 // whole row, 32 sums a border.
+//
+// bf16 logits take few values, so that their rows need less: a histogram over
+// the values themselves (those of the 17 largest binades that count; smaller
+// ones, next to zero, are few and weighed one by one) gives every sum of the
+// row exactly from one weight a value, and the border's value with it. Only a
+// border next to zero goes the general way.
 #pragma once
 
 #include <cstdint>
@@ -47,6 +53,10 @@ constexpr int kListEach = 6;                 // entries of a thread
 constexpr int kList = kListEach * kSampleThreads;
 constexpr int kQueue = 160;                  // values a warp holds back
 constexpr int kSampleExtra = kBins * 4 + kList * 8;
+constexpr int kSide = 17 * 128;              // bf16 magnitudes of 17 binades
+constexpr int kValues = 2 * kSide + 1;       // in order: positive, next to zero, negative
+constexpr int kValuesEach = (kValues + kSampleThreads - 1) / kSampleThreads;
+static_assert(kValuesEach * kSampleThreads * 4 <= kSampleExtra, "over the histogram and the list");
 static_assert(kSampleWarps * kQueue * 4 <= kList * 8, "the queues lie over the list");
 
 typedef unsigned long long u64;
@@ -111,10 +121,14 @@ struct SampleShared {
   double warp_d[kSampleWarps];
   uint32_t warp_u[kSampleWarps];
   uint32_t bin_lo, bin_hi, n_lo, n_hi;  // of the first CTA, and what it tells the others:
-  uint32_t told[4];
+  uint32_t told[5];
   uint32_t border[2];              // key, index
   uint32_t answer;
   u64 list_sum[kSampleWarps];
+  u64 tiny_weight, tiny_one;       // of the values next to zero
+  u64 one_all;
+  float border_value;
+  uint32_t border_count, settled;
   u64 range_sum[8 * kSampleWarps]; // of the first CTA: kept doubtful entries of every warp
 };
 
@@ -372,6 +386,35 @@ struct SampleRow {
     return warp_total(s);
   }
 
+  // bf16: the place of a value among kValues, by its 15 low bits less those of
+  // the smallest counted magnitude (below 0: next to zero; from kSide on: too
+  // far down to count).
+  __device__ __forceinline__ static int value_place(int i, bool negative) {
+    return negative ? kSide + 1 + i : kSide - 1 - i;
+  }
+
+  // Sum over the CTA, and over the threads before this one.
+  __device__ __forceinline__ u64 cta_scan(u64 v, u64& low) {
+    u64 up = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 t = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += t;
+    }
+    __syncthreads();
+    if (lane == 31) sh->list_sum[warp] = up;
+    __syncthreads();
+    u64 all = 0;
+    low = up - v;
+#pragma unroll
+    for (int w = 0; w < kSampleWarps; ++w) {
+      const u64 t = sh->list_sum[w];
+      if (w < warp) low += t;
+      all += t;
+    }
+    return all;
+  }
+
   // The entries that `in` holds for, in the order of their indices, into the
   // first CTA's list (at most kList of them).
   template <class P>
@@ -590,7 +633,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
 #pragma unroll 4
   for (int i = i0 + tid; i < len; i += kSampleThreads) seg[i] = src[i];
   for (int i = len + tid; i < padded; i += kSampleThreads) seg[i] = nothing;
-  for (int i = tid; i < kBins; i += kSampleThreads) row.hist[i] = 0;
+  for (int i = tid; i < (sizeof(T) == 2 ? kValuesEach * kSampleThreads : kBins);
+       i += kSampleThreads)
+    row.hist[i] = 0;
+  if (tid == 0) sh.tiny_weight = sh.tiny_one = 0;
   for (int i = tid; i < 8 * kSampleWarps; i += kSampleThreads) sh.range_sum[i] = 0;
   __syncthreads();
   auto drop = [&](int id) {
@@ -666,6 +712,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
   };
 
   int token = 0;
+  u64 one_all = 0;  // exp(l - m) over the row in steps of 2^-40, once known
   if (m != -INFINITY) {
     SampleWeights wt;
     wt.m = m;
@@ -688,7 +735,208 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
       };
       const bool by_k = top_k > 0 && top_k < p.n_vocab, by_p = top_p < 1.f;
       bool done = false;
-      if (by_k || by_p) {
+      if constexpr (sizeof(T) == 2) {
+        if (by_k || by_p) {
+          // What counts lies between m and `far`, for the weights and for prob (whose
+          // terms are below 1e-13 from there on); its magnitudes' binades.
+          const float far = fmaxf(m - fmaxf(static_cast<float>(46.0 / wt.c), 32.f), -3e38f);
+          const int top = static_cast<int>(
+              __float_as_uint(fmaxf(fmaxf(fabsf(m), fabsf(far)), 0x1p-100f)) >> 23);
+          const int least_bits = (top - 16) << 7;  // of the smallest counted magnitude
+          uint32_t* const values = row.hist;
+          u64 tiny = 0, tiny_one = 0;
+          uint32_t tiny_n = 0;
+          auto one_of = [&](float l) -> u64 {  // exp(l - m) in steps of 2^-40
+            return static_cast<u64>(static_cast<double>(expf(l - m)) * 0x1p40);
+          };
+          for (int i = 8 * tid; i < padded; i += 8 * kSampleThreads) {
+            const uint4 a = *reinterpret_cast<const uint4*>(seg + i);
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const uint32_t bits = (j & 1) ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu;
+              const int k = static_cast<int>(bits & 0x7fffu) - least_bits;
+              const bool negative = bits >> 15;
+              if (static_cast<uint32_t>(k) < static_cast<uint32_t>(kSide)) {
+                atomicAdd(values + row.value_place(k, negative), 1u);
+              } else if (k < 0) {
+                const float l = __uint_as_float(bits << 16);
+                tiny_one += one_of(l);
+                if (!wt.none(l)) {
+                  ++tiny_n;
+                  tiny += fixed44(wt.weight(l));
+                }
+              }
+            }
+          }
+          if (tiny_one) {
+            atomicAdd(&sh.tiny_one, tiny_one);
+            atomicAdd(values + kSide, tiny_n);
+            atomicAdd(&sh.tiny_weight, tiny);
+          }
+          __syncwarp();
+          cluster_sync_all();
+          if (row.rank == 0) {
+            // The values tid kValuesEach and on, from the whole row.
+            uint32_t n[kValuesEach];
+            u64 w[kValuesEach], one = 0;
+            for (int i = 4 * tid; row.n_ranks > 1 && i < kValuesEach * kSampleThreads;
+                 i += 4 * kSampleThreads) {
+              uint4 c = *reinterpret_cast<const uint4*>(values + i);
+              for (uint32_t r = 1; r < row.n_ranks; ++r) {
+                uint4 t;
+                asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(t.x), "=r"(t.y), "=r"(t.z), "=r"(t.w)
+                             : "r"(map_to_rank(row.smem_addr(values + i), r)) : "memory");
+                c.x += t.x;
+                c.y += t.y;
+                c.z += t.z;
+                c.w += t.w;
+              }
+              *reinterpret_cast<uint4*>(values + i) = c;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int h = 0; h < kValuesEach; ++h) n[h] = values[tid * kValuesEach + h];
+            u64 tiny_all = 0, tiny_ones = 0;
+            if (tid == kSide / kValuesEach) {
+              for (uint32_t r = 0; r < row.n_ranks; ++r) {
+                tiny_all += ld_cluster_u64(map_to_rank(row.smem_addr(&sh.tiny_weight), r));
+                tiny_ones += ld_cluster_u64(map_to_rank(row.smem_addr(&sh.tiny_one), r));
+              }
+            }
+            auto value_at = [&](int o) {
+              const int k = o < kSide ? kSide - 1 - o : o - kSide - 1;
+              const uint32_t bits =
+                  static_cast<uint32_t>(k + least_bits) | (o > kSide ? 0x8000u : 0u);
+              return __uint_as_float(bits << 16);
+            };
+            u64 sum = 0;
+#pragma unroll
+            for (int h = 0; h < kValuesEach; ++h) {
+              const int o = tid * kValuesEach + h;
+              w[h] = 0;
+              if (o == kSide) {
+                sum += tiny_all;
+                one += tiny_ones;
+              } else if (n[h]) {
+                const float l = value_at(o);
+                one += n[h] * one_of(l);
+                if (wt.none(l)) {
+                  n[h] = 0;
+                } else {
+                  w[h] = fixed44(wt.weight(l));
+                  sum += n[h] * w[h];
+                }
+              }
+            }
+            if (tid == 0) {
+              sh.settled = 1;
+              sh.border_value = -INFINITY;  // every entry with a weight is kept
+              sh.border_count = 0;
+            }
+            u64 low;
+            const u64 ones = row.cta_scan(one, low);
+            if (tid == 0) sh.one_all = ones;
+            if (by_k) {
+              u64 c = 0;
+#pragma unroll
+              for (int h = 0; h < kValuesEach; ++h) c += n[h];
+              row.cta_scan(c, low);
+              const u64 k = static_cast<u64>(top_k);
+#pragma unroll
+              for (int h = 0; h < kValuesEach; ++h) {
+                const int o = tid * kValuesEach + h;
+                const u64 upto = low + n[h];
+                if (low < k && k < upto) {  // cut within this value
+                  if (o == kSide) sh.settled = 0;
+                  sh.border_value = value_at(o);
+                  sh.border_count = static_cast<uint32_t>(k - low);
+                  n[h] = static_cast<uint32_t>(k - low);
+                } else if (k <= low) {
+                  n[h] = 0;
+                } else if (k == upto && n[h]) {  // cut behind it
+                  if (o == kSide) sh.settled = 0;
+                  sh.border_value = value_at(o);
+                  sh.border_count = n[h];
+                }
+                low = upto;
+              }
+              sum = 0;
+#pragma unroll
+              for (int h = 0; h < kValuesEach; ++h)
+                sum += tid * kValuesEach + h == kSide ? (n[h] ? tiny_all : 0) : n[h] * w[h];
+            }
+            __syncthreads();
+            if (by_p) {
+              const u64 all = row.cta_scan(sum, low);
+              const u64 need = need_of(top_p, all);
+#pragma unroll
+              for (int h = 0; h < kValuesEach; ++h) {
+                const int o = tid * kValuesEach + h;
+                const u64 here = o == kSide ? (n[h] ? tiny_all : 0) : n[h] * w[h];
+                if (low < need && need <= low + here) {
+                  if (o == kSide) sh.settled = 0;
+                  sh.border_value = value_at(o);
+                  sh.border_count =
+                      o == kSide ? 0 : static_cast<uint32_t>((need - low + w[h] - 1) / w[h]);
+                }
+                low += here;
+              }
+            }
+            __syncthreads();
+            if (tid < 8 * row.n_ranks && (tid & 7) < 5) {
+              const int k = tid & 7;
+              const uint32_t x = k == 0   ? __float_as_uint(sh.border_value)
+                                 : k == 1 ? sh.border_count
+                                 : k == 2 ? sh.settled
+                                 : k == 3 ? static_cast<uint32_t>(sh.one_all)
+                                          : static_cast<uint32_t>(sh.one_all >> 32);
+              st_cluster_u32(map_to_rank(row.smem_addr(&sh.told[k]), tid >> 3), x);
+            }
+          }
+          __syncwarp();
+          cluster_sync_all();
+          one_all = sh.told[3] | static_cast<u64>(sh.told[4]) << 32;
+          if (sh.told[2]) {
+            // Kept: what is above the border's value, and the first `count` of it.
+            const float at = __uint_as_float(sh.told[0]);
+            const uint32_t count = sh.told[1];
+            auto equal = [&](float l, int) -> u64 { return l == at; };
+            u64 lower;
+            const u64 mine_eq = count ? row.part(equal) : 0;
+            u64 kept_eq = 0, w_at = 0;
+            K = key_of(at);
+            if (count) {
+              const u64 all_eq = row.gather(mine_eq, lower);
+              u64 up = lower;
+              for (int w = 0; w < row.warp; ++w) up += sh.warp_sum[w];
+              if (up < count) kept_eq = min(mine_eq, count - up);
+              w_at = kept_weight(at);
+              __syncthreads();
+              I = count < all_eq ? static_cast<uint32_t>(row.find(equal, count - 1, lower))
+                                 : 0xffffffffu;
+            }
+            const float behind = count ? at : -INFINITY;
+            u64 mine = row.part_of(
+                [&](float l) { return l > behind && wt.place(l) < kNowhere; },
+                [&](float l) -> u64 {
+                  const double w = wt.weight(l);
+                  return w >= wt.least ? fixed44(w) : 0;
+                });
+            mine += kept_eq * w_at;
+            const u64 kept = row.gather(mine, lower);
+            token = row.find(
+                [&](float l, int i) -> u64 { return before(l, i) ? kept_weight(l) : 0; },
+                share_of(kept), lower);
+            done = true;
+          } else {
+            for (int i = tid; i < kBins; i += kSampleThreads) row.hist[i] = 0;
+            __syncthreads();
+          }
+        }
+      }
+      if (!done && (by_k || by_p)) {
         // The histogram, and where the nucleus is cut from the whole row, its weight.
         u64 s = 0;
         for (int i = row.lo + 4 * row.lane; i < row.hi; i += 128) {
@@ -968,20 +1216,23 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
       auto e = [&](float l) {  // (NaN: as far below the maximum as counts)
         return l == m ? 1.f : ex2_approx(fmaxf(l - m, -200.f) * 1.4426950408889634f);
       };
-      float s = 0.f;
-      for (int i = row.lo + 4 * row.lane; i < row.hi; i += 128) {
-        float v[4];
-        row.load4(i, v);
-        s += (e(v[0]) + e(v[1])) + (e(v[2]) + e(v[3]));
+      if (!one_all) {
+        float s = 0.f;
+        for (int i = row.lo + 4 * row.lane; i < row.hi; i += 128) {
+          float v[4];
+          row.load4(i, v);
+          s += (e(v[0]) + e(v[1])) + (e(v[2]) + e(v[3]));
+        }
+        u64 before;
+        one_all = row.gather(
+            row.warp_total(static_cast<u64>(static_cast<double>(s) * 0x1p40)), before);
       }
-      u64 before;
-      const u64 all = row.gather(row.warp_total(static_cast<u64>(static_cast<double>(s) * 0x1p40)), before);
       const int i = token - row.first;
       if (i >= 0 && i < len && tid == 0) {
         const float l = sizeof(T) == 4 ? reinterpret_cast<const float*>(seg)[i]
                                        : __uint_as_float(static_cast<uint32_t>(seg[i]) << 16);
         p.prob[cand] = static_cast<float>(
-            (l == m ? 1.0 : static_cast<double>(expf(l - m))) / (static_cast<double>(all) * 0x1p-40));
+            (l == m ? 1.0 : static_cast<double>(expf(l - m))) / (static_cast<double>(one_all) * 0x1p-40));
       }
     } else if (tid == 0 && row.rank == 0) {
       p.prob[cand] = 0.f;

@@ -245,3 +245,19 @@ def test_wide_kept_sets(kind, kw):
 def test_wide_kept_sets_of_many_rows():
     # One CTA a row, and a vocabulary that leaves the last warps without entries.
     check(logits_of(21, 300, 12289, scale=0.5), us(22, 300), top_p=0.95)
+
+
+@pytest.mark.parametrize("kw", [dict(top_p=0.9), dict(top_k=20003), dict(top_p=0.7, top_k=20003),
+                                dict(top_p=0.50001, temperature=float("inf")),
+                                dict(top_p=0.3, temperature=0.01), dict(top_k=5, temperature=50.0)])
+def test_bf16_borders_next_to_zero(kw):
+    # Entries within 2^-16 of the row's largest magnitude, zeros of both signs
+    # among them, hold the border; and rows of small values alone.
+    x = logits_of(23, 4, 30000)
+    x[0] *= 1e-6
+    x[0, :50] = 3.0
+    x[1, 100:] = 0.0
+    x[1, 101::3] = -0.0
+    x[2] = x[2] * 1e-30
+    x[3] = x[3] * 1e-3 + 200.0
+    check(x.to(torch.bfloat16), us(24, 4), **kw)
