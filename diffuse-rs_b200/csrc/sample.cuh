@@ -121,14 +121,11 @@ struct SampleShared {
   double warp_d[kSampleWarps];
   uint32_t warp_u[kSampleWarps];
   uint32_t bin_lo, bin_hi, n_lo, n_hi;  // of the first CTA, and what it tells the others:
-  uint32_t told[5];
-  uint32_t border[2];              // key, index
+  uint32_t told[4];
+  uint32_t border[3];              // key and index; bf16: value, how many of it, whether it holds
   uint32_t answer;
   u64 list_sum[kSampleWarps];
   u64 tiny_weight, tiny_one;       // of the values next to zero
-  u64 one_all;
-  float border_value;
-  uint32_t border_count, settled;
   u64 range_sum[8 * kSampleWarps]; // of the first CTA: kept doubtful entries of every warp
 };
 
@@ -199,6 +196,7 @@ struct SampleRow {
   // The sum of the warps' `mine` over the row; `before`: over lower ranks.
   // `second`: another sum, made that of the row.
   __device__ __forceinline__ u64 gather(u64 mine, u64& before, u64* second = nullptr) {
+    __syncthreads();  // the last ones are read
     if (lane == 0) {
       sh->warp_sum[warp] = mine;
       if (second) sh->warp_sum2[warp] = *second;
@@ -252,6 +250,12 @@ struct SampleRow {
   // lower ranks hold; the warps' parts are those of the last gather.
   template <class Q>
   __device__ __forceinline__ int find(Q q, u64 target, u64 before) {
+    return find_from(target, before, [](int, int, int) {}, q);
+  }
+  // `begin`(warp, first entry, one behind the last) is called by all threads
+  // of the CTA that it falls in, before q is.
+  template <class B, class Q>
+  __device__ __forceinline__ int find_from(u64 target, u64 before, B begin, Q q) {
     // The warp whose entries it falls in; its CTA's warps then take a part of
     // them each, one warp would take many rounds.
     int owner = -1;
@@ -267,6 +271,7 @@ struct SampleRow {
     }
     if (owner >= 0) {  // the same for the whole CTA
       const int lo0 = min(owner * share, padded), hi0 = min(lo0 + share, padded);
+      begin(owner, lo0, hi0);
       const int sub = (share / 128 + kSampleWarps - 1) / kSampleWarps * 128;
       const int lo1 = min(lo0 + warp * sub, hi0), hi1 = min(lo1 + sub, hi0);
       u64 c = 0;
@@ -359,8 +364,10 @@ struct SampleRow {
 
   // This warp's part of the sum of q over the entries that `in` holds for:
   // those are queued, so that a warp's lanes have one each to weigh.
+  // `equal`, if given: how many entries are `at`.
   template <class P, class Q>
-  __device__ __forceinline__ u64 part_of(P in, Q q) {
+  __device__ __forceinline__ u64 part_of(P in, Q q, float at = 0.f, u64* equal = nullptr) {
+    uint32_t same = 0;
     float* queue = reinterpret_cast<float*>(list_key) + warp * kQueue;
     u64 s = 0;
     int n = 0;
@@ -370,6 +377,7 @@ struct SampleRow {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const bool t = in(v[j]);
+        if (equal) same += v[j] == at ? 1 : 0;
         const uint32_t who = __ballot_sync(0xffffffffu, t);
         if (t) queue[n + __popc(who & ((1u << lane) - 1))] = v[j];
         n += __popc(who);
@@ -383,7 +391,33 @@ struct SampleRow {
     }
     if (lane < n) s += q(queue[lane]);
     __syncwarp();
+    if (equal) *equal = __reduce_add_sync(0xffffffffu, same);
     return warp_total(s);
+  }
+
+  // The index of the n-th entry of the segment's from .. to - 1 whose value is
+  // `at` (the last one's if there are fewer; every warp looks for itself).
+  __device__ __forceinline__ uint32_t nth_equal(float at, u64 n, int from, int to) {
+    uint32_t last = 0;
+    u64 seen = 0;
+    for (int i0 = from; i0 < to && seen < n; i0 += 32) {
+      const float l = value(i0 + lane);
+      const uint32_t who = __ballot_sync(0xffffffffu, l == at);
+      const int here = __popc(who);
+      if (here) {
+        // The (n - seen)-th of them, or the last.
+        const int k = seen + here >= n ? static_cast<int>(n - seen) : here;
+        last = static_cast<uint32_t>(first + i0 + __fns(who, 0, k));
+        seen += here;
+      }
+    }
+    return last;
+  }
+  __device__ __forceinline__ float value(int i) const {
+    if constexpr (sizeof(T) == 4)
+      return seg[i];
+    else
+      return __uint_as_float(static_cast<uint32_t>(seg[i]) << 16);
   }
 
   // bf16: the place of a value among kValues, by its 15 low bits less those of
@@ -391,28 +425,6 @@ struct SampleRow {
   // far down to count).
   __device__ __forceinline__ static int value_place(int i, bool negative) {
     return negative ? kSide + 1 + i : kSide - 1 - i;
-  }
-
-  // Sum over the CTA, and over the threads before this one.
-  __device__ __forceinline__ u64 cta_scan(u64 v, u64& low) {
-    u64 up = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 t = __shfl_up_sync(0xffffffffu, up, o);
-      if (lane >= o) up += t;
-    }
-    __syncthreads();
-    if (lane == 31) sh->list_sum[warp] = up;
-    __syncthreads();
-    u64 all = 0;
-    low = up - v;
-#pragma unroll
-    for (int w = 0; w < kSampleWarps; ++w) {
-      const u64 t = sh->list_sum[w];
-      if (w < warp) low += t;
-      all += t;
-    }
-    return all;
   }
 
   // The entries that `in` holds for, in the order of their indices, into the
@@ -636,7 +648,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
   for (int i = tid; i < (sizeof(T) == 2 ? kValuesEach * kSampleThreads : kBins);
        i += kSampleThreads)
     row.hist[i] = 0;
-  if (tid == 0) sh.tiny_weight = sh.tiny_one = 0;
+  if (tid == 0) {
+    sh.tiny_weight = sh.tiny_one = 0;
+    sh.border[0] = __float_as_uint(-INFINITY);  // no border
+    sh.border[1] = 0;
+    sh.border[2] = 1;
+  }
   for (int i = tid; i < 8 * kSampleWarps; i += kSampleThreads) sh.range_sum[i] = 0;
   __syncthreads();
   auto drop = [&](int id) {
@@ -776,14 +793,16 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
           }
           __syncwarp();
           cluster_sync_all();
-          if (row.rank == 0) {
-            // The values tid kValuesEach and on, from the whole row.
-            uint32_t n[kValuesEach];
-            u64 w[kValuesEach], one = 0;
-            for (int i = 4 * tid; row.n_ranks > 1 && i < kValuesEach * kSampleThreads;
-                 i += 4 * kSampleThreads) {
-              uint4 c = *reinterpret_cast<const uint4*>(values + i);
-              for (uint32_t r = 1; r < row.n_ranks; ++r) {
+          // Each CTA takes a share of the values, from the whole row, and of those
+          // a thread the `each` from `o0` on.
+          const int Q = kValuesEach * kSampleThreads / static_cast<int>(row.n_ranks);
+          const int each = (Q + kSampleThreads - 1) / kSampleThreads;
+          const int q0 = Q * static_cast<int>(row.rank), o0 = q0 + each * tid;
+          if (row.n_ranks > 1) {
+            for (int i = q0 + 4 * tid; i < q0 + Q; i += 4 * kSampleThreads) {
+              uint4 c = make_uint4(0, 0, 0, 0);
+#pragma unroll 4
+              for (uint32_t r = 0; r < row.n_ranks; ++r) {
                 uint4 t;
                 asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
                              : "=r"(t.x), "=r"(t.y), "=r"(t.z), "=r"(t.w)
@@ -795,140 +814,132 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
               }
               *reinterpret_cast<uint4*>(values + i) = c;
             }
-            __syncthreads();
+          }
+          __syncthreads();
+          auto value_at = [&](int o) {
+            const int k = o < kSide ? kSide - 1 - o : o - kSide - 1;
+            return __uint_as_float((static_cast<uint32_t>(k + least_bits) << 16) |
+                                   (o > kSide ? 0x80000000u : 0u));
+          };
+          uint32_t n[kValuesEach];
+          u64 w[kValuesEach], ones = 0, tiny_all = 0;
 #pragma unroll
-            for (int h = 0; h < kValuesEach; ++h) n[h] = values[tid * kValuesEach + h];
-            u64 tiny_all = 0, tiny_ones = 0;
-            if (tid == kSide / kValuesEach) {
-              for (uint32_t r = 0; r < row.n_ranks; ++r) {
-                tiny_all += ld_cluster_u64(map_to_rank(row.smem_addr(&sh.tiny_weight), r));
-                tiny_ones += ld_cluster_u64(map_to_rank(row.smem_addr(&sh.tiny_one), r));
-              }
-            }
-            auto value_at = [&](int o) {
-              const int k = o < kSide ? kSide - 1 - o : o - kSide - 1;
-              const uint32_t bits =
-                  static_cast<uint32_t>(k + least_bits) | (o > kSide ? 0x8000u : 0u);
-              return __uint_as_float(bits << 16);
-            };
-            u64 sum = 0;
-#pragma unroll
-            for (int h = 0; h < kValuesEach; ++h) {
-              const int o = tid * kValuesEach + h;
-              w[h] = 0;
+          for (int h = 0; h < kValuesEach; ++h) {
+            const int o = o0 + h;
+            n[h] = 0;
+            w[h] = 0;
+            if (h < each && o < q0 + Q && o < kValues) {
+              n[h] = values[o];
               if (o == kSide) {
-                sum += tiny_all;
-                one += tiny_ones;
+                for (uint32_t r = 0; r < row.n_ranks; ++r) {
+                  tiny_all += ld_cluster_u64(map_to_rank(row.smem_addr(&sh.tiny_weight), r));
+                  ones += ld_cluster_u64(map_to_rank(row.smem_addr(&sh.tiny_one), r));
+                }
               } else if (n[h]) {
                 const float l = value_at(o);
-                one += n[h] * one_of(l);
-                if (wt.none(l)) {
+                ones += n[h] * one_of(l);
+                if (wt.none(l))
                   n[h] = 0;
-                } else {
+                else
                   w[h] = fixed44(wt.weight(l));
-                  sum += n[h] * w[h];
-                }
               }
             }
-            if (tid == 0) {
-              sh.settled = 1;
-              sh.border_value = -INFINITY;  // every entry with a weight is kept
-              sh.border_count = 0;
+          }
+          // What a value weighs, by how many of it count.
+          auto here = [&](int h) -> u64 {
+            return o0 + h == kSide ? (n[h] ? tiny_all : 0) : n[h] * w[h];
+          };
+          // Sum over the row; `low`: over the values before this thread's.
+          auto scan = [&](u64 v, u64& low, u64* second) {
+            u64 up = v;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const u64 t = __shfl_up_sync(0xffffffffu, up, o);
+              if (row.lane >= o) up += t;
             }
-            u64 low;
-            const u64 ones = row.cta_scan(one, low);
-            if (tid == 0) sh.one_all = ones;
-            if (by_k) {
-              u64 c = 0;
+            const u64 all = row.gather(__shfl_sync(0xffffffffu, up, 31), low, second);
+            for (int i = 0; i < row.warp; ++i) low += sh.warp_sum[i];
+            low += up - v;
+            return all;
+          };
+          auto tell = [&](float value, uint32_t count, bool settled) {
+            const uint32_t x[3] = {__float_as_uint(value), count, settled ? 1u : 0u};
+            for (uint32_t r = 0; r < row.n_ranks; ++r)
 #pragma unroll
-              for (int h = 0; h < kValuesEach; ++h) c += n[h];
-              row.cta_scan(c, low);
-              const u64 k = static_cast<u64>(top_k);
+              for (int i = 0; i < 3; ++i)
+                st_cluster_u32(map_to_rank(row.smem_addr(&sh.border[i]), r), x[i]);
+          };
+          u64 low, second = row.warp_total(ones);
+          if (by_k) {
+            u64 c = 0;
 #pragma unroll
-              for (int h = 0; h < kValuesEach; ++h) {
-                const int o = tid * kValuesEach + h;
-                const u64 upto = low + n[h];
-                if (low < k && k < upto) {  // cut within this value
-                  if (o == kSide) sh.settled = 0;
-                  sh.border_value = value_at(o);
-                  sh.border_count = static_cast<uint32_t>(k - low);
-                  n[h] = static_cast<uint32_t>(k - low);
-                } else if (k <= low) {
-                  n[h] = 0;
-                } else if (k == upto && n[h]) {  // cut behind it
-                  if (o == kSide) sh.settled = 0;
-                  sh.border_value = value_at(o);
-                  sh.border_count = n[h];
-                }
-                low = upto;
+            for (int h = 0; h < kValuesEach; ++h) c += n[h];
+            scan(c, low, &second);
+            one_all = second;
+            const u64 k = static_cast<u64>(top_k);
+#pragma unroll
+            for (int h = 0; h < kValuesEach; ++h) {
+              const u64 upto = low + n[h];
+              if (k <= low) {
+                n[h] = 0;
+              } else if (k <= upto && n[h]) {
+                n[h] = static_cast<uint32_t>(k - low);  // the last of them to be kept
+                tell(value_at(o0 + h), n[h], o0 + h != kSide);
               }
-              sum = 0;
-#pragma unroll
-              for (int h = 0; h < kValuesEach; ++h)
-                sum += tid * kValuesEach + h == kSide ? (n[h] ? tiny_all : 0) : n[h] * w[h];
+              low = upto;
             }
-            __syncthreads();
-            if (by_p) {
-              const u64 all = row.cta_scan(sum, low);
-              const u64 need = need_of(top_p, all);
+          }
+          if (by_p) {
+            u64 c = 0;
 #pragma unroll
-              for (int h = 0; h < kValuesEach; ++h) {
-                const int o = tid * kValuesEach + h;
-                const u64 here = o == kSide ? (n[h] ? tiny_all : 0) : n[h] * w[h];
-                if (low < need && need <= low + here) {
-                  if (o == kSide) sh.settled = 0;
-                  sh.border_value = value_at(o);
-                  sh.border_count =
-                      o == kSide ? 0 : static_cast<uint32_t>((need - low + w[h] - 1) / w[h]);
-                }
-                low += here;
-              }
-            }
-            __syncthreads();
-            if (tid < 8 * row.n_ranks && (tid & 7) < 5) {
-              const int k = tid & 7;
-              const uint32_t x = k == 0   ? __float_as_uint(sh.border_value)
-                                 : k == 1 ? sh.border_count
-                                 : k == 2 ? sh.settled
-                                 : k == 3 ? static_cast<uint32_t>(sh.one_all)
-                                          : static_cast<uint32_t>(sh.one_all >> 32);
-              st_cluster_u32(map_to_rank(row.smem_addr(&sh.told[k]), tid >> 3), x);
+            for (int h = 0; h < kValuesEach; ++h) c += here(h);
+            const u64 all = scan(c, low, by_k ? nullptr : &second);
+            if (!by_k) one_all = second;
+            const u64 need = need_of(top_p, all);
+#pragma unroll
+            for (int h = 0; h < kValuesEach; ++h) {
+              const u64 x = here(h);
+              if (low < need && need <= low + x)
+                tell(value_at(o0 + h),
+                     o0 + h == kSide ? 0 : static_cast<uint32_t>((need - low + w[h] - 1) / w[h]),
+                     o0 + h != kSide);
+              low += x;
             }
           }
           __syncwarp();
           cluster_sync_all();
-          one_all = sh.told[3] | static_cast<u64>(sh.told[4]) << 32;
-          if (sh.told[2]) {
-            // Kept: what is above the border's value, and the first `count` of it.
-            const float at = __uint_as_float(sh.told[0]);
-            const uint32_t count = sh.told[1];
-            auto equal = [&](float l, int) -> u64 { return l == at; };
-            u64 lower;
-            const u64 mine_eq = count ? row.part(equal) : 0;
-            u64 kept_eq = 0, w_at = 0;
-            K = key_of(at);
-            if (count) {
-              const u64 all_eq = row.gather(mine_eq, lower);
-              u64 up = lower;
-              for (int w = 0; w < row.warp; ++w) up += sh.warp_sum[w];
-              if (up < count) kept_eq = min(mine_eq, count - up);
-              w_at = kept_weight(at);
-              __syncthreads();
-              I = count < all_eq ? static_cast<uint32_t>(row.find(equal, count - 1, lower))
-                                 : 0xffffffffu;
-            }
-            const float behind = count ? at : -INFINITY;
-            u64 mine = row.part_of(
-                [&](float l) { return l > behind && wt.place(l) < kNowhere; },
-                [&](float l) -> u64 {
-                  const double w = wt.weight(l);
-                  return w >= wt.least ? fixed44(w) : 0;
-                });
-            mine += kept_eq * w_at;
+          if (sh.border[2]) {
+            // Kept: what is above the border's value, and the first `count` of it
+            // (without a border: every entry that has a weight).
+            const float at = __uint_as_float(sh.border[0]);
+            const u64 count = sh.border[1];
+            u64 equal = 0, lower;
+            u64 mine = row.part_of([&](float l) { return l > at && wt.place(l) < kNowhere; },
+                                   [&](float l) -> u64 {
+                                     const double x = wt.weight(l);
+                                     return x >= wt.least ? fixed44(x) : 0;
+                                   },
+                                   at, &equal);
+            // How many of the border's value a warp keeps.
+            u64 eq_low;
+            row.gather(equal, eq_low);
+            u64 eq_at = eq_low;
+            for (int i = 0; i < row.warp; ++i) eq_at += sh.warp_sum[i];
+            const u64 w_at = count ? kept_weight(at) : 0;
+            mine += (eq_at >= count ? 0 : min(equal, count - eq_at)) * w_at;
+            if (row.lane == 0) sh.warp_sum2[row.warp] = eq_at;
             const u64 kept = row.gather(mine, lower);
-            token = row.find(
-                [&](float l, int i) -> u64 { return before(l, i) ? kept_weight(l) : 0; },
-                share_of(kept), lower);
+            // Within a warp's entries: those above, and of the border's value as
+            // many as `count` leaves after the warps before.
+            token = row.find_from(
+                share_of(kept), lower,
+                [&](int owner, int from, int to) {
+                  const u64 before_eq = sh.warp_sum2[owner];
+                  I = before_eq >= count ? 0 : row.nth_equal(at, count - before_eq, from, to) + 1;
+                },
+                [&](float l, int i) -> u64 {
+                  return l > at || (l == at && static_cast<uint32_t>(i) < I) ? kept_weight(l) : 0;
+                });
             done = true;
           } else {
             for (int i = tid; i < kBins; i += kSampleThreads) row.hist[i] = 0;
