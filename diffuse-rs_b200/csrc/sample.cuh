@@ -113,11 +113,12 @@ __device__ __forceinline__ double exp2_64(double a) {
 }
 
 struct SampleShared {
-  u64 warp_sum[kSampleWarps], warp_sum2[kSampleWarps];
-  u64 cta_sum[2], cta_sum2[2];
-  uint32_t found[2];
-  float max_v[kSampleWarps];
-  float cta_max;
+  u64 warp_sum[kSampleWarps], warp_second[kSampleWarps];
+  u64 cta_sum[2][8], cta_second[2][8];  // of every rank
+  uint32_t found[2], first_found[2][8];
+  float max_v[kSampleWarps], cta_max[8];
+  u64 equal_before[kSampleWarps];       // bf16: entries of the border's value
+  uint32_t equal[kSampleWarps];
   double warp_d[kSampleWarps];
   uint32_t warp_u[kSampleWarps];
   uint32_t bin_lo, bin_hi, n_lo, n_hi;  // of the first CTA, and what it tells the others:
@@ -194,35 +195,38 @@ struct SampleRow {
   }
 
   // The sum of the warps' `mine` over the row; `before`: over lower ranks.
-  // `second`: another sum, made that of the row.
+  // `second`: another sum, made that of the row. A CTA's sums are written to
+  // every CTA before the barrier: reads of one another's after it cost about
+  // 1000 clocks each.
   __device__ __forceinline__ u64 gather(u64 mine, u64& before, u64* second = nullptr) {
     __syncthreads();  // the last ones are read
     if (lane == 0) {
       sh->warp_sum[warp] = mine;
-      if (second) sh->warp_sum2[warp] = *second;
+      if (second) sh->warp_second[warp] = *second;
     }
     __syncthreads();
     turn ^= 1;
     if (warp == 0) {
-      u64 c = lane < kSampleWarps ? sh->warp_sum[lane] : 0;
-      c = warp_total(c);
-      if (lane == 0) sh->cta_sum[turn] = c;
+      const u64 c = warp_total(lane < kSampleWarps ? sh->warp_sum[lane] : 0);
+      if (lane < n_ranks) st_cluster_u64(map_to_rank(smem_addr(&sh->cta_sum[turn][rank]), lane), c);
       if (second) {
-        c = lane < kSampleWarps ? sh->warp_sum2[lane] : 0;
-        c = warp_total(c);
-        if (lane == 0) sh->cta_sum2[turn] = c;
+        const u64 d = warp_total(lane < kSampleWarps ? sh->warp_second[lane] : 0);
+        if (lane < n_ranks)
+          st_cluster_u64(map_to_rank(smem_addr(&sh->cta_second[turn][rank]), lane), d);
       }
     }
     __syncwarp();
     cluster_sync_all();
     u64 all = 0, all2 = 0;
     before = 0;
-#pragma unroll 1
-    for (uint32_t r = 0; r < n_ranks; ++r) {
-      const u64 c = ld_cluster_u64(map_to_rank(smem_addr(&sh->cta_sum[turn]), r));
-      if (r < rank) before += c;
-      all += c;
-      if (second) all2 += ld_cluster_u64(map_to_rank(smem_addr(&sh->cta_sum2[turn]), r));
+#pragma unroll
+    for (uint32_t r = 0; r < 8; ++r) {
+      if (r < n_ranks) {
+        const u64 c = sh->cta_sum[turn][r];
+        if (r < rank) before += c;
+        all += c;
+        if (second) all2 += sh->cta_second[turn][r];
+      }
     }
     if (second) *second = all2;
     return all;
@@ -348,17 +352,13 @@ struct SampleRow {
     turn ^= 1;
     if (warp == 0) {
       best = __reduce_min_sync(0xffffffffu, lane < kSampleWarps ? sh->warp_u[lane] : 0xffffffffu);
-      if (lane == 0) sh->found[turn] = best;
+      if (lane < n_ranks)
+        st_cluster_u32(map_to_rank(smem_addr(&sh->first_found[turn][rank]), lane), best);
     }
     __syncwarp();
     cluster_sync_all();
     best = 0xffffffffu;
-    for (uint32_t r = 0; r < n_ranks; ++r) {
-      uint32_t t;
-      asm volatile("ld.shared::cluster.u32 %0, [%1];"
-                   : "=r"(t) : "r"(map_to_rank(smem_addr(&sh->found[turn]), r)) : "memory");
-      best = min(best, t);
-    }
+    for (uint32_t r = 0; r < n_ranks; ++r) best = min(best, sh->first_found[turn][r]);
     return static_cast<int>(best);
   }
 
@@ -396,7 +396,7 @@ struct SampleRow {
   }
 
   // The index of the n-th entry of the segment's from .. to - 1 whose value is
-  // `at` (the last one's if there are fewer; every warp looks for itself).
+  // `at` (there are as many; every warp looks for itself).
   __device__ __forceinline__ uint32_t nth_equal(float at, u64 n, int from, int to) {
     uint32_t last = 0;
     u64 seen = 0;
@@ -404,12 +404,9 @@ struct SampleRow {
       const float l = value(i0 + lane);
       const uint32_t who = __ballot_sync(0xffffffffu, l == at);
       const int here = __popc(who);
-      if (here) {
-        // The (n - seen)-th of them, or the last.
-        const int k = seen + here >= n ? static_cast<int>(n - seen) : here;
-        last = static_cast<uint32_t>(first + i0 + __fns(who, 0, k));
-        seen += here;
-      }
+      if (seen + here >= n)
+        last = static_cast<uint32_t>(first + i0 + __fns(who, 0, static_cast<int>(n - seen)));
+      seen += here;
     }
     return last;
   }
@@ -688,13 +685,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
     m = row.lane < kSampleWarps ? sh.max_v[row.lane] : -INFINITY;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (row.lane == 0) sh.cta_max = m;
+    if (row.lane < row.n_ranks)
+      st_cluster_u32(map_to_rank(row.smem_addr(&sh.cta_max[row.rank]), row.lane),
+                     __float_as_uint(m));
   }
   __syncwarp();
   cluster_sync_all();
   m = -INFINITY;
-  for (uint32_t r = 0; r < row.n_ranks; ++r)
-    m = fmaxf(m, ld_cluster_f32(map_to_rank(row.smem_addr(&sh.cta_max), r)));
+  for (uint32_t r = 0; r < row.n_ranks; ++r) m = fmaxf(m, sh.cta_max[r]);
 
   m += 0.f;  // -0 as +0
   if (m == INFINITY) {
@@ -927,15 +925,20 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
             for (int i = 0; i < row.warp; ++i) eq_at += sh.warp_sum[i];
             const u64 w_at = count ? kept_weight(at) : 0;
             mine += (eq_at >= count ? 0 : min(equal, count - eq_at)) * w_at;
-            if (row.lane == 0) sh.warp_sum2[row.warp] = eq_at;
+            if (row.lane == 0) {
+              sh.equal_before[row.warp] = eq_at;
+              sh.equal[row.warp] = static_cast<uint32_t>(equal);
+            }
             const u64 kept = row.gather(mine, lower);
             // Within a warp's entries: those above, and of the border's value as
             // many as `count` leaves after the warps before.
             token = row.find_from(
                 share_of(kept), lower,
                 [&](int owner, int from, int to) {
-                  const u64 before_eq = sh.warp_sum2[owner];
-                  I = before_eq >= count ? 0 : row.nth_equal(at, count - before_eq, from, to) + 1;
+                  const u64 n0 = sh.equal_before[owner], n1 = n0 + sh.equal[owner];
+                  I = n0 >= count   ? 0
+                      : n1 <= count ? 0xffffffffu
+                                    : row.nth_equal(at, count - n0, from, to) + 1;
                 },
                 [&](float l, int i) -> u64 {
                   return l > at || (l == at && static_cast<uint32_t>(i) < I) ? kept_weight(l) : 0;
@@ -1141,7 +1144,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
               const u64 target = share_of(sum);
 #pragma unroll
               for (int j = 0; j < kListEach; ++j) {
-                if (low <= target && target < low + e[j]) sh.answer = ls.idx[j];
+                if (low <= target && target < low + e[j])
+                  for (uint32_t r = 0; r < row.n_ranks; ++r)
+                    st_cluster_u32(map_to_rank(row.smem_addr(&sh.answer), r), ls.idx[j]);
                 low += e[j];
               }
             } else {
@@ -1154,22 +1159,19 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
                 }
               }
             }
-            if (tid == 0) {
-              sh.border[0] = K;
-              sh.border[1] = I;
+            ls.sync();
+            if (tid < row.n_ranks && !whole) {
+              st_cluster_u32(map_to_rank(row.smem_addr(&sh.border[0]), tid), K);
+              st_cluster_u32(map_to_rank(row.smem_addr(&sh.border[1]), tid), I);
             }
           }
           __syncwarp();
           cluster_sync_all();
           if (whole) {
-            uint32_t t;
-            asm volatile("ld.shared::cluster.u32 %0, [%1];"
-                         : "=r"(t) : "r"(map_to_rank(row.smem_addr(&sh.answer), 0)) : "memory");
-            token = static_cast<int>(t);
+            token = static_cast<int>(sh.answer);
           } else {
-            const uint32_t b0 = map_to_rank(row.smem_addr(&sh.border[0]), 0);
-            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(K) : "r"(b0) : "memory");
-            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(I) : "r"(b0 + 4) : "memory");
+            K = sh.border[0];
+            I = sh.border[1];
             if (!thin) {
               mine += ld_cluster_u64(map_to_rank(
                   row.smem_addr(&sh.range_sum[row.rank * kSampleWarps + row.warp]), 0));
