@@ -34,11 +34,38 @@ bool aligned_to(const void* p, int bytes) {
   return (reinterpret_cast<uintptr_t>(p) & static_cast<uintptr_t>(bytes - 1)) == 0;
 }
 
-template <int NT, int C>
-int launch_rows_as(const RowsParams& p, bool vec, cudaStream_t st) {
-  const dim3 grid(static_cast<unsigned>(p.rows));
-  return vec ? launch_after(rows_kernel<NT, C, true>, grid, NT, 0, st, p)
-             : launch_after(rows_kernel<NT, C, false>, grid, NT, 0, st, p);
+template <bool XF32, int RES, int OUT>
+int launch_rows(const RowsParams& p, cudaStream_t st) {
+  const int chunks = p.cols / 8;
+  auto threads = [&](int c) { return ((chunks + c - 1) / c + 31) / 32 * 32; };
+  auto grid = [&](int threads) {
+    return dim3(static_cast<unsigned>(
+        std::min<int64_t>(p.rows, static_cast<int64_t>(kSms) * std::min(32, 1024 / threads))));
+  };
+  // Few rows: as many threads a row as it has chunks, for the shortest way.
+  if ((p.rows <= 2 * kSms && chunks <= 1024) || chunks <= 64) {
+    const int t = threads(1);
+    return launch_after(rows_kernel<XF32, RES, OUT, 1>, grid(t), t, 0, st, p);
+  }
+  if (chunks <= 1024) {
+    const int t = threads(2);
+    return launch_after(rows_kernel<XF32, RES, OUT, 2>, grid(t), t, 0, st, p);
+  }
+  const int t = threads(4);
+  return launch_after(rows_kernel<XF32, RES, OUT, 4>, grid(t), t, 0, st, p);
+}
+
+template <bool XF32, int RES>
+int launch_rows_out(const RowsParams& p, cudaStream_t st) {
+  if (p.out_type == kOutE4m3) return launch_rows<XF32, RES, kOutE4m3>(p, st);
+  if (p.out_type == kOutF32) return launch_rows<XF32, RES, kOutF32>(p, st);
+  return launch_rows<XF32, RES, kOutBf16>(p, st);
+}
+
+template <bool XF32>
+int launch_rows_res(const RowsParams& p, cudaStream_t st) {
+  if (!p.res) return launch_rows_out<XF32, 0>(p, st);
+  return p.res_f32 ? launch_rows_out<XF32, 2>(p, st) : launch_rows_out<XF32, 1>(p, st);
 }
 
 int rms_norm_impl(const ca_rms_norm_args* a, cudaStream_t st) {
@@ -68,7 +95,7 @@ int rms_norm_impl(const ca_rms_norm_args* a, cudaStream_t st) {
   if (!aligned_to(a->x, xs) || !aligned_to(a->out, os) || !aligned_to(a->w, 4) ||
       !aligned_to(a->residual, rs) || !aligned_to(a->sum_out, rs) || !aligned_to(a->out_scale, 4))
     return CA_ERR_INVALID;
-  if (a->cols > 32768 || a->rows > INT_MAX) return CA_ERR_UNSUPPORTED;
+  if (a->cols > INT_MAX - 1024) return CA_ERR_UNSUPPORTED;
   p.x = a->x;
   p.res = a->residual;
   p.sum = a->sum_out;
@@ -88,17 +115,12 @@ int rms_norm_impl(const ca_rms_norm_args* a, cudaStream_t st) {
                    aligned16(p.w) &&
                    (os == 1 ? aligned_to(p.out, 8) && p.out_stride % 8 == 0
                             : rows16(p.out, p.out_stride * os));
-  if (p.rows < 4 * kSms && p.cols <= 8192) {
-    if (p.cols <= 1024) return launch_rows_as<128, 1>(p, vec, st);
-    if (p.cols <= 2048) return launch_rows_as<256, 1>(p, vec, st);
-    if (p.cols <= 4096) return launch_rows_as<512, 1>(p, vec, st);
-    return launch_rows_as<1024, 1>(p, vec, st);
-  }
-  if (p.cols <= 1024) return launch_rows_as<128, 1>(p, vec, st);
-  if (p.cols <= 4096) return launch_rows_as<128, 4>(p, vec, st);
-  if (p.cols <= 8192) return launch_rows_as<256, 4>(p, vec, st);
-  if (p.cols <= 16384) return launch_rows_as<512, 4>(p, vec, st);
-  return launch_rows_as<1024, 4>(p, vec, st);
+  // Registers hold 16384 columns.
+  if (vec && p.cols <= 16384)
+    return p.x_f32 ? launch_rows_res<true>(p, st) : launch_rows_res<false>(p, st);
+  return launch_after(rows_any_kernel,
+                      dim3(static_cast<unsigned>(std::min<int64_t>(p.rows, 4 * kSms))), 256, 0, st,
+                      p);
 }
 
 // A row-major matrix of 1- or 2-byte elements in boxes of 128 bytes of

@@ -5,11 +5,13 @@
 //   e4m3: scale = 2^k, the smallest k with amax |y| <= 448 2^k; y / scale is
 //   exact in fp32, so each value is rounded once.
 //
-// One CTA per row, the row in registers between the passes (sum of squares,
-// largest magnitude, output), so HBM sees each input once and each output
-// once; the two reductions over the CTA are what a row waits for, and several
-// CTAs per SM hide them. Sums in fp32: a thread adds at most 32 squares, the
-// rest is a tree.
+// A CTA takes a row at a time, the row in registers between the passes (sum of
+// squares, largest magnitude, output), so HBM sees each input once and each
+// output once. What a row waits for are its loads and two reductions over the
+// CTA. rows_kernel, for rows that start on 16 bytes, therefore keeps the gain
+// in registers, asks for the next row before it works on the one it has, and
+// stays resident. Sums in fp32: a thread adds 8 squares to each of up to four
+// accumulators, the rest is a tree.
 #pragma once
 
 #include <cstdint>
@@ -89,142 +91,225 @@ __device__ __forceinline__ void* row_at(void* p, int f32, long long off) {
   return static_cast<char*>(p) + (off << (f32 ? 2 : 1));
 }
 
-// A sum or a maximum over the CTA's NT threads; `red` holds NT / 32 floats
-// that no other reduction uses.
-template <int NT, bool MAX>
-__device__ __forceinline__ float cta_reduce(float v, float* red) {
+// Eight elements as they are loaded, and as fp32.
+template <bool F32>
+struct Raw8 {
+  uint4 a, b;
+  __device__ __forceinline__ void load(const void* p, long long i) {
+    if constexpr (F32) {
+      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const float*>(p) + i);
+      a = q[0];
+      b = q[1];
+    } else {
+      a = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + i);
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (F32) {
+        v[k] = __uint_as_float(x[k]);
+        v[4 + k] = __uint_as_float(y[k]);
+      } else {
+        v[2 * k] = __uint_as_float(x[k] << 16);
+        v[2 * k + 1] = __uint_as_float(x[k] & 0xffff0000u);
+      }
+    }
+  }
+};
+
+// Over the CTA's `warps` warps; `red` holds a float for each.
+template <bool MAX>
+__device__ __forceinline__ float cta_reduce_n(float v, float* red, int warps) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float t = __shfl_xor_sync(0xffffffffu, v, o);
     v = MAX ? fmaxf(v, t) : v + t;
   }
-  if (NT == 32) return v;
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  if (warps == 1) return v;
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = red[0];
+  v = lane < warps ? red[lane] : 0.f;
 #pragma unroll
-  for (int i = 1; i < NT / 32; ++i) v = MAX ? fmaxf(v, red[i]) : v + red[i];
+  for (int o = 16; o > 0; o >>= 1) {
+    const float t = __shfl_xor_sync(0xffffffffu, v, o);
+    v = MAX ? fmaxf(v, t) : v + t;
+  }
   return v;
 }
 
-// Rows of at most NT * C * 8 columns, eight a chunk, C chunks a thread. VEC:
-// every row of every tensor starts on 16 bytes and cols is a multiple of 8;
-// otherwise elements are taken one by one, side by side across the threads.
-template <int NT, int C, bool VEC>
-__global__ void __launch_bounds__(NT) rows_kernel(const RowsParams p) {
-  __shared__ float red[2][NT / 32];
-  dependency_wait();
-  const long long r = blockIdx.x;
-  const int tid = threadIdx.x, cols = p.cols;
-  const void* x = row_at(p.x, p.x_f32, r * p.x_stride);
-  float v[C][8];
-  auto elem = [&](int c, int j) { return VEC ? (c * NT + tid) * 8 + j : (c * 8 + j) * NT + tid; };
+// C chunks of eight elements a thread; blockDim.x * C * 8 >= cols. RES: 0 none,
+// 1 bf16, 2 fp32.
+template <bool XF32, int RES, int OUT, int C>
+__global__ void __launch_bounds__(C == 1 ? 1024 : 512, C == 2 ? 2 : 1)
+    rows_kernel(const RowsParams p) {
+  __shared__ float red[2][2][32];  // of a row and the next
+  const int tid = threadIdx.x, cols = p.cols, warps = blockDim.x >> 5;
+  int at[C];
+  bool in[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    if (VEC) {
-      if (elem(c, 0) < cols) {
-        load8(x, p.x_f32, elem(c, 0), v[c]);
-      } else {
+    at[c] = (c * static_cast<int>(blockDim.x) + tid) * 8;
+    in[c] = at[c] < cols;
+  }
+  dependency_wait();
+  float g[C][8];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[c][j] = 1.f;
+    if (p.w && in[c]) load8(p.w, 1, at[c], g[c]);
+  }
+  Raw8<XF32> x[C];
+  Raw8<RES == 2> res[C];
+  auto fetch = [&](long long r) {
+    const void* px = row_at(p.x, XF32, r * p.x_stride);
+    const void* pr = RES ? row_at(p.res, RES == 2, r * p.res_stride) : nullptr;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if (in[c]) {
+        x[c].load(px, at[c]);
+        if constexpr (RES != 0) res[c].load(pr, at[c]);
+      }
+    }
+  };
+  long long r = blockIdx.x;
+  fetch(r);
+  const float inv_cols = 1.f / static_cast<float>(cols);
+  for (int turn = 0; r < p.rows; r += gridDim.x, turn ^= 1) {
+    float v[C][8];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      x[c].get(v[c]);
+      if constexpr (RES != 0) {
+        float t[8];
+        res[c].get(t);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[c][j] += t[j];
+        void* sum = row_at(p.sum, RES == 2, r * p.sum_stride);
+        if constexpr (RES == 1) {
+          const uint4 o = pack8(v[c]);
+          if (in[c])
+            *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(sum) + at[c]) = o;
+          Raw8<false> back;
+          back.a = o;
+          back.get(v[c]);
+        } else if (in[c]) {
+          store8(sum, 1, at[c], v[c]);
+        }
+      }
+      if (!in[c]) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[c][j] = 0.f;
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[c][j] = elem(c, j) < cols ? load1(x, p.x_f32, elem(c, j)) : 0.f;
     }
-  }
-  if (p.res) {
-    const void* res = row_at(p.res, p.res_f32, r * p.res_stride);
-    void* sum = row_at(p.sum, p.res_f32, r * p.sum_stride);
+    if (r + gridDim.x < p.rows) fetch(r + gridDim.x);
+    float rs = 1.f;
+    if (p.norm) {
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[c & 3] = fmaf(v[c][j], v[c][j], s[c & 3]);
+      const float ss = cta_reduce_n<false>((s[0] + s[1]) + (s[2] + s[3]), red[0][turn], warps);
+      rs = static_cast<float>(1.0 / sqrt(static_cast<double>(fmaf(ss, inv_cols, p.eps))));
+    }
+    float amax = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      float t[8];
-      if (VEC) {
-        if (elem(c, 0) < cols) {
-          load8(res, p.res_f32, elem(c, 0), t);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            v[c][j] += t[j];
-            if (!p.res_f32) v[c][j] = __bfloat162float(__float2bfloat16_rn(v[c][j]));
-          }
-          store8(sum, p.res_f32, elem(c, 0), v[c]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (elem(c, j) < cols) {
-            v[c][j] += load1(res, p.res_f32, elem(c, j));
-            if (!p.res_f32) v[c][j] = __bfloat162float(__float2bfloat16_rn(v[c][j]));
-            store1(sum, p.res_f32, elem(c, j), v[c][j]);
-          }
+      for (int j = 0; j < 8; ++j) {
+        v[c][j] = v[c][j] * rs * g[c][j];
+        // Infinities and NaN have no part in the scale.
+        if (OUT == kOutE4m3) {
+          const float m = fabsf(v[c][j]);
+          amax = fmaxf(amax, m < INFINITY ? m : 0.f);
         }
       }
     }
+    if constexpr (OUT != kOutE4m3) {
+      void* out = row_at(p.out, OUT == kOutF32, r * p.out_stride);
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (in[c]) store8(out, OUT == kOutF32, at[c], v[c]);
+    } else {
+      amax = cta_reduce_n<true>(amax, red[1][turn], warps);
+      const int k = e4m3_exp(amax, kKv8MinExp, kKv8MaxExp);
+      const float inv = exp2_int(-k);
+      if (tid == 0) p.out_scale[r] = exp2_int(k);
+      uint8_t* out = static_cast<uint8_t*>(p.out) + r * p.out_stride;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        uint32_t q[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          q[h] = cvt_e4m3x2(v[c][4 * h] * inv, v[c][4 * h + 1] * inv) |
+                 (cvt_e4m3x2(v[c][4 * h + 2] * inv, v[c][4 * h + 3] * inv) << 16);
+        if (in[c]) *reinterpret_cast<uint2*>(out + at[c]) = make_uint2(q[0], q[1]);
+      }
+    }
   }
-  float rs = 1.f;
-  if (p.norm) {
+}
+
+// Rows of any alignment, or of more columns than rows_kernel holds: elements
+// one by one, side by side across the threads. Each thread goes back to its
+// own elements, which it finds in the sum (or in x) as it left them.
+__global__ void __launch_bounds__(256) rows_any_kernel(const RowsParams p) {
+  __shared__ float red[2][2][32];
+  dependency_wait();
+  const int tid = threadIdx.x, cols = p.cols;
+  int turn = 0;
+  for (long long r = blockIdx.x; r < p.rows; r += gridDim.x, turn ^= 1) {
+    const void* x = row_at(p.x, p.x_f32, r * p.x_stride);
+    const void* res = p.res ? row_at(p.res, p.res_f32, r * p.res_stride) : nullptr;
+    void* sum = p.res ? row_at(p.sum, p.res_f32, r * p.sum_stride) : nullptr;
     float ss = 0.f;
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(v[c][j], v[c][j], ss);
-    ss = cta_reduce<NT, false>(ss, red[0]);
-    rs = 1.f / sqrtf(ss / static_cast<float>(cols) + p.eps);
-  }
-  float amax = 0.f;
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    float g[8];
-    if (p.w) {
-      if (VEC) {
-        if (elem(c, 0) < cols) load8(p.w, 1, elem(c, 0), g);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = elem(c, j) < cols ? p.w[elem(c, j)] : 0.f;
+    if (p.res || p.norm) {
+#pragma unroll 4
+      for (int i = tid; i < cols; i += 256) {
+        float v = load1(x, p.x_f32, i);
+        if (p.res) {
+          v += load1(res, p.res_f32, i);
+          if (!p.res_f32) v = __bfloat162float(__float2bfloat16_rn(v));
+          store1(sum, p.res_f32, i, v);
+        }
+        ss = fmaf(v, v, ss);
       }
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (p.norm) v[c][j] *= rs;
-      if (p.w) v[c][j] *= g[j];
-      const bool in = VEC ? elem(c, 0) < cols : elem(c, j) < cols;
-      // Infinities and NaN have no part in the scale.
-      if (in && fabsf(v[c][j]) <= 3.402823466e38f) amax = fmaxf(amax, fabsf(v[c][j]));
+    const void* from = p.res ? sum : x;
+    const int from_f32 = p.res ? p.res_f32 : p.x_f32;
+    float rs = 1.f;
+    if (p.norm) {
+      ss = cta_reduce_n<false>(ss, red[0][turn], 8);
+      rs = static_cast<float>(
+          1.0 / sqrt(static_cast<double>(ss / static_cast<float>(cols) + p.eps)));
     }
-  }
-  if (p.out_type != kOutE4m3) {
-    void* out = row_at(p.out, p.out_type, r * p.out_stride);
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      if (VEC) {
-        if (elem(c, 0) < cols) store8(out, p.out_type, elem(c, 0), v[c]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (elem(c, j) < cols) store1(out, p.out_type, elem(c, j), v[c][j]);
-      }
+    auto value = [&](int i) {
+      const float v = load1(from, from_f32, i) * rs;
+      return p.w ? v * p.w[i] : v;
+    };
+    if (p.out_type != kOutE4m3) {
+      void* out = row_at(p.out, p.out_type, r * p.out_stride);
+#pragma unroll 4
+      for (int i = tid; i < cols; i += 256) store1(out, p.out_type, i, value(i));
+      continue;
     }
-    return;
-  }
-  amax = cta_reduce<NT, true>(amax, red[1]);
-  const int k = e4m3_exp(amax, kKv8MinExp, kKv8MaxExp);
-  const float inv = exp2_int(-k);
-  if (tid == 0) p.out_scale[r] = exp2_int(k);
-  uint8_t* out = static_cast<uint8_t*>(p.out) + r * p.out_stride;
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    uint32_t q[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      q[h] = cvt_e4m3x2(v[c][4 * h] * inv, v[c][4 * h + 1] * inv) |
-             (cvt_e4m3x2(v[c][4 * h + 2] * inv, v[c][4 * h + 3] * inv) << 16);
-    if (VEC) {
-      if (elem(c, 0) < cols) *reinterpret_cast<uint2*>(out + elem(c, 0)) = make_uint2(q[0], q[1]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (elem(c, j) < cols) out[elem(c, j)] = static_cast<uint8_t>(q[j >> 2] >> (8 * (j & 3)));
+    float amax = 0.f;
+#pragma unroll 4
+    for (int i = tid; i < cols; i += 256) {
+      const float m = fabsf(value(i));
+      amax = fmaxf(amax, m < INFINITY ? m : 0.f);
     }
+    amax = cta_reduce_n<true>(amax, red[1][turn], 8);
+    const int k = e4m3_exp(amax, kKv8MinExp, kKv8MaxExp);
+    const float inv = exp2_int(-k);
+    if (tid == 0) p.out_scale[r] = exp2_int(k);
+    uint8_t* out = static_cast<uint8_t*>(p.out) + r * p.out_stride;
+#pragma unroll 4
+    for (int i = tid; i < cols; i += 256)
+      out[i] = static_cast<uint8_t>(cvt_e4m3x2(value(i) * inv, 0.f));
   }
 }
 

@@ -28,7 +28,7 @@ NORM = dict(x=FAKE, x_type=0, w=FAKE, norm=1, eps=1e-6, out=FAKE, out_type=0, ro
     (dict(residual=FAKE, sum_out=FAKE, residual_type=2), INV), (dict(out_type=2), INV),
     (dict(eps=-1.0), INV), (dict(eps=float("nan")), INV), (dict(x_stride=63), INV),
     (dict(out_stride=63), INV), (dict(x=FAKE + 1), INV), (dict(w=FAKE + 2), INV),
-    (dict(cols=32769), UNS), (dict(rows=1 << 31), UNS), (dict(rows=0), ca.CA_OK),
+    (dict(cols=1 << 31), UNS), (dict(rows=0), ca.CA_OK),
     (dict(rows=0, x=None, out=None), ca.CA_OK),
 ])
 def test_rms_norm(kw, status):
