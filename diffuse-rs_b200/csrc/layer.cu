@@ -42,8 +42,11 @@ int launch_rows(const RowsParams& p, cudaStream_t st) {
     return dim3(static_cast<unsigned>(
         std::min<int64_t>(p.rows, static_cast<int64_t>(kSms) * std::min(32, 1024 / threads))));
   };
-  // Few rows: as many threads a row as it has chunks, for the shortest way.
-  if ((p.rows <= 2 * kSms && chunks <= 1024) || chunks <= 64) {
+  // A chunk a thread where rows are few (the shortest way through one: 888 rows
+  // of 4096 in bf16 6.5 us, two chunks 7.1; 1184 rows 8.1 and 7.2) and where a
+  // chunk of fp32 takes twice the registers (2000 rows of 3584 12.8 us, two
+  // chunks 15.3).
+  if (chunks <= 1024 && (p.rows <= 6 * kSms || XF32 || RES == 2 || chunks <= 64)) {
     const int t = threads(1);
     return launch_after(rows_kernel<XF32, RES, OUT, 1>, grid(t), t, 0, st, p);
   }
@@ -51,8 +54,12 @@ int launch_rows(const RowsParams& p, cudaStream_t st) {
     const int t = threads(2);
     return launch_after(rows_kernel<XF32, RES, OUT, 2>, grid(t), t, 0, st, p);
   }
-  const int t = threads(4);
-  return launch_after(rows_kernel<XF32, RES, OUT, 4>, grid(t), t, 0, st, p);
+  if (chunks <= 1536) {
+    const int t = threads(3);
+    return launch_after(rows_kernel<XF32, RES, OUT, 3>, grid(t), t, 0, st, p);
+  }
+  const int t = threads(5);
+  return launch_after(rows_kernel<XF32, RES, OUT, 5>, grid(t), t, 0, st, p);
 }
 
 template <bool XF32, int RES>
@@ -115,8 +122,8 @@ int rms_norm_impl(const ca_rms_norm_args* a, cudaStream_t st) {
                    aligned16(p.w) &&
                    (os == 1 ? aligned_to(p.out, 8) && p.out_stride % 8 == 0
                             : rows16(p.out, p.out_stride * os));
-  // Registers hold 16384 columns.
-  if (vec && p.cols <= 16384)
+  // Registers hold 20480 columns.
+  if (vec && p.cols <= 20480)
     return p.x_f32 ? launch_rows_res<true>(p, st) : launch_rows_res<false>(p, st);
   return launch_after(rows_any_kernel,
                       dim3(static_cast<unsigned>(std::min<int64_t>(p.rows, 4 * kSms))), 256, 0, st,

@@ -10,8 +10,8 @@
 // output once. What a row waits for are its loads and two reductions over the
 // CTA. rows_kernel, for rows that start on 16 bytes, therefore keeps the gain
 // in registers, asks for the next row before it works on the one it has, and
-// stays resident. Sums in fp32: a thread adds 8 squares to each of up to four
-// accumulators, the rest is a tree.
+// stays resident. Eight squares are added in fp32, the rest in 64 bits, as the
+// reference adds all of them.
 #pragma once
 
 #include <cstdint>
@@ -119,33 +119,40 @@ struct Raw8 {
   }
 };
 
-// Over the CTA's `warps` warps; `red` holds a float for each.
-template <bool MAX>
-__device__ __forceinline__ float cta_reduce_n(float v, float* red, int warps) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float t = __shfl_xor_sync(0xffffffffu, v, o);
-    v = MAX ? fmaxf(v, t) : v + t;
-  }
+// The largest over the CTA's `warps` warps; `red` holds a float for each.
+__device__ __forceinline__ float cta_max_n(float v, float* red, int warps) {
+  // (Of numbers that are not negative, whose bits have their order.)
+  v = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
   if (warps == 1) return v;
   const int lane = threadIdx.x & 31;
   if (lane == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   v = lane < warps ? red[lane] : 0.f;
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+}
+
+__device__ __forceinline__ double cta_sum_n(double v, double* red, int warps) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float t = __shfl_xor_sync(0xffffffffu, v, o);
-    v = MAX ? fmaxf(v, t) : v + t;
-  }
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (warps == 1) return v;
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = lane < warps ? red[lane] : 0.0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// C chunks of eight elements a thread; blockDim.x * C * 8 >= cols. RES: 0 none,
+// C chunks of eight elements a thread; blockDim.x * C * 8 >= cols. At most 64
+// registers (128 of five chunks), so that an SM holds 1024 threads; of three
+// or five chunks the gain is read for each row (from L1). RES: 0 none,
 // 1 bf16, 2 fp32.
 template <bool XF32, int RES, int OUT, int C>
-__global__ void __launch_bounds__(C == 1 ? 1024 : 512, C == 2 ? 2 : 1)
+__global__ void __launch_bounds__(C >= 3 ? 512 : 1024, C == 3 ? 2 : 1)
     rows_kernel(const RowsParams p) {
-  __shared__ float red[2][2][32];  // of a row and the next
+  __shared__ double red_d[2][32];  // of a row and the next
+  __shared__ float red[2][32];
   const int tid = threadIdx.x, cols = p.cols, warps = blockDim.x >> 5;
   int at[C];
   bool in[C];
@@ -155,12 +162,13 @@ __global__ void __launch_bounds__(C == 1 ? 1024 : 512, C == 2 ? 2 : 1)
     in[c] = at[c] < cols;
   }
   dependency_wait();
-  float g[C][8];
+  constexpr bool kHeld = C < 3;
+  float g[kHeld ? C : 1][8];
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
+  for (int c = 0; c < (kHeld ? C : 1); ++c) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) g[c][j] = 1.f;
-    if (p.w && in[c]) load8(p.w, 1, at[c], g[c]);
+    if (kHeld && p.w && in[c]) load8(p.w, 1, at[c], g[c]);
   }
   Raw8<XF32> x[C];
   Raw8<RES == 2> res[C];
@@ -177,7 +185,7 @@ __global__ void __launch_bounds__(C == 1 ? 1024 : 512, C == 2 ? 2 : 1)
   };
   long long r = blockIdx.x;
   fetch(r);
-  const float inv_cols = 1.f / static_cast<float>(cols);
+  const double inv_cols = 1.0 / static_cast<double>(cols);
   for (int turn = 0; r < p.rows; r += gridDim.x, turn ^= 1) {
     float v[C][8];
 #pragma unroll
@@ -208,20 +216,25 @@ __global__ void __launch_bounds__(C == 1 ? 1024 : 512, C == 2 ? 2 : 1)
     if (r + gridDim.x < p.rows) fetch(r + gridDim.x);
     float rs = 1.f;
     if (p.norm) {
-      float s[4] = {0.f, 0.f, 0.f, 0.f};
+      float s[C];
+      double d = 0.0;
 #pragma unroll
-      for (int c = 0; c < C; ++c)
+      for (int c = 0; c < C; ++c) {
+        s[c] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[c & 3] = fmaf(v[c][j], v[c][j], s[c & 3]);
-      const float ss = cta_reduce_n<false>((s[0] + s[1]) + (s[2] + s[3]), red[0][turn], warps);
-      rs = static_cast<float>(1.0 / sqrt(static_cast<double>(fmaf(ss, inv_cols, p.eps))));
+        for (int j = 0; j < 8; ++j) s[c] = fmaf(v[c][j], v[c][j], s[c]);
+        d += static_cast<double>(s[c]);
+      }
+      const double ss = cta_sum_n(d, red_d[turn], warps);
+      rs = static_cast<float>(1.0 / sqrt(ss * inv_cols + static_cast<double>(p.eps)));
     }
     float amax = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
+      if (!kHeld && p.w && in[c]) load8(p.w, 1, at[c], g[0]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[c][j] = v[c][j] * rs * g[c][j];
+        v[c][j] = v[c][j] * rs * g[kHeld ? c : 0][j];
         // Infinities and NaN have no part in the scale.
         if (OUT == kOutE4m3) {
           const float m = fabsf(v[c][j]);
@@ -235,7 +248,7 @@ __global__ void __launch_bounds__(C == 1 ? 1024 : 512, C == 2 ? 2 : 1)
       for (int c = 0; c < C; ++c)
         if (in[c]) store8(out, OUT == kOutF32, at[c], v[c]);
     } else {
-      amax = cta_reduce_n<true>(amax, red[1][turn], warps);
+      amax = cta_max_n(amax, red[turn], warps);
       const int k = e4m3_exp(amax, kKv8MinExp, kKv8MaxExp);
       const float inv = exp2_int(-k);
       if (tid == 0) p.out_scale[r] = exp2_int(k);
@@ -257,7 +270,8 @@ __global__ void __launch_bounds__(C == 1 ? 1024 : 512, C == 2 ? 2 : 1)
 // one by one, side by side across the threads. Each thread goes back to its
 // own elements, which it finds in the sum (or in x) as it left them.
 __global__ void __launch_bounds__(256) rows_any_kernel(const RowsParams p) {
-  __shared__ float red[2][2][32];
+  __shared__ double red_d[2][32];
+  __shared__ float red[2][32];
   dependency_wait();
   const int tid = threadIdx.x, cols = p.cols;
   int turn = 0;
@@ -265,7 +279,7 @@ __global__ void __launch_bounds__(256) rows_any_kernel(const RowsParams p) {
     const void* x = row_at(p.x, p.x_f32, r * p.x_stride);
     const void* res = p.res ? row_at(p.res, p.res_f32, r * p.res_stride) : nullptr;
     void* sum = p.res ? row_at(p.sum, p.res_f32, r * p.sum_stride) : nullptr;
-    float ss = 0.f;
+    double ss = 0.0;
     if (p.res || p.norm) {
 #pragma unroll 4
       for (int i = tid; i < cols; i += 256) {
@@ -275,16 +289,15 @@ __global__ void __launch_bounds__(256) rows_any_kernel(const RowsParams p) {
           if (!p.res_f32) v = __bfloat162float(__float2bfloat16_rn(v));
           store1(sum, p.res_f32, i, v);
         }
-        ss = fmaf(v, v, ss);
+        ss += static_cast<double>(v) * v;
       }
     }
     const void* from = p.res ? sum : x;
     const int from_f32 = p.res ? p.res_f32 : p.x_f32;
     float rs = 1.f;
     if (p.norm) {
-      ss = cta_reduce_n<false>(ss, red[0][turn], 8);
-      rs = static_cast<float>(
-          1.0 / sqrt(static_cast<double>(ss / static_cast<float>(cols) + p.eps)));
+      ss = cta_sum_n(ss, red_d[turn], 8);
+      rs = static_cast<float>(1.0 / sqrt(ss / cols + static_cast<double>(p.eps)));
     }
     auto value = [&](int i) {
       const float v = load1(from, from_f32, i) * rs;
@@ -302,7 +315,7 @@ __global__ void __launch_bounds__(256) rows_any_kernel(const RowsParams p) {
       const float m = fabsf(value(i));
       amax = fmaxf(amax, m < INFINITY ? m : 0.f);
     }
-    amax = cta_reduce_n<true>(amax, red[1][turn], 8);
+    amax = cta_max_n(amax, red[turn], 8);
     const int k = e4m3_exp(amax, kKv8MinExp, kKv8MaxExp);
     const float inv = exp2_int(-k);
     if (tid == 0) p.out_scale[r] = exp2_int(k);

@@ -83,7 +83,7 @@ def test_norm_types(x, res, out):
 
 
 @pytest.mark.parametrize("cols", [1, 7, 8, 100, 1024, 1032, 2048, 3584, 4104, 8192, 8200, 16384,
-                                  16392, 18944, 32767, 32768, 40000])
+                                  16392, 18944, 20480, 20488, 32767, 32768, 40000])
 @pytest.mark.parametrize("rows", [1, 700])
 def test_norm_widths(rows, cols):
     norm_case(rows, cols, res="bf16", out="e4m3")
