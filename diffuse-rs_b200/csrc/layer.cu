@@ -179,14 +179,19 @@ int launch_skinny(const Product& q, cudaStream_t st) {
   }
   const int64_t tiles = (q.p.rows + 127) / 128, tok = (q.p.n + NT - 1) / NT;
   if (tiles > INT_MAX / 8 || tok > 65535) return CA_ERR_UNSUPPORTED;
-  // Columns are split while that fills SMs (two CTAs fit on one) and leaves a
-  // CTA at least four stages of work.
+  // Columns are split until there is a CTA for each SM, down to four pieces a
+  // CTA, and once more (two fit on an SM) if that leaves twelve. One token, us at
+  // 1, 2, 4 and 8 splits: 4096 x 4096 11.3, 8.1, 6.3, 7.1; 1024 x 4096 11.1, 8.0,
+  // 5.9, 5.1; 12288 -> 4096 28, 16.5, 10.5, 9.9; gated 4096 -> 12288 in bf16 51,
+  // 36, 40, 38.
   // fp32 outputs of bf16 operands: few additions to an accumulator, too, which
   // truncates (pair.cuh).
   const int64_t most = KIND == kKindBf16 && q.p.out_f32 ? 16 : INT_MAX;
   int S = 1;
   while (S < 8 && q.p.kblocks > most * S) S *= 2;
-  while (S < 8 && tiles * tok * S * 2 <= 2 * kSms && q.p.kblocks >= 8 * S) S *= 2;
+  while (S < 8 && ((tiles * tok * S * 2 <= kSms && q.p.kblocks >= 8 * S) ||
+                   (tiles * tok * S * 2 <= 2 * kSms && q.p.kblocks >= 24 * S)))
+    S *= 2;
   return launch_cluster_after(skinny_kernel<C>,
                               dim3(static_cast<unsigned>(tiles * S), static_cast<unsigned>(tok)),
                               C::kThreads, C::kSmem, S, st, tw, tu, tx, q.p);

@@ -9,9 +9,9 @@
 // weights' way from HBM: each is read once. A stage holds 128 bytes of each
 // row; the ring of stages (about 100 KB, so that two CTAs share an SM) keeps
 // the loads in flight. Where 128 rows a CTA would leave SMs idle, the S CTAs
-// of a cluster split the columns between them and add their parts through
-// distributed shared memory, in the order of their ranks: no workspace, no
-// atomics, the same bits every time.
+// of a cluster split the columns between them. Each sends its part of a token
+// to the shared memory of the CTA that finishes it, which adds the parts in
+// the order of their ranks: no workspace, no atomics, the same bits every time.
 //
 // Lane = weight row, TMEM column = token, so that a warp's 32 threads store 32
 // neighbours of an output row.
@@ -142,12 +142,16 @@ struct SkinnyCfg {
   static constexpr int G = G_;        // weight matrices
   static constexpr int NT = NT_;      // tokens of a CTA
   static constexpr int kStage = G * 16384 + NT * 128;
-  static constexpr int kStages = 104 * 1024 / kStage;
+  static constexpr int kParts = G * NT * 512;  // of a sum, from every rank
+  // Few tokens' parts have memory of their own, so that they can be sent while
+  // another CTA still multiplies; more lie over the ring.
+  static constexpr bool kApart = NT == 16;
+  static constexpr int kStages = (104 * 1024 - (kApart ? kParts : 0)) / kStage;
   static constexpr int kRing = kStages * kStage;
-  static_assert(kRing >= G * NT * 512, "the parts of a sum are laid over the ring");
+  static_assert(kApart || kRing >= kParts, "the parts of a sum are laid over the ring");
   static constexpr int kThreads = 192;
   static constexpr int kBars = 2 * kStages + 1;
-  static constexpr int kSmem = 1024 + kRing + 8 * kBars + 16;
+  static constexpr int kSmem = 1024 + kRing + (kApart ? kParts : 0) + 8 * kBars + 16;
   static constexpr int kTmemCols = G * NT < 32 ? 32 : G * NT;
   static constexpr int kElems = KIND == kKindBf16 ? 64 : 128;  // of 128 bytes
 };
@@ -158,7 +162,9 @@ __global__ void __launch_bounds__(C::kThreads)
                   const __grid_constant__ CUtensorMap tm_x, const LinearParams p) {
   extern __shared__ uint8_t raw_smem[];
   const uint32_t base = (smem_u32(raw_smem) + 1023u) & ~1023u;
-  const uint32_t bars = base + C::kRing, slot = bars + 8 * C::kBars;
+  const uint32_t parts = C::kApart ? base + C::kRing : base;
+  const uint32_t bars = base + C::kRing + (C::kApart ? C::kParts : 0);
+  const uint32_t slot = bars + 8 * C::kBars;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   auto full = [&](int s) { return bars + 8 * s; };
   auto empty = [&](int s) { return bars + 8 * (C::kStages + s); };
@@ -169,7 +175,20 @@ __global__ void __launch_bounds__(C::kThreads)
   const int kb0 = static_cast<int>(static_cast<long long>(p.kblocks) * rank / S);
   const int kb1 = static_cast<int>(static_cast<long long>(p.kblocks) * (rank + 1) / S);
 
+  bool dead = false;
+  int filled = 0;  // stages, by the loading thread
+  auto fill = [&](int i) {
+    const int s = i % C::kStages, x = (kb0 + i) * C::kElems;
+    const uint32_t dst = base + s * C::kStage;
+    mbar_arrive_expect_tx(full(s), C::kStage);
+    tma_load_2d(dst, &tm_w, full(s), x, r0);
+    if constexpr (C::G == 2) tma_load_2d(dst + 16384, &tm_u, full(s), x, r0);
+    tma_load_2d(dst + C::G * 16384, &tm_x, full(s), x, t0);
+  };
   if (tid == 0) {
+    tma_prefetch_desc(&tm_w);
+    if constexpr (C::G == 2) tma_prefetch_desc(&tm_u);
+    tma_prefetch_desc(&tm_x);
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
@@ -179,8 +198,12 @@ __global__ void __launch_bounds__(C::kThreads)
     fence_proxy_async_smem();
   }
   // TMEM is taken only once the kernel before is complete, and the next one
-  // let in only then: neither can hold columns that the other waits for.
+  // let in only then: neither can hold columns that the other waits for. The
+  // first loads need no TMEM.
   wait_prior_kernel();
+  if (tid == 0)
+    for (; filled < min(C::kStages, kb1 - kb0); ++filled) fill(filled);
+  __syncwarp();
   if (warp == 1) {
     tmem_alloc(slot, C::kTmemCols);
     tmem_relinquish();
@@ -191,24 +214,18 @@ __global__ void __launch_bounds__(C::kThreads)
   let_next_kernel();
   uint32_t tmem;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
-  bool dead = false;
 
   if (warp == 0) {
     if (lane == 0) {
-      int i = 0;
-      for (int kb = kb0; kb < kb1; ++kb, ++i) {
-        const int s = i % C::kStages;
-        if (i >= C::kStages && !mbar_wait(empty(s), ((i / C::kStages) - 1) & 1, dead, p.err)) break;
-        const uint32_t dst = base + s * C::kStage;
-        mbar_arrive_expect_tx(full(s), C::kStage);
-        tma_load_2d(dst, &tm_w, full(s), kb * C::kElems, r0);
-        if constexpr (C::G == 2) tma_load_2d(dst + 16384, &tm_u, full(s), kb * C::kElems, r0);
-        tma_load_2d(dst + C::G * 16384, &tm_x, full(s), kb * C::kElems, t0);
+      for (; filled < kb1 - kb0; ++filled) {
+        if (!mbar_wait(empty(filled % C::kStages), ((filled / C::kStages) - 1) & 1, dead, p.err))
+          break;
+        fill(filled);
       }
       // After an expired wait the copies in flight still have to land.
       if (dead) {
         bool late = false;
-        for (int j = max(0, i - C::kStages); j < i; ++j)
+        for (int j = max(0, filled - C::kStages); j < filled; ++j)
           mbar_wait(full(j % C::kStages), (j / C::kStages) & 1, late, p.err);
       }
     }
@@ -244,6 +261,17 @@ __global__ void __launch_bounds__(C::kThreads)
   auto combine = [&](float a, float b, float sa) {
     return C::G == 2 ? activate(a * sa * w0, p.act) * (b * sa * w1) : a * sa * w0 + bias;
   };
+  const int live = static_cast<int>(min(static_cast<long long>(C::NT), p.n - t0));  // tokens
+  const int each = C::NT / static_cast<int>(S);  // tokens that a rank finishes, from `first` on
+  const int shift = 31 - __clz(each);            // (a power of two)
+  const int first = each * static_cast<int>(rank), mine = max(0, min(each, live - first));
+  const bool on = warp >= 2 && r < p.rows;
+  // Residuals of its first tokens are asked for before the wait: a row's
+  // latency each time was most of what 64 tokens took (4 us of 15 without
+  // splits, 11 of 19 with two).
+  constexpr int kGroup = C::NT < 32 ? C::NT : 32;
+  float x[kGroup];
+  if (C::G == 1 && on && p.residual) load_residual(p, x, t0 + first, r, mine);
   if (warp >= 2) {
     if (r < p.rows) {
       if (p.w_scale) w0 = p.w_scale[r];
@@ -251,69 +279,83 @@ __global__ void __launch_bounds__(C::kThreads)
       if (C::G == 1 && p.bias) bias = p.bias[r];
     }
     mbar_wait(done, 0, dead, p.err);
+    __syncwarp();
     tc_fence_after();
+  }
+  if (S > 1 && !C::kApart) cluster_sync_all();  // every ring is free
+  if (warp >= 2) {
     const uint32_t col = tmem + (static_cast<uint32_t>(warp & 3) << 21);
-#pragma unroll 1
+#pragma unroll
     for (int j0 = 0; j0 < C::NT; j0 += 16) {
+      if (j0 >= live) break;
       uint32_t d0[16], d1[16];
       tmem_ld16(col + j0, d0);
       if constexpr (C::G == 2) tmem_ld16(col + C::NT + j0, d1);
       const float sa = act_scale_of(p, t0 + j0 + (lane & 15));
       tmem_wait_ld();
       if (S == 1) {
-        const int m = tokens_in<16>(p, t0 + j0, r < p.rows);
-        // Residuals are all asked for before the first store: out may be the
-        // same memory, so the compiler may not move them up itself.
-        float v[16], x[16];
-        if (p.residual) load_residual(p, x, t0 + j0, r, m);
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          v[j] = combine(__uint_as_float(d0[j]), C::G == 2 ? __uint_as_float(d1[j]) : 0.f,
-                         __shfl_sync(0xffffffffu, sa, j));
-        if (p.residual) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] += x[j];
-        }
-        store_tokens(p, v, t0 + j0, r, m);
-      } else {
+        float v[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          st_shared_f32(base + ((j0 + j) * 128 + f) * 4, __uint_as_float(d0[j]));
-          if constexpr (C::G == 2)
-            st_shared_f32(base + ((C::NT + j0 + j) * 128 + f) * 4, __uint_as_float(d1[j]));
+          v[j] = combine(__uint_as_float(d0[j]), C::G == 2 ? __uint_as_float(d1[j]) : 0.f,
+                         __shfl_sync(0xffffffffu, sa, j));
+          if (C::G == 1 && p.residual) v[j] += x[j0 % kGroup + j];
+        }
+        store_tokens(p, v, t0 + j0, r, tokens_in<16>(p, t0 + j0, r < p.rows));
+        // (out may be the residual: the next ones are not asked for earlier.)
+        if (C::G == 1 && p.residual && on && (j0 + 16) % kGroup == 0 && j0 + 16 < C::NT)
+          load_residual(p, x, t0 + j0 + 16, r, live - j0 - 16);
+      } else {
+        // Token j goes to rank j / each, place (this rank, j % each).
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if (j0 + j < live) {
+            const int to = (j0 + j) >> shift, k = (j0 + j) & (each - 1);
+            const uint32_t at = map_to_rank(
+                parts + ((static_cast<int>(rank) * each + k) * C::G * 128 + f) * 4, to);
+            st_cluster_f32(at, __uint_as_float(d0[j]));
+            if constexpr (C::G == 2) st_cluster_f32(at + 512, __uint_as_float(d1[j]));
+          }
         }
       }
     }
     tc_fence_before();
   }
   if (S > 1) {
-    // Rank i joins tokens NT i / S .. NT (i + 1) / S - 1, parts in the order
-    // of the ranks.
     __syncwarp();
     cluster_sync_all();
-    if (warp >= 2 && r < p.rows) {
-      const int j1 = min(static_cast<long long>(C::NT * (rank + 1) / S), p.n - t0);
-      for (int j = C::NT * rank / S; j < j1; ++j) {
-        float a = 0.f, b = 0.f;
-        for (uint32_t q = 0; q < S; ++q) {
-          a += ld_cluster_f32(map_to_rank(base + (j * 128 + f) * 4, q));
-          if constexpr (C::G == 2)
-            b += ld_cluster_f32(map_to_rank(base + ((C::NT + j) * 128 + f) * 4, q));
+    if (on) {
+#pragma unroll
+      for (int j0 = 0; j0 < (C::NT < 32 ? C::NT : 32); j0 += 4) {  // two ranks: 32 tokens each
+        if (j0 >= mine) break;
+        const int k = min(mine - j0, 4);
+        float d[2][4] = {};
+        for (int q = 0; q < static_cast<int>(S); ++q) {
+          const uint32_t at = parts + ((q * each + j0) * C::G * 128 + f) * 4;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int g = 0; g < C::G; ++g) {
+              float t = 0.f;
+              if (j < k)
+                asm volatile("ld.shared.f32 %0, [%1];"
+                             : "=f"(t) : "r"(at + (j * C::G + g) * 512) : "memory");
+              d[g][j] += t;
+            }
+          }
         }
-        float v[1] = {combine(a, b, p.act_scale ? p.act_scale[t0 + j] : 1.f)};
-        if (p.residual) {
-          float x[1];
-          load_residual(p, x, t0 + j, r, 1);
-          v[0] += x[0];
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float sa = j < k && p.act_scale ? p.act_scale[t0 + first + j0 + j] : 1.f;
+          v[j] = combine(d[0][j], d[1][j], sa);
+          if (C::G == 1 && p.residual) v[j] += x[j0 + j];
         }
-        store_tokens(p, v, t0 + j, r, 1);
+        store_tokens(p, v, t0 + first + j0, r, k);
       }
     }
-    __syncwarp();
-    cluster_sync_all();  // no CTA leaves while its parts are read
-  } else {
-    __syncthreads();
   }
+  __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, C::kTmemCols);
