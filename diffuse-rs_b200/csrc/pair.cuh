@@ -131,7 +131,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::kThreads)
   const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
   const int tiles = p.r_tiles * p.t_tiles;
 
+  bool dead = false;
+  // The loading thread's place: stages filled, and the piece of the tile.
+  int filled = 0, tile = pair, kb = 0, r0 = 0, t0 = 0;
+  auto fill = [&]() {
+    if (kb == 0) {
+      int rt, tt;
+      pair_tile(p, tile, rt, tt);
+      r0 = rt * C::kRows + static_cast<int>(rank) * (C::kRows / 2);
+      t0 = tt * C::NT + static_cast<int>(rank) * (C::NT / 2);
+    }
+    const int s = filled % C::kStages;
+    if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * C::kStage);
+    const uint32_t dst = base + s * C::kStage, bar = map_to_rank(full(s), 0);
+    tma_load_2d_pair(dst, &tm_w, bar, kb * C::kElems, r0);
+    if constexpr (C::G == 2) tma_load_2d_pair(dst + 8192, &tm_u, bar, kb * C::kElems, r0);
+    tma_load_2d_pair(dst + 16384, &tm_x, bar, kb * C::kElems, t0);
+    ++filled;
+    if (++kb == p.kblocks) {
+      kb = 0;
+      tile += n_pairs;
+    }
+  };
   if (tid == 0) {
+    tma_prefetch_desc(&tm_w);
+    if constexpr (C::G == 2) tma_prefetch_desc(&tm_u);
+    tma_prefetch_desc(&tm_x);
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
@@ -143,6 +168,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::kThreads)
     fence_barrier_init();
     fence_proxy_async_smem();
   }
+  __syncwarp();
+  cluster_sync_all();   // the barriers of both are set
   wait_prior_kernel();  // before TMEM is taken, as in skinny.cuh
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot),
@@ -151,37 +178,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::kThreads)
   }
   __syncwarp();
   tc_fence_before();
-  cluster_sync_all();  // the barriers of both are set
+  cluster_arrive();
+  if (tid == 0)
+    while (filled < C::kStages && tile < tiles) fill();  // the first loads need no TMEM
+  __syncwarp();
+  cluster_wait();  // both CTAs have theirs
   tc_fence_after();
   let_next_kernel();
   uint32_t tmem;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
-  bool dead = false;
 
   if (warp == 0) {
     if (lane == 0) {
-      int i = 0;  // stages filled
-      for (int tile = pair; tile < tiles && !dead; tile += n_pairs) {
-        int rt, tt;
-        pair_tile(p, tile, rt, tt);
-        const int r0 = rt * C::kRows + static_cast<int>(rank) * (C::kRows / 2);
-        const int t0 = tt * C::NT + static_cast<int>(rank) * (C::NT / 2);
-        for (int kb = 0; kb < p.kblocks; ++kb, ++i) {
-          const int s = i % C::kStages;
-          if (i >= C::kStages && !mbar_wait(empty(s), ((i / C::kStages) - 1) & 1, dead, p.err))
-            break;
-          if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * C::kStage);
-          const uint32_t dst = base + s * C::kStage, bar = map_to_rank(full(s), 0);
-          tma_load_2d_pair(dst, &tm_w, bar, kb * C::kElems, r0);
-          if constexpr (C::G == 2) tma_load_2d_pair(dst + 8192, &tm_u, bar, kb * C::kElems, r0);
-          tma_load_2d_pair(dst + 16384, &tm_x, bar, kb * C::kElems, t0);
-        }
+      while (tile < tiles) {
+        if (!mbar_wait(empty(filled % C::kStages), ((filled / C::kStages) - 1) & 1, dead, p.err))
+          break;
+        fill();
       }
       // After an expired wait the copies in flight still have to land; the
       // even CTA's barriers count those of both.
       if (dead && rank == 0) {
         bool late = false;
-        for (int j = max(0, i - C::kStages); j < i; ++j)
+        for (int j = max(0, filled - C::kStages); j < filled; ++j)
           mbar_wait(full(j % C::kStages), (j / C::kStages) & 1, late, p.err);
       }
     }

@@ -145,7 +145,7 @@ struct SkinnyCfg {
   static constexpr int kParts = G * NT * 512;  // of a sum, from every rank
   // Few tokens' parts have memory of their own, so that they can be sent while
   // another CTA still multiplies; more lie over the ring.
-  static constexpr bool kApart = NT == 16;
+  static constexpr bool kApart = kParts <= 16384;
   static constexpr int kStages = (104 * 1024 - (kApart ? kParts : 0)) / kStage;
   static constexpr int kRing = kStages * kStage;
   static_assert(kApart || kRing >= kParts, "the parts of a sum are laid over the ring");
