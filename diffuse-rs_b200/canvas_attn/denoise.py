@@ -24,6 +24,7 @@ from typing import Optional, Sequence
 import numpy as np
 
 from . import CaError, _check, _ptr, _stream, lib
+from .layer import one_device
 
 COSINE, LINEAR = 0, 1
 ENTROPY_EXIT, LOW_CONFIDENCE, MARGIN, CONFIDENCE, ENTROPY_BOUND, RANDOM = range(6)
@@ -126,9 +127,10 @@ def make_sample_args(logits, rows, u, token, prob=None, *, n_vocab: Optional[int
         scalars.append((int if name == "top_k" else float)(0 if each else x))
     if rows is None and n > logits.shape[0]:
         raise ValueError("more candidates than rows")
+    if logits.shape[0] > 1 and logits.stride(0) < v:
+        raise ValueError("logits: rows must not overlap")
     kept = (logits, rows, u, token, prob, suppress, *tensors)
-    if len({x.device for x in kept if x is not None}) > 1:
-        raise ValueError("tensors of one call are on several devices")
+    one_device(*kept)
     n_sup = 0 if suppress is None else int(suppress.numel())
     a = CaSampleArgs(_ptr(logits), kind, int(logits.shape[0]), v,
                      int(logits.stride(0)) if logits.shape[0] > 1 else 0, _ptr(rows), n,

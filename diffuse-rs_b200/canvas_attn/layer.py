@@ -74,6 +74,8 @@ def _matrix(name, x, types, shape=None):
                          f"got {list(x.shape)}")
     if x.shape[1] > 1 and x.stride(1) != 1:
         raise ValueError(f"{name}: columns must be next to one another")
+    if x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+        raise ValueError(f"{name}: rows must not overlap")
     return kind, int(x.stride(0)) if x.shape[0] > 1 else 0
 
 
@@ -84,7 +86,8 @@ def _vector(name, x, n):
         raise ValueError(f"{name} must be contiguous float32 with {n} entries")
 
 
-def _one_device(*xs):
+def one_device(*xs):
+    """The tensors of a call are on one device, and that is the current one."""
     devices = {x.device for x in xs if x is not None}
     if len(devices) > 1:
         raise ValueError(f"tensors of one call are on {sorted(map(str, devices))}")
@@ -117,7 +120,7 @@ def make_rms_norm_args(x, out, *, w=None, eps: float = 1e-6, norm: bool = True, 
     _vector("out_scale", out_scale, shape[0])
     if ot == E4M3 and out_scale is None:
         raise ValueError("an e4m3 output needs out_scale")
-    _one_device(x, out, residual, sum_out, w, out_scale)
+    one_device(x, out, residual, sum_out, w, out_scale)
     a = CaRmsNormArgs(_ptr(x), xt, xs, _ptr(residual), rt, rs, _ptr(sum_out), ss, _ptr(w),
                       1 if norm else 0, float(eps), _ptr(out), ot, os_, _ptr(out_scale),
                       shape[0], shape[1])
@@ -167,7 +170,7 @@ def make_linear_q8_args(act, act_scale, w, w_scale, out, *, bias=None, residual=
     _vector("act_scale", act_scale, n)
     _vector("w_scale", w_scale, rows)
     _vector("bias", bias, rows)
-    _one_device(act, act_scale, w, w_scale, out, bias, residual, status)
+    one_device(act, act_scale, w, w_scale, out, bias, residual, status)
     a = CaLinearQ8Args(_ptr(act), as_, _ptr(act_scale), _ptr(w), _ptr(w_scale), _ptr(bias),
                        _ptr(residual), rs, _ptr(out), 1 if ot == F32 else 0, os_, n, rows, cols,
                        _ptr(status))
@@ -205,7 +208,7 @@ def make_gated_linear_args(act, w_gate, w_up, out, *, activation: str = "silu",
     _vector("act_scale", act_scale, n)
     _vector("gate_scale", gate_scale, rows)
     _vector("up_scale", up_scale, rows)
-    _one_device(act, act_scale, w_gate, w_up, gate_scale, up_scale, out, status)
+    one_device(act, act_scale, w_gate, w_up, gate_scale, up_scale, out, status)
     a = CaGatedLinearArgs(_ptr(act), kind, as_, _ptr(act_scale), _ptr(w_gate), _ptr(w_up),
                           _ptr(gate_scale), _ptr(up_scale), ACTIVATIONS[activation], _ptr(out),
                           1 if ot == F32 else 0, os_, n, rows, cols, _ptr(status))

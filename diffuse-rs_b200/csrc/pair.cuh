@@ -211,7 +211,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::kThreads)
         uint32_t acc = 0;
         int first = 0;
         for (int kb = 0; kb < p.kblocks; ++kb, ++i) {
-          if (kb == 0 || (C::CHUNK > 0 && kb % C::CHUNK == 0)) {
+          if (kb == 0 || (C::CHUNK > 0 && kb % (C::CHUNK > 0 ? C::CHUNK : 1) == 0)) {
             if (kb > 0) umma_commit_pair(acc_full(n++ & 1));
             if (n >= 2 && !mbar_wait(acc_empty(n & 1), ((n >> 1) - 1) & 1, dead, p.err)) break;
             tc_fence_after();

@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(256) rows_any_kernel(const RowsParams p) {
           if (!p.res_f32) v = __bfloat162float(__float2bfloat16_rn(v));
           store1(sum, p.res_f32, i, v);
         }
-        ss += static_cast<double>(v) * v;
+        ss += static_cast<double>(v * v);
       }
     }
     const void* from = p.res ? sum : x;

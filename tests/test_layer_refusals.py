@@ -114,6 +114,11 @@ F8, F32, I32 = torch.float8_e4m3fn, torch.float32, torch.int32
     lambda: layer.make_gated_linear_args(z(2, 32), z(4, 32), z(4, 32), z(2, 4), activation="relu"),
     lambda: layer.make_gated_linear_args(z(2, 32), z(4, 32), z(4, 32), z(2, 4),
                                          act_scale=z(2, t=F32)),
+    lambda: layer.make_rms_norm_args(z(1, 8).expand(4, 8), z(4, 8)),
+    lambda: layer.make_rms_norm_args(z(4, 8), z(1, 8).expand(4, 8)),
+    lambda: layer.make_linear_q8_args(z(1, 32, t=F8).expand(2, 32), None, z(4, 32, t=F8), None,
+                                      z(2, 4)),
+    lambda: dn.make_sample_args(z(1, 9).expand(2, 9), None, z(2, t=F32), z(2, t=I32)),
     lambda: dn.make_sample_args(z(2, 9, t=torch.float16), None, z(2, t=F32), z(2, t=I32)),
     lambda: dn.make_sample_args(z(2, 9), None, z(3, t=F32), z(2, t=I32)),
     lambda: dn.make_sample_args(z(2, 9), None, z(3, t=F32), z(3, t=I32)),
