@@ -117,6 +117,7 @@ struct SampleShared {
   u64 cta_sum[2][8], cta_second[2][8];  // of every rank
   uint32_t found[2], first_found[2][8];
   float max_v[kSampleWarps], cta_max[8];
+  uint32_t cta_cut[8];
   u64 equal_before[kSampleWarps];       // bf16: entries of the border's value
   uint32_t equal[kSampleWarps];
   double warp_d[kSampleWarps];
@@ -232,16 +233,29 @@ struct SampleRow {
     return all;
   }
 
-  // This warp's part of the sum of q(value, index).
+  // exp(l - m) in fp32 (NaN as far below the maximum as counts for nothing).
+  __device__ __forceinline__ static float term(float l, float m) {
+    return ex2_approx(fmaxf(l - m, -200.f) * 1.4426950408889634f);
+  }
+  // A thread's sum of them as a warp's, in steps of 2^-40.
+  __device__ __forceinline__ static u64 terms_total(float s) {
+    return warp_total(static_cast<u64>(static_cast<double>(s) * 0x1p40));
+  }
+
+  // This warp's part of the sum of q(value, index); `terms`, if given: that of
+  // exp(value - m).
   template <class Q>
-  __device__ __forceinline__ u64 part(Q q) {
+  __device__ __forceinline__ u64 part(Q q, float m = 0.f, u64* terms = nullptr) {
     u64 s = 0;
+    float e = 0.f;
     for (int i = lo + 4 * lane; i < hi; i += 128) {
       float v[4];
       load4(i, v);
 #pragma unroll
       for (int j = 0; j < 4; ++j) s += q(v[j], first + i + j);
+      if (terms) e += (term(v[0], m) + term(v[1], m)) + (term(v[2], m) + term(v[3], m));
     }
+    if (terms) *terms = terms_total(e);
     return warp_total(s);
   }
   template <class Q>
@@ -417,6 +431,40 @@ struct SampleRow {
       return __uint_as_float(static_cast<uint32_t>(seg[i]) << 16);
   }
 
+  // The first k (k < n <= kSampleThreads) of the n entries in this CTA's list,
+  // whose keys lie between low and high, in the order of their indices again.
+  // An entry a thread: a barrier counts.
+  __device__ __forceinline__ void narrow(int n, int k, uint32_t low, uint32_t high) {
+    const int tid = threadIdx.x;
+    const uint32_t key = tid < n ? list_key[tid] : 0, idx = tid < n ? list_idx[tid] : 0;
+    const int bits = low == high ? 0 : 32 - __clz(low ^ high);
+    uint32_t K = bits == 32 ? 0 : high >> bits << bits;
+#pragma unroll 1
+    for (int b = bits - 1; b >= 0; --b) {
+      const uint32_t t = K | (1u << b);
+      if (__syncthreads_count(key >= t) >= k) K = t;
+    }
+    const int room = k - __syncthreads_count(key > K);  // for those of key K
+    const uint32_t lower = (1u << lane) - 1;
+    const uint32_t same = __ballot_sync(0xffffffffu, tid < n && key == K);
+    if (lane == 0) sh->warp_u[warp] = __popc(same);
+    __syncthreads();
+    int at = __popc(same & lower);
+    for (int w = 0; w < warp; ++w) at += sh->warp_u[w];
+    const bool keep = tid < n && (key > K || (key == K && at < room));
+    const uint32_t kept = __ballot_sync(0xffffffffu, keep);
+    __syncthreads();
+    if (lane == 0) sh->warp_u[warp] = __popc(kept);
+    __syncthreads();
+    at = __popc(kept & lower);
+    for (int w = 0; w < warp; ++w) at += sh->warp_u[w];
+    if (keep) {
+      list_key[at] = key;
+      list_idx[at] = idx;
+    }
+    __syncthreads();
+  }
+
   // bf16: the place of a value among kValues, by its 15 low bits less those of
   // the smallest counted magnitude (below 0: next to zero; from kSide on: too
   // far down to count).
@@ -425,19 +473,22 @@ struct SampleRow {
   }
 
   // The entries that `in` holds for, in the order of their indices, into the
-  // first CTA's list (at most kList of them).
+  // first CTA's list (at most kList of them; none if there are more).
   template <class P>
-  __device__ __forceinline__ int collect(P in) {
-    u64 n = 0;
+  __device__ __forceinline__ int collect(P in, float m = 0.f, u64* terms = nullptr) {
+    uint32_t mine = 0;
+    float e = 0.f;
     for (int i = lo + 4 * lane; i < hi; i += 128) {
       float v[4];
       load4(i, v);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) n += in(v[j]) ? 1 : 0;
+      for (int j = 0; j < 4; ++j) mine += in(v[j]) ? 1 : 0;
+      if (terms) e += (term(v[0], m) + term(v[1], m)) + (term(v[2], m) + term(v[3], m));
     }
-    n = warp_total(n);
+    if (terms) *terms = terms_total(e);
+    const u64 n = __reduce_add_sync(0xffffffffu, mine);
     u64 before;
-    const int all = static_cast<int>(gather(n, before));
+    const int all = static_cast<int>(gather(n, before, terms));
     u64 at = before;
     for (int w = 0; w < warp; ++w) at += sh->warp_sum[w];
     if (n > 0 && all <= kList) {
@@ -677,6 +728,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
     }
     m = fmaxf(__uint_as_float(mm << 16), __uint_as_float(mm & 0xffff0000u));
   }
+  float own_max = m;  // over this thread's share of the segment
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (row.lane == 0) sh.max_v[row.warp] = m;
@@ -705,6 +757,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
         seg[i] = seg[i] == 0x7f80 ? 0 : 0xff80;
     }
     m = 0.f;
+    own_max = own_max == INFINITY ? 0.f : -INFINITY;
     __syncthreads();
   }
 
@@ -750,8 +803,115 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
       };
       const bool by_k = top_k > 0 && top_k < p.n_vocab, by_p = top_p < 1.f;
       bool done = false;
+      // The first CTA's list of n entries, by its warps that have any: borders
+      // (of top_k, if `above` entries not listed come before; of top_p, if
+      // entries of weight sure_all do), min_p, and the draw from a list that is
+      // whole.
+      auto settle = [&](int n, bool whole, u64 above, u64 need, u64 sure_all) {
+        if (row.rank == 0 && row.warp * 32 * kListEach < max(n, 1)) {
+          SampleList ls;
+          ls.sh = &sh;
+          ls.lane = row.lane;
+          ls.warp = row.warp;
+          ls.warps = (max(n, 1) + 32 * kListEach - 1) / (32 * kListEach);
+          u64 e[kListEach];
+#pragma unroll
+          for (int j = 0; j < kListEach; ++j) {
+            const int i = tid * kListEach + j;
+            ls.in[j] = i < n;
+            ls.key[j] = i < n ? row.list_key[i] : 0;
+            ls.idx[j] = i < n ? row.list_idx[i] : 0;
+            ls.w[j] = 0;
+            if (i < n) ls.w[j] = fixed44(wt.weight(value_of(ls.key[j])));
+          }
+          if (by_k) {
+            if (above + n > need) {  // otherwise all of them are kept
+#pragma unroll
+              for (int j = 0; j < kListEach; ++j) e[j] = ls.in[j];
+              ls.border(e, need - above, K, I);
+            }
+          }
+          if (by_p) {
+            u64 c = 0;
+#pragma unroll
+            for (int j = 0; j < kListEach; ++j) c += e[j] = ls.in[j] ? ls.w[j] : 0;
+            const u64 here = ls.sum(c);
+            if (by_k) need = need_of(top_p, here);
+            if (sure_all + here > need) ls.border(e, need - sure_all, K, I);
+          }
+          // min_p, and the draw: over a whole list in the order of the
+          // indices; doubtful entries join what their warps are sure of.
+          u64 c = 0, low;
+#pragma unroll
+          for (int j = 0; j < kListEach; ++j) {
+            if (ls.in[j] && wt.least > 0.0 && wt.weight(value_of(ls.key[j])) < wt.least)
+              ls.in[j] = false;
+            c += e[j] = ls.in[j] ? ls.w[j] : 0;
+          }
+          if (whole) {
+            const u64 sum = ls.sum(c, &low);
+            const u64 target = share_of(sum);
+#pragma unroll
+            for (int j = 0; j < kListEach; ++j) {
+              if (low <= target && target < low + e[j])
+                for (uint32_t r = 0; r < row.n_ranks; ++r)
+                  st_cluster_u32(map_to_rank(row.smem_addr(&sh.answer), r), ls.idx[j]);
+              low += e[j];
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < kListEach; ++j) {
+              if (e[j]) {
+                const int rank = static_cast<int>(ls.idx[j]) / p.seg;
+                const int w = (static_cast<int>(ls.idx[j]) - rank * p.seg) / share_in(rank);
+                atomicAdd(&sh.range_sum[rank * kSampleWarps + w], e[j]);
+              }
+            }
+          }
+          ls.sync();
+          if (tid < row.n_ranks && !whole) {
+            st_cluster_u32(map_to_rank(row.smem_addr(&sh.border[0]), tid), K);
+            st_cluster_u32(map_to_rank(row.smem_addr(&sh.border[1]), tid), I);
+          }
+        }
+      };
+      // Few entries of top_k: no fewer than top_k entries reach the top_k-th largest
+      // of the threads' maxima in any CTA (to its upper 24 bits), so all that
+      // may be kept is at or above the largest of these; few more if top_k is
+      // well below the number of threads (k of t threads in each of c CTAs leave
+      // at most -c t ln(1 - k / t) entries of a row without order, 1200 at the
+      // limit below).
+      if (by_k && top_k <= kSampleThreads / 2 &&
+          static_cast<uint32_t>(top_k) * row.n_ranks <= 2 * kSampleThreads) {
+        const uint32_t mine = key_of(own_max);
+        uint32_t cut = 0;
+#pragma unroll 1
+        for (int b = 31; b >= 8; --b) {
+          const uint32_t t = cut | (1u << b);
+          if (__syncthreads_count(mine >= t) >= top_k) cut = t;
+        }
+        if (tid < row.n_ranks)
+          st_cluster_u32(map_to_rank(row.smem_addr(&sh.cta_cut[row.rank]), tid), cut);
+        __syncwarp();
+        cluster_sync_all();
+        for (uint32_t r = 0; r < row.n_ranks; ++r) cut = max(cut, sh.cta_cut[r]);
+        const float least = value_of(max(cut, 0x007fffffu));
+        u64 terms = 0;
+        const int n = row.collect([&](float l) { return l >= least && wt.place(l) < kNowhere; }, m,
+                                  p.prob ? &terms : nullptr);
+        one_all = terms;
+        if (n <= kList) {
+          const bool few = n > top_k && n <= kSampleThreads;
+          if (few && row.rank == 0) row.narrow(n, top_k, cut, key_of(m));
+          settle(few ? top_k : n, true, 0, top_k, 0);
+          __syncwarp();
+          cluster_sync_all();
+          token = static_cast<int>(sh.answer);
+          done = true;
+        }
+      }
       if constexpr (sizeof(T) == 2) {
-        if (by_k || by_p) {
+        if (!done && (by_k || by_p)) {
           // What counts lies between m and `far`, for the weights and for prob (whose
           // terms are below 1e-13 from there on); its magnitudes' binades.
           const float far = fmaxf(m - fmaxf(static_cast<float>(46.0 / wt.c), 32.f), -3e38f);
@@ -951,8 +1111,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
         }
       }
       if (!done && (by_k || by_p)) {
-        // The histogram, and where the nucleus is cut from the whole row, its weight.
+        // The histogram, and where the nucleus is cut from the whole row, its
+        // weight; prob's sum on the way.
         u64 s = 0;
+        float terms = 0.f;
+        const bool with_terms = p.prob && !one_all;
         for (int i = row.lo + 4 * row.lane; i < row.hi; i += 128) {
           float v[4];
           row.load4(i, v);
@@ -962,6 +1125,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
             const float at = wt.place(v[j]);
             t[j] = at < kNowhere;
             if (t[j]) atomicAdd(row.hist + wt.bin(at), 1u);
+            if (with_terms) terms += row.term(v[j], m);
           }
           if (!by_k && (t[0] || t[1] || t[2] || t[3])) {
 #pragma unroll
@@ -972,7 +1136,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
           }
         }
         u64 lower;
-        const u64 all = row.gather(row.warp_total(s), lower);  // the histograms are complete
+        u64 second = with_terms ? row.terms_total(terms) : 0;
+        // (The barrier within completes the histograms.)
+        const u64 all = row.gather(row.warp_total(s), lower, with_terms ? &second : nullptr);
+        if (with_terms) one_all = second;
         u64 need = by_k ? static_cast<u64>(top_k) : need_of(top_p, all);
         // The first CTA joins the histograms, finds the bins and tells the others:
         // every CTA reading all of them cost 20 us at 32 rows of 8 CTAs.
@@ -1098,73 +1265,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
             const float at = wt.place(l);
             return at >= from && at <= to;
           });
-          if (row.rank == 0 && row.warp * 32 * kListEach < max(n, 1)) {
-            SampleList ls;
-            ls.sh = &sh;
-            ls.lane = row.lane;
-            ls.warp = row.warp;
-            ls.warps = (max(n, 1) + 32 * kListEach - 1) / (32 * kListEach);
-            u64 e[kListEach];
-#pragma unroll
-            for (int j = 0; j < kListEach; ++j) {
-              const int i = tid * kListEach + j;
-              ls.in[j] = i < n;
-              ls.key[j] = i < n ? row.list_key[i] : 0;
-              ls.idx[j] = i < n ? row.list_idx[i] : 0;
-              ls.w[j] = 0;
-              if (i < n) ls.w[j] = fixed44(wt.weight(value_of(ls.key[j])));
-            }
-            if (by_k) {
-              const u64 above = whole ? 0 : n_lo;
-              if (above + n > need) {  // otherwise all of them are kept
-#pragma unroll
-                for (int j = 0; j < kListEach; ++j) e[j] = ls.in[j];
-                ls.border(e, need - above, K, I);
-              }
-            }
-            if (by_p) {
-              u64 c = 0;
-#pragma unroll
-              for (int j = 0; j < kListEach; ++j) c += e[j] = ls.in[j] ? ls.w[j] : 0;
-              const u64 here = ls.sum(c);
-              if (by_k) need = need_of(top_p, here);
-              if (sure_all + here > need) ls.border(e, need - sure_all, K, I);
-            }
-            // min_p, and the draw: over a whole list in the order of the
-            // indices; doubtful entries join what their warps are sure of.
-            u64 c = 0, low;
-#pragma unroll
-            for (int j = 0; j < kListEach; ++j) {
-              if (ls.in[j] && wt.least > 0.0 && wt.weight(value_of(ls.key[j])) < wt.least)
-                ls.in[j] = false;
-              c += e[j] = ls.in[j] ? ls.w[j] : 0;
-            }
-            if (whole) {
-              const u64 sum = ls.sum(c, &low);
-              const u64 target = share_of(sum);
-#pragma unroll
-              for (int j = 0; j < kListEach; ++j) {
-                if (low <= target && target < low + e[j])
-                  for (uint32_t r = 0; r < row.n_ranks; ++r)
-                    st_cluster_u32(map_to_rank(row.smem_addr(&sh.answer), r), ls.idx[j]);
-                low += e[j];
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < kListEach; ++j) {
-                if (e[j]) {
-                  const int rank = static_cast<int>(ls.idx[j]) / p.seg;
-                  const int w = (static_cast<int>(ls.idx[j]) - rank * p.seg) / share_in(rank);
-                  atomicAdd(&sh.range_sum[rank * kSampleWarps + w], e[j]);
-                }
-              }
-            }
-            ls.sync();
-            if (tid < row.n_ranks && !whole) {
-              st_cluster_u32(map_to_rank(row.smem_addr(&sh.border[0]), tid), K);
-              st_cluster_u32(map_to_rank(row.smem_addr(&sh.border[1]), tid), I);
-            }
-          }
+          settle(n, whole, whole ? 0 : n_lo, need, sure_all);
           __syncwarp();
           cluster_sync_all();
           if (whole) {
@@ -1218,27 +1319,23 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
         if (by_k || by_p)
           token = row.find(
               [&](float l, int i) -> u64 { return before(l, i) ? kept_weight(l) : 0; }, share_of);
-        else
-          token = row.find([&](float l, int) -> u64 { return kept_weight(l); }, share_of);
+        else {
+          auto q = [&](float l, int) -> u64 { return kept_weight(l); };
+          u64 terms = 0, lower;
+          const u64 mine = row.part(q, m, p.prob ? &terms : nullptr);
+          const u64 all = row.gather(mine, lower, p.prob ? &terms : nullptr);
+          one_all = terms;
+          token = row.find(q, share_of(all), lower);
+        }
       }
     }
   }
   if (p.prob) {
     if (m != -INFINITY) {
-      // exp(l - m) in fp32, sums of a thread's few entries too.
-      auto e = [&](float l) {  // (NaN: as far below the maximum as counts)
-        return l == m ? 1.f : ex2_approx(fmaxf(l - m, -200.f) * 1.4426950408889634f);
-      };
       if (!one_all) {
-        float s = 0.f;
-        for (int i = row.lo + 4 * row.lane; i < row.hi; i += 128) {
-          float v[4];
-          row.load4(i, v);
-          s += (e(v[0]) + e(v[1])) + (e(v[2]) + e(v[3]));
-        }
-        u64 before;
-        one_all = row.gather(
-            row.warp_total(static_cast<u64>(static_cast<double>(s) * 0x1p40)), before);
+        u64 terms, before;
+        row.part([](float, int) -> u64 { return 0; }, m, &terms);
+        one_all = row.gather(terms, before);
       }
       const int i = token - row.first;
       if (i >= 0 && i < len && tid == 0) {

@@ -261,3 +261,19 @@ def test_bf16_borders_next_to_zero(kw):
     x[2] = x[2] * 1e-30
     x[3] = x[3] * 1e-3 + 200.0
     check(x.to(torch.bfloat16), us(24, 4), **kw)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("k", [2, 7, 128, 129, 256, 257])
+def test_small_top_k(kind, k):
+    # Rows whose largest entries stand in one place, are equal, or are fewer
+    # than k; and rows without any order.
+    x = logits_of(25, 5, 40000, kind).float()
+    x[0, 10000:10000 + k] += 30.0
+    x[1] = 0.0
+    x[1, 5::2000] = 9.0
+    x[2, 3:] = -float("inf")
+    x[3] = torch.arange(40000) * 1e-3
+    x = x.to(torch.bfloat16) if kind == "bf16" else x
+    check(x, us(26, 5), top_k=k)
+    check(x, us(27, 5), top_k=k, top_p=0.8003, temperature=0.7)
