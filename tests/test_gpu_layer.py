@@ -136,6 +136,21 @@ def test_norm_of_unusual_values():
     assert torch.isnan(y[1, 3]) and (y[1, :3] == 0).all()
 
 
+def test_quantisation_of_rows_with_infinities():
+    # Every other row has infinities, at widths of one and of several warps.
+    for cols in (64, 1000, 4096, 9000):
+        x = torch.randn(50, cols, generator=gen(cols))
+        x[::2, 5] = float("inf")
+        x[::4, cols - 1] = -float("inf")
+        x[8] = float("inf")
+        sc = torch.zeros(50, device="cuda")
+        out = torch.zeros(50, cols, device="cuda").to(F8)
+        layer.quantize_rows(x.cuda(), out, sc)
+        q, s = quantise_ref(x.double())
+        assert torch.equal(sc.cpu().double(), s)
+        assert torch.equal(out.cpu().float().double(), q)
+
+
 def test_norm_of_no_rows():
     x = torch.zeros(0, 64, device="cuda")
     layer.rms_norm(x, torch.zeros(0, 64, device="cuda"))
