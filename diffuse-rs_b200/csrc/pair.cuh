@@ -274,10 +274,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::kThreads)
           st_shared_f32(sa_at + 4 * j, t0 + j < p.n ? p.act_scale[t0 + j] : 1.f);
         __syncwarp();
       }
-      float next[16];  // residuals of the sixteen tokens to come
-      if (C::G == 1 && p.residual) load_residual(p, next, t0, r, tokens_in<16>(p, t0, ok));
-      // Sixteen tokens from t0 + j0 on.
-      auto finish = [&](float (&d)[16], int j0) {
+      // Residuals of the 32 tokens to come; the first ones are asked for before
+      // the tile is there.
+      float next[2][16];
+      auto ask = [&](int j0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          load_residual(p, next[h], t0 + j0 + 16 * h, r, tokens_in<16>(p, t0 + j0 + 16 * h, ok));
+      };
+      if (C::G == 1 && p.residual) ask(0);
+      // Sixteen tokens from t0 + j0 on, `h`: the second of 32.
+      auto finish = [&](float (&d)[16], int j0, int h) {
         if (p.act_scale) {
 #pragma unroll
           for (int j = 0; j < 16; j += 4) {
@@ -312,9 +319,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::kThreads)
           for (int j = 0; j < 16; ++j) d[j] = fmaf(d[j], w0, bias);
           if (p.residual) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) d[j] += next[j];
-            const long long t = t0 + j0 + 16;
-            if (j0 + 16 < C::kHalf) load_residual(p, next, t, r, tokens_in<16>(p, t, ok));
+            for (int j = 0; j < 16; ++j) d[j] += next[h][j];
+            if (h == 1 && j0 + 16 < C::kHalf) ask(j0 + 16);
           }
           store_tokens(p, d, t0 + j0, r, tokens_in<16>(p, t0 + j0, ok));
         }
@@ -336,18 +342,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::kThreads)
           give();
         }
 #pragma unroll
-        for (int j0 = 0; j0 < C::kHalf; j0 += 16) finish(v[j0 / 16], j0);
+        for (int j0 = 0; j0 < C::kHalf; j0 += 16) finish(v[j0 / 16], j0, j0 / 16 & 1);
       } else {
         const uint32_t col = take();
 #pragma unroll 1
-        for (int j0 = 0; j0 < C::kHalf; j0 += 16) {
-          uint32_t d[16];
-          tmem_ld16(col + j0, d);
-          tmem_wait_ld();
-          float v[16];
+        for (int j0 = 0; j0 < C::kHalf; j0 += 32) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(d[j]);
-          finish(v, j0);
+          for (int h = 0; h < 2; ++h) {
+            uint32_t d[16];
+            tmem_ld16(col + j0 + 16 * h, d);
+            tmem_wait_ld();
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(d[j]);
+            finish(v, j0 + 16 * h, h);
+          }
         }
         give();
       }

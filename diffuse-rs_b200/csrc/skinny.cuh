@@ -94,18 +94,24 @@ __device__ __forceinline__ int tokens_in(const LinearParams& p, long long t, boo
   return ok ? static_cast<int>(max(0ll, min(static_cast<long long>(N), p.n - t))) : 0;
 }
 
-// The residual's element r of the first m of N tokens from t on.
+// The residual's element r of the first m of N tokens from t on. Loads without
+// conditions (tokens behind the m-th read the m-th's), so that all N are on
+// their way before the first is waited for.
 template <int N>
 __device__ __forceinline__ void load_residual(const LinearParams& p, float (&x)[N], long long t,
                                               long long r, int m) {
+  if (m <= 0) return;
   if (p.out_f32) {
     const float* s = static_cast<const float*>(p.residual) + t * p.res_stride + r;
 #pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = j < m ? s[j * p.res_stride] : 0.f;
+    for (int j = 0; j < N; ++j) x[j] = s[min(j, m - 1) * p.res_stride];
   } else {
-    const __nv_bfloat16* s = static_cast<const __nv_bfloat16*>(p.residual) + t * p.res_stride + r;
+    const uint16_t* s = static_cast<const uint16_t*>(p.residual) + t * p.res_stride + r;
+    uint16_t raw[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = j < m ? __bfloat162float(s[j * p.res_stride]) : 0.f;
+    for (int j = 0; j < N; ++j) raw[j] = s[min(j, m - 1) * p.res_stride];
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = __uint_as_float(static_cast<uint32_t>(raw[j]) << 16);
   }
 }
 
