@@ -227,24 +227,34 @@ int launch_pair(const Product& q, cudaStream_t st) {
   return launch_after(pair_kernel<C>, dim3(2 * pairs), C::kThreads, C::kSmem, st, tw, tu, tx, p);
 }
 
+// Few tokens, or few enough tiles that single CTAs of 128 rows by 64 tokens get
+// through them at once (two on an SM; the gated form's, which hold two matrices,
+// one on every other SM) where pairs of SMs would leave some idle or pay their
+// longer way for little: us, single CTAs and pairs, in e4m3: 128 tokens 4096 ->
+// 4096 13.5 and 17.1, 512 tokens 16.0 and 18.1, 768 tokens (384 tiles) 28.6 and
+// 21.9; 443 tokens 3584 -> 4608 14.0 and 15.9; 512 tokens 12288 -> 4096 34.9 and
+// 40.0; gated in bf16 128 tokens 4096 -> 4096 20.5 and 28.1, 256 tokens (128
+// tiles) 31.7 and 28.6.
 template <int KIND, int G>
 int launch_product(const Product& q, cudaStream_t st) {
-  if (q.p.n > 64) {
-    // 16 pieces of 64 bf16 are 64 additions to an accumulator.
-    if (KIND == kKindBf16 && q.p.out_f32) return launch_pair<KIND, G, 128, 16>(q, st);
-    // Tiles of 128 tokens where they take fewer rounds of the pairs: one costs
-    // about 0.6 of a tile of 256 (its operands' way out of shared memory is the
-    // bound).
-    const int64_t rt = (q.p.rows + 256 / G - 1) / (256 / G);
-    auto rounds = [&](int64_t nt) {
-      return (rt * ((q.p.n + nt - 1) / nt) + kSms / 2 - 1) / (kSms / 2);
-    };
-    if (6 * rounds(128) < 10 * rounds(256)) return launch_pair<KIND, G, 128>(q, st);
-    return launch_pair<KIND, G, 256>(q, st);
+  const int64_t tiles = (q.p.rows + 127) / 128 * ((q.p.n + 63) / 64);
+  if (q.p.n <= 64 || tiles <= (G == 1 ? 2 * kSms : kSms / 2)) {
+    if (q.p.n <= 16) return launch_skinny<KIND, G, 16>(q, st);
+    if (q.p.n <= 32) return launch_skinny<KIND, G, 32>(q, st);
+    return launch_skinny<KIND, G, 64>(q, st);
   }
-  if (q.p.n <= 16) return launch_skinny<KIND, G, 16>(q, st);
-  if (q.p.n <= 32) return launch_skinny<KIND, G, 32>(q, st);
-  return launch_skinny<KIND, G, 64>(q, st);
+  // 16 pieces of 64 bf16 are 64 additions to an accumulator.
+  if (KIND == kKindBf16 && q.p.out_f32) return launch_pair<KIND, G, 128, 16>(q, st);
+  // A tile of 128 tokens takes a pair about as long as one of 256 (0.31 us a
+  // piece alone: the weights' way into shared memory is the bound), so that it
+  // pays only where there are no more rounds of them: 1536 tokens 4096 -> 4096 in
+  // three rounds 40 us, in two of 256 tokens 30.
+  const int64_t rt = (q.p.rows + 256 / G - 1) / (256 / G);
+  auto rounds = [&](int64_t nt) {
+    return (rt * ((q.p.n + nt - 1) / nt) + kSms / 2 - 1) / (kSms / 2);
+  };
+  if (rounds(128) <= rounds(256)) return launch_pair<KIND, G, 128>(q, st);
+  return launch_pair<KIND, G, 256>(q, st);
 }
 
 // Shapes, strides and alignment of a product; es: bytes of an operand's element.
