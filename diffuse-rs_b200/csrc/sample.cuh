@@ -1141,129 +1141,195 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
         const u64 all = row.gather(row.warp_total(s), lower, with_terms ? &second : nullptr);
         if (with_terms) one_all = second;
         u64 need = by_k ? static_cast<u64>(top_k) : need_of(top_p, all);
-        // The first CTA joins the histograms, finds the bins and tells the others:
-        // every CTA reading all of them cost 20 us at 32 rows of 8 CTAs.
-        if (row.rank == 0) {
-          // Bins kBinsEach tid and on of the whole row, and what is before them.
-          uint32_t own[kBinsEach];
+        // What the histograms say of the border: the first bin that is not before it
+        // for certain and the last that is not behind it for certain, and how many
+        // entries come before these two's ends. Bin i holds weights within a factor
+        // `more` of 2^-(x0 + i step); entries of weight sure_w, sure_n of them, come
+        // before the first bin; total_w: what all entries weigh, the histogram's
+        // among them (0: not known). The first CTA joins the histograms and tells
+        // the others: every CTA reading all of them cost 20 us at 32 rows of 8 CTAs.
+        struct Bins {
+          int lo, hi;
+          uint32_t n_lo, n_hi;
+        };
+        auto locate = [&](double sure_w, uint32_t sure_n, double total_w, float x0, float step,
+                          double more) -> Bins {
+          if (row.rank == 0) {
+            // Bins kBinsEach tid and on of the whole row, and what is before them.
+            uint32_t own[kBinsEach];
 #pragma unroll
-          for (int h = 0; h < kBinsEach; ++h) own[h] = 0;
-          if (tid < kBins / kBinsEach) {
+            for (int h = 0; h < kBinsEach; ++h) own[h] = 0;
+            if (tid < kBins / kBinsEach) {
 #pragma unroll 4
-            for (uint32_t r = 0; r < row.n_ranks; ++r) {
-              uint32_t a[4];
-              asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
-                           : "r"(map_to_rank(row.smem_addr(row.hist), r) + 4 * kBinsEach * tid)
-                           : "memory");
+              for (uint32_t r = 0; r < row.n_ranks; ++r) {
+                uint32_t a[4];
+                asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
+                             : "r"(map_to_rank(row.smem_addr(row.hist), r) + 4 * kBinsEach * tid)
+                             : "memory");
 #pragma unroll
-              for (int h = 0; h < kBinsEach; ++h) own[h] += a[h];
-            }
-          }
-          if (tid == 0) {
-            sh.bin_lo = kBins;
-            sh.bin_hi = 0;
-            sh.n_lo = sh.n_hi = 0;
-          }
-          double q = 0.0, own_q[kBinsEach];
-          uint32_t n = 0;
-#pragma unroll
-          for (int h = 0; h < kBinsEach; ++h) {
-            own_q[h] = static_cast<double>(
-                           exp2f(static_cast<float>(kBinsEach * tid + h) / -kBinsPerOctave)) *
-                       own[h];
-            q += own_q[h];
-            n += own[h];
-          }
-          double before_q = q;
-          uint32_t before_n = n;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double tq = __shfl_up_sync(0xffffffffu, before_q, o);
-            const uint32_t tn = __shfl_up_sync(0xffffffffu, before_n, o);
-            if (row.lane >= o) {
-              before_q += tq;
-              before_n += tn;
-            }
-          }
-          if (row.lane == 31) {
-            sh.warp_d[row.warp] = before_q;
-            sh.warp_u[row.warp] = before_n;
-          }
-          __syncthreads();
-          before_q -= q;
-          before_n -= n;
-          double base_q = 0.0;
-#pragma unroll
-          for (int w = 0; w < kSampleWarps; ++w) {
-            if (w < row.warp) {
-              before_q += sh.warp_d[w];
-              before_n += sh.warp_u[w];
-            }
-            base_q += sh.warp_d[w];
-          }
-          // Whether a bin is before the border for certain, or behind it.
-          const double total_w = static_cast<double>(all) * 0x1p-44;
-          const double need_w = static_cast<double>(need) * 0x1p-44;
-          const double more = 1.0111, less = 1.0 / 1.0111;  // 2^(1/64), and roundings
-#pragma unroll
-          for (int h = 0; h < kBinsEach; ++h) {
-            const uint32_t bin = kBinsEach * tid + h;
-            const uint32_t upto_n = before_n + own[h];
-            const double upto_q = before_q + own_q[h];
-            if (own[h]) {
-              bool sure, behind;
-              if (by_k) {
-                sure = upto_n <= need;
-                behind = before_n >= need;
-              } else {
-                sure = fmin(upto_q * more, total_w - (base_q - upto_q) * less) < need_w * (1 - 1e-6);
-                behind =
-                    fmax(before_q * less, total_w - (base_q - before_q) * more) > need_w * (1 + 1e-6);
+                for (int h = 0; h < kBinsEach; ++h) own[h] += a[h];
               }
-              if (!sure) atomicMin(&sh.bin_lo, bin);
-              if (!behind) {
-                atomicMax(&sh.bin_hi, bin);
-                atomicMax(&sh.n_hi, upto_n);
-              }
-              if (sure) atomicMax(&sh.n_lo, upto_n);
             }
-            before_n = upto_n;
-            before_q = upto_q;
+            if (tid == 0) {
+              sh.bin_lo = kBins;
+              sh.bin_hi = 0;
+              sh.n_lo = sure_n;
+              sh.n_hi = sure_n;
+            }
+            double q = 0.0, own_q[kBinsEach];
+            uint32_t n = 0;
+#pragma unroll
+            for (int h = 0; h < kBinsEach; ++h) {
+              own_q[h] = static_cast<double>(exp2f(
+                             -fmaf(static_cast<float>(kBinsEach * tid + h), step, x0))) *
+                         own[h];
+              q += own_q[h];
+              n += own[h];
+            }
+            double before_q = q;
+            uint32_t before_n = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const double tq = __shfl_up_sync(0xffffffffu, before_q, o);
+              const uint32_t tn = __shfl_up_sync(0xffffffffu, before_n, o);
+              if (row.lane >= o) {
+                before_q += tq;
+                before_n += tn;
+              }
+            }
+            if (row.lane == 31) {
+              sh.warp_d[row.warp] = before_q;
+              sh.warp_u[row.warp] = before_n;
+            }
+            __syncthreads();
+            before_q -= q;
+            before_n += sure_n - n;
+            double base_q = 0.0;
+#pragma unroll
+            for (int w = 0; w < kSampleWarps; ++w) {
+              if (w < row.warp) {
+                before_q += sh.warp_d[w];
+                before_n += sh.warp_u[w];
+              }
+              base_q += sh.warp_d[w];
+            }
+            const double need_w = static_cast<double>(need) * 0x1p-44, less = 1.0 / more;
+#pragma unroll
+            for (int h = 0; h < kBinsEach; ++h) {
+              const uint32_t bin = kBinsEach * tid + h;
+              const uint32_t upto_n = before_n + own[h];
+              const double upto_q = before_q + own_q[h];
+              if (own[h]) {
+                bool sure, behind;
+                if (by_k) {
+                  sure = upto_n <= need;
+                  behind = before_n >= need;
+                } else {
+                  double most = sure_w + upto_q * more, fewest = sure_w + before_q * less;
+                  if (total_w > 0.0) {
+                    most = fmin(most, total_w - (base_q - upto_q) * less);
+                    fewest = fmax(fewest, total_w - (base_q - before_q) * more);
+                  }
+                  sure = most < need_w * (1 - 1e-9);
+                  behind = fewest > need_w * (1 + 1e-9);
+                }
+                if (!sure) atomicMin(&sh.bin_lo, bin);
+                if (!behind) {
+                  atomicMax(&sh.bin_hi, bin);
+                  atomicMax(&sh.n_hi, upto_n);
+                }
+                if (sure) atomicMax(&sh.n_lo, upto_n);
+              }
+              before_n = upto_n;
+              before_q = upto_q;
+            }
+            __syncthreads();
+            if (tid < 4 * row.n_ranks) {
+              const uint32_t* from = tid & 2 ? (tid & 1 ? &sh.n_hi : &sh.n_lo)
+                                             : (tid & 1 ? &sh.bin_hi : &sh.bin_lo);
+              st_cluster_u32(map_to_rank(row.smem_addr(&sh.told[tid & 3]), tid >> 2), *from);
+            }
           }
-          __syncthreads();
-          if (tid < 4 * row.n_ranks) {
-            const uint32_t* from = tid & 2 ? (tid & 1 ? &sh.n_hi : &sh.n_lo)
-                                           : (tid & 1 ? &sh.bin_hi : &sh.bin_lo);
-            st_cluster_u32(map_to_rank(row.smem_addr(&sh.told[tid & 3]), tid >> 2), *from);
-          }
-        }
-        __syncwarp();
-        cluster_sync_all();
-        const int b_lo = static_cast<int>(sh.told[0]), b_hi = static_cast<int>(sh.told[1]);
-        const uint32_t n_lo = sh.told[2], n_hi = sh.told[3];
+          __syncwarp();
+          cluster_sync_all();
+          return Bins{static_cast<int>(sh.told[0]), static_cast<int>(sh.told[1]), sh.told[2],
+                      sh.told[3]};
+        };
+        const Bins bins = locate(0.0, 0, static_cast<double>(all) * 0x1p-44, 0.f,
+                                 1.f / kBinsPerOctave, 1.0111);  // 2^(1/64), and roundings
+        const int b_lo = bins.lo, b_hi = bins.hi;
+        uint32_t n_lo = bins.n_lo, n_hi = bins.n_hi;
         // A list of every entry up to the last bin that may be kept, or of the
-        // doubtful bins; sums of whole rows otherwise.
+        // doubtful ones, found with a finer histogram of their bins where they are
+        // too many; sums of whole rows otherwise.
         const bool whole = n_hi <= kList;
-        const bool doubt = !whole && n_hi - n_lo <= kList && !(by_k && by_p) && b_lo <= b_hi;
+        bool doubt = !whole && !(by_k && by_p) && b_lo <= b_hi;
         const bool thin = by_p && wt.least > 0.0;  // min_p thins out a wide nucleus
         u64 sure_all = 0, mine = 0;
+        float fine_c = 0.f, fine_0 = 0.f;  // place in the finer one
+        float fine_lo = -INFINITY, fine_hi = INFINITY;
+        auto fine = [&](float l) { return fmaf(l - m, -fine_c, fine_0); };
+        auto kept_for_sure = [&](float l) -> u64 {
+          const double w = wt.weight(l);
+          return by_k && w < wt.least ? 0 : fixed44(w);  // the nucleus is cut first
+        };
         if (doubt) {  // what is before the border for certain
           const float below = 8388608.f + static_cast<float>(b_lo);  // whole numbers, exact
-          mine = row.part_of(
-              [&](float l) { return wt.place(l) < below; },
-              [&](float l) -> u64 {
-                const double w = wt.weight(l);
-                return by_k && w < wt.least ? 0 : fixed44(w);  // the nucleus is cut first
-              });
+          mine = row.part_of([&](float l) { return wt.place(l) < below; }, kept_for_sure);
           sure_all = row.gather(mine, lower);
+          if (n_hi - n_lo > kList && (b_hi - b_lo + 1) * 2 >= kBins) {
+            doubt = false;
+          } else if (n_hi - n_lo > kList) {
+            int R = 2;  // bins of one: as many as there are room for
+            while ((b_hi - b_lo + 1) * 2 * R < kBins) R *= 2;
+            fine_c = wt.bin_c * static_cast<float>(R);
+            fine_0 = 8388608.f - static_cast<float>(b_lo * R - R / 2);
+            const float to = 8388608.f + static_cast<float>(b_hi);
+            for (int i = tid; i < kBins; i += kSampleThreads) row.hist[i] = 0;
+            __syncthreads();
+            for (int i = row.lo + 4 * row.lane; i < row.hi; i += 128) {
+              float v[4];
+              row.load4(i, v);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float at = wt.place(v[j]);
+                if (at >= below && at <= to)
+                  atomicAdd(row.hist + min(wt.bin(fmaxf(fine(v[j]), 8388608.f)),
+                                           static_cast<uint32_t>(kBins - 1)), 1u);
+              }
+            }
+            __syncwarp();
+            cluster_sync_all();
+            const float step = 1.f / (kBinsPerOctave * static_cast<float>(R));
+            // (Weights of a nucleus' sure entries are whole here: by_k has no need of them.)
+            const Bins f = locate(by_k ? 0.0 : static_cast<double>(sure_all) * 0x1p-44, n_lo, 0.0,
+                                  static_cast<float>(b_lo * R - R / 2) * step, step,
+                                  (1.0 + 0.35 * step) * (1.0 + 1e-5));
+            n_lo = f.n_lo;
+            n_hi = f.n_hi;
+            fine_lo = 8388608.f + static_cast<float>(f.lo);
+            fine_hi = f.hi == kBins - 1 ? INFINITY : 8388608.f + static_cast<float>(f.hi);
+            doubt = f.lo <= f.hi && n_hi - n_lo <= kList;
+            if (doubt) {
+              mine += row.part_of(
+                  [&](float l) {
+                    const float at = wt.place(l);
+                    return at >= below && at <= to && fmaxf(fine(l), 8388608.f) < fine_lo;
+                  },
+                  kept_for_sure);
+              sure_all = row.gather(mine, lower);
+            }
+          }
         }
         if (whole || doubt) {
           const float from = 8388608.f + static_cast<float>(whole ? 0 : b_lo);
           const float to = 8388608.f + static_cast<float>(b_hi);
           const int n = row.collect([&](float l) {
             const float at = wt.place(l);
-            return at >= from && at <= to;
+            if (!(at >= from && at <= to)) return false;
+            const float x = fmaxf(fine(l), 8388608.f);
+            return x >= fine_lo && x <= fine_hi;
           });
           settle(n, whole, whole ? 0 : n_lo, need, sure_all);
           __syncwarp();

@@ -277,3 +277,15 @@ def test_small_top_k(kind, k):
     x = x.to(torch.bfloat16) if kind == "bf16" else x
     check(x, us(26, 5), top_k=k)
     check(x, us(27, 5), top_k=k, top_p=0.8003, temperature=0.7)
+
+
+@pytest.mark.parametrize("kw", [dict(top_p=0.9), dict(top_p=0.9, temperature=1.5),
+                                dict(top_p=0.3, min_p=0.4), dict(top_k=5000),
+                                dict(top_k=100000, min_p=0.31), dict(top_p=0.999),
+                                dict(top_p=1e-4)])
+def test_flat_rows_of_large_vocabularies(kw):
+    # Thousands of entries in the border's bin of the first histogram.
+    x = logits_of(28, 3, 250000, scale=0.2)
+    x[1] *= 1e-3
+    x[2, :1000] += 2.0
+    check(x, us(29, 3), **kw)
