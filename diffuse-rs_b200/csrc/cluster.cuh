@@ -22,23 +22,31 @@ __device__ __forceinline__ void cluster_sync_all() {
       "barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
           : "memory");
 }
-// Its two halves: a thread that has arrived may go on until it waits.
-__device__ __forceinline__ void cluster_arrive() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-}
+// The wait of a barrier whose arrival is a call of its own.
 __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// An arrival that orders no memory: it says that the CTA has started, which has
+// to be known before its shared memory is written from another. (With the
+// release of the other form it costs a microsecond at a kernel's start.)
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+// The same as cluster_sync_all with one warp's release for the whole CTA, whose
+// writes the CTA's own barrier puts before it.
+__device__ __forceinline__ void cluster_sync_cta() {
+  __syncthreads();
+  if (threadIdx.x < 32)
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  else
+    cluster_arrive_relaxed();
+  cluster_wait();
 }
 // The address of this CTA's shared `addr` in the CTA of rank `rank`.
 __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
-}
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
 }
 __device__ __forceinline__ unsigned long long ld_cluster_u64(uint32_t addr) {
   unsigned long long v;

@@ -169,16 +169,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::kThreads)
     fence_proxy_async_smem();
   }
   __syncwarp();
-  cluster_sync_all();   // the barriers of both are set
+  cluster_arrive_relaxed();  // (the barriers' initialisation has a fence of its own)
+  cluster_wait();            // the barriers of both are set
   wait_prior_kernel();  // before TMEM is taken, as in skinny.cuh
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot),
                  "r"(C::kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
   }
-  __syncwarp();
   tc_fence_before();
-  cluster_arrive();
+  __syncthreads();
+  cluster_arrive_relaxed();
   if (tid == 0)
     while (filled < C::kStages && tile < tiles) fill();  // the first loads need no TMEM
   __syncwarp();
@@ -370,7 +371,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::kThreads)
                  "r"(C::kTmemCols));
   }
   __syncwarp();
-  cluster_sync_all();
+  cluster_arrive_relaxed();
+  cluster_wait();
 }
 
 }  // namespace ca

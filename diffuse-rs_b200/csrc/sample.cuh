@@ -216,8 +216,7 @@ struct SampleRow {
           st_cluster_u64(map_to_rank(smem_addr(&sh->cta_second[turn][rank]), lane), d);
       }
     }
-    __syncwarp();
-    cluster_sync_all();
+    cluster_sync_cta();
     u64 all = 0, all2 = 0;
     before = 0;
 #pragma unroll
@@ -335,8 +334,7 @@ struct SampleRow {
         }
       }
     }
-    __syncwarp();
-    cluster_sync_all();
+    cluster_sync_cta();
     return static_cast<int>(sh->found[turn]);
   }
   template <class Q, class F>
@@ -369,8 +367,7 @@ struct SampleRow {
       if (lane < n_ranks)
         st_cluster_u32(map_to_rank(smem_addr(&sh->first_found[turn][rank]), lane), best);
     }
-    __syncwarp();
-    cluster_sync_all();
+    cluster_sync_cta();
     best = 0xffffffffu;
     for (uint32_t r = 0; r < n_ranks; ++r) best = min(best, sh->first_found[turn][r]);
     return static_cast<int>(best);
@@ -520,8 +517,7 @@ struct SampleRow {
         at += __shfl_sync(0xffffffffu, up, 31);
       }
     }
-    __syncwarp();
-    cluster_sync_all();
+    cluster_sync_cta();
     return all;
   }
 };
@@ -645,6 +641,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
     }
     return;
   }
+  cluster_arrive_relaxed();  // (waited for before anything is written to another CTA)
   row.seg = seg;
   row.first = static_cast<int>(row.rank) * p.seg;
   auto len_in = [&](int rank) { return max(0, min(p.seg, p.n_vocab - rank * p.seg)); };
@@ -733,6 +730,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (row.lane == 0) sh.max_v[row.warp] = m;
   __syncthreads();
+  cluster_wait();  // every CTA of the cluster has started
   if (row.warp == 0) {
     m = row.lane < kSampleWarps ? sh.max_v[row.lane] : -INFINITY;
 #pragma unroll
@@ -741,8 +739,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
       st_cluster_u32(map_to_rank(row.smem_addr(&sh.cta_max[row.rank]), row.lane),
                      __float_as_uint(m));
   }
-  __syncwarp();
-  cluster_sync_all();
+  cluster_sync_cta();
   m = -INFINITY;
   for (uint32_t r = 0; r < row.n_ranks; ++r) m = fmaxf(m, sh.cta_max[r]);
 
@@ -892,8 +889,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
         }
         if (tid < row.n_ranks)
           st_cluster_u32(map_to_rank(row.smem_addr(&sh.cta_cut[row.rank]), tid), cut);
-        __syncwarp();
-        cluster_sync_all();
+        cluster_sync_cta();
         for (uint32_t r = 0; r < row.n_ranks; ++r) cut = max(cut, sh.cta_cut[r]);
         const float least = value_of(max(cut, 0x007fffffu));
         u64 terms = 0;
@@ -904,8 +900,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
           const bool few = n > top_k && n <= kSampleThreads;
           if (few && row.rank == 0) row.narrow(n, top_k, cut, key_of(m));
           settle(few ? top_k : n, true, 0, top_k, 0);
-          __syncwarp();
-          cluster_sync_all();
+          cluster_sync_cta();
           token = static_cast<int>(sh.answer);
           done = true;
         }
@@ -944,13 +939,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
               }
             }
           }
-          if (tiny_one) {
+          if (tiny_n || tiny_one) {
             atomicAdd(&sh.tiny_one, tiny_one);
             atomicAdd(values + kSide, tiny_n);
             atomicAdd(&sh.tiny_weight, tiny);
           }
-          __syncwarp();
-          cluster_sync_all();
+          cluster_sync_cta();
           // Each CTA takes a share of the values, from the whole row, and of those
           // a thread the `each` from `o0` on.
           const int Q = kValuesEach * kSampleThreads / static_cast<int>(row.n_ranks);
@@ -1054,18 +1048,19 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
             const u64 all = scan(c, low, by_k ? nullptr : &second);
             if (!by_k) one_all = second;
             const u64 need = need_of(top_p, all);
+            // (Where top_k cuts next to zero, what it leaves there is not known.)
+            const bool known = sh.border[2];
 #pragma unroll
             for (int h = 0; h < kValuesEach; ++h) {
               const u64 x = here(h);
-              if (low < need && need <= low + x)
+              if (known && low < need && need <= low + x)
                 tell(value_at(o0 + h),
                      o0 + h == kSide ? 0 : static_cast<uint32_t>((need - low + w[h] - 1) / w[h]),
                      o0 + h != kSide);
               low += x;
             }
           }
-          __syncwarp();
-          cluster_sync_all();
+          cluster_sync_cta();
           if (sh.border[2]) {
             // Kept: what is above the border's value, and the first `count` of it
             // (without a border: every entry that has a weight).
@@ -1251,8 +1246,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
               st_cluster_u32(map_to_rank(row.smem_addr(&sh.told[tid & 3]), tid >> 2), *from);
             }
           }
-          __syncwarp();
-          cluster_sync_all();
+          cluster_sync_cta();
           return Bins{static_cast<int>(sh.told[0]), static_cast<int>(sh.told[1]), sh.told[2],
                       sh.told[3]};
         };
@@ -1299,8 +1293,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
                                            static_cast<uint32_t>(kBins - 1)), 1u);
               }
             }
-            __syncwarp();
-            cluster_sync_all();
+            cluster_sync_cta();
             const float step = 1.f / (kBinsPerOctave * static_cast<float>(R));
             // (Weights of a nucleus' sure entries are whole here: by_k has no need of them.)
             const Bins f = locate(by_k ? 0.0 : static_cast<double>(sure_all) * 0x1p-44, n_lo, 0.0,
@@ -1332,8 +1325,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
             return x >= fine_lo && x <= fine_hi;
           });
           settle(n, whole, whole ? 0 : n_lo, need, sure_all);
-          __syncwarp();
-          cluster_sync_all();
+          cluster_sync_cta();
           if (whole) {
             token = static_cast<int>(sh.answer);
           } else {
@@ -1415,7 +1407,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
     }
   }
   if (tid == 0 && row.rank == 0) p.token[cand] = token;
-  cluster_sync_all();  // no CTA leaves while another reads its shared memory
+  // No CTA leaves while another reads its shared memory (those reads are over).
+  __syncwarp();
+  cluster_arrive_relaxed();
+  cluster_wait();
 }
 
 }  // namespace ca

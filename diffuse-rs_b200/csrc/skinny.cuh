@@ -203,6 +203,8 @@ __global__ void __launch_bounds__(C::kThreads)
     fence_barrier_init();
     fence_proxy_async_smem();
   }
+  __syncwarp();
+  cluster_arrive_relaxed();  // (waited for before anything is written to another CTA)
   // TMEM is taken only once the kernel before is complete, and the next one
   // let in only then: neither can hold columns that the other waits for. The
   // first loads need no TMEM.
@@ -288,6 +290,8 @@ __global__ void __launch_bounds__(C::kThreads)
     __syncwarp();
     tc_fence_after();
   }
+  __syncwarp();
+  cluster_wait();                               // every CTA of the cluster has started
   if (S > 1 && !C::kApart) cluster_sync_all();  // every ring is free
   if (warp >= 2) {
     const uint32_t col = tmem + (static_cast<uint32_t>(warp & 3) << 21);

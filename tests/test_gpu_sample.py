@@ -289,3 +289,17 @@ def test_flat_rows_of_large_vocabularies(kw):
     x[1] *= 1e-3
     x[2, :1000] += 2.0
     check(x, us(29, 3), **kw)
+
+
+def test_bf16_cuts_and_weights_next_to_zero():
+    # top_k ends among tens of thousands of zeros, the nucleus of what it leaves
+    # among the entries above them; and a temperature at which values next to
+    # zero weigh although exp(l - m) of them is nothing.
+    x = torch.zeros(2, 30000)
+    x[0, 7:30000:300] = 3.0
+    x[1, ::2] = 100.0
+    x[1, 1::2] = torch.arange(15000) * 1e-7
+    x = x.to(torch.bfloat16)
+    check(x, [0.3141, 0.2718], top_k=15000, top_p=0.1003)
+    check(x, [0.7141, 0.6718], temperature=50.0, top_p=0.9003)
+    check(x, [0.9141, 0.8718], temperature=50.0, top_k=20000, top_p=0.97)
