@@ -125,6 +125,17 @@ int rms_norm_impl(const ca_rms_norm_args* a, cudaStream_t st) {
   // Registers hold 20480 columns.
   if (vec && p.cols <= 20480)
     return p.x_f32 ? launch_rows_res<true>(p, st) : launch_rows_res<false>(p, st);
+  if (p.cols <= 20480) {
+    auto odd = [&](auto kernel, int n) {
+      const int t = ((p.cols + n - 1) / n + 31) / 32 * 32;
+      const int64_t most = static_cast<int64_t>(kSms) * std::min(32, std::max(1, (n == 4 ? 2048 : 1024) / t));
+      return launch_after(kernel, dim3(static_cast<unsigned>(std::min<int64_t>(p.rows, most))), t,
+                          0, st, p);
+    };
+    if (p.cols <= 4096) return odd(rows_odd_kernel<4>, 4);
+    if (p.cols <= 8192) return odd(rows_odd_kernel<8>, 8);
+    return odd(rows_odd_kernel<20>, 20);
+  }
   return launch_after(rows_any_kernel,
                       dim3(static_cast<unsigned>(std::min<int64_t>(p.rows, 4 * kSms))), 256, 0, st,
                       p);

@@ -283,8 +283,113 @@ __global__ void __launch_bounds__(C >= 3 ? 512 : 1024, C == 3 ? 2 : 1)
   }
 }
 
-// Rows of any alignment, or of more columns than rows_kernel holds: elements
-// one by one, side by side across the threads. Each thread goes back to its
+// The bits of N elements tid, tid + threads, ... of a row of `cols` that lie
+// side by side across the threads; 0 behind its end. As fp32 they are these
+// bits, of bf16 16 places up: a step of its own, so that what several tensors
+// are asked for is on its way before the first is waited for.
+template <int N>
+__device__ __forceinline__ void load_strided(const void* row, int f32, int cols, uint32_t (&v)[N]) {
+  const int tid = threadIdx.x, step = blockDim.x;
+  if (f32) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      v[j] = tid + j * step < cols ? static_cast<const uint32_t*>(row)[tid + j * step] : 0;
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      v[j] = tid + j * step < cols ? static_cast<const uint16_t*>(row)[tid + j * step] : 0;
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_strided(void* row, int f32, int cols, const float (&v)[N]) {
+  const int tid = threadIdx.x, step = blockDim.x;
+  if (f32) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (tid + j * step < cols) static_cast<float*>(row)[tid + j * step] = v[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (tid + j * step < cols)
+        static_cast<__nv_bfloat16*>(row)[tid + j * step] = __float2bfloat16_rn(v[j]);
+  }
+}
+
+// Rows of any alignment, element by element, N a thread (N * blockDim.x >=
+// cols), otherwise as rows_kernel: held in registers between the passes, the
+// gain among them. Several CTAs on an SM hide what a row waits for.
+template <int N>
+__global__ void __launch_bounds__(1024) rows_odd_kernel(const RowsParams p) {
+  __shared__ double red_d[2][32];
+  __shared__ float red[2][32];
+  const int tid = threadIdx.x, step = blockDim.x, cols = p.cols, warps = blockDim.x >> 5;
+  dependency_wait();
+  uint32_t g[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) g[j] = __float_as_uint(1.f);
+  if (p.w) load_strided(p.w, 1, cols, g);
+  const double inv_cols = 1.0 / static_cast<double>(cols);
+  const int x_up = p.x_f32 ? 0 : 16, res_up = p.res_f32 ? 0 : 16;
+  int turn = 0;
+  for (long long r = blockIdx.x; r < p.rows; r += gridDim.x, turn ^= 1) {
+    uint32_t x[N], t[N];
+    load_strided(row_at(p.x, p.x_f32, r * p.x_stride), p.x_f32, cols, x);
+    if (p.res) load_strided(row_at(p.res, p.res_f32, r * p.res_stride), p.res_f32, cols, t);
+    float v[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = __uint_as_float(x[j] << x_up);
+    if (p.res) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        v[j] += __uint_as_float(t[j] << res_up);
+        if (!p.res_f32) v[j] = __bfloat162float(__float2bfloat16_rn(v[j]));
+      }
+      store_strided(row_at(p.sum, p.res_f32, r * p.sum_stride), p.res_f32, cols, v);
+    }
+    float rs = 1.f;
+    if (p.norm) {
+      double d = 0.0;
+#pragma unroll
+      for (int j0 = 0; j0 < N; j0 += 4) {
+        float s = 0.f;
+#pragma unroll
+        for (int j = j0; j < (j0 + 4 < N ? j0 + 4 : N); ++j) s = fmaf(v[j], v[j], s);
+        d += static_cast<double>(s);
+      }
+      rs = inv_root(fma(cta_sum_n(d, red_d[turn], warps), inv_cols, static_cast<double>(p.eps)));
+    }
+    float amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      v[j] = v[j] * rs * __uint_as_float(g[j]);
+      amax = fmaxf(amax, fabsf(v[j]));
+    }
+    if (p.out_type != kOutE4m3) {
+      store_strided(row_at(p.out, p.out_type, r * p.out_stride), p.out_type, cols, v);
+      continue;
+    }
+    amax = cta_max_n(amax, red[turn], warps);
+    if (amax == INFINITY) {  // infinities have no part in the scale
+      amax = 0.f;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (fabsf(v[j]) < INFINITY) amax = fmaxf(amax, fabsf(v[j]));
+      __syncthreads();  // the infinity is read
+      amax = cta_max_n(amax, red[turn], warps);
+    }
+    const int k = e4m3_exp(amax, kKv8MinExp, kKv8MaxExp);
+    const float inv = exp2_int(-k);
+    if (tid == 0) p.out_scale[r] = exp2_int(k);
+    uint8_t* out = static_cast<uint8_t*>(p.out) + r * p.out_stride;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (tid + j * step < cols)
+        out[tid + j * step] = static_cast<uint8_t>(cvt_e4m3x2(v[j] * inv, 0.f));
+  }
+}
+
+// Rows of more columns than registers hold, of any alignment: elements one by
+// one, side by side across the threads. Each thread goes back to its
 // own elements, which it finds in the sum (or in x) as it left them.
 __global__ void __launch_bounds__(256) rows_any_kernel(const RowsParams p) {
   __shared__ double red_d[2][32];
