@@ -281,7 +281,10 @@ int check_product(Product* q, int es, int out_f32) {
       (q->up && !aligned16(q->up)))
     return CA_ERR_INVALID;
   const int os = out_f32 ? 4 : 2;
-  if (!aligned_to(p.out, os) || !aligned_to(p.residual, os)) return CA_ERR_INVALID;
+  if (!aligned_to(p.out, os) || !aligned_to(p.residual, os) || !aligned_to(p.act_scale, 4) ||
+      !aligned_to(p.w_scale, 4) || !aligned_to(p.up_scale, 4) || !aligned_to(p.bias, 4) ||
+      !aligned_to(p.err, 4))
+    return CA_ERR_INVALID;
   if (q->cols * es % 16) return CA_ERR_UNSUPPORTED;
   if (p.n > INT_MAX - 256 || p.rows > INT_MAX - 256 || q->cols > INT_MAX - 256)
     return CA_ERR_UNSUPPORTED;

@@ -47,6 +47,14 @@ int sample_impl(const ca_sample_args* a, cudaStream_t st) {
   if (rs < a->n_vocab) return CA_ERR_INVALID;
   if (!a->rows && a->n_cand > a->n_rows) return CA_ERR_INVALID;
   if (reinterpret_cast<uintptr_t>(a->logits) & (a->logits_bf16 ? 1u : 3u)) return CA_ERR_INVALID;
+  for (const void* q : {static_cast<const void*>(a->rows), static_cast<const void*>(a->suppress),
+                        static_cast<const void*>(a->u), static_cast<const void*>(a->token),
+                        static_cast<const void*>(a->prob),
+                        static_cast<const void*>(a->temperature_row),
+                        static_cast<const void*>(a->top_k_row),
+                        static_cast<const void*>(a->top_p_row),
+                        static_cast<const void*>(a->min_p_row)})
+    if (reinterpret_cast<uintptr_t>(q) & 3u) return CA_ERR_INVALID;
   if (a->n_vocab > 8ll * kSampleSegBytes / (a->logits_bf16 ? 2 : 4)) return CA_ERR_UNSUPPORTED;
   SampleParams p{};
   p.logits = a->logits;

@@ -130,3 +130,23 @@ F8, F32, I32 = torch.float8_e4m3fn, torch.float32, torch.int32
 def test_python_arguments(make):
     with pytest.raises(ValueError):
         make()
+
+
+OFF = FAKE + 2  # 4-byte vectors that start between two entries
+
+
+@pytest.mark.parametrize("name", ["act_scale", "w_scale", "bias", "status"])
+def test_linear_q8_misaligned_vectors(name):
+    assert call(ca.lib.ca_linear_q8, layer.CaLinearQ8Args, LINEAR, {name: OFF}) == INV
+
+
+@pytest.mark.parametrize("name", ["act_scale", "gate_scale", "up_scale", "status"])
+def test_gated_linear_misaligned_vectors(name):
+    assert call(ca.lib.ca_gated_linear, layer.CaGatedLinearArgs, GATED, {name: OFF}) == INV
+
+
+@pytest.mark.parametrize("name", ["rows", "u", "token", "prob", "temperature_row", "top_k_row",
+                                  "top_p_row", "min_p_row", "suppress"])
+def test_sample_misaligned_vectors(name):
+    assert call(ca.lib.ca_sample, dn.CaSampleArgs, SAMPLE,
+                {name: OFF, "n_suppress": int(name == "suppress")}) == INV
