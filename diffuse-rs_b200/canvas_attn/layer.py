@@ -86,14 +86,22 @@ def _vector(name, x, n):
         raise ValueError(f"{name} must be contiguous float32 with {n} entries")
 
 
+def _status(x):
+    if x is not None and (str(x.dtype) != "torch.int32" or x.numel() < 1):
+        raise ValueError("status must be int32")
+
+
 def one_device(*xs):
-    """The tensors of a call are on one device, and that is the current one."""
+    """The tensors of a call are on one device, a GPU where there is one, and
+    that is the current one."""
     devices = {x.device for x in xs if x is not None}
     if len(devices) > 1:
         raise ValueError(f"tensors of one call are on {sorted(map(str, devices))}")
     dev = devices.pop()
+    import torch
+    if dev.type != "cuda" and torch.cuda.is_available():
+        raise ValueError(f"tensors are on {dev}")
     if dev.type == "cuda":
-        import torch
         if dev.index not in (None, torch.cuda.current_device()):
             raise ValueError(f"tensors are on {dev}, which is not the current device")
 
@@ -170,6 +178,7 @@ def make_linear_q8_args(act, act_scale, w, w_scale, out, *, bias=None, residual=
     _vector("act_scale", act_scale, n)
     _vector("w_scale", w_scale, rows)
     _vector("bias", bias, rows)
+    _status(status)
     one_device(act, act_scale, w, w_scale, out, bias, residual, status)
     a = CaLinearQ8Args(_ptr(act), as_, _ptr(act_scale), _ptr(w), _ptr(w_scale), _ptr(bias),
                        _ptr(residual), rs, _ptr(out), 1 if ot == F32 else 0, os_, n, rows, cols,
@@ -208,6 +217,7 @@ def make_gated_linear_args(act, w_gate, w_up, out, *, activation: str = "silu",
     _vector("act_scale", act_scale, n)
     _vector("gate_scale", gate_scale, rows)
     _vector("up_scale", up_scale, rows)
+    _status(status)
     one_device(act, act_scale, w_gate, w_up, gate_scale, up_scale, out, status)
     a = CaGatedLinearArgs(_ptr(act), kind, as_, _ptr(act_scale), _ptr(w_gate), _ptr(w_up),
                           _ptr(gate_scale), _ptr(up_scale), ACTIVATIONS[activation], _ptr(out),

@@ -150,3 +150,25 @@ def test_gated_linear_misaligned_vectors(name):
 def test_sample_misaligned_vectors(name):
     assert call(ca.lib.ca_sample, dn.CaSampleArgs, SAMPLE,
                 {name: OFF, "n_suppress": int(name == "suppress")}) == INV
+
+
+@pytest.mark.parametrize("make", [
+    lambda: layer.make_rms_norm_args(z(2, 8), z(2, 8)),
+    lambda: layer.make_linear_q8_args(z(2, 32, t=F8), None, z(4, 32, t=F8), None, z(2, 4)),
+    lambda: layer.make_gated_linear_args(z(2, 32), z(4, 32), z(4, 32), z(2, 4)),
+    lambda: dn.make_sample_args(z(2, 9, t=F32), None, z(2, t=F32), z(2, t=I32)),
+])
+def test_host_tensors_where_there_is_a_gpu(make, monkeypatch):
+    make()
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    with pytest.raises(ValueError, match="cpu"):
+        make()
+
+
+@pytest.mark.parametrize("status", [z(1, t=F32), z(0, t=I32)])
+def test_status_type(status):
+    with pytest.raises(ValueError, match="status"):
+        layer.make_linear_q8_args(z(2, 32, t=F8), None, z(4, 32, t=F8), None, z(2, 4),
+                                  status=status)
+    with pytest.raises(ValueError, match="status"):
+        layer.make_gated_linear_args(z(2, 32), z(4, 32), z(4, 32), z(2, 4), status=status)
