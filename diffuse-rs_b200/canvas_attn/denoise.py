@@ -197,11 +197,24 @@ def collect_candidates(state: DenoiseState, logits, n_vocab: int, rng: range, sh
     GPU. `logits`: device fp32 [len(seq), n_vocab]; its suppressed entries of
     the candidate rows are set to -inf, as process_logits does. At
     params.temperature > 0 token and prob are those of the draw, entropy and
-    margin the row's; draw_rng gives the random numbers."""
+    margin the row's; draw_rng gives the random numbers. Everything runs on
+    `stream` (None: the legacy default stream), the copies to the host too."""
     import torch
     pos = [p for p in rng if state.is_masked[p]]
     if not pos:
         return []
+    dev = logits.device
+    if dev.type == "cuda":
+        handle = _stream(stream)
+        on = (torch.cuda.ExternalStream(handle, device=dev) if handle
+              else torch.cuda.default_stream(dev))
+        with torch.cuda.stream(on):
+            return _collect(state, logits, n_vocab, pos, shift, params, handle, draw_rng)
+    return _collect(state, logits, n_vocab, pos, shift, params, stream, draw_rng)
+
+
+def _collect(state, logits, n_vocab, pos, shift, params, stream, draw_rng):
+    import torch
     dev = logits.device
     rows = torch.tensor([max(p - shift, 0) for p in pos], dtype=torch.int32, device=dev)
     n = len(pos)

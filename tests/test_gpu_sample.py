@@ -232,6 +232,31 @@ def test_denoising_step_with_temperature():
     assert min(want[i][1] for i in done) >= max(rest) * (1 - 2e-5)
 
 
+@pytest.mark.parametrize("temperature", [0.0, 0.8])
+def test_denoising_step_on_another_stream(temperature):
+    # The results are read after the work of the stream that was given, which
+    # is still busy when the call is made.
+    L, vocab, mask_id = 24, 5000, 4999
+    x = logits_of(31, L, vocab)
+    params = dn.StepParams(remasking=dn.CONFIDENCE, temperature=temperature, top_k=60)
+    host = x.cuda()
+    u = np.random.default_rng(6).random(L, dtype=np.float32)
+    want = [sample_ref(x[i].numpy(), u[i], temperature=temperature, top_k=60, dead=[mask_id])
+            for i in range(L)]
+    assert temperature == 0 or all(w[2] > vocab * STEP for w in want)
+    side = torch.cuda.Stream()
+    lg = torch.zeros_like(host)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # about a tenth of a second
+        lg.copy_(host)
+    st = dn.DenoiseState([mask_id] * L, [True] * L, mask_id)
+    got = dn.collect_candidates(st, lg, vocab, range(L), 0, params, stream=side,
+                                draw_rng=np.random.default_rng(6))
+    torch.cuda.synchronize()
+    assert [c.token for c in got] == [w[0] for w in want]
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("kw", [dict(top_p=0.9), dict(top_p=0.6, min_p=0.003),
                                 dict(top_k=9000), dict(top_k=9000, min_p=0.01),
