@@ -169,6 +169,12 @@ struct Product {
   LinearParams p;
 };
 
+// How many pieces of 128 bytes of the columns (four additions each) an
+// accumulator takes where the output is fp32, see pair.cuh: 1024 columns of
+// bf16, 4096 of e4m3, whose products have eight bits and leave less to cut off
+// (sums of one sign over 4096 columns 5e-7 off in 2-norm, over 18944 9e-6).
+constexpr int pieces_of_an_accumulator(int kind) { return kind == kKindBf16 ? 16 : 32; }
+
 template <int KIND, int G, int NT>
 int launch_skinny(const Product& q, cudaStream_t st) {
   using C = SkinnyCfg<KIND, G, NT>;
@@ -195,9 +201,9 @@ int launch_skinny(const Product& q, cudaStream_t st) {
   // 1, 2, 4 and 8 splits: 4096 x 4096 11.3, 8.1, 6.3, 7.1; 1024 x 4096 11.1, 8.0,
   // 5.9, 5.1; 12288 -> 4096 28, 16.5, 10.5, 9.9; gated 4096 -> 12288 in bf16 51,
   // 36, 40, 38.
-  // fp32 outputs of bf16 operands: few additions to an accumulator, too, which
-  // truncates (pair.cuh).
-  const int64_t most = KIND == kKindBf16 && q.p.out_f32 ? 16 : INT_MAX;
+  // fp32 outputs: few additions to an accumulator, too, which truncates
+  // (pair.cuh).
+  const int64_t most = q.p.out_f32 ? pieces_of_an_accumulator(KIND) : INT_MAX;
   int S = 1;
   while (S < 8 && q.p.kblocks > most * S) S *= 2;
   while (S < 8 && ((tiles * tok * S * 2 <= kSms && q.p.kblocks >= 8 * S) ||
@@ -249,13 +255,17 @@ int launch_pair(const Product& q, cudaStream_t st) {
 template <int KIND, int G>
 int launch_product(const Product& q, cudaStream_t st) {
   const int64_t tiles = (q.p.rows + 127) / 128 * ((q.p.n + 63) / 64);
-  if (q.p.n <= 64 || tiles <= (G == 1 ? 2 * kSms : kSms / 2)) {
+  constexpr int kPieces = pieces_of_an_accumulator(KIND);
+  const bool pieces = q.p.out_f32 && q.p.kblocks > kPieces;
+  // Long sums of e4m3 would need more splits here than tiles leave room for (512
+  // tokens 12288 -> 4096 to fp32 87 us in eight, pairs 38); bf16 tokens stay
+  // (gated, 128 tokens 8192 -> 1024 23 us, pairs 58).
+  if (q.p.n <= 64 || (tiles <= (G == 1 ? 2 * kSms : kSms / 2) &&
+                      !(KIND == kKindE4m3 && pieces))) {
     if (q.p.n <= 16) return launch_skinny<KIND, G, 16>(q, st);
     if (q.p.n <= 32) return launch_skinny<KIND, G, 32>(q, st);
     return launch_skinny<KIND, G, 64>(q, st);
   }
-  // 16 pieces of 64 bf16 are 64 additions to an accumulator.
-  if (KIND == kKindBf16 && q.p.out_f32) return launch_pair<KIND, G, 128, 16>(q, st);
   // A tile of 128 tokens takes a pair about as long as one of 256 (0.31 us a
   // piece alone: the weights' way into shared memory is the bound), so that it
   // pays only where there are no more rounds of them: 1536 tokens 4096 -> 4096 in
@@ -264,7 +274,12 @@ int launch_product(const Product& q, cudaStream_t st) {
   auto rounds = [&](int64_t nt) {
     return (rt * ((q.p.n + nt - 1) / nt) + kSms / 2 - 1) / (kSms / 2);
   };
-  if (rounds(128) <= rounds(256)) return launch_pair<KIND, G, 128>(q, st);
+  const bool small = rounds(128) <= rounds(256);
+  if constexpr (KIND == kKindE4m3) {
+    if (pieces && !small) return launch_pair<KIND, G, 256, kPieces>(q, st);
+  }
+  if (pieces) return launch_pair<KIND, G, 128, kPieces>(q, st);
+  if (small) return launch_pair<KIND, G, 128>(q, st);
   return launch_pair<KIND, G, 256>(q, st);
 }
 

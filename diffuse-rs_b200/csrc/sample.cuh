@@ -22,9 +22,14 @@
 // before a border for certain and which may hold it. Then either every entry
 // up to there fits a list of the cluster's first CTA, which settles the rest
 // by itself (a top-k, a sharp nucleus), or the entries of the doubtful bins do
-// (a wide nucleus). What fits neither (thousands of entries in one bin, as
-// rows of equal logits have) is settled by bisection of the keys over the
-// whole row, 32 sums a border.
+// (a wide nucleus); doubtful bins that hold too many get a histogram of their
+// own, finer by their number (32 rows of 250000 flat logits at top-p 0.9 189 us,
+// bisected 1.5 ms). What fits none of these (thousands of equal logits; in fp32
+// a top_k of more entries than the list has, together with top_p) is settled by
+// bisection of the keys over the whole row, 32 sums a border (1.5 ms).
+//
+// A small top_k needs no histogram: each thread's maximum gives a value that
+// at least top_k entries reach, and the entries from there on go to the list.
 //
 // bf16 logits take few values, so that their rows need less: a histogram over
 // the values themselves (those of the 17 largest binades that count; smaller

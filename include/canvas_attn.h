@@ -311,7 +311,8 @@ typedef struct {
     int32_t n_suppress;
     const float* u;           /* fp32 [n_cand]: a number in [0, 1) for each candidate (others are
                                  taken as the nearest in it, NaN as 0) */
-    float temperature;        /* <= 0 (or NaN): the maximum's first index, filters and u unused */
+    float temperature;        /* <= 0 (or NaN): the maximum's first index, filters and u unused;
+                                 below 2^-100: 2^-100 */
     int32_t top_k;            /* <= 0: off */
     float top_p;              /* >= 1 (or NaN): off; <= 0: the first entry alone */
     float min_p;              /* <= 0 (or NaN): off */

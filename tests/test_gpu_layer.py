@@ -295,6 +295,49 @@ def test_gated_sizes(n, rows, cols, kind):
     gated_case(n, rows, cols, kind=kind)
 
 
+# fp32 outputs of positive operands, where what the tensor core cuts off in its
+# additions is cut off in one direction. An accumulator takes at most 128
+# additions (32 pieces of 128 columns, four each), each cutting off less than
+# 2^-23 of what is there so far, half the end's on average over a sum that grows
+# evenly, to which 5% are given for its unevenness: 128 / 2 * 1.05 * 2^-23 =
+# 8.0e-6 of an entry; joining up to ten of them and rounding takes 10 * 2^-24 =
+# 6e-7.
+ONE_SIGN = 67.2 * 2.0 ** -23 + 10 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("n,rows", [(1, 9600), (16, 640), (40, 9600), (100, 640), (600, 4000),
+                                    (2048, 4096)])
+@pytest.mark.parametrize("cols", [4112, 18944])
+def test_linear_sums_of_one_sign(n, rows, cols):
+    torch.manual_seed(n + cols)
+    x = torch.rand(n, cols, device="cuda").to(F8)
+    w = torch.rand(rows, cols, device="cuda").to(F8)
+    o = torch.empty(n, rows, device="cuda")
+    layer.linear_q8(x, None, w, None, o)
+    y = x.double() @ w.double().T
+    assert float(((o.double() - y).abs() / y).max()) < ONE_SIGN
+
+
+@pytest.mark.parametrize("n", [1, 100, 300, 1100])
+def test_linear_long_to_fp32(n):
+    linear_case(n, 1300, 4368, bias=True, res=True, out="f32", pad=1)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n", [16, 100, 2048])
+def test_gated_sums_of_one_sign(n, kind):
+    # Both factors are off by ONE_SIGN at most; the gates are above 100, where
+    # silu(g) is g to less than 2^-24, and the three products round once each.
+    torch.manual_seed(n)
+    x = torch.rand(n, 8208, device="cuda").to(TYPE.get(kind, F8))
+    g, u = (torch.rand(2000, 8208, device="cuda").to(x.dtype) for _ in range(2))
+    o = torch.empty(n, 2000, device="cuda")
+    layer.gated_linear(x, g, u, o)
+    a, b = x.double() @ g.double().T, x.double() @ u.double().T
+    assert float(a.min()) > 100
+    assert float(((o.double() - a * b).abs() / (a * b)).max()) < 2 * ONE_SIGN + 6 * 2.0 ** -24
+
+
 def test_products_in_a_graph_on_another_stream_twice():
     g = gen(31)
     x, xs = (t.cuda() for t in operand(g, 100, 1024, "e4m3"))
