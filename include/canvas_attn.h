@@ -624,7 +624,8 @@ typedef struct {
  * ca_rms_norm -- residual_add and rms_norm_inplace (src/model/ops.rs:107-114,
  * src/model/forward.rs:345-370) of the rows between a layer's products, in one
  * pass: s = x + residual rounded to the residual stream's type (x itself
- * without one), y = s * w / sqrt(sum s^2 / cols + eps), sums in fp32. e4m3
+ * without one), y = s * w / sqrt(sum s^2 / cols + eps), squares in fp32, their
+ * sums in fp32 or more (so |s| below 6e18). e4m3
  * output: scale = 2^k with the smallest k in [-64, 120] such that no finite
  * |y| of the row exceeds 448 * 2^k, value = y / scale to nearest even;
  * infinities saturate, NaN stays NaN and takes no part in the scale (the rule

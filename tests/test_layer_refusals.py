@@ -159,6 +159,7 @@ def test_sample_misaligned_vectors(name):
     lambda: dn.make_sample_args(z(2, 9, t=F32), None, z(2, t=F32), z(2, t=I32)),
 ])
 def test_host_tensors_where_there_is_a_gpu(make, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: False)
     make()
     monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
     with pytest.raises(ValueError, match="cpu"):
