@@ -99,21 +99,23 @@ __device__ __forceinline__ u64 fixed44(double w) {
   return static_cast<u64>(__double_as_longlong(w + 256.0) - __double_as_longlong(256.0));
 }
 
-// 2^a for -1000 < a < 1000 to 2e-14: a = n + f with n the nearest whole number
-// (the low bits of a sum with 1.5 * 2^52), 2^f by the Chebyshev interpolation
-// of degree 9 on [-1/2, 1/2], n added to the exponent. The coefficients stand
-// in constant memory, where an instruction takes them from directly: as
-// immediates they cost two moves each, more than the arithmetic.
-__constant__ double kExp2[10] = {
-    1.000000000000014,      0.6931471805599526,     0.24022650695631514,    0.05550410866428854,
-    0.009618129195951041,   0.001333355825801874,   0.00015403432339553542, 1.5252640059770786e-05,
-    1.3259945262689143e-06, 1.0212097549811005e-07};
+// 2^a for -1000 < a < 1000 to 5e-16 and the roundings of its sums: a = n + f
+// with n the nearest whole number (the low bits of a sum with 1.5 * 2^52), 2^f
+// by the Chebyshev interpolation of degree 10 on [-1/2, 1/2], n added to the
+// exponent. Its eleven nodes hold 0, so that 2^0 is 1 to the bit: a row's
+// largest entry weighs exactly 1, which is what min_p counts on. The
+// coefficients stand in constant memory, where an instruction takes them from
+// directly: as immediates they cost two moves each, more than the arithmetic.
+__constant__ double kExp2[11] = {
+    1.0,                    0.69314718055995,       0.24022650695910097,   0.05550410866444772,
+    0.009618129107606888,   0.0013333558230164974,  0.0001540353044173605, 1.5252657260200837e-05,
+    1.321544258792169e-06,  1.0208690299958306e-07, 7.072585949269223e-09};
 __device__ __forceinline__ double exp2_64(double a) {
   const double t = a + 6755399441055744.0;
   const double f = a - (t - 6755399441055744.0);
-  double p = kExp2[9];
+  double p = kExp2[10];
 #pragma unroll
-  for (int i = 8; i >= 0; --i) p = fma(p, f, kExp2[i]);
+  for (int i = 9; i >= 0; --i) p = fma(p, f, kExp2[i]);
   return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
 }
 
@@ -140,7 +142,7 @@ struct SampleShared {
 struct SampleWeights {
   float m;
   float bin_c;    // place = -bin_c (l - m) + 2^23, whose low bits are the bin
-  double c, b;    // log2 w = c l + b
+  double c, top;  // log2 w = c (l - top), top: m in 64 bits
   double least;   // min_p
 
   // To the nearest bin; not below kNowhere for an entry without a weight (NaN
@@ -152,8 +154,11 @@ struct SampleWeights {
   __device__ __forceinline__ static uint32_t bin(float place) {
     return __float_as_uint(place) - 0x4B000000u;
   }
-  __device__ __forceinline__ double weight(float l) const {  // of an entry that is not none()
-    return exp2_64(fma(static_cast<double>(l), c, b));
+  // Of an entry that is not none(). The difference comes first: it is exact or
+  // off by 2^-53 of itself, 0 for the maximum. c l - c m would be off by 2^-53 of
+  // c m, which at low temperatures or far from 0 is more than there are bits.
+  __device__ __forceinline__ double weight(float l) const {
+    return exp2_64((static_cast<double>(l) - top) * c);
   }
   __device__ __forceinline__ u64 fixed(float l) const {
     return none(l) ? 0 : fixed44(weight(l));
@@ -703,6 +708,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
     sh.border[0] = __float_as_uint(-INFINITY);  // no border
     sh.border[1] = 0;
     sh.border[2] = 1;
+    sh.found[0] = sh.found[1] = sh.answer = 0;
   }
   for (int i = tid; i < 8 * kSampleWarps; i += kSampleThreads) sh.range_sum[i] = 0;
   __syncthreads();
@@ -792,7 +798,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
     } else {
       // (Temperatures below 2^-100 as 2^-100.)
       wt.c = 1.4426950408889634 / static_cast<double>(fmaxf(temp, 0x1p-100f));
-      wt.b = -static_cast<double>(m) * wt.c;
+      wt.top = static_cast<double>(m);
       wt.bin_c = static_cast<float>(wt.c) * kBinsPerOctave;
       uint32_t K = 0, I = 0xffffffffu;
       auto before = [&](float l, int i) {
