@@ -805,9 +805,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
         const uint32_t k = key_of(l);
         return k > K || (k == K && static_cast<uint32_t>(i) <= I);
       };
+      float end = kNowhere;  // places from here on have no weight, or are cut
       auto kept_weight = [&](float l) -> u64 {  // of any entry: 0 without a weight
         const double w = wt.weight(l);
-        return wt.place(l) < kNowhere && w >= wt.least ? fixed44(w) : 0;
+        return wt.place(l) < end && w >= wt.least ? fixed44(w) : 0;
       };
       const bool by_k = top_k > 0 && top_k < p.n_vocab, by_p = top_p < 1.f;
       bool done = false;
@@ -1352,7 +1353,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
             }
           }
           done = whole || !thin;
-        } else if (b_lo <= b_hi || by_p) {  // else: fewer entries than top_k have a weight
+        } else if (b_lo > b_hi && !by_p) {
+          // No bin is in doubt: the first top_k entries end with a bin, the last
+          // before b_lo, or (b_lo is behind all bins) no more than those have a
+          // weight.
+          if (b_lo < kBins) end = 8388608.f + static_cast<float>(b_lo);
+        } else {
           if (by_k) {
             uint32_t key = 0;  // the largest key that top_k entries reach
             for (int b = 31; b >= 0; --b) {
