@@ -175,9 +175,10 @@ struct Product {
 // (sums of one sign over 4096 columns 5e-7 off in 2-norm, over 18944 9e-6).
 constexpr int pieces_of_an_accumulator(int kind) { return kind == kKindBf16 ? 16 : 32; }
 
-template <int KIND, int G, int NT>
-int launch_skinny(const Product& q, cudaStream_t st) {
-  using C = SkinnyCfg<KIND, G, NT>;
+// tiles x tok tiles of 128 rows by NT tokens, each by a cluster of S CTAs.
+template <class C>
+int launch_skinny_as(const Product& q, int64_t tiles, int64_t tok, int S, cudaStream_t st) {
+  constexpr int KIND = C::KIND, G = C::G, NT = C::NT;
   static bool attr_done[kMaxDevices] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return CA_ERR_CUDA;
@@ -194,6 +195,13 @@ int launch_skinny(const Product& q, cudaStream_t st) {
       return CA_ERR_CUDA;
     attr_done[dev] = true;
   }
+  return launch_cluster_after(skinny_kernel<C>,
+                              dim3(static_cast<unsigned>(tiles * S), static_cast<unsigned>(tok)),
+                              C::kThreads, C::kSmem, S, st, tw, tu, tx, q.p);
+}
+
+template <int KIND, int G, int NT>
+int launch_skinny(const Product& q, cudaStream_t st) {
   const int64_t tiles = (q.p.rows + 127) / 128, tok = (q.p.n + NT - 1) / NT;
   if (tiles > INT_MAX / 8 || tok > 65535) return CA_ERR_UNSUPPORTED;
   // Columns are split until there is a CTA for each SM, down to four pieces a
@@ -202,16 +210,17 @@ int launch_skinny(const Product& q, cudaStream_t st) {
   // 5.9, 5.1; 12288 -> 4096 28, 16.5, 10.5, 9.9; gated 4096 -> 12288 in bf16 51,
   // 36, 40, 38.
   // fp32 outputs: few additions to an accumulator, too, which truncates
-  // (pair.cuh).
-  const int64_t most = q.p.out_f32 ? pieces_of_an_accumulator(KIND) : INT_MAX;
+  // (pair.cuh), by more splits and, beyond eight, by more accumulators.
+  constexpr int kPieces = pieces_of_an_accumulator(KIND);
+  const int64_t most = q.p.out_f32 ? kPieces : INT_MAX;
   int S = 1;
   while (S < 8 && q.p.kblocks > most * S) S *= 2;
   while (S < 8 && ((tiles * tok * S * 2 <= kSms && q.p.kblocks >= 8 * S) ||
                    (tiles * tok * S * 2 <= 2 * kSms && q.p.kblocks >= 24 * S)))
     S *= 2;
-  return launch_cluster_after(skinny_kernel<C>,
-                              dim3(static_cast<unsigned>(tiles * S), static_cast<unsigned>(tok)),
-                              C::kThreads, C::kSmem, S, st, tw, tu, tx, q.p);
+  if (q.p.kblocks > most * S)
+    return launch_skinny_as<SkinnyCfg<KIND, G, NT, kPieces>>(q, tiles, tok, S, st);
+  return launch_skinny_as<SkinnyCfg<KIND, G, NT>>(q, tiles, tok, S, st);
 }
 
 template <int KIND, int G, int NT, int CHUNK = 0>

@@ -13,10 +13,15 @@
 // to the shared memory of the CTA that finishes it, which adds the parts in
 // the order of their ranks: no workspace, no atomics, the same bits every time.
 //
+// CHUNK > 0 (fp32 outputs of more columns than the largest split takes): as in
+// pair.cuh an accumulator takes CHUNK pieces of 128 bytes at most, which the
+// storing warps add up in registers while the next one fills.
+//
 // Lane = weight row, TMEM column = token, so that a warp's 32 threads store 32
 // neighbours of an output row.
 #pragma once
 
+#include <climits>
 #include <cstdint>
 #include <cuda_bf16.h>
 
@@ -142,8 +147,9 @@ __device__ __forceinline__ float act_scale_of(const LinearParams& p, long long t
   return p.act_scale && t < p.n ? p.act_scale[t] : 1.f;
 }
 
-template <int KIND_, int G_, int NT_>
+template <int KIND_, int G_, int NT_, int CHUNK_ = 0>
 struct SkinnyCfg {
+  static constexpr int CHUNK = CHUNK_;
   static constexpr int KIND = KIND_;  // operands
   static constexpr int G = G_;        // weight matrices
   static constexpr int NT = NT_;      // tokens of a CTA
@@ -156,14 +162,20 @@ struct SkinnyCfg {
   static constexpr int kRing = kStages * kStage;
   static_assert(kApart || kRing >= kParts, "the parts of a sum are laid over the ring");
   static constexpr int kThreads = 192;
-  static constexpr int kBars = 2 * kStages + 1;
+  static constexpr int kBufs = CHUNK > 0 ? 2 : 1;  // accumulators
+  static constexpr int kBars = 2 * kStages + 2 * kBufs;
   static constexpr int kSmem = 1024 + kRing + (kApart ? kParts : 0) + 8 * kBars + 16;
-  static constexpr int kTmemCols = G * NT < 32 ? 32 : G * NT;
+  static constexpr int kBuf = G * NT;  // TMEM columns of an accumulator
+  static constexpr int kTmemCols = kBufs * kBuf < 32 ? 32 : kBufs * kBuf;
+  static_assert(kTmemCols <= 256, "two CTAs share an SM");
   static constexpr int kElems = KIND == kKindBf16 ? 64 : 128;  // of 128 bytes
 };
 
+// CHUNK: two CTAs an SM (168 registers, with 84 bytes of spills at 64 tokens of
+// two matrices, which would take 175: gated, 64 tokens 18944 -> 4096 in bf16 43
+// us, one CTA an SM 91).
 template <class C>
-__global__ void __launch_bounds__(C::kThreads)
+__global__ void __launch_bounds__(C::kThreads, C::CHUNK > 0 ? 2 : 1)
     skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_u,
                   const __grid_constant__ CUtensorMap tm_x, const LinearParams p) {
   extern __shared__ uint8_t raw_smem[];
@@ -174,7 +186,8 @@ __global__ void __launch_bounds__(C::kThreads)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   auto full = [&](int s) { return bars + 8 * s; };
   auto empty = [&](int s) { return bars + 8 * (C::kStages + s); };
-  const uint32_t done = bars + 8 * (2 * C::kStages);
+  auto acc_full = [&](int b) { return bars + 8 * (2 * C::kStages + b); };
+  auto acc_empty = [&](int b) { return bars + 8 * (2 * C::kStages + C::kBufs + b); };
   const uint32_t S = cluster_size(), rank = cluster_rank();
   const int r0 = static_cast<int>(blockIdx.x / S) * 128;
   const int t0 = static_cast<int>(blockIdx.y) * C::NT;
@@ -199,7 +212,10 @@ __global__ void __launch_bounds__(C::kThreads)
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
     }
-    mbar_init(done, 1);
+    for (int b = 0; b < C::kBufs; ++b) {
+      mbar_init(acc_full(b), 1);
+      mbar_init(acc_empty(b), 4);
+    }
     fence_barrier_init();
     fence_proxy_async_smem();
   }
@@ -241,8 +257,17 @@ __global__ void __launch_bounds__(C::kThreads)
   } else if (warp == 1) {
     if (lane == 0) {
       constexpr uint32_t idesc = linear_idesc(C::KIND, 128, C::NT);
-      int i = 0;
-      for (int kb = kb0; kb < kb1; ++kb, ++i) {
+      constexpr int kChunk = C::CHUNK > 0 ? C::CHUNK : INT_MAX;
+      int i = 0, n = 0, in = 0;  // pieces taken; accumulators filled; pieces in this one
+      uint32_t acc = tmem;
+      for (int kb = kb0; kb < kb1; ++kb, ++i, ++in) {
+        if (in == kChunk) {
+          umma_commit(acc_full(n++ & 1));
+          in = 0;
+          if (n >= 2 && !mbar_wait(acc_empty(n & 1), ((n >> 1) - 1) & 1, dead, p.err)) break;
+          tc_fence_after();
+          acc = tmem + (n & 1) * C::kBuf;
+        }
         const int s = i % C::kStages;
         if (!mbar_wait(full(s), (i / C::kStages) & 1, dead, p.err)) break;
         tc_fence_after();
@@ -251,13 +276,13 @@ __global__ void __launch_bounds__(C::kThreads)
         const uint64_t dx = umma_desc_sw128(at + C::G * 16384, 16, 1024);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
-          mma_ss<C::KIND>(tmem, dw + 2 * kk, dx + 2 * kk, idesc, i | kk);
+          mma_ss<C::KIND>(acc, dw + 2 * kk, dx + 2 * kk, idesc, in | kk);
           if constexpr (C::G == 2)
-            mma_ss<C::KIND>(tmem + C::NT, dw + 1024 + 2 * kk, dx + 2 * kk, idesc, i | kk);
+            mma_ss<C::KIND>(acc + C::NT, dw + 1024 + 2 * kk, dx + 2 * kk, idesc, in | kk);
         }
         umma_commit(empty(s));
       }
-      umma_commit(done);
+      umma_commit(acc_full(n & 1));
     }
     __syncwarp();
   }
@@ -280,29 +305,66 @@ __global__ void __launch_bounds__(C::kThreads)
   constexpr int kGroup = C::NT < 32 ? C::NT : 32;
   float x[kGroup];
   if (C::G == 1 && on && p.residual) load_residual(p, x, t0 + first, r, mine);
+  const uint32_t col = tmem + (static_cast<uint32_t>(warp & 3) << 21);
+  float v0[C::CHUNK > 0 ? C::NT : 1], v1[C::CHUNK > 0 && C::G == 2 ? C::NT : 1];  // CHUNK's sums
   if (warp >= 2) {
     if (r < p.rows) {
       if (p.w_scale) w0 = p.w_scale[r];
       if (C::G == 2 && p.up_scale) w1 = p.up_scale[r];
       if (C::G == 1 && p.bias) bias = p.bias[r];
     }
-    mbar_wait(done, 0, dead, p.err);
-    __syncwarp();
-    tc_fence_after();
+    if constexpr (C::CHUNK == 0) {
+      mbar_wait(acc_full(0), 0, dead, p.err);
+      __syncwarp();
+      tc_fence_after();
+    } else {
+#pragma unroll
+      for (int j = 0; j < C::NT; ++j) {
+        v0[j] = 0.f;
+        if constexpr (C::G == 2) v1[j] = 0.f;
+      }
+      for (int n = 0; n * C::CHUNK < kb1 - kb0; ++n) {
+        mbar_wait(acc_full(n & 1), (n >> 1) & 1, dead, p.err);
+        __syncwarp();
+        tc_fence_after();
+#pragma unroll
+        for (int j0 = 0; j0 < C::NT; j0 += 16) {
+          uint32_t d0[16], d1[16];
+          tmem_ld16(col + (n & 1) * C::kBuf + j0, d0);
+          if constexpr (C::G == 2) tmem_ld16(col + (n & 1) * C::kBuf + C::NT + j0, d1);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            v0[j0 + j] += __uint_as_float(d0[j]);
+            if constexpr (C::G == 2) v1[j0 + j] += __uint_as_float(d1[j]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty(n & 1));
+      }
+    }
   }
   __syncwarp();
   cluster_wait();                               // every CTA of the cluster has started
   if (S > 1 && !C::kApart) cluster_sync_all();  // every ring is free
   if (warp >= 2) {
-    const uint32_t col = tmem + (static_cast<uint32_t>(warp & 3) << 21);
 #pragma unroll
     for (int j0 = 0; j0 < C::NT; j0 += 16) {
       if (j0 >= live) break;
       uint32_t d0[16], d1[16];
-      tmem_ld16(col + j0, d0);
-      if constexpr (C::G == 2) tmem_ld16(col + C::NT + j0, d1);
+      if constexpr (C::CHUNK == 0) {
+        tmem_ld16(col + j0, d0);
+        if constexpr (C::G == 2) tmem_ld16(col + C::NT + j0, d1);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          d0[j] = __float_as_uint(v0[j0 + j]);
+          if constexpr (C::G == 2) d1[j] = __float_as_uint(v1[j0 + j]);
+        }
+      }
       const float sa = act_scale_of(p, t0 + j0 + (lane & 15));
-      tmem_wait_ld();
+      if constexpr (C::CHUNK == 0) tmem_wait_ld();
       if (S == 1) {
         float v[16];
 #pragma unroll
