@@ -175,7 +175,7 @@ struct SkinnyCfg {
 // two matrices, which would take 175: gated, 64 tokens 18944 -> 4096 in bf16 43
 // us, one CTA an SM 91).
 template <class C>
-__global__ void __launch_bounds__(C::kThreads, C::CHUNK > 0 ? 2 : 1)
+__global__ void __launch_bounds__(C::kThreads, C::CHUNK > 0 ? 2 : 0)
     skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_u,
                   const __grid_constant__ CUtensorMap tm_x, const LinearParams p) {
   extern __shared__ uint8_t raw_smem[];
