@@ -314,7 +314,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::kThreads)
             float other;
             asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(theirs + j * 128) : "memory");
             const float g = up ? other : d[j], u = up ? d[8 + j] : other;
-            v[j] = activate(g * w0, p.act) * (u * w1);
+            v[j] = activate(g * w0, p.act, p.out_f32) * (u * w1);
           }
           const long long t = t0 + j0 + (up ? 8 : 0);
           store_tokens(p, v, t, r, tokens_in<8>(p, t, ok));

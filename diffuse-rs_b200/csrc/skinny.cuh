@@ -86,11 +86,22 @@ __device__ __forceinline__ void st_shared_f32(uint32_t addr, float v) {
 
 // The gate's activation, in fp32: g / (1 + e^-g), and with y = sqrt(2/pi) (g +
 // 0.044715 g^3), 0.5 g (1 + tanh y) = g / (1 + e^-2y). Exponentials that run to
-// infinity give 0.
-__device__ __forceinline__ float activate(float g, int act) {
-  if (act == 0) return __fdividef(g, 1.f + __expf(-g));
-  const float y = 0.7978845608028654f * (g + 0.044715f * g * g * g);
-  return __fdividef(g, 1.f + __expf(-2.f * y));
+// infinity give 0. 2^(x log2 e) of a rounded product is off by 2 + 1.16 |x| units
+// of 2^-23 (1e-5 at -80), which a bf16 output does not show (2e-3). For fp32 ones
+// (`exact`) what the product lost, and the constant, come back as a factor: 2
+// units, one for the factor and 2 for the quotient. (expf and a division took
+// 2048 gated tokens 4096 -> 12288 in e4m3 from 160 to 256 us.)
+__device__ __forceinline__ float activate(float g, int act, bool exact) {
+  constexpr float kLog2E = 1.44269502f, kLog2ERest = 1.92596299e-8f, kLn2 = 0.693147182f;
+  const float x =
+      act == 0 ? -g : -2.f * (0.7978845608028654f * (g + 0.044715f * g * g * g));
+  float e = ex2_approx(x * kLog2E);
+  if (exact) {
+    const float c = fminf(fmaxf(x, -200.f), 200.f);  // (beyond, e is 0 or infinite)
+    const float lost = fmaf(c, kLog2ERest, fmaf(c, kLog2E, -(c * kLog2E)));
+    e *= fmaf(lost, kLn2, 1.f);
+  }
+  return __fdividef(g, 1.f + e);
 }
 
 // How many of the N tokens from t on have an element r of their own.
@@ -292,7 +303,7 @@ __global__ void __launch_bounds__(C::kThreads, C::CHUNK > 0 ? 2 : 0)
   const long long r = r0 + f;
   float w0 = 1.f, w1 = 1.f, bias = 0.f;
   auto combine = [&](float a, float b, float sa) {
-    return C::G == 2 ? activate(a * sa * w0, p.act) * (b * sa * w1) : a * sa * w0 + bias;
+    return C::G == 2 ? activate(a * sa * w0, p.act, p.out_f32) * (b * sa * w1) : a * sa * w0 + bias;
   };
   const int live = static_cast<int>(min(static_cast<long long>(C::NT), p.n - t0));  // tokens
   const int each = C::NT / static_cast<int>(S);  // tokens that a rank finishes, from `first` on
