@@ -117,6 +117,16 @@ __device__ __forceinline__ void pair_tile(const LinearParams& p, int i, int& rt,
   tt = j / size;
 }
 
+// A row's scale w as factors of a sum before and after the token's scale, one of
+// them 1: below 1 it goes first, to the same end as in `scaled`, whose choice for
+// each element took 512 tokens 4096 -> 4096 from 15.5 to 16.4 us here. Without a
+// token's scale: all of it after.
+struct RowScale {
+  float before, after;
+  __device__ __forceinline__ RowScale(float w, bool alone)
+      : before(!alone && fabsf(w) < 1.f ? w : 1.f), after(!alone && fabsf(w) < 1.f ? 1.f : w) {}
+};
+
 template <class C>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::kThreads)
     pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_u,
@@ -266,10 +276,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::kThreads)
       const long long r = static_cast<long long>(rt) * C::kRows + rank * (C::kRows / 2) + q;
       const long long t0 = static_cast<long long>(tt) * C::NT + half0;
       const bool ok = r < p.rows;
-      float w0 = 1.f, w1 = 1.f, bias = 0.f;
+      RowScale w0(1.f, true), w1(1.f, true);
+      float bias = 0.f;
       if (ok) {
-        if (p.w_scale) w0 = p.w_scale[r];
-        if (C::G == 2 && p.up_scale) w1 = p.up_scale[r];
+        if (p.w_scale) w0 = RowScale(p.w_scale[r], !p.act_scale);
+        if (C::G == 2 && p.up_scale) w1 = RowScale(p.up_scale[r], !p.act_scale);
         if (C::G == 1 && p.bias) bias = p.bias[r];
       }
       if (p.act_scale) {
@@ -278,6 +289,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::kThreads)
           st_shared_f32(sa_at + 4 * j, t0 + j < p.n ? p.act_scale[t0 + j] : 1.f);
         __syncwarp();
       }
+      const float before = up ? w1.before : w0.before;  // of the rows that this warp holds
       // Residuals of the 32 tokens to come; the first ones are asked for before
       // the tile is there.
       float next[2][16];
@@ -297,7 +309,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::kThreads)
                          : "=f"(s[0]), "=f"(s[1]), "=f"(s[2]), "=f"(s[3])
                          : "r"(sa_at + 4 * (j0 + j)));
 #pragma unroll
-            for (int k = 0; k < 4; ++k) d[j + k] *= s[k];
+            for (int k = 0; k < 4; ++k) d[j + k] = d[j + k] * before * s[k];
           }
         }
         if constexpr (C::G == 2) {
@@ -314,13 +326,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(C::kThreads)
             float other;
             asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(theirs + j * 128) : "memory");
             const float g = up ? other : d[j], u = up ? d[8 + j] : other;
-            v[j] = activate(g * w0, p.act, p.out_f32) * (u * w1);
+            v[j] = activate(g * w0.after, p.act, p.out_f32) * (u * w1.after);
           }
           const long long t = t0 + j0 + (up ? 8 : 0);
           store_tokens(p, v, t, r, tokens_in<8>(p, t, ok));
         } else {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) d[j] = fmaf(d[j], w0, bias);
+          for (int j = 0; j < 16; ++j) d[j] = fmaf(d[j], w0.after, bias);
           if (p.residual) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) d[j] += next[h][j];

@@ -104,6 +104,15 @@ __device__ __forceinline__ float activate(float g, int act, bool exact) {
   return __fdividef(g, 1.f + e);
 }
 
+// A sum times its two scales, a token's and a row's, the smaller one first: it is
+// out of range in between only where the result is (rows quantised at 2^100 and
+// more times weights of 2^-10 are finite). No operand's scale from ca_rms_norm
+// takes a sum below the normal numbers.
+__device__ __forceinline__ float scaled(float a, float s, float w) {
+  const bool first = fabsf(s) < fabsf(w);
+  return a * (first ? s : w) * (first ? w : s);
+}
+
 // How many of the N tokens from t on have an element r of their own.
 template <int N>
 __device__ __forceinline__ int tokens_in(const LinearParams& p, long long t, bool ok) {
@@ -303,7 +312,8 @@ __global__ void __launch_bounds__(C::kThreads, C::CHUNK > 0 ? 2 : 0)
   const long long r = r0 + f;
   float w0 = 1.f, w1 = 1.f, bias = 0.f;
   auto combine = [&](float a, float b, float sa) {
-    return C::G == 2 ? activate(a * sa * w0, p.act, p.out_f32) * (b * sa * w1) : a * sa * w0 + bias;
+    const float s = scaled(a, sa, w0);
+    return C::G == 2 ? activate(s, p.act, p.out_f32) * scaled(b, sa, w1) : s + bias;
   };
   const int live = static_cast<int>(min(static_cast<long long>(C::NT), p.n - t0));  // tokens
   const int each = C::NT / static_cast<int>(S);  // tokens that a rank finishes, from `first` on
