@@ -50,9 +50,11 @@ int launch_rows(const RowsParams& p, cudaStream_t st) {
     const int t = threads(1);
     return launch_after(rows_kernel<XF32, RES, OUT, 1>, grid(t), t, 0, st, p);
   }
-  if (chunks <= 1024) {
-    const int t = threads(2);
-    return launch_after(rows_kernel<XF32, RES, OUT, 2>, grid(t), t, 0, st, p);
+  if constexpr (!XF32 && RES != 2) {
+    if (chunks <= 1024) {
+      const int t = threads(2);
+      return launch_after(rows_kernel<XF32, RES, OUT, 2>, grid(t), t, 0, st, p);
+    }
   }
   if (chunks <= 1536) {
     const int t = threads(3);
