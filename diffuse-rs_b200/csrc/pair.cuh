@@ -23,8 +23,11 @@
 // as it accumulates: without it fp32 results of bf16 operands of 4112 columns
 // were 9e-6 off in 2-norm, those of e4m3 ones over 18944 columns 9e-6 where all
 // products have one sign (5e-7 over 4096 columns, and with it). It is for fp32
-// outputs alone; a bf16 one rounds by 2e-3. 8192 tokens 12288 -> 4096 in e4m3 to
-// fp32: 320 us without it, 342 with it, 530 to 580 in tiles of 128 tokens.
+// outputs alone; a bf16 one rounds by 2e-3. (512 gated tokens 4096 -> 12288 in
+// bf16: one rounding in 220 falls to the other side of that of exact sums, 2e-4
+// in 2-norm; results are as far from the exact ones, 1.6567e-3.) 8192 tokens
+// 12288 -> 4096 in e4m3 to fp32: 320 us without it, 342 with it (128 sums a
+// thread, 848 bytes of spills), 530 to 580 in tiles of 128 tokens.
 //
 // Warps: 0 loads (TMA, both CTAs, completing on the even CTA's barriers), 1
 // issues (the even CTA alone), 2-9 store, half the tokens of 32 lanes each.

@@ -157,8 +157,9 @@ __device__ __forceinline__ float inv_root(double x) {
 
 // C chunks of eight elements a thread; blockDim.x * C * 8 >= cols. At most 64
 // registers (128 of five chunks), so that an SM holds 1024 threads; of three
-// or five chunks the gain is read for each row (from L1). RES: 0 none,
-// 1 bf16, 2 fp32.
+// or five chunks the gain is read for each row (from L1). Forms of three and five
+// chunks with a residual or fp32 rows spill 8 to 350 bytes. RES: 0 none, 1 bf16,
+// 2 fp32.
 template <bool XF32, int RES, int OUT, int C>
 __global__ void __launch_bounds__(C >= 3 ? 512 : 1024, C == 3 ? 2 : 1)
     rows_kernel(const RowsParams p) {
@@ -317,7 +318,8 @@ __device__ __forceinline__ void store_strided(void* row, int f32, int cols, cons
 
 // Rows of any alignment, element by element, N a thread (N * blockDim.x >=
 // cols), otherwise as rows_kernel: held in registers between the passes, the
-// gain among them. Several CTAs on an SM hide what a row waits for.
+// gain among them. Several CTAs on an SM hide what a row waits for. (N = 20: 88
+// bytes of spills.)
 template <int N>
 __global__ void __launch_bounds__(1024) rows_odd_kernel(const RowsParams p) {
   __shared__ double red_d[2][32];

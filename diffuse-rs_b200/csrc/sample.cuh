@@ -630,6 +630,7 @@ struct SampleList {
   }
 };
 
+// Two CTAs an SM: 64 registers, with 80 bytes of spills (44 for bf16 rows).
 template <class T>
 __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) uint8_t raw_smem[];

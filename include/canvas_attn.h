@@ -657,8 +657,11 @@ typedef struct {
 /*
  * ca_linear_q8 -- ca_linear over 8-bit operands: out = act_scale * w_scale *
  * (act . W^T) (+ bias) (+ residual), products of e4m3 rows summed in fp32 on
- * the tensor cores, one rounding to out's type. Asynchronous on `stream`;
- * allocates nothing.
+ * the tensor cores, one rounding to out's type. The tensor cores truncate as
+ * they add: sums for fp32 outputs are joined every 4096 columns, those for bf16
+ * ones are not (about 1e-5 of a long sum, before its rounding). After an expired
+ * wait (status, ca_device_status) the contents of out are undefined.
+ * Asynchronous on `stream`; allocates nothing.
  */
 int ca_linear_q8(const ca_linear_q8_args* a, void* stream);
 
@@ -689,7 +692,8 @@ typedef struct {
  * ca_gated_linear -- the first half of ffn_block (src/model/forward.rs:
  * 354-370, :439-461): out = activation(act . Wgate^T) * (act . Wup^T), both
  * products in fp32 on the tensor cores, the activation and the product of the
- * two in the same kernel, one rounding. Neither product goes to memory.
+ * two in the same kernel, one rounding. Neither product goes to memory. Sums are
+ * taken as in ca_linear_q8 (joined every 1024 columns of bf16 for fp32 outputs).
  * Asynchronous on `stream`; allocates nothing.
  */
 int ca_gated_linear(const ca_gated_linear_args* a, void* stream);
