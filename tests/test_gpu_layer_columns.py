@@ -55,3 +55,37 @@ def test_both_signs(n):
         gated_case(n, 300, cols, kind="bf16", act="gelu", out="f32", scale_w=0.01)
     gated_case(n, 140, 40000, kind="e4m3", out="f32", scale_w=0.01)
     gated_case(n, 140, 12288, kind="bf16")
+
+
+def test_in_a_graph_and_on_two_streams_at_once():
+    torch.manual_seed(5)
+    x = torch.randn(50, 12288, device="cuda").to(torch.bfloat16)
+    g, u = ((torch.randn(2000, 12288, device="cuda") * 0.01).to(x.dtype) for _ in range(2))
+    y = torch.randn(40, 33008, device="cuda").to(F8)
+    w = torch.randn(1500, 33008, device="cuda").to(F8)
+    want = torch.empty(50, 2000, device="cuda"), torch.empty(40, 1500, device="cuda")
+    layer.gated_linear(x, g, u, want[0])
+    layer.linear_q8(y, None, w, None, want[1])
+    got = [torch.zeros_like(o) for o in want]
+    a = layer.make_gated_linear_args(x, g, u, got[0])
+    b = layer.make_linear_q8_args(y, None, w, None, got[1])
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=st):
+        layer.gated_linear_args(a, st)
+        layer.linear_q8_args(b, st)
+    for _ in range(3):
+        got[0].zero_()
+        got[1].zero_()
+        gr.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for o in got:
+        o.zero_()
+    torch.cuda.synchronize()
+    for i in range(10):
+        layer.gated_linear_args(a, st if i % 2 else None)
+        layer.linear_q8_args(b, None if i % 2 else st)
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
